@@ -535,6 +535,83 @@ int sspmm_attention_fm_ragged_f16(int batch, int heads, int seq, int head_dim, c
                                   void *hip_stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Serving: attention over whole prompts, and a paged cache in 8 bits that single tokens read.  No counterpart in the reference, whose
+ * models are encoders over sequences of one length (end2end/sspmm_e2e/end_to_end.py:123-153).
+ *
+ * Types of activations: fp16 and bf16 (bit patterns either way).  Formats of the cache: int8 and e4m3 (finite values up to 448, as
+ * in torch.float8_e4m3fn).  Heads have 32, 64 or 128 features; heads is a multiple of kv_heads, query head h goes with head
+ * h / (heads / kv_heads) of keys and values.  scale positive, and finite times log2(e).  Activations are 16-byte aligned with
+ * strides in elements that are multiples of 8; strides between tokens are at least head_dim.
+ * ---------------------------------------------------------------------------------------- */
+#define SSPMM_TYPE_F16 0
+#define SSPMM_TYPE_BF16 1
+#define SSPMM_CACHE_INT8 0
+#define SSPMM_CACHE_E4M3 1
+
+/*
+ * out_i = softmax over j of (q_i . k_j * scale) times v_j per sequence and head; sequence b is tokens offsets[b] .. offsets[b + 1] - 1
+ * (device, sequences + 1 of them, ascending within 0 .. tokens; others are taken to the nearest of these).  causal: j <= i.  Token i,
+ * head h of q is at q + i * q_row + h * q_head elements, and so on.  Tokens of no sequence are neither read nor written.  A row whose scores
+ * are all -infinity is zeros.  Row strides below 2^23.
+ */
+int sspmm_prompt_attention(int type, int sequences, int tokens, int heads, int kv_heads, int head_dim, const int32_t *offsets,
+                           const sspmm_half_t *q, int64_t q_row, int64_t q_head, const sspmm_half_t *k, int64_t k_row, int64_t k_head,
+                           const sspmm_half_t *v, int64_t v_row, int64_t v_head, int causal, float scale, sspmm_half_t *out,
+                           int64_t out_row, int64_t out_head, void *hip_stream);
+
+/*
+ * The cache: keys [pages, kv_heads, page_size, head_dim], values [pages, kv_heads, head_dim, page_size], one byte an element, scales
+ * [pages, 2, kv_heads] (keys, values): element = code * scale.  page_size 32, 64 or 128; all of it dense, 16-byte aligned.
+ * page_table [rows, slots]: the page of positions slot * page_size .. of a row; an entry outside 0 .. pages - 1 is no page: what would be
+ * written there is dropped, and what would be read is masked.
+ *
+ * sspmm_cache_write: tokens offsets[b] .. offsets[b + 1] - 1 of k and v to positions starts[b] on of row b.  A page has one scale per head for its
+ * keys and one for its values: max |x| / 127 (int8), or the smallest power of two that brings it to 448 or less (e4m3), codes are rounded to
+ * nearest, ties to even.  Tokens in front of the new ones in their page are kept: the scale is then the larger of the page's and the new
+ * tokens', and if it grows the kept codes are brought to it.  What lies behind the new ones in their page counts as unwritten.  A block that is
+ * given an infinity or NaN has scale NaN until it is written from its page's first position again.  No two rows of a call may write to the same page.
+ */
+int sspmm_cache_write(int type, int format, int sequences, int tokens, const int32_t *offsets, const int32_t *starts,
+                      const sspmm_half_t *k, int64_t k_row, int64_t k_head, const sspmm_half_t *v, int64_t v_row, int64_t v_head,
+                      const int32_t *page_table, int slots, int pages, int kv_heads, int page_size, int head_dim, void *keys,
+                      void *values, float *scales, void *hip_stream);
+
+/*
+ * out[b, i, h] = attention of q[b, i, h] ([sequences, queries, heads, head_dim]) over positions 0 .. lengths[b] - queries + i of row b: the
+ * queries are the row's newest tokens, whose keys and values are in the cache already.  A query without any position is zeros.
+ * workspace: sspmm_cache_attention_workspace_bytes of the same sizes, 16-byte aligned (may be 0 bytes).
+ */
+size_t sspmm_cache_attention_workspace_bytes(int sequences, int queries, int heads, int kv_heads, int head_dim, int slots, int page_size);
+int sspmm_cache_attention(int type, int format, int sequences, int queries, int heads, const sspmm_half_t *q, int64_t q_seq,
+                          int64_t q_row, int64_t q_head, const int32_t *page_table, int slots, const int32_t *lengths, int pages,
+                          int kv_heads, int page_size, int head_dim, const void *keys, const void *values, const float *scales,
+                          float scale, sspmm_half_t *out, int64_t out_seq, int64_t out_row, int64_t out_head, void *workspace,
+                          size_t workspace_bytes, void *hip_stream);
+
+/*
+ * Pages.  page_refs[pages]: how many table entries name a page; it is free where that is not positive.  Free pages are taken lowest
+ * first, in the order of rows and slots or of children.
+ *   reserve   gives a page to every slot that holds positions starts[b] .. of row b's new tokens (offsets as above, one row of the table a
+ *             sequence) and has none; when no page is free the rest go without
+ *   release   the pages that the named rows hold lose a reference each, the rows' entries become -1, their lengths 0
+ *   fork      row children[i], which holds no pages, becomes a copy of row parents[i]: full pages are shared, a last page that is not full is
+ *             copied to a free one.  A child that finds none, or whose parent is no row or itself a child in the call, is left empty with
+ *             length 0.  A row named several times as a child becomes its last naming.
+ *   compact   with n pages in use, the contents of those at n and behind go to the free ones below n, and the table and counts with them
+ * Indices outside the table are passed over.  workspace: sspmm_page_workspace_bytes(pages, rows, slots, count of rows named), 16-byte aligned.
+ */
+size_t sspmm_page_workspace_bytes(int pages, int rows, int slots, int count);
+int sspmm_reserve_pages(int32_t *page_refs, int pages, int32_t *page_table, int rows, int slots, const int32_t *starts,
+                        const int32_t *offsets, int page_size, void *workspace, size_t workspace_bytes, void *hip_stream);
+int sspmm_release_pages(int32_t *page_refs, int pages, int32_t *page_table, int rows, int slots, int32_t *lengths, const int32_t *named,
+                        int count, void *hip_stream);
+int sspmm_fork_pages(int32_t *page_refs, int pages, int32_t *page_table, int rows, int slots, int32_t *lengths, const int32_t *parents,
+                     const int32_t *children, int count, int kv_heads, int page_size, int head_dim, void *keys, void *values,
+                     float *scales, void *workspace, size_t workspace_bytes, void *hip_stream);
+int sspmm_compact_pages(int32_t *page_refs, int pages, int32_t *page_table, int rows, int slots, int kv_heads, int page_size, int head_dim,
+                        void *keys, void *values, float *scales, void *workspace, size_t workspace_bytes, void *hip_stream);
+
+/* ------------------------------------------------------------------------------------------
  * Coordinate list -> CSR, the step between a Matrix Market file and the RowMerge in the
  * reference's SuiteSparse path: `csr = self.coo.tocsr()` in suite_matrix.coo2csr, reference
  * RowMerge/suit_sparse_matrix.py:109-111 (scipy: rows ascending, inside a row the columns

@@ -68,6 +68,16 @@ SIGNATURES = {
     "sspmm_linear_f16": (_int, [_int, _int, _int, _int, _vp, _vp, _vp, _vp, _vp, _int, _vp, _vp]),
     "sspmm_attention_fm_f16": (_int, [_int, _int, _int, _int, _vp, _vp, _vp, ctypes.c_int64, _vp, ctypes.c_int64, ctypes.c_float, _vp]),
     "sspmm_attention_fm_ragged_f16": (_int, [_int, _int, _int, _int, _vp, _vp, _vp, ctypes.c_int64, _vp, ctypes.c_int64, ctypes.c_float, _vp]),
+    "sspmm_prompt_attention": (_int, [_int] * 6 + [_vp] + [_vp, _i64, _i64] * 3 + [_int, ctypes.c_float, _vp, _i64, _i64, _vp]),
+    "sspmm_cache_write": (_int, [_int] * 4 + [_vp, _vp] + [_vp, _i64, _i64] * 2 + [_vp] + [_int] * 5 + [_vp] * 4),
+    "sspmm_cache_attention_workspace_bytes": (ctypes.c_size_t, [_int] * 7),
+    "sspmm_cache_attention": (_int, [_int] * 5 + [_vp, _i64, _i64, _i64, _vp, _int, _vp] + [_int] * 4 + [_vp] * 3 + [ctypes.c_float, _vp, _i64, _i64, _i64,
+                                                                                                               _vp, ctypes.c_size_t, _vp]),
+    "sspmm_page_workspace_bytes": (ctypes.c_size_t, [_int] * 4),
+    "sspmm_reserve_pages": (_int, [_vp, _int, _vp, _int, _int, _vp, _vp, _int, _vp, ctypes.c_size_t, _vp]),
+    "sspmm_release_pages": (_int, [_vp, _int, _vp, _int, _int, _vp, _vp, _int, _vp]),
+    "sspmm_fork_pages": (_int, [_vp, _int, _vp, _int, _int, _vp, _vp, _vp] + [_int] * 4 + [_vp] * 4 + [ctypes.c_size_t, _vp]),
+    "sspmm_compact_pages": (_int, [_vp, _int, _vp, _int, _int] + [_int] * 3 + [_vp] * 4 + [ctypes.c_size_t, _vp]),
     "svc_coo_workspace_bytes": (ctypes.c_size_t, [_i64]),
     "svc_coo_to_csr": (_int, [_int, _int, _i64, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
     "svc_reorder_workspace_bytes": (ctypes.c_size_t, [_int]),

@@ -1,0 +1,369 @@
+// Attention of the newest tokens of every sequence over its paged cache in 8 bits:
+//   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^((q . k_j) scale log2(e) - m),  k_j and v_j codes times their block's scale.
+// Bound by the cache's bytes, each read once: a wave's loads go from memory to the registers that the products read.
+#include "cache_kernels.h"
+
+#include "lane_ops.h"
+#include "sixteen_bit.h"
+
+namespace sspmm {
+
+namespace {
+
+constexpr int kWaves = 4;
+
+typedef Fp16::vec8 half8;
+
+__device__ __forceinline__ floatx4 mfma(uintx4 a, uintx4 b, floatx4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+}
+
+// Eight codes as fp16, which holds either format's values exactly.
+template <int FORMAT>
+__device__ __forceinline__ uintx4 as_halfs(uint32_t lo, uint32_t hi) {
+  uintx4 r;
+  const uint32_t w[2] = {lo, hi};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if constexpr (FORMAT == 0) {
+      // 0x6400 + u is 1024 + u in fp16, u = code + 128
+      const uint32_t u = w[i] ^ 0x80808080u;
+      const Fp16::vec2 off = {(_Float16)1152, (_Float16)1152};
+      r[2 * i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(Fp16::vec2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - off);
+      r[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(Fp16::vec2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - off);
+    } else {
+      r[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i], 1.0f, false));
+      r[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i], 1.0f, true));
+    }
+  }
+  return r;
+}
+
+__device__ __forceinline__ long long partial_floats(int rows, int d) { return (long long)rows * (d + 2); }
+
+// A workgroup owns 16 * TILES rows (queries x heads of one head of the cache; row i * group + j is query i, head j of the group) of one
+// sequence and one of its `splits` shares of the keys, a wave a quarter of those, UNIT keys at a time, all of them in one page.  Scores are
+// made transposed, K Q^T: the lane of row m and group g holds keys UNIT / 4 * g .. of the unit, which is the operand of the second product
+// V^T P^T as it is, and the order in which values lie in a page.
+template <typename T, int FORMAT, int D, int TILES, int UNIT>
+__global__ __launch_bounds__(64 * kWaves, 2) void cache_attention_kernel(const CacheAttentionArgs p) {
+  constexpr int kKeyTiles = UNIT / 16, kParts = D / 16, kSteps = D / 32, kShares = UNIT / 32, kRows = 16 * TILES;
+  constexpr int kKeyWords = D >= 64 ? 4 : 2;  // of a load of K: 16 bytes, or 8 where a group's share of a row is no more
+  constexpr int kKeyLoads = D / (16 * kKeyWords);  // of a row by a lane
+  constexpr int kValueWords = UNIT / 16;
+  typedef uint32_t KeyWords __attribute__((ext_vector_type(kKeyWords)));
+  typedef uint32_t ValueWords __attribute__((ext_vector_type(kValueWords)));
+  __shared__ float state[kWaves][2][kRows];
+  __shared__ __align__(16) float sums[kWaves][kRows][D];
+  const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const CachePool pool = p.pool;
+  const int group = p.heads / pool.kv_heads, rows = p.queries * group, tiles = (rows + kRows - 1) / kRows;
+  const int split = blockIdx.x, head = blockIdx.y % pool.kv_heads, tile = blockIdx.y / pool.kv_heads, seq = blockIdx.z;
+  const int length = max(0, (int)min((long long)p.lengths[seq], (long long)pool.slots * pool.page_size));
+  const int units = (length + UNIT - 1) / UNIT, pieces = p.splits * kWaves, piece = split * kWaves + wave;
+  const int unit0 = (int)((long long)units * piece / pieces), unit1 = (int)((long long)units * (piece + 1) / pieces);
+
+  // ---- queries.  bf16 goes to fp16 by way of a power of two for the row, which leaves its largest magnitude in 2^14 .. 2^15
+  uintx4 q[TILES][kSteps];
+  float c[TILES];
+  int seen[TILES];  // keys that the row sees: those below
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) {
+    const int row = tile * kRows + 16 * t + m, r = row < rows ? row : 0, i = r / group;
+    seen[t] = length - p.queries + 1 + i;
+    const uint16_t *const at = p.q + (long long)seq * p.q_seq + (long long)i * p.q_row + (long long)(head * group + r % group) * p.q_head;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int d = D >= 64 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 8 * g;
+      q[t][s] = *reinterpret_cast<const uintx4 *>(at + d);
+    }
+    c[t] = p.scale_log2e;
+    if constexpr (!__is_same(T, Fp16)) {
+      float most = 0.f;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) most = fmaxf(most, fmaxf(fabsf(T::lower(q[t][s][j])), fabsf(T::upper(q[t][s][j]))));
+      most = max_over_rows(most);
+      const int e = max((int)(__float_as_uint(most) >> 23) - 127 - 14, -126);
+      const bool usual = most < INFINITY;  // (else as they are)
+      const float up = usual ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.f;
+      c[t] *= usual ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.f;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q[t][s][j] = Fp16::pack(T::lower(q[t][s][j]) * up, T::upper(q[t][s][j]) * up);
+    }
+  }
+
+  floatx4 o[TILES][kParts];  // features 16 part + 4 g + i of row m
+  float run_max[TILES], run_sum[TILES];
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) {
+    run_max[t] = -3.0e38f;
+    run_sum[t] = 0.f;
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) o[t][part] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  const int32_t *const table = p.pool.table + (long long)seq * pool.slots;
+  const long long block = (long long)pool.page_size * D;
+  KeyWords kk[kKeyTiles][kKeyLoads];
+  ValueWords vv[kParts];
+  int page = 0, page_next = 0;
+  const int page_units = pool.page_size / UNIT, page_bits = 31 - __builtin_clz(page_units);  // (1 or 2)
+  const auto page_of = [&](int u) { return __builtin_amdgcn_readfirstlane(table[u >> page_bits]); };
+  const auto place_of = [&](int u) { return (u & (page_units - 1)) * UNIT; };  // in its page
+  const auto usable = [&](int pg) { return pg >= 0 && pg < pool.pages; };
+  const auto load_k = [&](int u, int pg) {
+    const unsigned char *const at = pool.keys + ((long long)(usable(pg) ? pg : 0) * pool.kv_heads + head) * block + place_of(u) * D;
+#pragma unroll
+    for (int kt = 0; kt < kKeyTiles; ++kt) {
+      const unsigned char *const row = at + (UNIT / 4 * (m >> 2) + 4 * kt + (m & 3)) * D + 4 * kKeyWords * g;
+#pragma unroll
+      for (int i = 0; i < kKeyLoads; ++i) {
+        kk[kt][i] = *reinterpret_cast<const KeyWords *>(row + 64 * i);
+      }
+    }
+  };
+  const auto load_v = [&](int u, int pg) {
+    const unsigned char *const at = pool.values + ((long long)(usable(pg) ? pg : 0) * pool.kv_heads + head) * block + place_of(u) + UNIT / 4 * g;
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) {
+      const unsigned char *const row = at + (16 * part + m) * pool.page_size;
+      vv[part] = *reinterpret_cast<const ValueWords *>(row);
+    }
+  };
+
+  if (unit0 < unit1) {
+    page = page_of(unit0);
+    load_k(unit0, page);
+    load_v(unit0, page);
+    page_next = unit0 + 1 < unit1 ? page_of(unit0 + 1) : page;
+  }
+  for (int u = unit0; u < unit1; ++u) {
+    const bool more = u + 1 < unit1, there = usable(page);
+    const float *const scale = pool.scales + (long long)(there ? page : 0) * 2 * pool.kv_heads + head;
+    const float k_scale = scale[0], v_scale = scale[pool.kv_heads];
+    const int after = u + 2 < unit1 ? page_of(u + 2) : page_next;
+    floatx4 s[TILES][kKeyTiles];
+#pragma unroll
+    for (int kt = 0; kt < kKeyTiles; ++kt) {
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) s[t][kt] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int step = 0; step < kSteps; ++step) {
+        const int i = D >= 64 ? step / 2 : 0, w = D >= 64 ? 2 * (step % 2) : 0;
+        const uintx4 k = as_halfs<FORMAT>(kk[kt][i][w], kk[kt][i][w + 1]);
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) s[t][kt] = mfma(k, q[t][step], s[t][kt]);
+      }
+    }
+    if (more) load_k(u + 1, page_next);
+    const int key0 = u * UNIT, key = key0 + UNIT / 4 * g;
+    const bool cut = !there || key0 + UNIT > length - p.queries + 1;  // uniform: some row does not see some key
+    uintx4 pt[TILES][kShares];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+      const float f = k_scale * c[t];
+      float most = -INFINITY;
+#pragma unroll
+      for (int kt = 0; kt < kKeyTiles; ++kt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[t][kt][i] *= f;
+          if (cut && (!there || key + 4 * kt + i >= seen[t])) s[t][kt][i] = -INFINITY;
+          most = fmaxf(most, s[t][kt][i]);
+        }
+      most = max_over_rows(most);
+      // the reference point moves only when a row's maximum has grown by more than 2^8, which fp16 holds
+      const float new_max = fmaxf(run_max[t], most);
+      if (__ballot(new_max - run_max[t] > 8.0f) != 0) {
+        const float alpha = __builtin_amdgcn_exp2f(fmaxf(run_max[t] - new_max, -126.0f));
+        run_max[t] = new_max;
+        run_sum[t] *= alpha;
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) o[t][part] *= alpha;
+      }
+#pragma unroll
+      for (int kt = 0; kt < kKeyTiles; ++kt)
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          const float a = __builtin_amdgcn_exp2f(s[t][kt][i] - run_max[t]), b = __builtin_amdgcn_exp2f(s[t][kt][i + 1] - run_max[t]);
+          run_sum[t] += a + b;
+          pt[t][kt / 2][2 * (kt % 2) + i / 2] = Fp16::pack(a, b);
+        }
+    }
+    // (Nothing: but the compiler of ROCm 7.2 loses half of such a pair of words between here and there, and reuses its register, unless both are
+    // wanted at one place.  -verify-machineinstrs finds it; the build asks for that.)
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) asm volatile("" : "+v"(vv[part]));
+    if (FORMAT == 1 && key0 + UNIT > length) {  // (what lies behind the sequence may be NaN)
+#pragma unroll
+      for (int w = 0; w < kValueWords; ++w) {
+        const int left = max(0, min(4, length - key - 4 * w));
+        const uint32_t mask = left == 4 ? 0xffffffffu : (1u << (8 * left)) - 1u;
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) vv[part][w] &= mask;
+      }
+    }
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) {
+      floatx4 sum[TILES];
+#pragma unroll
+      for (int w = 0; w < kShares; ++w) {
+        const uintx4 v = as_halfs<FORMAT>(vv[part][2 * w], vv[part][2 * w + 1]);
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) sum[t] = mfma(v, pt[t][w], w == 0 ? floatx4{0.f, 0.f, 0.f, 0.f} : sum[t]);
+      }
+#pragma unroll
+      for (int t = 0; t < TILES; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          // (a row that sees nothing of the page does not see that its scale is NaN either)
+          const float x = fmaf(sum[t][i], v_scale, o[t][part][i]);
+          o[t][part][i] = cut && (!there || key0 >= seen[t]) ? o[t][part][i] : x;
+        }
+    }
+    if (more) load_v(u + 1, page_next);
+    page = page_next;
+    page_next = after;
+  }
+
+  // ---- the waves' states as one
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) {
+    run_sum[t] = sum_over_rows(run_sum[t]);
+    if (g == 0) {
+      state[wave][0][16 * t + m] = run_max[t];
+      state[wave][1][16 * t + m] = run_sum[t];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) {
+    float most = state[0][0][16 * t + m];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) most = fmaxf(most, state[w][0][16 * t + m]);
+    const float weight = __builtin_amdgcn_exp2f(fmaxf(run_max[t] - most, -126.0f));
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) *reinterpret_cast<floatx4 *>(&sums[wave][16 * t + m][16 * part + 4 * g]) = o[t][part] * weight;
+  }
+  __syncthreads();
+  const int r0 = tile * kRows;
+  float *const partial =
+      p.splits > 1 ? p.partial + ((((long long)seq * pool.kv_heads + head) * tiles + tile) * p.splits + split) * partial_floats(kRows, D) : nullptr;
+  for (int at = threadIdx.x; at < kRows * D / 4; at += 64 * kWaves) {
+    const int r = at / (D / 4), d = (at % (D / 4)) * 4, row = r0 + r;
+    if (row >= rows) continue;
+    float most = state[0][0][r], total = 0.f;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) most = fmaxf(most, state[w][0][r]);
+    floatx4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      x += *reinterpret_cast<const floatx4 *>(&sums[w][r][d]);
+      total += state[w][1][r] * __builtin_amdgcn_exp2f(fmaxf(state[w][0][r] - most, -126.0f));
+    }
+    if (partial) {
+      *reinterpret_cast<floatx4 *>(partial + (long long)r * D + d) = x;
+      if (d == 0) {
+        partial[(long long)kRows * D + r] = most;
+        partial[(long long)kRows * D + kRows + r] = total;
+      }
+    } else {
+      const float inv = total > 0.f || total != total ? 1.0f / total : 0.f;
+      const int i = row / group, h = head * group + row % group;
+      uint16_t *const to = p.out + (long long)seq * p.out_seq + (long long)i * p.out_row + (long long)h * p.out_head + d;
+      *reinterpret_cast<uintx2 *>(to) = uintx2{T::pack(x[0] * inv, x[1] * inv), T::pack(x[2] * inv, x[3] * inv)};
+    }
+  }
+}
+
+// The splits' states of one row as one: D / 4 threads for the features, 1024 / D sets of them that take every so manyth split.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void cache_attention_join_kernel(const CacheAttentionArgs p, int row_tiles) {
+  constexpr int kSets = 1024 / D;
+  __shared__ float weight_sum[kSets];
+  __shared__ __align__(16) float part[kSets][D];
+  __shared__ float largest[4];
+  const int kRows = 16 * row_tiles, group = p.heads / p.pool.kv_heads, rows = p.queries * group, tiles = (rows + kRows - 1) / kRows;
+  const int row = blockIdx.x, head = blockIdx.y, seq = blockIdx.z, tile = row / kRows, r = row % kRows;
+  const long long pitch = partial_floats(kRows, D);
+  const float *const base = p.partial + (((long long)seq * p.pool.kv_heads + head) * tiles + tile) * p.splits * pitch;
+  const float *const maxima = base + (long long)kRows * D + r, *const totals = maxima + kRows;
+  const int set = threadIdx.x / (D / 4), d = (threadIdx.x % (D / 4)) * 4;
+  float most = -3.0e38f;
+  for (int s = threadIdx.x; s < p.splits; s += 256) most = fmaxf(most, maxima[s * pitch]);
+  most = wave_max_all(most);
+  if ((threadIdx.x & 63) == 0) largest[threadIdx.x >> 6] = most;
+  __syncthreads();
+  most = fmaxf(fmaxf(largest[0], largest[1]), fmaxf(largest[2], largest[3]));
+  floatx4 x = {0.f, 0.f, 0.f, 0.f};
+  float total = 0.f;
+  for (int s = set; s < p.splits; s += kSets) {
+    const float w = __builtin_amdgcn_exp2f(fmaxf(maxima[s * pitch] - most, -126.0f));
+    total += totals[s * pitch] * w;
+    x += *reinterpret_cast<const floatx4 *>(base + s * pitch + (long long)r * D + d) * w;
+  }
+  *reinterpret_cast<floatx4 *>(&part[set][d]) = x;
+  if (d == 0) weight_sum[set] = total;
+  __syncthreads();
+  if (set != 0) return;
+  for (int i = 1; i < kSets; ++i) {
+    x += *reinterpret_cast<const floatx4 *>(&part[i][d]);
+    total += weight_sum[i];
+  }
+  // (total of set 0 is in its first thread's registers only as its own share: all of them hold the same)
+  const float inv = total > 0.f || total != total ? 1.0f / total : 0.f;
+  const int i = row / group, h = head * group + row % group;
+  uint16_t *const to = p.out + (long long)seq * p.out_seq + (long long)i * p.out_row + (long long)h * p.out_head + d;
+  *reinterpret_cast<uintx2 *>(to) = uintx2{T::pack(x[0] * inv, x[1] * inv), T::pack(x[2] * inv, x[3] * inv)};
+}
+
+int row_tiles(int queries, int group) { return queries * group > 16 ? 2 : 1; }
+
+template <typename T, int FORMAT, int D>
+hipError_t launch(const CacheAttentionArgs &a, hipStream_t stream) {
+  const int group = a.heads / a.pool.kv_heads, rows = a.queries * group, two = row_tiles(a.queries, group);
+  const int tiles = (rows + 16 * two - 1) / (16 * two);
+  const dim3 grid(a.splits, a.pool.kv_heads * tiles, a.sequences), threads(64 * kWaves);
+  if (a.pool.page_size == 32) {
+    if (two == 1) hipLaunchKernelGGL((cache_attention_kernel<T, FORMAT, D, 1, 32>), grid, threads, 0, stream, a);
+    else hipLaunchKernelGGL((cache_attention_kernel<T, FORMAT, D, 2, 32>), grid, threads, 0, stream, a);
+  } else {
+    if (two == 1) hipLaunchKernelGGL((cache_attention_kernel<T, FORMAT, D, 1, 64>), grid, threads, 0, stream, a);
+    else hipLaunchKernelGGL((cache_attention_kernel<T, FORMAT, D, 2, 64>), grid, threads, 0, stream, a);
+  }
+  if (a.splits > 1)
+    hipLaunchKernelGGL((cache_attention_join_kernel<T, D>), dim3(rows, a.pool.kv_heads, a.sequences), dim3(256), 0, stream, a, two);
+  return hipGetLastError();
+}
+
+template <typename T, int FORMAT>
+hipError_t launch(const CacheAttentionArgs &a, hipStream_t stream) {
+  return a.pool.d == 128 ? launch<T, FORMAT, 128>(a, stream) : a.pool.d == 64 ? launch<T, FORMAT, 64>(a, stream) : launch<T, FORMAT, 32>(a, stream);
+}
+
+}  // namespace
+
+int cache_attention_splits(int sequences, int queries, int heads, int kv_heads, int d, long long longest) {
+  const int group = heads / kv_heads, rows = queries * group, two = row_tiles(queries, group), tiles = (rows + 16 * two - 1) / (16 * two);
+  const long long wide = (long long)sequences * kv_heads * tiles;
+  const long long wanted = (1024 + wide - 1) / wide, most = (longest + 255) / 256;
+  return (int)max(1ll, min(min(wanted, most), 256ll));
+}
+
+size_t cache_attention_workspace(int sequences, int queries, int heads, int kv_heads, int d, int splits) {
+  if (splits <= 1) return 0;
+  const int group = heads / kv_heads, rows = queries * group, two = row_tiles(queries, group), tiles = (rows + 16 * two - 1) / (16 * two);
+  return (size_t)sequences * kv_heads * tiles * splits * (size_t)(16 * two) * (d + 2);
+}
+
+hipError_t launch_cache_attention(int type, int format, const CacheAttentionArgs &a, hipStream_t stream) {
+  if (type == 0) return format == 0 ? launch<Fp16, 0>(a, stream) : launch<Fp16, 1>(a, stream);
+  return format == 0 ? launch<Bf16, 0>(a, stream) : launch<Bf16, 1>(a, stream);
+}
+
+}  // namespace sspmm

@@ -5,9 +5,12 @@
 #include "../../include/sspmm.h"
 #include "attention_kernels.h"
 #include "block_kernels.h"
+#include "cache_kernels.h"
+#include "cache_pages.h"
 #include "coo_kernels.h"
 #include "layer_kernels.h"
 #include "plan.h"
+#include "prompt_kernels.h"
 #include "reorder_kernels.h"
 #include "spmm_kernels.h"
 #include "svc_kernels.h"
@@ -60,6 +63,23 @@ int plan_entry(const sspmm_plan_t *plan, int batch, int N, const int32_t *row_of
   if (hipGetDevice(&dev) != hipSuccess || dev != pl->device) return kInvalid;  // the plan's memory lives on its device
   return spmm_entry(batch, pl->m_vec, pl->V, N, pl->K, nullptr, row_offsets, col_idx, values, stride_values, B, stride_B,
                     C, stride_C, out_f16, stream, pl);
+}
+
+// What the serving entry points ask of heads, scales and strided activations.
+bool heads_fit(int heads, int kv_heads, int head_dim) {
+  return kv_heads >= 1 && heads >= 1 && heads % kv_heads == 0 && heads <= 65535 && (head_dim == 32 || head_dim == 64 || head_dim == 128);
+}
+bool scale_fits(float scale) { return scale > 0.f && std::isfinite(scale * 1.4426950408889634f); }
+bool operand_fits(const void *p, int64_t row, int64_t head, int head_dim) {
+  return p && reinterpret_cast<uintptr_t>(p) % 16 == 0 && row % 8 == 0 && head % 8 == 0 && row >= head_dim && head >= 0 && row < (1ll << 23);
+}
+bool pool_fits(int pages, int kv_heads, int page_size, int head_dim, const void *keys, const void *values, const void *scales) {
+  return pages >= 1 && pages <= (1 << 30) && kv_heads >= 1 && kv_heads <= 65535 && (page_size == 32 || page_size == 64 || page_size == 128) &&
+         (head_dim == 32 || head_dim == 64 || head_dim == 128) && keys && values && scales && reinterpret_cast<uintptr_t>(keys) % 16 == 0 &&
+         reinterpret_cast<uintptr_t>(values) % 16 == 0 && reinterpret_cast<uintptr_t>(scales) % 4 == 0;
+}
+bool table_fits(const void *refs, int pages, const void *table, int rows, int slots) {
+  return refs && table && pages >= 1 && pages <= (1 << 30) && rows >= 1 && slots >= 1 && (int64_t)rows * slots < (1ll << 31);
 }
 
 }  // namespace
@@ -769,6 +789,151 @@ int sspmm_attention_fm_ragged_f16(int batch, int heads, int seq, int head_dim, c
   if (!q || !k || !v || !out || ld < (int64_t)batch * seq || ld_out < (int64_t)batch * seq) return kInvalid;
   if (!sspmm::attention_fm_ragged_applies(batch, heads, seq, head_dim, q, k, v, out)) return kInvalid;
   return (int)sspmm::launch_attention_fm(batch, heads, seq, q, k, v, ld, out, ld_out, scale, static_cast<hipStream_t>(hip_stream));
+}
+
+int sspmm_prompt_attention(int type, int sequences, int tokens, int heads, int kv_heads, int head_dim, const int32_t *offsets,
+                           const sspmm_half_t *q, int64_t q_row, int64_t q_head, const sspmm_half_t *k, int64_t k_row, int64_t k_head,
+                           const sspmm_half_t *v, int64_t v_row, int64_t v_head, int causal, float scale, sspmm_half_t *out,
+                           int64_t out_row, int64_t out_head, void *hip_stream) {
+  if (type != SSPMM_TYPE_F16 && type != SSPMM_TYPE_BF16) return kInvalid;
+  if (sequences < 0 || tokens < 0 || !heads_fit(heads, kv_heads, head_dim) || !scale_fits(scale)) return kInvalid;
+  if (sequences == 0 || tokens == 0) return 0;
+  if (!offsets || !operand_fits(q, q_row, q_head, head_dim) || !operand_fits(k, k_row, k_head, head_dim) ||
+      !operand_fits(v, v_row, v_head, head_dim) || !operand_fits(out, out_row, out_head, head_dim))
+    return kInvalid;
+  if (tokens > (1 << 30)) return kInvalid;
+  sspmm::PromptArgs a{};
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.out = out;
+  a.offsets = offsets;
+  a.q_row = q_row;
+  a.q_head = q_head;
+  a.k_row = k_row;
+  a.k_head = k_head;
+  a.v_row = v_row;
+  a.v_head = v_head;
+  a.out_row = out_row;
+  a.out_head = out_head;
+  a.sequences = sequences;
+  a.tokens = tokens;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.scale_log2e = scale * 1.4426950408889634f;
+  return (int)sspmm::launch_prompt_attention(type, head_dim, causal != 0, a, static_cast<hipStream_t>(hip_stream));
+}
+
+int sspmm_cache_write(int type, int format, int sequences, int tokens, const int32_t *offsets, const int32_t *starts,
+                      const sspmm_half_t *k, int64_t k_row, int64_t k_head, const sspmm_half_t *v, int64_t v_row, int64_t v_head,
+                      const int32_t *page_table, int slots, int pages, int kv_heads, int page_size, int head_dim, void *keys,
+                      void *values, float *scales, void *hip_stream) {
+  if ((type != SSPMM_TYPE_F16 && type != SSPMM_TYPE_BF16) || (format != SSPMM_CACHE_INT8 && format != SSPMM_CACHE_E4M3)) return kInvalid;
+  if (sequences < 0 || tokens < 0 || slots < 0) return kInvalid;
+  if (sequences == 0 || tokens == 0 || slots == 0) return 0;
+  if (tokens > (1 << 30) || !offsets || !starts || !page_table || !pool_fits(pages, kv_heads, page_size, head_dim, keys, values, scales)) return kInvalid;
+  if (!operand_fits(k, k_row, k_head, head_dim) || !operand_fits(v, v_row, v_head, head_dim)) return kInvalid;
+  sspmm::CacheWriteArgs a{};
+  a.pool = {static_cast<unsigned char *>(keys), static_cast<unsigned char *>(values), scales, page_table, pages, kv_heads, page_size, head_dim, slots};
+  a.k = k;
+  a.v = v;
+  a.k_row = k_row;
+  a.k_head = k_head;
+  a.v_row = v_row;
+  a.v_head = v_head;
+  a.offsets = offsets;
+  a.starts = starts;
+  a.sequences = sequences;
+  a.tokens = tokens;
+  return (int)sspmm::launch_cache_write(type, format, a, static_cast<hipStream_t>(hip_stream));
+}
+
+size_t sspmm_cache_attention_workspace_bytes(int sequences, int queries, int heads, int kv_heads, int head_dim, int slots, int page_size) {
+  if (sequences <= 0 || queries <= 0 || slots < 0 || page_size <= 0 || !heads_fit(heads, kv_heads, head_dim)) return 0;
+  const int splits = sspmm::cache_attention_splits(sequences, queries, heads, kv_heads, head_dim, (long long)slots * page_size);
+  return 4 * sspmm::cache_attention_workspace(sequences, queries, heads, kv_heads, head_dim, splits);
+}
+
+int sspmm_cache_attention(int type, int format, int sequences, int queries, int heads, const sspmm_half_t *q, int64_t q_seq,
+                          int64_t q_row, int64_t q_head, const int32_t *page_table, int slots, const int32_t *lengths, int pages,
+                          int kv_heads, int page_size, int head_dim, const void *keys, const void *values, const float *scales,
+                          float scale, sspmm_half_t *out, int64_t out_seq, int64_t out_row, int64_t out_head, void *workspace,
+                          size_t workspace_bytes, void *hip_stream) {
+  if ((type != SSPMM_TYPE_F16 && type != SSPMM_TYPE_BF16) || (format != SSPMM_CACHE_INT8 && format != SSPMM_CACHE_E4M3)) return kInvalid;
+  if (sequences < 0 || queries < 0 || slots < 1 || !heads_fit(heads, kv_heads, head_dim) || !scale_fits(scale)) return kInvalid;
+  if (sequences == 0 || queries == 0) return 0;
+  if (sequences > 65535 || (int64_t)queries * heads > (1 << 20) || (int64_t)slots * page_size > (1ll << 31) - 256) return kInvalid;
+  if (!page_table || !lengths || !pool_fits(pages, kv_heads, page_size, head_dim, keys, values, scales)) return kInvalid;
+  if (!operand_fits(q, q_row, q_head, head_dim) || !operand_fits(out, out_row, out_head, head_dim) || q_seq % 8 || q_seq < 0 || out_seq % 8 || out_seq < 0)
+    return kInvalid;
+  sspmm::CacheAttentionArgs a{};
+  a.pool = {static_cast<unsigned char *>(const_cast<void *>(keys)), static_cast<unsigned char *>(const_cast<void *>(values)), const_cast<float *>(scales),
+            page_table, pages, kv_heads, page_size, head_dim, slots};
+  a.q = q;
+  a.out = out;
+  a.q_seq = q_seq;
+  a.q_row = q_row;
+  a.q_head = q_head;
+  a.out_seq = out_seq;
+  a.out_row = out_row;
+  a.out_head = out_head;
+  a.lengths = lengths;
+  a.sequences = sequences;
+  a.queries = queries;
+  a.heads = heads;
+  a.splits = sspmm::cache_attention_splits(sequences, queries, heads, kv_heads, head_dim, (long long)slots * page_size);
+  a.scale_log2e = scale * 1.4426950408889634f;
+  a.partial = static_cast<float *>(workspace);
+  const size_t need = 4 * sspmm::cache_attention_workspace(sequences, queries, heads, kv_heads, head_dim, a.splits);
+  if (workspace_bytes < need || (need > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16))) return kInvalid;
+  return (int)sspmm::launch_cache_attention(type, format, a, static_cast<hipStream_t>(hip_stream));
+}
+
+size_t sspmm_page_workspace_bytes(int pages, int rows, int slots, int count) {
+  if (pages < 1 || rows < 1 || slots < 1 || count < 0) return 0;
+  return 4 * sspmm::page_workspace_ints(pages, rows, slots, count);
+}
+
+int sspmm_reserve_pages(int32_t *page_refs, int pages, int32_t *page_table, int rows, int slots, const int32_t *starts,
+                        const int32_t *offsets, int page_size, void *workspace, size_t workspace_bytes, void *hip_stream) {
+  if (rows == 0 || slots == 0) return 0;
+  if (!table_fits(page_refs, pages, page_table, rows, slots) || !starts || !offsets || page_size < 1) return kInvalid;
+  if (!workspace || workspace_bytes < sspmm_page_workspace_bytes(pages, rows, slots, 0)) return kInvalid;
+  return (int)sspmm::launch_reserve_pages({page_refs, page_table, pages, rows, slots}, starts, offsets, page_size, static_cast<int32_t *>(workspace),
+                                          static_cast<hipStream_t>(hip_stream));
+}
+
+int sspmm_release_pages(int32_t *page_refs, int pages, int32_t *page_table, int rows, int slots, int32_t *lengths, const int32_t *named,
+                        int count, void *hip_stream) {
+  if (count < 0) return kInvalid;
+  if (count == 0 || rows == 0 || slots == 0) return 0;
+  if (!table_fits(page_refs, pages, page_table, rows, slots) || !lengths || !named) return kInvalid;
+  return (int)sspmm::launch_release_pages({page_refs, page_table, pages, rows, slots}, lengths, named, count, static_cast<hipStream_t>(hip_stream));
+}
+
+int sspmm_fork_pages(int32_t *page_refs, int pages, int32_t *page_table, int rows, int slots, int32_t *lengths, const int32_t *parents,
+                     const int32_t *children, int count, int kv_heads, int page_size, int head_dim, void *keys, void *values,
+                     float *scales, void *workspace, size_t workspace_bytes, void *hip_stream) {
+  if (count < 0) return kInvalid;
+  if (count == 0 || rows == 0 || slots == 0) return 0;
+  if (!table_fits(page_refs, pages, page_table, rows, slots) || !lengths || !parents || !children) return kInvalid;
+  if (!pool_fits(pages, kv_heads, page_size, head_dim, keys, values, scales)) return kInvalid;
+  if (!workspace || workspace_bytes < sspmm_page_workspace_bytes(pages, rows, slots, count)) return kInvalid;
+  const sspmm::PagePool pool = {static_cast<unsigned char *>(keys), static_cast<unsigned char *>(values), scales, (long long)kv_heads * page_size * head_dim,
+                                2 * kv_heads};
+  return (int)sspmm::launch_fork_pages({page_refs, page_table, pages, rows, slots}, pool, lengths, parents, children, count, page_size,
+                                       static_cast<int32_t *>(workspace), static_cast<hipStream_t>(hip_stream));
+}
+
+int sspmm_compact_pages(int32_t *page_refs, int pages, int32_t *page_table, int rows, int slots, int kv_heads, int page_size, int head_dim,
+                        void *keys, void *values, float *scales, void *workspace, size_t workspace_bytes, void *hip_stream) {
+  if (rows == 0 || slots == 0) return 0;
+  if (!table_fits(page_refs, pages, page_table, rows, slots)) return kInvalid;
+  if (!pool_fits(pages, kv_heads, page_size, head_dim, keys, values, scales)) return kInvalid;
+  if (!workspace || workspace_bytes < sspmm_page_workspace_bytes(pages, rows, slots, 0)) return kInvalid;
+  const sspmm::PagePool pool = {static_cast<unsigned char *>(keys), static_cast<unsigned char *>(values), scales, (long long)kv_heads * page_size * head_dim,
+                                2 * kv_heads};
+  return (int)sspmm::launch_compact_pages({page_refs, page_table, pages, rows, slots}, pool, static_cast<int32_t *>(workspace), static_cast<hipStream_t>(hip_stream));
 }
 
 int svc_split_row_ptr(int count, int groups, const int32_t *mat_groups, const int32_t *vec_row_ptr, int32_t *out_ptr, int32_t *bounds,

@@ -1,0 +1,400 @@
+"""The paged cache in 8 bits: writing it, bit for bit, and attention over it against the formula in 64 bits."""
+import math
+
+import pytest
+import torch
+
+import sspmm_amd
+from serving_util import attention, check, check_step, codes_for, offsets_of, row_of_cache, scale_for, write
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float16, torch.bfloat16]
+FORMATS = [torch.int8, torch.float8_e4m3fn]
+
+
+def _randn(shape, seed, scale=1.0):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return torch.randn(shape, generator=g, device="cuda") * scale
+
+
+def _ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _filled(pages, kv, page, d, dtype, seed):
+    """A pool of quantised normal values, blocks of different size."""
+    keys, values, scales = sspmm_amd.new_cache(pages, kv, page, d, dtype)
+    for i, pool in enumerate((keys, values)):
+        x = _randn(pool.shape, seed + i) * torch.exp(_randn((pages, kv, 1, 1), seed + 10 + i))
+        s = scale_for(x.abs().amax((2, 3)), dtype)
+        pool.view(torch.int8).copy_(codes_for(x, s[:, :, None, None], dtype))
+        scales[:, i] = s
+    return keys, values, scales
+
+
+def _table(lengths, page, seed, spare=3):
+    g = torch.Generator()
+    g.manual_seed(seed)
+    held = [-(-n // page) for n in lengths]
+    order = torch.randperm(sum(held) + spare, generator=g)
+    table = torch.full((len(lengths), max(held + [1]) + 1), -1, dtype=torch.int32)
+    at = 0
+    for i, n in enumerate(held):
+        table[i, :n] = order[at:at + n]
+        at += n
+    return table.cuda(), sum(held) + spare
+
+
+# ---- writing
+
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("page,d,kv", [(32, 64, 3), (64, 128, 2), (128, 32, 1), (128, 128, 2), (64, 32, 5)])
+def test_writes_bit_for_bit(built_library, page, d, kv, dtype, form):
+    starts = [0, 5, page - 1, page, 3 * page + 7, 0, 11, 2 * page - 3]
+    counts = [1, 1, 2, page, 2 * page + 9, 3 * page, 0, 3]
+    table, pages = _table([s + n for s, n in zip(starts, counts)], page, seed=page)
+    keys, values, scales = _filled(pages, kv, page, d, form, seed=d)
+    tokens = sum(counts)
+    x = (_randn((tokens, 2, kv, d), 5) * torch.exp(_randn((tokens, 1, kv, 1), 6))).to(dtype)
+    k, v = x.unbind(1)
+    host = [t.cpu().clone() for t in (keys, values, scales)]
+    write(k.cpu(), v.cpu(), offsets_of(counts).cpu(), starts, table.cpu(), *host)
+    print(page, d, kv, dtype, form, flush=True)
+    sspmm_amd.cache_write(k, v, offsets_of(counts), _ints(starts), table, keys, values, scales)
+    for name, got, want in zip(("keys", "values", "scales"), (keys, values, scales), host):
+        same = got.cpu().view(torch.int8 if got.dtype in FORMATS else torch.int32) == want.view(torch.int8 if want.dtype in FORMATS else torch.int32)
+        assert same.all(), "%s: %d of %d differ" % (name, (~same).sum(), same.numel())
+
+
+@pytest.mark.parametrize("form", FORMATS)
+def test_token_by_token_is_as_the_rule_says(built_library, form):
+    """A page filled one token at a time, sizes rising and falling: each growth of the scale brings the codes to it once more."""
+    page, kv, d = 32, 2, 64
+    keys, values, scales = _filled(4, kv, page, d, form, seed=1)
+    host = [t.cpu().clone() for t in (keys, values, scales)]
+    table = _ints([[2, 0]])
+    for i in range(40):
+        x = (_randn((1, 2, kv, d), 100 + i) * 2.0 ** ((7 * i) % 11 - 5)).half()
+        k, v = x.unbind(1)
+        write(k.cpu(), v.cpu(), [0, 1], [i], table.cpu(), *host)
+        sspmm_amd.cache_write(k, v, offsets_of([1]), _ints([i]), table, keys, values, scales)
+    for got, want in zip((keys, values, scales), host):
+        assert torch.equal(got.cpu().view(torch.int8), want.view(torch.int8))
+    # what was written is there: within half a step of the block's scale for each time it was brought to a larger one, and its own rounding
+    k, v = row_of_cache(table[0], keys, values, scales, 40)
+    x = torch.stack([(_randn((1, 2, kv, d), 100 + i) * 2.0 ** ((7 * i) % 11 - 5)).half() for i in range(40)]).double()[:, 0]
+    step = 0.5 if form is torch.int8 else 0.0
+    for i, got in enumerate((k, v)):
+        s = scales[table[0].long(), i].double().repeat_interleave(page, 0)[:40, :, None]  # [40, kv, 1]
+        # e4m3: 2^-4 of the value, or half of the smallest step, which is 2^-9 of the scale.  Scales grow by powers of two, so codes that stay
+        # normal numbers move without a rounding, and those that do not are off by half a smallest step of each scale they had in turn,
+        # the last one's and at most half of it, a quarter, ...: 2^-9 of the scale in all.
+        near = 12 * s * step if step else x[:, i].abs() * 2.0 ** -4 + s * 2.0 ** -9
+        assert ((got - x[:, i]).abs() <= near).all()
+
+
+def test_every_e4m3_code_and_every_tie(built_library):
+    """All halves below 448 against torch's conversion (the block's largest is 448, so its scale is one)."""
+    bits = torch.arange(0, 0x6000, dtype=torch.int32, device="cuda").to(torch.int16)
+    x = bits.view(torch.float16)
+    x = x[x <= 448]
+    x = torch.cat([x, -x])
+    d, page = 128, 128
+    n = -(-x.numel() // (d - 1))
+    x = torch.nn.functional.pad(x, (0, n * (d - 1) - x.numel())).view(n, 1, d - 1)
+    x = torch.cat([torch.full((n, 1, 1), 448.0, device="cuda", dtype=torch.float16), x], 2)
+    pages = -(-n // page)
+    keys, values, scales = sspmm_amd.new_cache(pages, 1, page, d, torch.float8_e4m3fn)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    sspmm_amd.cache_write(x, x, offsets_of([n]), _ints([0]), table, keys, values, scales)
+    assert (scales == 1).all()
+    want = x[:, 0].to(torch.float8_e4m3fn).view(torch.int8)
+    assert torch.equal(keys.view(torch.int8).view(-1, d)[:n], want)
+    assert torch.equal(values.view(torch.int8).transpose(2, 3).reshape(-1, d)[:n], want)
+
+
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("most", [2.0 ** -126, 3e-39, 1e-45, 0.0, 3.0e38, 1.75 * 2.0 ** 20, 1.7578125 * 2.0 ** 20])
+def test_sizes_at_the_ends_of_the_range(built_library, form, most):
+    keys, values, scales = _filled(1, 1, 32, 32, form, seed=2)
+    x = torch.zeros(3, 1, 32, device="cuda", dtype=torch.bfloat16)
+    x[1, 0, 5], x[2, 0, 7] = most, -most / 2
+    host = [t.cpu().clone() for t in (keys, values, scales)]
+    write(x.cpu(), x.cpu(), [0, 3], [0], torch.zeros(1, 1, dtype=torch.int32), *host)
+    sspmm_amd.cache_write(x, x, offsets_of([3]), _ints([0]), _ints([[0]]), keys, values, scales)
+    for got, want in zip((keys, values, scales), host):
+        assert torch.equal(got.cpu().view(torch.int8), want.view(torch.int8))
+
+
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_what_is_not_finite_marks_its_block(built_library, form, bad):
+    page, kv, d = 32, 2, 32
+    keys, values, scales = _filled(3, kv, page, d, form, seed=3)
+    before = scales.clone()
+    k, v = _randn((4, kv, d), 1).half(), _randn((4, kv, d), 2).half()
+    k[1, 0, 3] = bad
+    table = _ints([[1, 2]])
+    sspmm_amd.cache_write(k, v, offsets_of([4]), _ints([10]), table, keys, values, scales)
+    assert torch.isnan(scales[1, 0, 0]) and torch.isfinite(scales[1, 0, 1]) and torch.isfinite(scales[1, 1]).all()
+    assert torch.equal(scales[[0, 2]], before[[0, 2]])
+    out = sspmm_amd.cache_attention(_randn((1, 1, 4, d), 3).half(), table, _ints([14]), keys, values, scales)
+    assert torch.isnan(out[0, 0, :2]).all() and torch.isfinite(out[0, 0, 2:]).all()
+    # it stays so until the page begins anew
+    ok = _randn((1, kv, d), 4).half()
+    sspmm_amd.cache_write(ok, ok, offsets_of([1]), _ints([14]), table, keys, values, scales)
+    assert torch.isnan(scales[1, 0, 0])
+    sspmm_amd.cache_write(ok, ok, offsets_of([1]), _ints([0]), table, keys, values, scales)
+    assert torch.isfinite(scales).all()
+
+
+def test_tokens_without_a_page_are_dropped(built_library):
+    page, kv, d = 32, 2, 32
+    keys, values, scales = _filled(4, kv, page, d, torch.int8, seed=4)
+    host = [t.cpu().clone() for t in (keys, values, scales)]
+    table = _ints([[-1, 1], [4, 2], [0, 2 ** 31 - 1], [3, -7]])
+    counts, starts = [40, 50, 5, 90], [0, 0, -3, 20]  # (a start below zero: nothing; the last row runs out of its slots)
+    k, v = _randn((sum(counts), kv, d), 5).half(), _randn((sum(counts), kv, d), 6).half()
+    write(k.cpu(), v.cpu(), offsets_of(counts).cpu(), starts, table.cpu(), *host)
+    sspmm_amd.cache_write(k, v, offsets_of(counts), _ints(starts), table, keys, values, scales)
+    for got, want in zip((keys, values, scales), host):
+        assert torch.equal(got.cpu().view(torch.int8), want.view(torch.int8))
+
+
+@pytest.mark.parametrize("order", ["heads first", "features first", "odd start"])
+def test_write_from_other_orders_in_memory(built_library, order):
+    k, v = _randn((70, 2, 64), 7).half(), _randn((70, 2, 64), 8).half()
+    table = _ints([[3, 0, 1]])
+    want = _filled(4, 2, 32, 64, torch.int8, seed=9)
+    sspmm_amd.cache_write(k, v, offsets_of([70]), _ints([9]), table, *want)
+    if order == "heads first":
+        k, v = (t.transpose(0, 1).contiguous().transpose(0, 1) for t in (k, v))
+    elif order == "features first":
+        k, v = (t.permute(1, 2, 0).contiguous().permute(2, 0, 1) for t in (k, v))
+    else:
+        k, v = (torch.nn.functional.pad(t.reshape(-1), (5, 0))[5:].view(t.shape) for t in (k, v))
+    got = _filled(4, 2, 32, 64, torch.int8, seed=9)
+    sspmm_amd.cache_write(k, v, offsets_of([70]), _ints([9]), table, *got)
+    assert all(torch.equal(a.view(torch.int8), b.view(torch.int8)) for a, b in zip(got, want))
+
+
+# ---- attention
+
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("page,d", [(32, 128), (64, 128), (128, 128), (32, 64), (64, 64), (128, 32), (32, 32), (64, 32)])
+@pytest.mark.parametrize("n,heads,kv", [(1, 4, 1), (1, 3, 3), (5, 8, 4), (3, 16, 2), (11, 6, 2)])
+def test_attention_against_the_formula(built_library, n, heads, kv, page, d, dtype, form):
+    lengths = [1, 0, 2, page - 1, page, page + 1, 5 * page + 17, 333]
+    table, pages = _table(lengths, page, seed=n)
+    pool = _filled(pages, kv, page, d, form, seed=d + n)
+    q = _randn((len(lengths), n, heads, d), 11, 1.5).to(dtype)
+    print(n, heads, kv, page, d, dtype, form, flush=True)
+    got = sspmm_amd.cache_attention(q, table, _ints(lengths), *pool)
+    check_step(got, q, table, lengths, *pool, 1 / math.sqrt(d))
+
+
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("lengths,n,heads,kv,page,d", [([9001], 1, 8, 2, 64, 128), ([20000, 17], 2, 4, 4, 128, 64), ([4096, 5000, 1], 9, 4, 1, 32, 128),
+                                                       ([7777], 1, 64, 1, 64, 64)])
+def test_long_rows_are_split_and_joined(built_library, lengths, n, heads, kv, page, d, form):
+    table, pages = _table(lengths, page, seed=1)
+    pool = _filled(pages, kv, page, d, form, seed=2)
+    q = _randn((len(lengths), n, heads, d), 12, 1.5).bfloat16()
+    got = sspmm_amd.cache_attention(q, table, _ints(lengths), *pool)
+    check_step(got, q, table, lengths, *pool, 1 / math.sqrt(d))
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e-4, 1.0, 3e4, 1e30])
+def test_queries_of_any_size(built_library, size):
+    lengths, d = [200, 65], 64
+    table, pages = _table(lengths, 64, seed=3)
+    pool = _filled(pages, 2, 64, d, torch.int8, seed=4)
+    q = _randn((2, 1, 4, d), 13, size).bfloat16()
+    scaling = 1 / (8 * size)
+    got = sspmm_amd.cache_attention(q, table, _ints(lengths), *pool, scaling=scaling)
+    check_step(got, q, table, lengths, *pool, scaling)
+
+
+def test_blocks_of_very_different_scales(built_library):
+    """One block of large values that the queries ignore beside small ones that they do not: nothing of the small ones is lost."""
+    page, d = 32, 64
+    keys, values, scales = _filled(4, 1, page, d, torch.int8, seed=5)
+    keys.zero_()
+    keys[0, 0, :, 0] = -127
+    scales[0], scales[1:] = 1.0, 1.0
+    scales[0, 1], scales[1:, 1] = 1e6, 1e-3
+    table, lengths = _ints([[0, 1, 2, 3]]), [4 * page]
+    q = torch.zeros(1, 1, 1, d, device="cuda", dtype=torch.float16)
+    q[..., 0] = 1.0
+    got = sspmm_amd.cache_attention(q, table, _ints(lengths), keys, values, scales, scaling=1.0)
+    k, v = row_of_cache(table[0], keys, values, scales, 128)
+    want, off = attention(q[0, 0], k[:, 0], v[:, 0], torch.tensor([128], device="cuda"), 1.0, torch.float16, torch.float16)
+    # (the first block's probabilities are 2^-183: neither they nor their rounding reach the result)
+    _, off = attention(q[0, 0], k[page:, 0], v[page:, 0], torch.tensor([96], device="cuda"), 1.0, torch.float16, torch.float16)
+    check(got[0, 0], want, off)
+
+
+@pytest.mark.parametrize("form", FORMATS)
+def test_nothing_comes_from_behind_the_row(built_library, form):
+    """Codes of NaN and scales of NaN in the rest of the last page, in pages behind it, and where a draft's earlier queries do not see."""
+    page, d, lengths = 32, 64, [40, 1, 33, 64]
+    table, pages = _table(lengths, page, seed=6)
+    pool = _filled(pages, 2, page, d, form, seed=7)
+    q = _randn((4, 3, 4, d), 14).half()
+    want = sspmm_amd.cache_attention(q, table, _ints(lengths), *pool)
+    nan = 0x7f if form is torch.float8_e4m3fn else -128
+    keys, values, scales = (t.clone() for t in pool)
+    kb, vb = keys.view(torch.int8), values.view(torch.int8)
+    for b, n in enumerate(lengths):
+        if n % page:
+            p = int(table[b, n // page])
+            kb[p, :, n % page:] = nan
+            vb[p, :, :, n % page:] = nan
+    free = [p for p in range(pages) if not (table == p).any()]
+    kb[free], vb[free], scales[free] = nan, nan, float("nan")
+    table2 = table.clone()
+    for b, n in enumerate(lengths):  # pages behind the row's end
+        table2[b, -(-n // page):] = free[0]
+    got = sspmm_amd.cache_attention(q, table2, _ints(lengths), keys, values, scales)
+    assert torch.equal(got, want)
+    # queries 0 of the row of 33 (sees 31) and 1 (sees 32): its second page is not theirs
+    p = int(table[2, 1])
+    scales[p] = float("nan")
+    got = sspmm_amd.cache_attention(q, table2, _ints(lengths), keys, values, scales)
+    assert torch.equal(got[2, :2], want[2, :2]) and torch.isnan(got[2, 2]).all() and torch.equal(got[[0, 1, 3]], want[[0, 1, 3]])
+
+
+def test_positions_without_a_page_are_masked(built_library):
+    page, d = 32, 64
+    pool = _filled(6, 1, page, d, torch.int8, seed=8)
+    table = _ints([[4, -1, 2], [6, 1, 2 ** 31 - 1], [-1, -1, -1]])
+    q = _randn((3, 1, 2, d), 15).half()
+    got = sspmm_amd.cache_attention(q, table, _ints([96, 96, 50]), *pool)
+    want = sspmm_amd.cache_attention(q, _ints([[4, 2], [1, 0], [0, 0]]), _ints([64, 32, 0]), *pool)
+    assert not got[2].any()
+    for b, part in ((0, [4, 2]), (1, [1])):
+        k, v = row_of_cache(_ints(part), *pool, 32 * len(part))
+        for h in range(2):
+            ref, off = attention(q[b, :, h], k[:, 0], v[:, 0], torch.tensor([32 * len(part)], device="cuda"), 0.125, torch.float16, torch.float16)
+            check(got[b, :, h], ref, off)
+            check(want[b, :, h], ref, off)
+    # lengths beyond the table end with it, lengths below zero are empty
+    got = sspmm_amd.cache_attention(q, table, _ints([2 ** 31 - 1, -5, 0]), *pool)
+    assert not got[1:].any()
+    check(got[0, :, 0], *attention(q[0, :, 0], *(t[:, 0] for t in row_of_cache(_ints([4, 2]), *pool, 64)), torch.tensor([64], device="cuda"), 0.125,
+                                   torch.float16, torch.float16))
+
+
+@pytest.mark.parametrize("order", ["heads first", "features first", "odd start", "out"])
+def test_attention_of_other_orders_in_memory(built_library, order):
+    lengths, d = [100, 31], 64
+    table, pages = _table(lengths, 32, seed=9)
+    pool = _filled(pages, 2, 32, d, torch.int8, seed=10)
+    q = _randn((2, 3, 4, d), 16).bfloat16()
+    want = sspmm_amd.cache_attention(q, table, _ints(lengths), *pool)
+    out = None
+    if order == "heads first":
+        q = q.transpose(1, 2).contiguous().transpose(1, 2)
+    elif order == "features first":
+        q = q.permute(0, 2, 3, 1).contiguous().permute(0, 3, 1, 2)
+    elif order == "odd start":
+        q = torch.nn.functional.pad(q.reshape(-1), (1, 0))[1:].view(q.shape)
+    else:
+        out = torch.full((2, 5, 4, d + 8), 7.0, device="cuda", dtype=torch.bfloat16)[:, 1:4, :, :d]
+    got = sspmm_amd.cache_attention(q, table, _ints(lengths), *pool, out=out)
+    assert torch.equal(got, want)
+    if out is not None:
+        assert (out._base[:, 0] == 7).all() and (out._base[:, 4] == 7).all() and (out._base[..., d:] == 7).all()
+
+
+def test_a_pool_beyond_32_bits(built_library):
+    """Pages whose bytes lie past 2^32."""
+    page, kv, d = 128, 8, 128
+    pages = (1 << 32) // (kv * page * d) + 40
+    keys = torch.empty(pages, kv, page, d, dtype=torch.int8, device="cuda")
+    values = torch.empty(pages, kv, d, page, dtype=torch.int8, device="cuda")
+    scales = torch.zeros(pages, 2, kv, device="cuda")
+    table = torch.arange(pages - 3, pages, dtype=torch.int32, device="cuda")[None].contiguous()
+    k, v = _randn((300, kv, d), 17).half(), _randn((300, kv, d), 18).half()
+    sspmm_amd.cache_write(k, v, offsets_of([300]), _ints([0]), table, keys, values, scales)
+    q = _randn((1, 1, kv, d), 19).half()
+    got = sspmm_amd.cache_attention(q, table, _ints([300]), keys, values, scales)
+    last = table[0].long()
+    small = keys[last].contiguous(), values[last].contiguous(), scales[last].contiguous()
+    want = sspmm_amd.cache_attention(q, _ints([[0, 1, 2]]), _ints([300]), *small)
+    assert torch.equal(got, want)
+    check_step(got, q, _ints([[0, 1, 2]]), [300], *small, 128 ** -0.5)
+
+
+def test_two_graphs_and_two_streams(built_library):
+    """Each call has a workspace of its own: two captured steps replayed one after the other, calls on two streams at once."""
+    lengths, d = [3000, 1700], 128
+    table, pages = _table(lengths, 64, seed=11)
+    pool = _filled(pages, 2, 64, d, torch.int8, seed=12)
+    n = _ints(lengths)
+    qs = [_randn((2, 1, 8, d), 30 + i).bfloat16() for i in range(2)]
+    outs, graphs = [torch.zeros_like(q) for q in qs], [torch.cuda.CUDAGraph() for _ in qs]
+    sspmm_amd.cache_attention(qs[0], table, n, *pool)
+    torch.cuda.synchronize()
+    for q, out, g in zip(qs, outs, graphs):
+        with torch.cuda.graph(g):
+            sspmm_amd.cache_attention(q, table, n, *pool, out=out)
+    for turn in range(4):
+        n.copy_(_ints([3000 - 500 * turn, 100 + turn]))
+        for i, q in enumerate(qs):
+            q.copy_(_randn((2, 1, 8, d), 40 + 2 * turn + i))
+        want = [sspmm_amd.cache_attention(q, table, n, *pool) for q in qs]
+        for g in graphs if turn % 2 else graphs[::-1]:
+            g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    torch.cuda.synchronize()
+    for turn in range(6):
+        for s, q in zip(streams, qs):
+            with torch.cuda.stream(s):
+                got.append(sspmm_amd.cache_attention(q, table, n, *pool))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i % 2]) for i, x in enumerate(got))
+
+
+def test_refusals(built_library):
+    keys, values, scales = sspmm_amd.new_cache(4, 2, 32, 64)
+    table, n, q = _ints([[0, 1]]), _ints([40]), _randn((1, 1, 4, 64), 1).half()
+    k = _randn((3, 2, 64), 2).half()
+    step, put = sspmm_amd.cache_attention, sspmm_amd.cache_write
+    for bad, kind in (((q.float(), table, n, keys, values, scales), TypeError), ((q, table.long(), n, keys, values, scales), TypeError),
+                      ((q, table, n.cpu(), keys, values, scales), TypeError), ((q, table, n, keys.float(), values, scales), TypeError),
+                      ((q, table, n, keys, values.view(torch.float8_e4m3fn), scales), TypeError), ((q, table, n, keys, values, scales.half()), TypeError),
+                      ((q[0], table, n, keys, values, scales), ValueError), ((q[..., :32], table, n, keys, values, scales), ValueError),
+                      ((q[:, :, :3], table, n, keys, values, scales), ValueError), ((q, table[0], n, keys, values, scales), ValueError),
+                      ((q, _ints([[0], [1]]), n, keys, values, scales), ValueError), ((q, table, _ints([1, 2]), keys, values, scales), ValueError),
+                      ((q, table, n, keys, values.transpose(2, 3).contiguous(), scales), ValueError), ((q, table, n, keys, values, scales[:, :, :1].contiguous()), ValueError),
+                      ((q, table, n, keys[1:3, :, ::2].contiguous(), values[1:3, :, :, ::2].contiguous(), scales[1:3]), ValueError),
+                      ((q, table, n, keys.transpose(0, 1), values, scales), ValueError), ((q, table[:, :0], n, keys, values, scales), ValueError)):
+        with pytest.raises(kind):
+            step(*bad)
+    with pytest.raises(ValueError):
+        step(q, table, n, keys, values, scales, scaling=float("inf"))
+    with pytest.raises(RuntimeError):
+        step(q.clone().requires_grad_(), table, n, keys, values, scales)
+    with pytest.raises(ValueError):
+        step(q, table, n, keys, values, scales, out=q[:, :, :2])
+    off, start = offsets_of([3]), _ints([0])
+    for bad, kind in (((k.float(), k, off, start, table, keys, values, scales), TypeError), ((k, k.bfloat16(), off, start, table, keys, values, scales), TypeError),
+                      ((k[:, :1], k[:, :1], off, start, table, keys, values, scales), ValueError), ((k, k[:2], off, start, table, keys, values, scales), ValueError),
+                      ((k, k, off[:1], start, table, keys, values, scales), ValueError), ((k, k, off, start.long(), table, keys, values, scales), TypeError),
+                      ((k, k, off, start, _ints([[0], [1]]), keys, values, scales), ValueError)):
+        with pytest.raises(kind):
+            put(*bad)
+    with pytest.raises(TypeError):
+        sspmm_amd.new_cache(4, 2, 32, 64, torch.float16)
+    for page, d in ((16, 64), (48, 64), (32, 80)):
+        with pytest.raises(ValueError):
+            sspmm_amd.new_cache(4, 2, page, d)
+    assert step(q[:0], table[:0], n[:0], keys, values, scales).shape == (0, 1, 4, 64)

@@ -1,0 +1,236 @@
+"""Attention over packed prompts against the formula in 64 bits."""
+import math
+
+import pytest
+import torch
+
+import sspmm_amd
+from serving_util import attention, check, check_prompt, offsets_of
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float16, torch.bfloat16]
+
+
+def _projection(tokens, heads, kv, d, dtype, seed=0):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    x = torch.randn(tokens, (heads + 2 * kv) * d, generator=g, device="cuda").to(dtype)
+    return (x[:, :heads * d].view(tokens, heads, d), x[:, heads * d:(heads + kv) * d].view(tokens, kv, d), x[:, (heads + kv) * d:].view(tokens, kv, d))
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lengths,heads,kv", [([1], 1, 1), ([2, 0, 65, 1], 4, 2), ([63, 64, 31, 32, 33], 3, 1), ([127, 128, 129], 2, 2), ([300, 5], 6, 2),
+                                              ([257, 0, 0, 96], 8, 8), ([150], 16, 8), ([700], 2, 1)])
+def test_against_the_formula(built_library, lengths, heads, kv, dtype, d, causal):
+    q, k, v = _projection(sum(lengths), heads, kv, d, dtype, seed=len(lengths) + d)
+    print(lengths, heads, kv, dtype, d, causal, flush=True)
+    got = sspmm_amd.prompt_attention(q, k, v, offsets_of(lengths), causal=causal)
+    check_prompt(got, q, k, v, lengths, causal, 1 / math.sqrt(d))
+
+
+@pytest.mark.parametrize("lengths,heads,kv,causal", [([2500, 1100], 4, 1, True), ([3001], 8, 8, True), ([1900, 2300], 2, 2, False)])
+def test_longer_ones(built_library, lengths, heads, kv, causal):
+    q, k, v = _projection(sum(lengths), heads, kv, 128, torch.bfloat16, seed=3)
+    got = sspmm_amd.prompt_attention(q, k, v, offsets_of(lengths), causal=causal)
+    check_prompt(got, q, k, v, lengths, causal, 128 ** -0.5)
+
+
+def test_hundreds_of_short_sequences(built_library):
+    lengths = [(7 * i * i + 3) % 40 for i in range(300)]
+    q, k, v = _projection(sum(lengths), 4, 4, 64, torch.float16, seed=5)
+    got = sspmm_amd.prompt_attention(q, k, v, offsets_of(lengths))
+    check_prompt(got, q, k, v, lengths, True, 0.125)
+
+
+@pytest.mark.parametrize("scaling", [1e-3, 0.125, 3.0, 100.0])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scores_small_and_large(built_library, dtype, scaling):
+    lengths = [200, 77]
+    q, k, v = _projection(sum(lengths), 2, 1, 64, dtype, seed=6)
+    got = sspmm_amd.prompt_attention(q, k, v, offsets_of(lengths), scaling=scaling)
+    check_prompt(got, q, k, v, lengths, True, scaling)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_maxima_that_grow_along_the_sequence(built_library, causal):
+    """Every tile's maximum is far above the one before: the reference point moves each time."""
+    n = 500
+    q, k, v = _projection(n, 2, 2, 64, torch.float16, seed=7)
+    k = (k * torch.linspace(0.1, 8, n, device="cuda")[:, None, None]).half()
+    got = sspmm_amd.prompt_attention(q, k, v, offsets_of([n]), causal=causal, scaling=1.0)
+    check_prompt(got, q, k, v, [n], causal, 1.0)
+
+
+def test_many_small_probabilities_beside_a_large_one(built_library):
+    """The sum is of the exponentials, not of what fp16 makes of them: 8000 keys of 2^-26 are together a part in 8000 of the one that is 1."""
+    n, d = 8000, 64
+    q = torch.zeros(n, 1, d, device="cuda", dtype=torch.float16)
+    k = torch.zeros_like(q)
+    q[-1, 0, 0], k[0, 0, 0] = 1.0, 26.0 * math.log(2)
+    v = torch.ones_like(q)
+    v[0] = 0.0
+    got = sspmm_amd.prompt_attention(q, k, v, offsets_of([n]), scaling=1.0)
+    want, off = attention(q[-1:, 0], k[:, 0], v[:, 0], torch.tensor([n], device="cuda"), 1.0, torch.float16, torch.float16)
+    check(got[-1:, 0], want, off)
+    v[0] = 1.0  # all ones: the result is one, whatever was rounded on the way, to what fp16 leaves out of these keys
+    got = sspmm_amd.prompt_attention(q, k, v, offsets_of([n]), scaling=1.0)
+    assert (got[-1].float() - 1).abs().max() <= n * 2.0 ** -26 + 2.0 ** -11
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [32, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_nothing_comes_from_masked_places(built_library, dtype, d, bad):
+    """NaN and infinities in k and v of tokens that a query does not see: later ones, other sequences', and rows behind the last."""
+    lengths = [130, 70, 1, 40]
+    q, k, v = (t.clone() for t in _projection(sum(lengths) + 30, 4, 2, d, dtype, seed=8))
+    k[sum(lengths):], v[sum(lengths):] = bad, bad
+    q[sum(lengths):] = bad
+    for at in (100, 129, 195, 200 + 1 + 5):  # tokens of three of the sequences
+        v[at, 0, 3] = bad
+        k[at, 1] = bad if bad != bad else k[at, 1]
+    got = sspmm_amd.prompt_attention(q, k, v, offsets_of(lengths))
+    # keys that are NaN: whoever sees one gets NaN, all others a finite result
+    group, at = 2, 0
+    for n in lengths:
+        for h in range(4):
+            qq, kk, vv = q[at:at + n, h], k[at:at + n, h // group], v[at:at + n, h // group]
+            nan_key = torch.isnan(kk).any(-1)
+            sees_nan = torch.cumsum(nan_key.int(), 0) > 0
+            visible = torch.arange(1, n + 1, device="cuda")
+            want, off = attention(qq, torch.where(nan_key[:, None], 0.0, kk.double()), vv, visible, d ** -0.5, dtype, dtype)
+            rows = ~sees_nan
+            check(got[at:at + n, h][rows], want[rows], off[rows], "head %d at %d" % (h, at))
+            assert torch.isnan(got[at:at + n, h][sees_nan]).all()
+        at += n
+
+
+def test_both_infinities_in_the_last_tile(built_library):
+    n = 40
+    q, k, v = (t.clone() for t in _projection(n, 1, 1, 64, torch.bfloat16, seed=9))
+    v[10, 0, 0], v[20, 0, 0], v[15, 0, 1], v[12, 0, 40] = float("inf"), float("-inf"), float("-inf"), float("nan")
+    got = sspmm_amd.prompt_attention(q, k, v, offsets_of([n]))[:, 0]
+    assert torch.isfinite(got[:10]).all() and (got[10:20, 0] == float("inf")).all() and torch.isnan(got[20:, 0]).all()
+    assert (got[15:, 1] == float("-inf")).all() and torch.isfinite(got[:15, 1]).all() and torch.isnan(got[12:, 40]).all() and torch.isfinite(got[:, 2:40]).all()
+
+
+def test_scores_of_minus_infinity_only_are_zeros(built_library):
+    q = torch.full((3, 1, 32), float("-inf"), device="cuda", dtype=torch.float16)
+    k = torch.ones_like(q)
+    got = sspmm_amd.prompt_attention(q, k, torch.ones_like(q), offsets_of([3]))
+    assert not got.any()
+
+
+def test_rows_of_no_sequence_stay_as_they_were(built_library):
+    lengths = [50, 0, 30]
+    q, k, v = _projection(100, 2, 1, 64, torch.float16, seed=10)
+    out = torch.full((100, 2, 64), 7.0, device="cuda", dtype=torch.float16)
+    offsets = offsets_of(lengths) + 5  # tokens 0 .. 4 and 85 .. belong to nobody
+    got = sspmm_amd.prompt_attention(q, k, v, offsets, out=out)
+    assert got is out and (out[:5] == 7).all() and (out[85:] == 7).all()
+    check_prompt(out[5:85], q[5:85], k[5:85], v[5:85], lengths, True, 0.125)
+
+
+def test_offsets_outside_the_tokens_are_taken_to_their_ends(built_library):
+    q, k, v = _projection(60, 2, 2, 32, torch.float16, seed=11)
+    out = torch.full((60, 2, 32), 7.0, device="cuda", dtype=torch.float16)
+    offsets = torch.tensor([-9, 20, 10, 50, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    # 0 .. 19; 20 .. 9, nothing; 10 .. 49; 50 .. 59
+    sspmm_amd.prompt_attention(q, k, v, offsets[[0, 1]].contiguous(), out=out)
+    check_prompt(out[:20], q[:20], k[:20], v[:20], [20], True, 32 ** -0.5)
+    sspmm_amd.prompt_attention(q, k, v, offsets[[1, 2]].contiguous(), out=out)
+    sspmm_amd.prompt_attention(q, k, v, offsets[[2, 3, 4]].contiguous(), out=out)
+    check_prompt(out[10:], q[10:], k[10:], v[10:], [40, 10], True, 32 ** -0.5)
+
+
+@pytest.mark.parametrize("order", ["heads first", "features first", "odd start", "out"])
+def test_other_orders_in_memory(built_library, order):
+    lengths, heads, kv, d = [90, 33], 4, 2, 64
+    q, k, v = _projection(123, heads, kv, d, torch.bfloat16, seed=12)
+    want = sspmm_amd.prompt_attention(q, k, v, offsets_of(lengths))
+    out = None
+    if order == "heads first":
+        q, k, v = (t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v))
+    elif order == "features first":  # as the SpMM leaves projections
+        q, k, v = (t.permute(1, 2, 0).contiguous().permute(2, 0, 1) for t in (q, k, v))
+    elif order == "odd start":
+        q, k, v = (torch.nn.functional.pad(t.reshape(-1), (3, 0))[3:].view(t.shape) for t in (q, k, v))
+        assert q.data_ptr() % 16
+    else:
+        out = torch.zeros(heads, 123, d + 8, device="cuda", dtype=torch.bfloat16)[:, :, :d].transpose(0, 1)
+    got = sspmm_amd.prompt_attention(q, k, v, offsets_of(lengths), out=out)
+    assert torch.equal(got, want)
+
+
+def test_rows_further_apart_than_32_bits_reach(built_library):
+    n, pitch = 520, 1 << 22  # 4.4 GB
+    room = torch.empty(n * pitch, dtype=torch.float16, device="cuda")
+    x = room.view(n, pitch)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(13)
+    q, k, v = (x[:, i * 64:(i + 1) * 64].view(n, 1, 64) for i in range(3))
+    for t in (q, k, v):
+        t.copy_(torch.randn(n, 1, 64, generator=g, device="cuda"))
+    out = x[:, 1024:1088].view(n, 1, 64)
+    sspmm_amd.prompt_attention(q, k, v, offsets_of([n]), out=out)
+    check_prompt(out, q, k, v, [n], True, 0.125)
+
+
+def test_captured_replayed_and_called_beside_it(built_library):
+    lengths = [300, 77]
+    q, k, v = (t.clone() for t in _projection(377, 8, 8, 128, torch.bfloat16, seed=14))
+    offsets, out = offsets_of(lengths), torch.zeros(377, 8, 128, device="cuda", dtype=torch.bfloat16)
+    eager = sspmm_amd.prompt_attention(q, k, v, offsets)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        sspmm_amd.prompt_attention(q, k, v, offsets, out=out)
+    for seed in range(4):
+        q.copy_(_projection(377, 8, 8, 128, torch.bfloat16, seed=20 + seed)[0])
+        offsets.copy_(offsets_of([100 + seed, 277 - seed]))  # (the graph reads them anew)
+        want = sspmm_amd.prompt_attention(q, k, v, offsets)
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    assert eager.shape == out.shape
+
+
+def test_on_another_stream(built_library):
+    q, k, v = _projection(200, 4, 2, 64, torch.float16, seed=15)
+    offsets = offsets_of([200])
+    want = sspmm_amd.prompt_attention(q, k, v, offsets)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = sspmm_amd.prompt_attention(q, k, v, offsets)
+    s.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_refusals(built_library):
+    q, k, v = _projection(10, 4, 2, 64, torch.float16)
+    offsets = offsets_of([10])
+    call = sspmm_amd.prompt_attention
+    for bad, kind in (((q.float(), k, v, offsets), TypeError), ((q, k.bfloat16(), v, offsets), TypeError), ((q, k, v, offsets.long()), TypeError),
+                      ((q, k, v, offsets.cpu()), TypeError), ((q.cpu(), k.cpu(), v.cpu(), offsets), TypeError), ((q[:, :3], k, v, offsets), ValueError),
+                      ((q, k[:, :, :32], v[:, :, :32], offsets), ValueError), ((q[:, :, :48], k[:, :, :48], v[:, :, :48], offsets), ValueError),
+                      ((q, k[:9], v[:9], offsets), ValueError), ((q[0], k[0], v[0], offsets), ValueError), ((q, k, v, offsets[None]), ValueError),
+                      ((q, k, v, offsets[:0]), ValueError), ((q, k[:, :0], v[:, :0], offsets), ValueError)):
+        with pytest.raises(kind):
+            call(*bad)
+    for scaling in (0.0, -1.0, float("nan"), float("inf"), 3e38):
+        with pytest.raises(ValueError):
+            call(q, k, v, offsets, scaling=scaling)
+    with pytest.raises(ValueError):
+        call(q, k, v, offsets, out=torch.empty(10, 4, 64, device="cuda", dtype=torch.bfloat16))
+    with pytest.raises(ValueError):
+        call(q, k, v, offsets, out=torch.empty(10, 64, 4, device="cuda", dtype=torch.float16).transpose(1, 2))
+    with pytest.raises(RuntimeError):
+        call(q.clone().requires_grad_(), k, v, offsets)
+    with torch.no_grad():
+        assert not call(q.clone().requires_grad_(), k, v, offsets).requires_grad
+    assert call(q[:0], k[:0], v[:0], offsets_of([])).shape == (0, 4, 64)
