@@ -6,6 +6,8 @@
 #include "lane_ops.h"
 #include "sixteen_bit.h"
 
+#include <type_traits>
+
 namespace sspmm {
 
 namespace {
@@ -25,11 +27,17 @@ __device__ __forceinline__ int swizzle_v(int r) {
   return D == 128 ? (r & 3) * 4 : D == 64 ? ((r >> 1) & 1) * 4 : 0;
 }
 
-// 16 bytes a lane from memory straight into LDS, one lane's behind the other's; what lies behind `bytes` comes as zeros.
-__device__ __forceinline__ void load_to_lds(const void *base, uint32_t bytes, uint32_t at, unsigned char *to) {
-  typedef __attribute__((address_space(3))) void lds_void;
-  const auto srd = __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, (int)bytes, kSrdWord3);
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(srd, (lds_void *)to, 16, (int)at, 0, 0, 0);
+// 16 bytes a lane from memory straight into LDS, one lane's behind the other's from `to` on; what lies behind the descriptor's bytes comes as
+// zeros.  As assembly because the compiler, which cannot tell one tile of LDS from another, makes every read of the tile that is worked on wait for
+// the next one's loads (16001 tokens, 8 heads: 619 us with the builtin); the waits for these are the ones before the barriers below.
+typedef int srd __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void load_to_lds(srd from, uint32_t at, uint32_t to) {
+  // (m0 is nobody else's here.  The wait is what a vector instruction that wrote one of the scalars just before would need.)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(at), "s"(from) : "memory");
+}
+__device__ __forceinline__ srd descriptor(const uint16_t *base, uint32_t bytes) {
+  const uint64_t b = reinterpret_cast<uint64_t>(base);
+  return srd{(int)(uint32_t)b, (int)((uint32_t)(b >> 32) & 0xffffu), (int)bytes, (int)kSrdWord3};
 }
 
 // Whether any of the eight values is infinite or NaN.
@@ -41,24 +49,15 @@ __device__ __forceinline__ bool not_finite(uintx4 v) {
   return bad;
 }
 
-// The eight values, with ones where the value is of a kind and zeros elsewhere: 0 = finite values as they are (zeros elsewhere),
-// 1 = +infinity, 2 = -infinity, 3 = NaN.
+// The eight values with zeros in place of infinities and NaN.
 template <typename T>
-__device__ __forceinline__ uintx4 of_kind(uintx4 v, int kind) {
-  uintx4 r;
+__device__ __forceinline__ uintx4 finite_part(uintx4 v) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    uint32_t u = 0;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t x = (v[i] >> (16 * h)) & 0xffffu;
-      const bool special = (x & T::kExponent) == T::kExponent;
-      const int is = !special ? 0 : x == T::kInfinity ? 1 : x == (0x8000u | T::kInfinity) ? 2 : 3;
-      u |= (is != kind ? 0u : kind == 0 ? x : T::kOne) << (16 * h);
-    }
-    r[i] = u;
+    if ((v[i] & T::kExponent) == T::kExponent) v[i] &= 0xffff0000u;
+    if (((v[i] >> 16) & T::kExponent) == T::kExponent) v[i] &= 0xffffu;
   }
-  return r;
+  return v;
 }
 
 // A workgroup of WAVES waves owns 32 * WAVES consecutive queries of one sequence and head, 32 a wave.
@@ -117,8 +116,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(const P
   const int kv_head = head / (p.heads / p.kv_heads);
   const int my = q0 + 32 * wave + n;  // this lane's query
   const int seen = CAUSAL ? min(my + 1, length) : length;  // keys it sees: those below
-  const int all_see = CAUSAL ? min(q0 + 32 * wave + 1, length) : length;  // (every query of the wave sees those below this)
-  const int most = CAUSAL ? min(q0 + 32 * wave + 32, length) : length;  // (and none of them one from here on)
+  const int most = CAUSAL ? min(q0 + 32 * wave + 32, length) : length;  // (no query of the wave sees one from here on)
   const int last = CAUSAL ? min(q0 + kQueries, length) : length;
   const int key_tiles = (last + kKeys - 1) / kKeys;
 
@@ -134,6 +132,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(const P
   const uint16_t *const k0 = p.k + (long long)first * p.k_row + (long long)kv_head * p.k_head;
   const uint16_t *const v0 = p.v + (long long)first * p.v_row + (long long)kv_head * p.v_head;
   const uint32_t k_pitch = (uint32_t)p.k_row * 2, v_pitch = (uint32_t)p.v_row * 2;
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)lds + wave * 1024;
   uint32_t k_at[kLoads], v_at[kLoads];
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
@@ -143,13 +142,24 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(const P
   }
   const auto fetch = [&](int t) {
     const int rows = min(kKeys, length - t * kKeys);
-    const uint16_t *const k = k0 + (long long)t * kKeys * p.k_row, *const v = v0 + (long long)t * kKeys * p.v_row;
-    unsigned char *const to = lds + (t & 1) * 2 * kTile + wave * 1024;
+    const srd sk = descriptor(k0 + (long long)t * kKeys * p.k_row, (rows - 1) * k_pitch + D * 2);
+    const srd sv = descriptor(v0 + (long long)t * kKeys * p.v_row, (rows - 1) * v_pitch + D * 2);
+    const uint32_t to = lds_at + (t & 1) * 2 * kTile;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) load_to_lds(k, (rows - 1) * k_pitch + D * 2, k_at[i], to + i * WAVES * 1024);
+    for (int i = 0; i < kLoads; ++i) load_to_lds(sk, k_at[i], to + i * WAVES * 1024);
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) load_to_lds(v, (rows - 1) * v_pitch + D * 2, v_at[i], to + kTile + i * WAVES * 1024);
+    for (int i = 0; i < kLoads; ++i) load_to_lds(sv, v_at[i], to + kTile + i * WAVES * 1024);
   };
+
+  // ---- where a lane's operands lie in a tile: of K in its first 32 rows by step, of V in the first 8 rows of a step by part
+  uint32_t k_rd[kSteps], v_rd[kParts];
+#pragma unroll
+  for (int step = 0; step < kSteps; ++step) k_rd[step] = n * (D * 2) + (((2 * step + half) ^ swizzle_k<D>(n)) * 16);  // (32 rows on: the same swizzle)
+#pragma unroll
+  for (int part = 0; part < kParts; ++part) {
+    const int r = 4 * half + ((lane & 15) >> 2), piece = 4 * part + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    v_rd[part] = kTile + r * (D * 2) + ((piece ^ swizzle_v<D>(r)) * 16) + (lane & 1) * 8;  // (8 rows on: the same swizzle)
+  }
 
   floatx16 o[kParts];  // lane (n, half): features 32 part + 8 (i / 4) + 4 half + i % 4 of its query
 #pragma unroll
@@ -159,35 +169,25 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(const P
   float run_max = -3.0e38f, run_sum = 0.f;  // of the scaled scores; this lane's share of the sum
   const float c = p.scale_log2e;
 
-  fetch(0);
-  for (int t = 0; t < key_tiles; ++t) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();  // tile t is there, and nobody reads tile t - 1 any more
-    if (t + 1 < key_tiles) fetch(t + 1);
-    const int key0 = t * kKeys;
-    if (key0 >= most) continue;  // (the barrier above is in every wave's path)
-    const unsigned char *const k_tile = lds + (t & 1) * 2 * kTile, *const v_tile = k_tile + kTile;
-
+  // Tile t, in `tile` of LDS.  cut: some query may not see all of its keys.
+  const auto work_on = [&](auto cut_, const unsigned char *tile, int key0) {
+    constexpr bool cut = decltype(cut_)::value;
     floatx16 s[2];
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
+    for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[kt][i] = 0.f;
-      const int r = 32 * kt + n;
 #pragma unroll
-      for (int step = 0; step < kSteps; ++step) {
-        const uintx4 k = *reinterpret_cast<const uintx4 *>(k_tile + r * (D * 2) + (((2 * step + half) ^ swizzle_k<D>(r)) * 16));
-        s[kt] = T::mfma_32x32x16(k, q[step], s[kt]);
-      }
-    }
-    const bool cut = key0 + kKeys > all_see;  // uniform in the wave
-    if (cut) {
+    for (int step = 0; step < kSteps; ++step)
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+        s[kt] = T::mfma_32x32x16(*reinterpret_cast<const uintx4 *>(tile + k_rd[step] + 32 * kt * (D * 2)), q[step], s[kt]);
+    if constexpr (cut) {
       const int left = seen - key0 - 4 * half;
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (32 * kt + 8 * (i / 4) + i % 4 >= left) s[kt][i] = -INFINITY;
+        for (int i = 0; i < 16; ++i) s[kt][i] = 32 * kt + 8 * (i / 4) + i % 4 >= left ? -INFINITY : s[kt][i];
     }
     float most_here = s[0][0];
 #pragma unroll
@@ -221,52 +221,72 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(const P
       }
 
     const auto read_v = [&](int part, int step) {
-      const int r = 16 * step + 4 * half + ((lane & 15) >> 2), piece = 4 * part + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-      const unsigned char *const at = v_tile + r * (D * 2) + ((piece ^ swizzle_v<D>(r)) * 16) + (lane & 1) * 8;
-      const uintx2 lo = lds_read_tr(at), hi = lds_read_tr(at + 8 * (D * 2));  // (swizzle_v is the same eight rows on)
+      const unsigned char *const at = tile + v_rd[part] + 16 * step * (D * 2);
+      const uintx2 lo = lds_read_tr(at), hi = lds_read_tr(at + 8 * (D * 2));
       return uintx4{lo[0], lo[1], hi[0], hi[1]};
     };
     bool bad = false;
-    if (cut) {
+    if constexpr (cut && CAUSAL) {  // (keys behind the sequence are zeros)
 #pragma unroll
       for (int part = 0; part < kParts; ++part)
 #pragma unroll
-        for (int step = 0; step < 4; ++step) bad |= not_finite<T>(read_v(part, step));
+        for (int step = 0; step < 4; ++step) {
+          bad |= not_finite<T>(read_v(part, step));
+          if (step % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+        }
       bad = __ballot(bad) != 0;
     }
-    if (!__builtin_expect(bad, 0)) {
+    if (!(cut && CAUSAL) || !__builtin_expect(bad, 0)) {
 #pragma unroll
       for (int part = 0; part < kParts; ++part)
 #pragma unroll
         for (int step = 0; step < 4; ++step) o[part] = T::mfma_32x32x16(read_v(part, step), pt[step], o[part]);
     } else {
-      // A masked key's probability is zero, but zero times an infinity or a NaN in its v is NaN.  Finite values as ever; of the others,
-      // those that a query sees are counted by the same instruction, kind by kind.
+      // A masked key's probability is zero, but zero times an infinity or a NaN in its v is NaN.  Finite values as ever; the others are
+      // added, key by key, to the queries that see them.
 #pragma unroll
       for (int part = 0; part < kParts; ++part)
 #pragma unroll
-        for (int step = 0; step < 4; ++step) o[part] = T::mfma_32x32x16(of_kind<T>(read_v(part, step), 0), pt[step], o[part]);
-      uintx4 sees[4];
-#pragma unroll
-      for (int step = 0; step < 4; ++step)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int key = 16 * step + 4 * half + 8 * (j >> 1) + 2 * (j & 1), left = seen - key0;
-          sees[step][j] = (key < left ? T::kOne : 0u) | (key + 1 < left ? T::kOne << 16 : 0u);
+        for (int step = 0; step < 4; ++step) {
+          o[part] = T::mfma_32x32x16(finite_part<T>(read_v(part, step)), pt[step], o[part]);
+          __builtin_amdgcn_sched_barrier(0);  // (one operand at a time: registers are short)
         }
+#pragma unroll 1
+      for (int r = 0; r < kKeys; ++r) {
+        const bool sees = key0 + r < seen;
 #pragma unroll
-      for (int part = 0; part < kParts; ++part)
-        for (int kind = 1; kind < 4; ++kind) {
-          floatx16 count;
+        for (int part = 0; part < kParts; ++part)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) count[i] = 0.f;
+          for (int i = 0; i < 16; i += 4) {
+            const int piece = 4 * part + i / 4;
+            const uintx2 v = *reinterpret_cast<const uintx2 *>(tile + kTile + r * (D * 2) + ((piece ^ swizzle_v<D>(r)) * 16) + 8 * half);
+            const float x[4] = {T::lower(v[0]), T::upper(v[0]), T::lower(v[1]), T::upper(v[1])};
 #pragma unroll
-          for (int step = 0; step < 4; ++step) count = T::mfma_32x32x16(of_kind<T>(read_v(part, step), kind), sees[step], count);
-          const float what = kind == 1 ? INFINITY : kind == 2 ? -INFINITY : NAN;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[part][i] += count[i] > 0.f ? what : 0.f;
-        }
+            for (int j = 0; j < 4; ++j) o[part][i + j] += sees && !(fabsf(x[j]) < INFINITY) ? x[j] : 0.f;
+          }
+      }
     }
+  };
+
+  const std::integral_constant<bool, false> whole{};
+  const std::integral_constant<bool, true> cut{};
+  const auto next = [&](int t) {  // tile t is there, and nobody reads tile t - 1 any more
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    __syncthreads();
+    if (t + 1 < key_tiles) fetch(t + 1);
+  };
+  const int whole_tiles = (CAUSAL ? min(q0 + 1, length) : length) / kKeys;  // that all queries of the workgroup see
+  fetch(0);
+  int t = 0;
+  for (; t + 2 <= whole_tiles; t += 2) {
+    next(t);
+    work_on(whole, lds, t * kKeys);
+    next(t + 1);
+    work_on(whole, lds + 2 * kTile, (t + 1) * kKeys);
+  }
+  for (; t < key_tiles; ++t) {
+    next(t);
+    if (t * kKeys < most) work_on(cut, lds + (t & 1) * 2 * kTile, t * kKeys);
   }
 
   {
