@@ -598,9 +598,11 @@ int sspmm_cache_attention(int type, int format, int sequences, int queries, int 
  *             copied to a free one.  A child that finds none, or whose parent is no row or itself a child in the call, is left empty with
  *             length 0.  A row named several times as a child becomes its last naming.
  *   compact   with n pages in use, the contents of those at n and behind go to the free ones below n, and the table and counts with them
- * Indices outside the table are passed over.  workspace: sspmm_page_workspace_bytes(pages, rows, slots, count of rows named), 16-byte aligned.
+ * Indices outside the table are passed over.  workspace: what the functions say (reserve: 0 where a workgroup's LDS holds it), 4-byte aligned.
  */
-size_t sspmm_page_workspace_bytes(int pages, int rows, int slots, int count);
+size_t sspmm_reserve_pages_workspace_bytes(int pages, int rows, int slots);
+size_t sspmm_fork_pages_workspace_bytes(int rows, int count);
+size_t sspmm_compact_pages_workspace_bytes(int pages);
 int sspmm_reserve_pages(int32_t *page_refs, int pages, int32_t *page_table, int rows, int slots, const int32_t *starts,
                         const int32_t *offsets, int page_size, void *workspace, size_t workspace_bytes, void *hip_stream);
 int sspmm_release_pages(int32_t *page_refs, int pages, int32_t *page_table, int rows, int slots, int32_t *lengths, const int32_t *named,

@@ -73,7 +73,9 @@ SIGNATURES = {
     "sspmm_cache_attention_workspace_bytes": (ctypes.c_size_t, [_int] * 7),
     "sspmm_cache_attention": (_int, [_int] * 5 + [_vp, _i64, _i64, _i64, _vp, _int, _vp] + [_int] * 4 + [_vp] * 3 + [ctypes.c_float, _vp, _i64, _i64, _i64,
                                                                                                                _vp, ctypes.c_size_t, _vp]),
-    "sspmm_page_workspace_bytes": (ctypes.c_size_t, [_int] * 4),
+    "sspmm_reserve_pages_workspace_bytes": (ctypes.c_size_t, [_int] * 3),
+    "sspmm_fork_pages_workspace_bytes": (ctypes.c_size_t, [_int] * 2),
+    "sspmm_compact_pages_workspace_bytes": (ctypes.c_size_t, [_int]),
     "sspmm_reserve_pages": (_int, [_vp, _int, _vp, _int, _int, _vp, _vp, _int, _vp, ctypes.c_size_t, _vp]),
     "sspmm_release_pages": (_int, [_vp, _int, _vp, _int, _int, _vp, _vp, _int, _vp]),
     "sspmm_fork_pages": (_int, [_vp, _int, _vp, _int, _int, _vp, _vp, _vp] + [_int] * 4 + [_vp] * 4 + [ctypes.c_size_t, _vp]),

@@ -10,7 +10,7 @@ namespace sspmm {
 
 namespace {
 
-constexpr int kWaves = 4;
+constexpr int kMostSplits = 256;
 
 typedef Fp16::vec8 half8;
 
@@ -39,13 +39,27 @@ __device__ __forceinline__ uintx4 as_halfs(uint32_t lo, uint32_t hi) {
   return r;
 }
 
+// The sequence that a workgroup takes: of 64 consecutive ones the longest go first, where not all workgroups find a place at once.
+__device__ __forceinline__ int longest_first(const int32_t *lengths, int sequences) {
+  const int z = blockIdx.z;
+  if (gridDim.x * gridDim.y * gridDim.z <= 256 || sequences == 1) return z;
+  const int lane = threadIdx.x & 63, first = z & ~63, count = min(64, sequences - first);
+  const int mine = lane < count ? lengths[first + lane] : -1;
+  int rank = lane < count ? 0 : 64;
+  for (int j = 0; j < count; ++j) {
+    const int other = __builtin_amdgcn_readlane(mine, j);
+    rank += other > mine || (other == mine && j < lane);
+  }
+  return first + __builtin_ctzll(__ballot(rank == z - first));
+}
+
 __device__ __forceinline__ long long partial_floats(int rows, int d) { return (long long)rows * (d + 2); }
 
 // A workgroup owns 16 * TILES rows (queries x heads of one head of the cache; row i * group + j is query i, head j of the group) of one
 // sequence and one of its `splits` shares of the keys, a wave a quarter of those, UNIT keys at a time, all of them in one page.  Scores are
 // made transposed, K Q^T: the lane of row m and group g holds keys UNIT / 4 * g .. of the unit, which is the operand of the second product
 // V^T P^T as it is, and the order in which values lie in a page.
-template <typename T, int FORMAT, int D, int TILES, int UNIT>
+template <typename T, int FORMAT, int D, int TILES, int UNIT, int kWaves>
 __global__ __launch_bounds__(64 * kWaves, 2) void cache_attention_kernel(const CacheAttentionArgs p) {
   constexpr int kKeyTiles = UNIT / 16, kParts = D / 16, kSteps = D / 32, kShares = UNIT / 32, kRows = 16 * TILES;
   constexpr int kKeyWords = D >= 64 ? 4 : 2;  // of a load of K: 16 bytes, or 8 where a group's share of a row is no more
@@ -59,7 +73,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_attention_kernel(const C
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const CachePool pool = p.pool;
   const int group = p.heads / pool.kv_heads, rows = p.queries * group, tiles = (rows + kRows - 1) / kRows;
-  const int split = blockIdx.x, head = blockIdx.y % pool.kv_heads, tile = blockIdx.y / pool.kv_heads, seq = blockIdx.z;
+  const int split = blockIdx.x, head = blockIdx.y % pool.kv_heads, tile = blockIdx.y / pool.kv_heads;
+  const int seq = longest_first(p.lengths, p.sequences);
   const int length = max(0, (int)min((long long)p.lengths[seq], (long long)pool.slots * pool.page_size));
   const int units = (length + UNIT - 1) / UNIT, pieces = p.splits * kWaves, piece = split * kWaves + wave;
   const int unit0 = (int)((long long)units * piece / pieces), unit1 = (int)((long long)units * (piece + 1) / pieces);
@@ -111,11 +126,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_attention_kernel(const C
   const long long block = (long long)pool.page_size * D;
   KeyWords kk[kKeyTiles][kKeyLoads];
   ValueWords vv[kParts];
-  int page = 0, page_next = 0;
   const int page_units = pool.page_size / UNIT, page_bits = 31 - __builtin_clz(page_units);  // (1 or 2)
-  const auto page_of = [&](int u) { return __builtin_amdgcn_readfirstlane(table[u >> page_bits]); };
   const auto place_of = [&](int u) { return (u & (page_units - 1)) * UNIT; };  // in its page
   const auto usable = [&](int pg) { return pg >= 0 && pg < pool.pages; };
+  // Pages and scales of 64 units at a time, one a lane, so that no unit waits for them.
+  int pages_of = 0;
+  float k_scales = 0.f, v_scales = 0.f;
+  const auto look_up = [&](int u) {
+    const int mine = min(u + lane, unit1 - 1);
+    pages_of = table[mine >> page_bits];
+    const float *const scale = pool.scales + (long long)(usable(pages_of) ? pages_of : 0) * 2 * pool.kv_heads + head;
+    k_scales = scale[0];
+    v_scales = scale[pool.kv_heads];
+  };
   const auto load_k = [&](int u, int pg) {
     const unsigned char *const at = pool.keys + ((long long)(usable(pg) ? pg : 0) * pool.kv_heads + head) * block + place_of(u) * D;
 #pragma unroll
@@ -136,17 +159,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_attention_kernel(const C
     }
   };
 
+  int page = 0;
   if (unit0 < unit1) {
-    page = page_of(unit0);
+    look_up(unit0);
+    page = __builtin_amdgcn_readlane(pages_of, 0);
     load_k(unit0, page);
     load_v(unit0, page);
-    page_next = unit0 + 1 < unit1 ? page_of(unit0 + 1) : page;
   }
   for (int u = unit0; u < unit1; ++u) {
     const bool more = u + 1 < unit1, there = usable(page);
-    const float *const scale = pool.scales + (long long)(there ? page : 0) * 2 * pool.kv_heads + head;
-    const float k_scale = scale[0], v_scale = scale[pool.kv_heads];
-    const int after = u + 2 < unit1 ? page_of(u + 2) : page_next;
+    const int at = (u - unit0) & 63;
+    const float k_scale = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(k_scales), at));
+    const float v_scale = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v_scales), at));
+    if (at == 63 && more) look_up(u + 1);
+    const int page_next = __builtin_amdgcn_readlane(pages_of, (at + 1) & 63);
     floatx4 s[TILES][kKeyTiles];
 #pragma unroll
     for (int kt = 0; kt < kKeyTiles; ++kt) {
@@ -228,7 +254,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_attention_kernel(const C
     }
     if (more) load_v(u + 1, page_next);
     page = page_next;
-    page_next = after;
   }
 
   // ---- the waves' states as one
@@ -281,89 +306,101 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_attention_kernel(const C
   }
 }
 
-// The splits' states of one row as one: D / 4 threads for the features, 1024 / D sets of them that take every so manyth split.
+// The splits' states of one row as one: their weights first, then D / 4 threads for the features and 1024 / D sets of them that take every so
+// manyth split.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void cache_attention_join_kernel(const CacheAttentionArgs p, int row_tiles) {
   constexpr int kSets = 1024 / D;
-  __shared__ float weight_sum[kSets];
+  __shared__ float weights[kMostSplits];
   __shared__ __align__(16) float part[kSets][D];
-  __shared__ float largest[4];
+  __shared__ float largest[4], totals_of[4];
   const int kRows = 16 * row_tiles, group = p.heads / p.pool.kv_heads, rows = p.queries * group, tiles = (rows + kRows - 1) / kRows;
-  const int row = blockIdx.x, head = blockIdx.y, seq = blockIdx.z, tile = row / kRows, r = row % kRows;
+  const int row = blockIdx.x, head = blockIdx.y, seq = blockIdx.z, tile = row / kRows, r = row % kRows, tid = threadIdx.x;
   const long long pitch = partial_floats(kRows, D);
   const float *const base = p.partial + (((long long)seq * p.pool.kv_heads + head) * tiles + tile) * p.splits * pitch;
-  const float *const maxima = base + (long long)kRows * D + r, *const totals = maxima + kRows;
-  const int set = threadIdx.x / (D / 4), d = (threadIdx.x % (D / 4)) * 4;
-  float most = -3.0e38f;
-  for (int s = threadIdx.x; s < p.splits; s += 256) most = fmaxf(most, maxima[s * pitch]);
-  most = wave_max_all(most);
-  if ((threadIdx.x & 63) == 0) largest[threadIdx.x >> 6] = most;
+  const float *const own = base + (long long)kRows * D + r;
+  // (a split a thread: there are no more than 256)
+  const bool mine = tid < p.splits;
+  const float max_here = mine ? own[tid * pitch] : -3.0e38f, sum_here = mine ? own[tid * pitch + kRows] : 0.f;
+  float most = wave_max_all(max_here);
+  if ((tid & 63) == 0) largest[tid >> 6] = most;
   __syncthreads();
   most = fmaxf(fmaxf(largest[0], largest[1]), fmaxf(largest[2], largest[3]));
+  const float weight = __builtin_amdgcn_exp2f(fmaxf(max_here - most, -126.0f));
+  if (mine) weights[tid] = weight;
+  const float sum = wave_sum_all(mine ? sum_here * weight : 0.f);
+  if ((tid & 63) == 0) totals_of[tid >> 6] = sum;
+  __syncthreads();
+  const float total = (totals_of[0] + totals_of[1]) + (totals_of[2] + totals_of[3]);
+  const int set = tid / (D / 4), d = (tid % (D / 4)) * 4;
   floatx4 x = {0.f, 0.f, 0.f, 0.f};
-  float total = 0.f;
-  for (int s = set; s < p.splits; s += kSets) {
-    const float w = __builtin_amdgcn_exp2f(fmaxf(maxima[s * pitch] - most, -126.0f));
-    total += totals[s * pitch] * w;
-    x += *reinterpret_cast<const floatx4 *>(base + s * pitch + (long long)r * D + d) * w;
-  }
+#pragma unroll 8
+  for (int s = set; s < p.splits; s += kSets) x += *reinterpret_cast<const floatx4 *>(base + s * pitch + (long long)r * D + d) * weights[s];
   *reinterpret_cast<floatx4 *>(&part[set][d]) = x;
-  if (d == 0) weight_sum[set] = total;
   __syncthreads();
   if (set != 0) return;
-  for (int i = 1; i < kSets; ++i) {
-    x += *reinterpret_cast<const floatx4 *>(&part[i][d]);
-    total += weight_sum[i];
-  }
-  // (total of set 0 is in its first thread's registers only as its own share: all of them hold the same)
+  for (int i = 1; i < kSets; ++i) x += *reinterpret_cast<const floatx4 *>(&part[i][d]);
   const float inv = total > 0.f || total != total ? 1.0f / total : 0.f;
   const int i = row / group, h = head * group + row % group;
   uint16_t *const to = p.out + (long long)seq * p.out_seq + (long long)i * p.out_row + (long long)h * p.out_head + d;
   *reinterpret_cast<uintx2 *>(to) = uintx2{T::pack(x[0] * inv, x[1] * inv), T::pack(x[2] * inv, x[3] * inv)};
 }
 
-int row_tiles(int queries, int group) { return queries * group > 16 ? 2 : 1; }
+// Rows of the largest tiles, workgroups for the rows and heads, waves of one, and shares of the keys.
+struct Shape {
+  int row_tiles, tiles, waves, splits;
+};
+Shape shape_of(int sequences, int queries, int heads, int kv_heads, long long longest) {
+  Shape s;
+  const int rows = queries * (heads / kv_heads);
+  s.row_tiles = rows > 16 ? 2 : 1;
+  s.tiles = (rows + 16 * s.row_tiles - 1) / (16 * s.row_tiles);
+  const long long wide = (long long)sequences * kv_heads * s.tiles;
+  const bool whole = wide >= 128 || longest <= 2048;
+  s.waves = whole ? 8 : 4;
+  s.splits = whole ? 1 : (int)max(1ll, min(min((256 + wide - 1) / wide, (longest + 511) / 512), (long long)kMostSplits));
+  return s;
+}
+
+template <typename T, int FORMAT, int D, int TILES, int UNIT>
+void launch(const CacheAttentionArgs &a, const Shape &s, const dim3 &grid, hipStream_t stream) {
+  if (s.waves == 8) hipLaunchKernelGGL((cache_attention_kernel<T, FORMAT, D, TILES, UNIT, 8>), grid, dim3(512), 0, stream, a);
+  else hipLaunchKernelGGL((cache_attention_kernel<T, FORMAT, D, TILES, UNIT, 4>), grid, dim3(256), 0, stream, a);
+}
 
 template <typename T, int FORMAT, int D>
-hipError_t launch(const CacheAttentionArgs &a, hipStream_t stream) {
-  const int group = a.heads / a.pool.kv_heads, rows = a.queries * group, two = row_tiles(a.queries, group);
-  const int tiles = (rows + 16 * two - 1) / (16 * two);
-  const dim3 grid(a.splits, a.pool.kv_heads * tiles, a.sequences), threads(64 * kWaves);
+hipError_t launch(const CacheAttentionArgs &a, const Shape &s, hipStream_t stream) {
+  const dim3 grid(a.splits, a.pool.kv_heads * s.tiles, a.sequences);
   if (a.pool.page_size == 32) {
-    if (two == 1) hipLaunchKernelGGL((cache_attention_kernel<T, FORMAT, D, 1, 32>), grid, threads, 0, stream, a);
-    else hipLaunchKernelGGL((cache_attention_kernel<T, FORMAT, D, 2, 32>), grid, threads, 0, stream, a);
+    if (s.row_tiles == 1) launch<T, FORMAT, D, 1, 32>(a, s, grid, stream);
+    else launch<T, FORMAT, D, 2, 32>(a, s, grid, stream);
   } else {
-    if (two == 1) hipLaunchKernelGGL((cache_attention_kernel<T, FORMAT, D, 1, 64>), grid, threads, 0, stream, a);
-    else hipLaunchKernelGGL((cache_attention_kernel<T, FORMAT, D, 2, 64>), grid, threads, 0, stream, a);
+    if (s.row_tiles == 1) launch<T, FORMAT, D, 1, 64>(a, s, grid, stream);
+    else launch<T, FORMAT, D, 2, 64>(a, s, grid, stream);
   }
   if (a.splits > 1)
-    hipLaunchKernelGGL((cache_attention_join_kernel<T, D>), dim3(rows, a.pool.kv_heads, a.sequences), dim3(256), 0, stream, a, two);
+    hipLaunchKernelGGL((cache_attention_join_kernel<T, D>), dim3(a.queries * (a.heads / a.pool.kv_heads), a.pool.kv_heads, a.sequences), dim3(256), 0, stream, a,
+                       s.row_tiles);
   return hipGetLastError();
 }
 
 template <typename T, int FORMAT>
-hipError_t launch(const CacheAttentionArgs &a, hipStream_t stream) {
-  return a.pool.d == 128 ? launch<T, FORMAT, 128>(a, stream) : a.pool.d == 64 ? launch<T, FORMAT, 64>(a, stream) : launch<T, FORMAT, 32>(a, stream);
+hipError_t launch(const CacheAttentionArgs &a, const Shape &s, hipStream_t stream) {
+  return a.pool.d == 128 ? launch<T, FORMAT, 128>(a, s, stream) : a.pool.d == 64 ? launch<T, FORMAT, 64>(a, s, stream) : launch<T, FORMAT, 32>(a, s, stream);
 }
 
 }  // namespace
 
-int cache_attention_splits(int sequences, int queries, int heads, int kv_heads, int d, long long longest) {
-  const int group = heads / kv_heads, rows = queries * group, two = row_tiles(queries, group), tiles = (rows + 16 * two - 1) / (16 * two);
-  const long long wide = (long long)sequences * kv_heads * tiles;
-  const long long wanted = (1024 + wide - 1) / wide, most = (longest + 255) / 256;
-  return (int)max(1ll, min(min(wanted, most), 256ll));
+size_t cache_attention_workspace(int sequences, int queries, int heads, int kv_heads, int d, long long longest) {
+  const Shape s = shape_of(sequences, queries, heads, kv_heads, longest);
+  return s.splits <= 1 ? 0 : (size_t)sequences * kv_heads * s.tiles * s.splits * (size_t)(16 * s.row_tiles) * (d + 2);
 }
 
-size_t cache_attention_workspace(int sequences, int queries, int heads, int kv_heads, int d, int splits) {
-  if (splits <= 1) return 0;
-  const int group = heads / kv_heads, rows = queries * group, two = row_tiles(queries, group), tiles = (rows + 16 * two - 1) / (16 * two);
-  return (size_t)sequences * kv_heads * tiles * splits * (size_t)(16 * two) * (d + 2);
-}
-
-hipError_t launch_cache_attention(int type, int format, const CacheAttentionArgs &a, hipStream_t stream) {
-  if (type == 0) return format == 0 ? launch<Fp16, 0>(a, stream) : launch<Fp16, 1>(a, stream);
-  return format == 0 ? launch<Bf16, 0>(a, stream) : launch<Bf16, 1>(a, stream);
+hipError_t launch_cache_attention(int type, int format, CacheAttentionArgs a, hipStream_t stream) {
+  const Shape s = shape_of(a.sequences, a.queries, a.heads, a.pool.kv_heads, (long long)a.pool.slots * a.pool.page_size);
+  a.splits = s.splits;
+  if (type == 0) return format == 0 ? launch<Fp16, 0>(a, s, stream) : launch<Fp16, 1>(a, s, stream);
+  return format == 0 ? launch<Bf16, 0>(a, s, stream) : launch<Bf16, 1>(a, s, stream);
 }
 
 }  // namespace sspmm

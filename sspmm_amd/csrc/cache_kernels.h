@@ -35,13 +35,14 @@ struct CacheAttentionArgs {
   uint16_t *out;
   long long q_seq, q_row, q_head, out_seq, out_row, out_head;
   const int32_t *lengths;
-  int sequences, queries, heads, splits;
+  int sequences, queries, heads;
   float scale_log2e;
-  float *partial;  // splits > 1: cache_attention_workspace floats
+  float *partial;  // cache_attention_workspace floats
+  int splits;      // (the launch's own)
 };
-int cache_attention_splits(int sequences, int queries, int heads, int kv_heads, int d, long long longest);
-size_t cache_attention_workspace(int sequences, int queries, int heads, int kv_heads, int d, int splits);  // floats
-hipError_t launch_cache_attention(int type, int format, const CacheAttentionArgs &args, hipStream_t stream);
+// longest: positions that a row of the table has room for
+size_t cache_attention_workspace(int sequences, int queries, int heads, int kv_heads, int d, long long longest);  // floats
+hipError_t launch_cache_attention(int type, int format, CacheAttentionArgs args, hipStream_t stream);
 
 }  // namespace sspmm
 #endif

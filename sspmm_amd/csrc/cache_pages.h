@@ -21,7 +21,9 @@ struct PagePool {
   int scale_floats;
 };
 
-size_t page_workspace_ints(int pages, int rows, long long slots, int named);
+size_t reserve_workspace_ints(int pages, int rows, int slots);  // 0: none wanted
+size_t fork_workspace_ints(int rows, int count);
+size_t compact_workspace_ints(int pages);
 
 hipError_t launch_reserve_pages(const PageTable &t, const int32_t *starts, const int32_t *offsets, int page_size, int32_t *workspace, hipStream_t stream);
 hipError_t launch_release_pages(const PageTable &t, int32_t *lengths, const int32_t *named, int count, hipStream_t stream);

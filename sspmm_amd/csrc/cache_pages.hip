@@ -10,6 +10,7 @@ namespace sspmm {
 namespace {
 
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
+constexpr size_t kPlanLds = 15 * 1024;  // integers of a plan that stay in LDS
 
 // Sum of v over the threads before this one, and over all of them.  Two barriers; `share` holds kPlanWaves values.
 __device__ __forceinline__ uint32_t block_exclusive_sum(uint32_t v, uint32_t *share, uint32_t *all) {
@@ -70,11 +71,13 @@ __device__ __forceinline__ void new_slots(const int32_t *starts, const int32_t *
 }
 
 // One workgroup: a wave counts a row's slots without a page, ranks follow in the order of rows and slots, the list of free pages is made, and
-// the slots take theirs.  workspace: rows + 1 ranks, then the list.
+// the slots take theirs.  workspace: the ranks, then the list; null: in LDS.
 __global__ __launch_bounds__(kPlanThreads) void reserve_pages_kernel(const PageTable t, const int32_t *starts, const int32_t *offsets, int page_size,
                                                                      int32_t *workspace) {
   __shared__ uint32_t share[kPlanWaves];
+  extern __shared__ int32_t plan_lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (!workspace) workspace = plan_lds;
   uint32_t *const ranks = reinterpret_cast<uint32_t *>(workspace);
   int32_t *const list = workspace + t.rows;
   for (int b = wave; b < t.rows; b += kPlanWaves) {
@@ -233,35 +236,48 @@ __global__ __launch_bounds__(kPlanThreads) void compact_count_kernel(const int32
 }
 
 // With U pages in use, those at U and behind move, in their order, to the free ones below U, in theirs.  rank_of[p] = its place among the
-// movers (-1: it stays), hole[i] / mover[i] = the i-th of either, counts[chunks] = how many.
-__global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(const int32_t *refs, int pages, int32_t *counts, int chunks, int32_t *rank_of, int32_t *hole,
-                                                                    int32_t *mover) {
+// movers (-1: it stays), hole[i] / mover[i] = the i-th of either, counts[chunks] = how many.  counted: counts[] are there.
+__global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(const int32_t *refs, int pages, int32_t *counts, int chunks, bool counted,
+                                                                    int32_t *rank_of, int32_t *hole, int32_t *mover) {
   __shared__ uint32_t share[kPlanWaves];
   const int tid = threadIdx.x;
-  uint32_t in_use = 0, mine = 0;  // of all chunks; of those before this one
-  for (int i0 = 0; i0 < chunks; i0 += kPlanThreads) {
-    const int i = i0 + tid;
-    const uint32_t v = i < chunks ? (uint32_t)counts[i] : 0u;
-    uint32_t all, part;
-    block_exclusive_sum(v, share, &all);
-    block_exclusive_sum(i < (int)blockIdx.x ? v : 0u, share, &part);
-    in_use += all;
-    mine += part;
-  }
-  // pages in use below U: those of the chunks before U's, and U's own chunk up to it
-  const int boundary = (int)in_use, its = boundary / kChunk;
-  uint32_t below = 0;
-  for (int i0 = 0; i0 < chunks; i0 += kPlanThreads) {
-    const int i = i0 + tid;
-    uint32_t all;
-    block_exclusive_sum(i < its && i < chunks ? (uint32_t)counts[i] : 0u, share, &all);
-    below += all;
-  }
-  {
+  uint32_t in_use = 0, mine = 0, below = 0;  // pages in use: all of them, in the chunks before this one, below U
+  int boundary;
+  if (counted) {
+    for (int i0 = 0; i0 < chunks; i0 += kPlanThreads) {
+      const int i = i0 + tid;
+      const uint32_t v = i < chunks ? (uint32_t)counts[i] : 0u;
+      uint32_t all, part;
+      block_exclusive_sum(v, share, &all);
+      block_exclusive_sum(i < (int)blockIdx.x ? v : 0u, share, &part);
+      in_use += all;
+      mine += part;
+    }
+    boundary = (int)in_use;
+    const int its = boundary / kChunk;  // the chunk that U lies in: those before it, and its own pages up to U
+    for (int i0 = 0; i0 < chunks; i0 += kPlanThreads) {
+      const int i = i0 + tid;
+      uint32_t all;
+      block_exclusive_sum(i < its && i < chunks ? (uint32_t)counts[i] : 0u, share, &all);
+      below += all;
+    }
     uint32_t used = 0, all;
     for (int p = its * kChunk + tid; p < min(boundary, pages); p += kPlanThreads) used += refs[p] > 0;
     block_exclusive_sum(used, share, &all);
     below += all;
+  } else {
+    uint32_t used = 0, before = 0;
+    for (int p = tid; p < pages; p += kPlanThreads) {
+      const bool is = refs[p] > 0;
+      used += is;
+      before += is && p < (int)blockIdx.x * kChunk;
+    }
+    block_exclusive_sum(used, share, &in_use);
+    block_exclusive_sum(before, share, &mine);
+    boundary = (int)in_use;
+    used = 0;
+    for (int p = tid; p < boundary; p += kPlanThreads) used += refs[p] > 0;
+    block_exclusive_sum(used, share, &below);
   }
   if (blockIdx.x == 0 && tid == 0) counts[chunks] = boundary - (int)below;
   uint32_t before = mine;
@@ -305,15 +321,21 @@ __global__ __launch_bounds__(256) void compact_move_kernel(const PageTable t, co
 
 }  // namespace
 
-size_t page_workspace_ints(int pages, int rows, long long slots, int named) {
-  // reserve: a rank a row and the pages taken; fork: a mark a row, the pages taken, what becomes of each child; compact: four lists
-  const size_t chunks = ((size_t)pages + kChunk - 1) / kChunk;
-  const size_t reserve = (size_t)rows + (size_t)min((long long)pages, (long long)rows * slots), fork = (size_t)rows + 6ull * named;
-  return max(max(reserve, fork), chunks + 1 + 3ull * pages) + 4;
+// a rank a row, and the pages taken
+static size_t reserve_ints(int pages, int rows, int slots) { return (size_t)rows + (size_t)min((long long)pages, (long long)rows * slots); }
+size_t reserve_workspace_ints(int pages, int rows, int slots) {
+  const size_t n = reserve_ints(pages, rows, slots);
+  return n <= kPlanLds ? 0 : n;
 }
+// a mark a row, the pages taken, what becomes of each child
+size_t fork_workspace_ints(int rows, int count) { return (size_t)rows + (size_t)count * (1 + sizeof(Fork) / 4); }
+// the chunks' counts and the moves', and three lists
+size_t compact_workspace_ints(int pages) { return ((size_t)pages + kChunk - 1) / kChunk + 1 + 3 * (size_t)pages; }
 
 hipError_t launch_reserve_pages(const PageTable &t, const int32_t *starts, const int32_t *offsets, int page_size, int32_t *workspace, hipStream_t stream) {
-  hipLaunchKernelGGL(reserve_pages_kernel, dim3(1), dim3(kPlanThreads), 0, stream, t, starts, offsets, page_size, workspace);
+  const size_t ints = reserve_ints(t.pages, t.rows, t.slots);
+  const bool inside = ints <= kPlanLds;
+  hipLaunchKernelGGL(reserve_pages_kernel, dim3(1), dim3(kPlanThreads), inside ? ints * 4 : 0, stream, t, starts, offsets, page_size, inside ? nullptr : workspace);
   return hipGetLastError();
 }
 
@@ -333,8 +355,10 @@ hipError_t launch_fork_pages(const PageTable &t, const PagePool &pool, int32_t *
 hipError_t launch_compact_pages(const PageTable &t, const PagePool &pool, int32_t *workspace, hipStream_t stream) {
   const int chunks = (t.pages + kChunk - 1) / kChunk;
   int32_t *const counts = workspace, *const rank_of = counts + chunks + 1, *const hole = rank_of + t.pages, *const mover = hole + t.pages;
-  hipLaunchKernelGGL(compact_count_kernel, dim3(chunks), dim3(kPlanThreads), 0, stream, t.refs, t.pages, counts);
-  hipLaunchKernelGGL(compact_plan_kernel, dim3(chunks), dim3(kPlanThreads), 0, stream, t.refs, t.pages, counts, chunks, rank_of, hole, mover);
+  // (a few chunks are counted by the plan itself, in each of its workgroups: a launch less)
+  const bool counted = chunks > 4;
+  if (counted) hipLaunchKernelGGL(compact_count_kernel, dim3(chunks), dim3(kPlanThreads), 0, stream, t.refs, t.pages, counts);
+  hipLaunchKernelGGL(compact_plan_kernel, dim3(chunks), dim3(kPlanThreads), 0, stream, t.refs, t.pages, counts, chunks, counted, rank_of, hole, mover);
   const int parts = (int)max(1ll, min(pool.block_bytes / 16384, 16ll));
   const unsigned grid = (unsigned)max(1ll, min(2048ll, (long long)t.pages * parts));
   hipLaunchKernelGGL(compact_move_kernel, dim3(grid), dim3(256), 0, stream, t, pool, counts + chunks, rank_of, hole, mover, parts);

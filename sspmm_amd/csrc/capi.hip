@@ -78,6 +78,7 @@ bool pool_fits(int pages, int kv_heads, int page_size, int head_dim, const void 
          (head_dim == 32 || head_dim == 64 || head_dim == 128) && keys && values && scales && reinterpret_cast<uintptr_t>(keys) % 16 == 0 &&
          reinterpret_cast<uintptr_t>(values) % 16 == 0 && reinterpret_cast<uintptr_t>(scales) % 4 == 0;
 }
+bool workspace_fits(const void *p, size_t bytes, size_t need) { return p && bytes >= need && reinterpret_cast<uintptr_t>(p) % 4 == 0; }
 bool table_fits(const void *refs, int pages, const void *table, int rows, int slots) {
   return refs && table && pages >= 1 && pages <= (1 << 30) && rows >= 1 && slots >= 1 && (int64_t)rows * slots < (1ll << 31);
 }
@@ -850,8 +851,7 @@ int sspmm_cache_write(int type, int format, int sequences, int tokens, const int
 
 size_t sspmm_cache_attention_workspace_bytes(int sequences, int queries, int heads, int kv_heads, int head_dim, int slots, int page_size) {
   if (sequences <= 0 || queries <= 0 || slots < 0 || page_size <= 0 || !heads_fit(heads, kv_heads, head_dim)) return 0;
-  const int splits = sspmm::cache_attention_splits(sequences, queries, heads, kv_heads, head_dim, (long long)slots * page_size);
-  return 4 * sspmm::cache_attention_workspace(sequences, queries, heads, kv_heads, head_dim, splits);
+  return 4 * sspmm::cache_attention_workspace(sequences, queries, heads, kv_heads, head_dim, (long long)slots * page_size);
 }
 
 int sspmm_cache_attention(int type, int format, int sequences, int queries, int heads, const sspmm_half_t *q, int64_t q_seq,
@@ -881,24 +881,25 @@ int sspmm_cache_attention(int type, int format, int sequences, int queries, int 
   a.sequences = sequences;
   a.queries = queries;
   a.heads = heads;
-  a.splits = sspmm::cache_attention_splits(sequences, queries, heads, kv_heads, head_dim, (long long)slots * page_size);
   a.scale_log2e = scale * 1.4426950408889634f;
   a.partial = static_cast<float *>(workspace);
-  const size_t need = 4 * sspmm::cache_attention_workspace(sequences, queries, heads, kv_heads, head_dim, a.splits);
+  const size_t need = 4 * sspmm::cache_attention_workspace(sequences, queries, heads, kv_heads, head_dim, (long long)slots * page_size);
   if (workspace_bytes < need || (need > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16))) return kInvalid;
   return (int)sspmm::launch_cache_attention(type, format, a, static_cast<hipStream_t>(hip_stream));
 }
 
-size_t sspmm_page_workspace_bytes(int pages, int rows, int slots, int count) {
-  if (pages < 1 || rows < 1 || slots < 1 || count < 0) return 0;
-  return 4 * sspmm::page_workspace_ints(pages, rows, slots, count);
+size_t sspmm_reserve_pages_workspace_bytes(int pages, int rows, int slots) {
+  return pages < 1 || rows < 1 || slots < 1 ? 0 : 4 * sspmm::reserve_workspace_ints(pages, rows, slots);
 }
+size_t sspmm_fork_pages_workspace_bytes(int rows, int count) { return rows < 1 || count < 1 ? 0 : 4 * sspmm::fork_workspace_ints(rows, count); }
+size_t sspmm_compact_pages_workspace_bytes(int pages) { return pages < 1 ? 0 : 4 * sspmm::compact_workspace_ints(pages); }
 
 int sspmm_reserve_pages(int32_t *page_refs, int pages, int32_t *page_table, int rows, int slots, const int32_t *starts,
                         const int32_t *offsets, int page_size, void *workspace, size_t workspace_bytes, void *hip_stream) {
   if (rows == 0 || slots == 0) return 0;
   if (!table_fits(page_refs, pages, page_table, rows, slots) || !starts || !offsets || page_size < 1) return kInvalid;
-  if (!workspace || workspace_bytes < sspmm_page_workspace_bytes(pages, rows, slots, 0)) return kInvalid;
+  const size_t need = sspmm_reserve_pages_workspace_bytes(pages, rows, slots);
+  if (need > 0 && !workspace_fits(workspace, workspace_bytes, need)) return kInvalid;
   return (int)sspmm::launch_reserve_pages({page_refs, page_table, pages, rows, slots}, starts, offsets, page_size, static_cast<int32_t *>(workspace),
                                           static_cast<hipStream_t>(hip_stream));
 }
@@ -918,7 +919,7 @@ int sspmm_fork_pages(int32_t *page_refs, int pages, int32_t *page_table, int row
   if (count == 0 || rows == 0 || slots == 0) return 0;
   if (!table_fits(page_refs, pages, page_table, rows, slots) || !lengths || !parents || !children) return kInvalid;
   if (!pool_fits(pages, kv_heads, page_size, head_dim, keys, values, scales)) return kInvalid;
-  if (!workspace || workspace_bytes < sspmm_page_workspace_bytes(pages, rows, slots, count)) return kInvalid;
+  if (!workspace_fits(workspace, workspace_bytes, sspmm_fork_pages_workspace_bytes(rows, count))) return kInvalid;
   const sspmm::PagePool pool = {static_cast<unsigned char *>(keys), static_cast<unsigned char *>(values), scales, (long long)kv_heads * page_size * head_dim,
                                 2 * kv_heads};
   return (int)sspmm::launch_fork_pages({page_refs, page_table, pages, rows, slots}, pool, lengths, parents, children, count, page_size,
@@ -930,7 +931,7 @@ int sspmm_compact_pages(int32_t *page_refs, int pages, int32_t *page_table, int 
   if (rows == 0 || slots == 0) return 0;
   if (!table_fits(page_refs, pages, page_table, rows, slots)) return kInvalid;
   if (!pool_fits(pages, kv_heads, page_size, head_dim, keys, values, scales)) return kInvalid;
-  if (!workspace || workspace_bytes < sspmm_page_workspace_bytes(pages, rows, slots, 0)) return kInvalid;
+  if (!workspace_fits(workspace, workspace_bytes, sspmm_compact_pages_workspace_bytes(pages))) return kInvalid;
   const sspmm::PagePool pool = {static_cast<unsigned char *>(keys), static_cast<unsigned char *>(values), scales, (long long)kv_heads * page_size * head_dim,
                                 2 * kv_heads};
   return (int)sspmm::launch_compact_pages({page_refs, page_table, pages, rows, slots}, pool, static_cast<int32_t *>(workspace), static_cast<hipStream_t>(hip_stream));

@@ -163,7 +163,7 @@ def test_running_out_of_pages(built_library):
 
 
 def test_every_page_of_a_large_pool_and_none(built_library):
-    for pages in (1, 4096, 8192, 12289):
+    for pages in (1, 4096, 8192, 12289, 16385, 20480):
         model, dev = Model(pages, 3, pages + 1, 32), Device(pages, 3, pages + 1, 32, kv=1)
         model.compact()
         sspmm_amd.compact_pages(dev.refs, dev.table, *dev.cache)

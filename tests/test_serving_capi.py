@@ -61,20 +61,21 @@ def test_cache_attention(L):
 
 
 def test_pages(L):
-    need = L.sspmm_page_workspace_bytes(100, 4, 8, 3)
-    assert need >= 4 * 100 and L.sspmm_page_workspace_bytes(0, 4, 8, 3) == 0 and L.sspmm_page_workspace_bytes(100, 4, 8, -1) == 0
+    many, need, lists = L.sspmm_reserve_pages_workspace_bytes(100000, 40, 800), L.sspmm_fork_pages_workspace_bytes(4, 3), L.sspmm_compact_pages_workspace_bytes(100)
+    assert L.sspmm_reserve_pages_workspace_bytes(100, 4, 8) == 0 and many == 4 * (40 + 32000) and need > 0 and lists > 1200
+    assert L.sspmm_reserve_pages_workspace_bytes(0, 4, 8) == 0 and L.sspmm_fork_pages_workspace_bytes(4, 0) == 0 and L.sspmm_compact_pages_workspace_bytes(-1) == 0
     # refs pages table rows slots ...
-    reserve = _changed([A, 100, A, 4, 8, A, A, 32, A, need, None], L.sspmm_reserve_pages)
-    for i, v in ((0, None), (1, 0), (2, None), (3, -1), (4, -1), (4, 1 << 30), (5, None), (6, None), (7, 0), (8, None), (9, 16)):
+    reserve = _changed([A, 100000, A, 40, 800, A, A, 32, A, many, None], L.sspmm_reserve_pages)
+    for i, v in ((0, None), (1, 0), (2, None), (3, -1), (4, -1), (4, 1 << 30), (5, None), (6, None), (7, 0), (8, None), (8, A + 2), (9, many - 1)):
         assert reserve((i, v)) == 1, (i, v)
     release = _changed([A, 100, A, 4, 8, A, A, 2, None], L.sspmm_release_pages)
     for i, v in ((0, None), (1, -1), (2, None), (5, None), (6, None), (7, -1)):
         assert release((i, v)) == 1, (i, v)
     fork = _changed([A, 100, A, 4, 8, A, A, A, 3, 2, 32, 64, A, A, A, A, need, None], L.sspmm_fork_pages)
-    for i, v in ((0, None), (2, None), (5, None), (6, None), (7, None), (8, -1), (9, 0), (10, 33), (11, 16), (12, None), (13, A + 1), (14, None), (15, None), (16, need - 4 * 150)):
+    for i, v in ((0, None), (2, None), (5, None), (6, None), (7, None), (8, -1), (9, 0), (10, 33), (11, 16), (12, None), (13, A + 1), (14, None), (15, None), (15, A + 1), (16, need - 1)):
         assert fork((i, v)) == 1, (i, v)
-    compact = _changed([A, 100, A, 4, 8, 2, 32, 64, A, A, A, A, need, None], L.sspmm_compact_pages)
-    for i, v in ((0, None), (1, 0), (2, None), (5, 0), (6, 0), (7, 33), (8, None), (9, None), (10, None), (11, None), (12, 8)):
+    compact = _changed([A, 100, A, 4, 8, 2, 32, 64, A, A, A, A, lists, None], L.sspmm_compact_pages)
+    for i, v in ((0, None), (1, 0), (2, None), (5, 0), (6, 0), (7, 33), (8, None), (9, None), (10, None), (11, None), (12, lists - 1)):
         assert compact((i, v)) == 1, (i, v)
     assert reserve((3, 0)) == 0 and release((7, 0)) == 0 and fork((8, 0)) == 0 and compact((4, 0)) == 0
 
