@@ -221,13 +221,13 @@ __global__ __launch_bounds__(256) void fork_copy_kernel(const PageTable t, const
   }
 }
 
-constexpr int kChunk = 4096;  // pages whose counts a workgroup of the compaction looks at
+constexpr int kPer = 4, kChunk = kPer * kPlanThreads;  // pages that a thread and a workgroup of the compaction look at
 
 __global__ __launch_bounds__(kPlanThreads) void compact_count_kernel(const int32_t *refs, int pages, int32_t *counts) {
   __shared__ uint32_t share[kPlanWaves];
   uint32_t used = 0, all;
 #pragma unroll
-  for (int i = 0; i < kChunk / kPlanThreads; ++i) {
+  for (int i = 0; i < kPer; ++i) {
     const int p = blockIdx.x * kChunk + i * kPlanThreads + threadIdx.x;
     used += p < pages && refs[p] > 0;
   }
@@ -240,10 +240,26 @@ __global__ __launch_bounds__(kPlanThreads) void compact_count_kernel(const int32
 __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(const int32_t *refs, int pages, int32_t *counts, int chunks, bool counted,
                                                                     int32_t *rank_of, int32_t *hole, int32_t *mover) {
   __shared__ uint32_t share[kPlanWaves];
-  const int tid = threadIdx.x;
-  uint32_t in_use = 0, mine = 0, below = 0;  // pages in use: all of them, in the chunks before this one, below U
+  const int tid = threadIdx.x, p0 = blockIdx.x * kChunk + tid * kPer;
+  bool used[kPer];
+  uint32_t count = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    used[i] = p0 + i < pages && refs[p0 + i] > 0;
+    count += used[i];
+  }
+  uint32_t in_chunk;
+  uint32_t ahead = block_exclusive_sum(count, share, &in_chunk);  // pages in use before the thread's, for now of the chunk
+  uint32_t in_use = 0, before = 0, below = 0;  // pages in use: all of them, in the chunks before this one, below U
   int boundary;
-  if (counted) {
+  if (chunks == 1) {
+    in_use = in_chunk;
+    boundary = (int)in_use;
+    uint32_t n = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) n += used[i] && p0 + i < boundary;
+    block_exclusive_sum(n, share, &below);
+  } else if (counted) {
     for (int i0 = 0; i0 < chunks; i0 += kPlanThreads) {
       const int i = i0 + tid;
       const uint32_t v = i < chunks ? (uint32_t)counts[i] : 0u;
@@ -251,7 +267,7 @@ __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(const int32_
       block_exclusive_sum(v, share, &all);
       block_exclusive_sum(i < (int)blockIdx.x ? v : 0u, share, &part);
       in_use += all;
-      mine += part;
+      before += part;
     }
     boundary = (int)in_use;
     const int its = boundary / kChunk;  // the chunk that U lies in: those before it, and its own pages up to U
@@ -261,41 +277,39 @@ __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(const int32_
       block_exclusive_sum(i < its && i < chunks ? (uint32_t)counts[i] : 0u, share, &all);
       below += all;
     }
-    uint32_t used = 0, all;
-    for (int p = its * kChunk + tid; p < min(boundary, pages); p += kPlanThreads) used += refs[p] > 0;
-    block_exclusive_sum(used, share, &all);
+    uint32_t n = 0, all;
+    for (int p = its * kChunk + tid; p < min(boundary, pages); p += kPlanThreads) n += refs[p] > 0;
+    block_exclusive_sum(n, share, &all);
     below += all;
   } else {
-    uint32_t used = 0, before = 0;
+    uint32_t n = 0, m = 0;
     for (int p = tid; p < pages; p += kPlanThreads) {
       const bool is = refs[p] > 0;
-      used += is;
-      before += is && p < (int)blockIdx.x * kChunk;
+      n += is;
+      m += is && p < (int)blockIdx.x * kChunk;
     }
-    block_exclusive_sum(used, share, &in_use);
-    block_exclusive_sum(before, share, &mine);
+    block_exclusive_sum(n, share, &in_use);
+    block_exclusive_sum(m, share, &before);
     boundary = (int)in_use;
-    used = 0;
-    for (int p = tid; p < boundary; p += kPlanThreads) used += refs[p] > 0;
-    block_exclusive_sum(used, share, &below);
+    n = 0;
+    for (int p = tid; p < boundary; p += kPlanThreads) n += refs[p] > 0;
+    block_exclusive_sum(n, share, &below);
   }
   if (blockIdx.x == 0 && tid == 0) counts[chunks] = boundary - (int)below;
-  uint32_t before = mine;
-  for (int i = 0; i < kChunk / kPlanThreads; ++i) {
-    const int p = blockIdx.x * kChunk + i * kPlanThreads + tid;
-    const bool used = p < pages && refs[p] > 0;
-    uint32_t all;
-    const uint32_t ahead = before + block_exclusive_sum(used ? 1u : 0u, share, &all);  // pages in use before p
-    before += all;
-    if (p >= pages) continue;
+  ahead += before;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int p = p0 + i;
+    if (p >= pages) break;
     int rank = -1;
-    if (used && p >= boundary) {
+    if (used[i] && p >= boundary) {
       rank = (int)(ahead - below);
       mover[rank] = p;
-    } else if (!used && p < boundary) {
+    } else if (!used[i] && p < boundary) {
       hole[p - (int)ahead] = p;
     }
     rank_of[p] = rank;
+    ahead += used[i];
   }
 }
 

@@ -53,15 +53,26 @@ __device__ __forceinline__ uint32_t rescaled(uint32_t c, float before, float now
   return codes<FORMAT>(x[0] * before, x[1] * before, x[2] * before, x[3] * before, now);
 }
 
-// A workgroup owns one block: the keys (blockIdx.z = 0) or values of one head in one page that gets new tokens.  Values lie transposed in the
-// page, so their codes pass through LDS.
+// Four words of four bytes, a token each, to a feature each.
+__device__ __forceinline__ void turn(uint32_t &a, uint32_t &b, uint32_t &c, uint32_t &d) {
+  // v_perm: selectors 0 .. 3 are bytes of the second operand, 4 .. 7 of the first
+  const uint32_t ab = __builtin_amdgcn_perm(b, a, 0x05010400u), ab2 = __builtin_amdgcn_perm(b, a, 0x07030602u);
+  const uint32_t cd = __builtin_amdgcn_perm(d, c, 0x05010400u), cd2 = __builtin_amdgcn_perm(d, c, 0x07030602u);
+  a = __builtin_amdgcn_perm(cd, ab, 0x05040100u);
+  b = __builtin_amdgcn_perm(cd, ab, 0x07060302u);
+  c = __builtin_amdgcn_perm(cd2, ab2, 0x05040100u);
+  d = __builtin_amdgcn_perm(cd2, ab2, 0x07060302u);
+}
+
+// A workgroup owns one block: the keys (blockIdx.z = 0) or values of one head in one page that gets new tokens.  A thread takes four places
+// of the page and eight features, side by side with threads of other features (keys) or other places (values, which lie transposed in the page), so that
+// either's stores are whole lines and nothing passes through LDS.
 template <typename T, int FORMAT, int D>
 __global__ __launch_bounds__(kThreads) void cache_write_kernel(const CacheWriteArgs p) {
-  constexpr int kPer = D / 8;  // pieces of eight elements of a token
-  constexpr int kMost = 128 * kPer / kThreads;  // of a thread, in the largest page
-  __shared__ __align__(16) unsigned char turned[D * 128];
+  constexpr int kPer = D / 8;  // threads for the features
+  constexpr int kMost = (128 / 4 * kPer + kThreads - 1) / kThreads;  // of a thread, in the largest page
   __shared__ uint32_t largest[kThreads / 64];
-  const int tid = threadIdx.x, lane = tid & 63, page_size = p.pool.page_size;
+  const int tid = threadIdx.x, lane = tid & 63, page_size = p.pool.page_size, quads = page_size / 4, items = quads * kPer;
   const int head = blockIdx.y, values = blockIdx.z;
 
   // ---- which page: the blockIdx.x-th of those that the sequences touch
@@ -98,89 +109,101 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(const CacheWriteA
   const int page = p.pool.table[(long long)row * p.pool.slots + slot];
   if (page < 0 || page >= p.pool.pages) return;
 
+  float *const scale_at = p.pool.scales + ((long long)page * 2 + values) * p.pool.kv_heads + head;
+  const float before = from > 0 ? *scale_at : 0.f;
+
   // ---- the new tokens, in registers
-  const uint16_t *const src = values ? p.v + token0 * p.v_row + (long long)head * p.v_head : p.k + token0 * p.k_row + (long long)head * p.k_head;
   const long long pitch = values ? p.v_row : p.k_row;
-  const int pieces = (upto - from) * kPer;
-  uintx4 x[kMost];
+  const uint16_t *const src = (values ? p.v + (long long)head * p.v_head : p.k + (long long)head * p.k_head) + (token0 - from) * pitch;  // place 0
+  const int bits = 31 - __builtin_clz(quads);
+  unsigned char *const block = (values ? p.pool.values : p.pool.keys) + ((long long)page * p.pool.kv_heads + head) * ((long long)page_size * D);
+  uintx4 x[kMost][4];
+  uint32_t old[kMost][8] = {};  // (values) words with both new places and others, as they are
   uint32_t most = 0;
 #pragma unroll
   for (int i = 0; i < kMost; ++i) {
     const int at = i * kThreads + tid;
-    x[i] = uintx4{0, 0, 0, 0};
-    if (at < pieces) x[i] = *reinterpret_cast<const uintx4 *>(src + (at / kPer) * pitch + (at % kPer) * 8);
+    const int quad = values ? at & (quads - 1) : at / kPer, octet = values ? at >> bits : at % kPer;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int place = 4 * quad + j;
+      x[i][j] = uintx4{0, 0, 0, 0};
+      if (at < items && place >= from && place < upto) x[i][j] = *reinterpret_cast<const uintx4 *>(src + place * pitch + 8 * octet);
+    }
+    if (values && at < items && 4 * quad < upto && 4 * quad + 4 > from && (4 * quad < from || 4 * quad + 4 > upto)) {
+#pragma unroll
+      for (int f = 0; f < 8; ++f) old[i][f] = *reinterpret_cast<const uint32_t *>(block + (8 * octet + f) * page_size + 4 * quad);
+    }
   }
 #pragma unroll
   for (int i = 0; i < kMost; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      // (bits of magnitudes order as the magnitudes do, infinities and NaN above all)
-      most = max(most, max(__float_as_uint(T::lower(x[i][j])) & 0x7fffffffu, __float_as_uint(T::upper(x[i][j])) & 0x7fffffffu));
-    }
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        // (bits of magnitudes order as the magnitudes do, infinities and NaN above all)
+        most = max(most, max(__float_as_uint(T::lower(x[i][j][w])) & 0x7fffffffu, __float_as_uint(T::upper(x[i][j][w])) & 0x7fffffffu));
+      }
   most = from_last_lane(wave_inclusive_max(most));
   if (lane == 0) largest[tid >> 6] = most;
-  __syncthreads();
+  __syncthreads();  // (behind it every wave has read the scale, too, that is about to be replaced)
 #pragma unroll
   for (int i = 0; i < kThreads / 64; ++i) most = max(most, largest[i]);
 
-  float *const scale_at = p.pool.scales + ((long long)page * 2 + values) * p.pool.kv_heads + head;
-  const float needed = scale_for<FORMAT>(most), before = from > 0 ? *scale_at : 0.f;
+  const float needed = scale_for<FORMAT>(most);
   const float scale = from > 0 ? larger_scale(before, needed) : needed;
   const bool grown = from > 0 && scale > before;  // (a NaN scale: what is there does not matter any more)
-  __syncthreads();  // (every wave has read the scale that is about to be replaced)
   if (tid == 0 && (from == 0 || scale != before)) *scale_at = scale;
 
-  unsigned char *const block = (values ? p.pool.values : p.pool.keys) + ((long long)page * p.pool.kv_heads + head) * ((long long)page_size * D);
-  if (!values) {
-    if (grown)
-      for (int at = tid; at < from * kPer; at += kThreads) {
-        uintx2 *const c = reinterpret_cast<uintx2 *>(block + at * 8);
-        const uintx2 old = *c;
-        *c = uintx2{rescaled<FORMAT>(old[0], before, scale), rescaled<FORMAT>(old[1], before, scale)};
-      }
-#pragma unroll
-    for (int i = 0; i < kMost; ++i) {
-      const int at = i * kThreads + tid;
-      if (at < pieces)
-        *reinterpret_cast<uintx2 *>(block + (from * kPer + at) * 8) =
-            uintx2{codes<FORMAT>(T::lower(x[i][0]), T::upper(x[i][0]), T::lower(x[i][1]), T::upper(x[i][1]), scale),
-                   codes<FORMAT>(T::lower(x[i][2]), T::upper(x[i][2]), T::lower(x[i][3]), T::upper(x[i][3]), scale)};
-    }
-    return;
-  }
 #pragma unroll
   for (int i = 0; i < kMost; ++i) {
     const int at = i * kThreads + tid;
-    if (at < pieces) {
-      const uint32_t a = codes<FORMAT>(T::lower(x[i][0]), T::upper(x[i][0]), T::lower(x[i][1]), T::upper(x[i][1]), scale);
-      const uint32_t b = codes<FORMAT>(T::lower(x[i][2]), T::upper(x[i][2]), T::lower(x[i][3]), T::upper(x[i][3]), scale);
-      unsigned char *const to = turned + (at % kPer) * 8 * page_size + from + at / kPer;
+    const int quad = values ? at & (quads - 1) : at / kPer, octet = values ? at >> bits : at % kPer, place = 4 * quad;
+    if (at >= items || place >= upto || (place + 4 <= from && !grown)) continue;
+    uint32_t c[4][2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      c[j][0] = c[j][1] = 0;
+      if (place + j < from || place + j >= upto) continue;  // (a division is a dozen instructions: a single token does one of four)
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+        c[j][w] = codes<FORMAT>(T::lower(x[i][j][2 * w]), T::upper(x[i][j][2 * w]), T::lower(x[i][j][2 * w + 1]), T::upper(x[i][j][2 * w + 1]), scale);
+    }
+    if (!values) {
+      uintx2 *to[4];
+      uintx2 kept[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        to[j * page_size] = (unsigned char)(a >> (8 * j));
-        to[(4 + j) * page_size] = (unsigned char)(b >> (8 * j));
+        to[j] = reinterpret_cast<uintx2 *>(block + (place + j) * D + 8 * octet);
+        kept[j] = grown && place + j < from ? *to[j] : uintx2{0, 0};
       }
-    }
-  }
-  __syncthreads();
-  const int words = page_size / 4;
-  for (int at = tid; at < D * words; at += kThreads) {
-    const int place = (at % words) * 4;
-    if (place >= upto || (place + 4 <= from && !grown)) continue;
-    uint32_t w = *reinterpret_cast<const uint32_t *>(turned + at * 4);
-    uint32_t *const to = reinterpret_cast<uint32_t *>(block + at * 4);
-    if (place < from || place + 4 > upto) {
-      uint32_t old = *to;
-      const uint32_t moved = grown ? rescaled<FORMAT>(old, before, scale) : old;
-      uint32_t r = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t m = 0xffu << (8 * j);
-        r |= (place + j < from ? moved : place + j < upto ? w : old) & m;
+        if (place + j >= from) {
+          if (place + j < upto) *to[j] = uintx2{c[j][0], c[j][1]};
+        } else if (grown) {
+          *to[j] = uintx2{rescaled<FORMAT>(kept[j][0], before, scale), rescaled<FORMAT>(kept[j][1], before, scale)};
+        }
       }
-      w = r;
+    } else {
+#pragma unroll
+      for (int w = 0; w < 2; ++w) turn(c[0][w], c[1][w], c[2][w], c[3][w]);  // c[j][w]: feature 4 w + j, a byte a place
+      if (place + 4 <= from) {  // (all of it kept, at a scale that has grown)
+#pragma unroll
+        for (int f = 0; f < 8; ++f) old[i][f] = *reinterpret_cast<const uint32_t *>(block + (8 * octet + f) * page_size + place);
+      }
+      uint32_t keep = 0, stale = 0;  // the bytes in front of the new places and behind them
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        keep |= place + j < from ? 0xffu << (8 * j) : 0u;
+        stale |= place + j >= upto ? 0xffu << (8 * j) : 0u;
+      }
+#pragma unroll
+      for (int f = 0; f < 8; ++f) {
+        const uint32_t moved = grown && keep != 0 ? rescaled<FORMAT>(old[i][f], before, scale) : old[i][f];
+        *reinterpret_cast<uint32_t *>(block + (8 * octet + f) * page_size + place) = (moved & keep) | (old[i][f] & stale) | (c[f % 4][f / 4] & ~(keep | stale));
+      }
     }
-    *to = w;
   }
 }
 
