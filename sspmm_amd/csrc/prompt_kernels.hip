@@ -13,6 +13,7 @@ namespace sspmm {
 namespace {
 
 constexpr int kKeys = 64;  // keys of a tile
+constexpr int kWaves = 4, kTileQueries = 32 * kWaves;  // of a group, and queries of a workgroup
 constexpr uint32_t kSrdWord3 = 0x00020000u;
 
 // A tile's row r is D elements in pieces of 16 bytes; piece c lies at place c ^ swizzle(r) of the row.  K's fragments are read by 32 lanes
@@ -65,33 +66,37 @@ __device__ __forceinline__ uintx4 finite_part(uintx4 v) {
 // inside the lane, but for one exchange with the lane 32 apart, and what the matrix instruction leaves is, rounded to 16 bits, the operand P^T
 // of the second product V^T P^T, whose contraction slots are numbered accordingly: slots of lane half h in step t are keys
 // 16 t + 4 h + {0 .. 3, 8 .. 11}.  V^T comes from transpose reads.
-template <typename T, int D, int WAVES, bool CAUSAL>
-__global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(const PromptArgs p, int tiles, int blocks) {
+template <typename T, int D, int WAVES, int GROUPS, bool CAUSAL>
+__global__ __launch_bounds__(64 * WAVES * GROUPS, 2) void prompt_attention_kernel(const PromptArgs p, int tiles) {
   constexpr int kQueries = 32 * WAVES, kPieces = D / 8, kTile = kKeys * D * 2;
   constexpr int kSteps = D / 16, kParts = D / 32;  // steps of the first product; parts of 32 features of the second
   constexpr int kLoads = kTile / (64 * WAVES * 16);  // pieces of 16 bytes of a tile that a thread fetches
-  __shared__ __align__(16) unsigned char lds[4 * kTile];  // K, V, K, V
+  __shared__ __align__(16) unsigned char tiles_lds[GROUPS * 4 * kTile];  // of each group K, V, K, V
+  __shared__ float states[GROUPS > 1 ? (GROUPS - 1) * WAVES * 2 * 64 : 1];
   const int lane = threadIdx.x & 63, n = lane & 31, half = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = GROUPS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * WAVES));
+  const int wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) % WAVES);
+  unsigned char *const lds = tiles_lds + group * 4 * kTile;
 
   // ---- which queries
   int tile, head;
   {
-    const int group = p.heads / p.kv_heads;
+    const int per_kv = p.heads / p.kv_heads;
     if (p.kv_heads % 8 == 0) {
       // Workgroup ids go round-robin to the 8 XCDs: a head of k and v stays with one of them and its L2.
-      const int xcd = blockIdx.x & 7, i = blockIdx.x >> 3, per = tiles * group;
+      const int xcd = blockIdx.x & 7, i = blockIdx.x >> 3, per = tiles * per_kv;
       const int kv = (i / per) * 8 + xcd, j = i % per;
-      tile = j / group;
-      head = kv * group + j % group;
+      tile = j / per_kv;
+      head = kv * per_kv + j % per_kv;
     } else {
       tile = blockIdx.x / p.heads;
       head = blockIdx.x % p.heads;
     }
   }
-  if ((int)blockIdx.x >= blocks) return;
+  // The tile-th of all sequences' tiles, those with the most keys first: of 64 sequences at a time, level x (a causal tile has about as many keys as
+  // places before it in its sequence, another as many as its sequence) is the largest at which more than `tile` tiles are of x or more.
   int first = 0, length = -1, q0 = 0;  // the sequence's first row and rows, the workgroup's first query in it
-  for (int b0 = 0, base = 0; b0 < p.sequences; b0 += 64) {
+  for (int b0 = 0, left = tile; b0 < p.sequences; b0 += 64) {
     const int b = b0 + lane;
     int lo = 0, hi = 0;
     if (b < p.sequences) {
@@ -99,17 +104,32 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(const P
       hi = max(lo, min(p.offsets[b + 1], p.tokens));
     }
     const int count = (int)(((long long)(hi - lo) + kQueries - 1) / kQueries);
-    const int upto = base + (int)wave_inclusive_sum((uint32_t)count);
-    const unsigned long long found = __ballot(upto > tile);
-    if (found != 0) {
-      const int at = __builtin_ctzll(found);
-      first = __builtin_amdgcn_readlane(lo, at);
-      length = __builtin_amdgcn_readlane(hi, at) - first;
-      // (the last queries first: with a causal mask these have the most keys)
-      q0 = (__builtin_amdgcn_readlane(upto, at) - 1 - tile) * kQueries;
-      break;
+    const int all = (int)from_last_lane(wave_inclusive_sum((uint32_t)count));
+    if (left >= all) {
+      left -= all;
+      continue;
     }
-    base = __builtin_amdgcn_readlane(upto, 63);
+    int x = 1, above = 0, end = (int)from_last_lane(wave_inclusive_max((uint32_t)count)) + 1;  // above: tiles of `end` or more
+    while (end - x > 1) {
+      const int mid = (x + end) >> 1;
+      const int n_mid = count < mid ? 0 : CAUSAL ? count - mid + 1 : count;
+      const int upwards = (int)from_last_lane(wave_inclusive_sum((uint32_t)n_mid));
+      if (upwards > left) {
+        x = mid;
+      } else {
+        end = mid;
+        above = upwards;
+      }
+    }
+    left -= above;  // which of level x
+    const unsigned long long those = __ballot(CAUSAL ? count >= x : count == x);
+    const int which = CAUSAL ? left : left / x;
+    const bool is = (those >> lane & 1) && __popcll(those & ((1ull << lane) - 1)) == which;
+    const int at = __builtin_ctzll(__ballot(is));
+    first = __builtin_amdgcn_readlane(lo, at);
+    length = __builtin_amdgcn_readlane(hi, at) - first;
+    q0 = (CAUSAL ? x - 1 : left % x) * kQueries;
+    break;
   }
   if (length < 0) return;  // (there are fewer tiles than the host could exclude)
 
@@ -144,7 +164,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(const P
     const int rows = min(kKeys, length - t * kKeys);
     const srd sk = descriptor(k0 + (long long)t * kKeys * p.k_row, (rows - 1) * k_pitch + D * 2);
     const srd sv = descriptor(v0 + (long long)t * kKeys * p.v_row, (rows - 1) * v_pitch + D * 2);
-    const uint32_t to = lds_at + (t & 1) * 2 * kTile;
+    const uint32_t to = lds_at + (t / GROUPS & 1) * 2 * kTile;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) load_to_lds(sk, k_at[i], to + i * WAVES * 1024);
 #pragma unroll
@@ -161,6 +181,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(const P
     v_rd[part] = kTile + r * (D * 2) + ((piece ^ swizzle_v<D>(r)) * 16) + (lane & 1) * 8;  // (8 rows on: the same swizzle)
   }
 
+  const bool ahead = D == 128 && key_tiles >= 64;
   floatx16 o[kParts];  // lane (n, half): features 32 part + 8 (i / 4) + 4 half + i % 4 of its query
 #pragma unroll
   for (int part = 0; part < kParts; ++part)
@@ -173,60 +194,68 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(const P
   const auto work_on = [&](auto cut_, const unsigned char *tile, int key0) {
     constexpr bool cut = decltype(cut_)::value;
     floatx16 s[2];
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+    uintx4 pt[4];
+    const auto scores = [&](int kt) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[kt][i] = 0.f;
 #pragma unroll
-    for (int step = 0; step < kSteps; ++step)
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+      for (int step = 0; step < kSteps; ++step)
         s[kt] = T::mfma_32x32x16(*reinterpret_cast<const uintx4 *>(tile + k_rd[step] + 32 * kt * (D * 2)), q[step], s[kt]);
-    if constexpr (cut) {
-      const int left = seen - key0 - 4 * half;
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[kt][i] = 32 * kt + 8 * (i / 4) + i % 4 >= left ? -INFINITY : s[kt][i];
-    }
-    float most_here = s[0][0];
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) most_here = fmaxf(most_here, s[kt][i]);
-    {
-      const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(most_here), __float_as_uint(most_here), false, false);
-      most_here = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
-    }
-    // The reference point moves only when some query's maximum has grown by more than 2^8: until then probabilities are up to 2^8
-    // too large, which either type holds, and the accumulators stay as they are.
-    const float new_max = fmaxf(run_max, most_here * c);
-    if (__ballot(new_max - run_max > 8.0f) != 0) {
-      const float alpha = __builtin_amdgcn_exp2f(fmaxf(run_max - new_max, -126.0f));
-      run_max = new_max;
-      run_sum *= alpha;
-#pragma unroll
-      for (int part = 0; part < kParts; ++part)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[part][i] *= alpha;
-    }
-    uintx4 pt[4];
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+    };
+    // The probabilities of 32 keys, by the reference point as it is.  That moves only when some query's maximum has grown by more than 2^8:
+    // until then probabilities are up to 2^8 too large, which either type holds, and the accumulators stay as they are.
+    float most_here = 0.f, sum = 0.f;
+    const auto exponentials = [&](int kt) {
+      sum = 0.f;
 #pragma unroll
       for (int i = 0; i < 16; i += 2) {
         const float a = __builtin_amdgcn_exp2f(fmaf(s[kt][i], c, -run_max)), b = __builtin_amdgcn_exp2f(fmaf(s[kt][i + 1], c, -run_max));
-        run_sum += a + b;  // (of the exponentials, not of what 16 bits make of them)
+        sum += a + b;  // (of the exponentials, not of what 16 bits make of them)
         pt[2 * kt + i / 8][(i % 8) / 2] = T::pack(a, b);
       }
-
+    };
+    const auto probabilities = [&](int kt) {
+      if constexpr (cut) {
+        const int left = seen - key0 - 4 * half;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[kt][i] = 32 * kt + 8 * (i / 4) + i % 4 >= left ? -INFINITY : s[kt][i];
+      }
+      most_here = s[kt][0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) most_here = fmaxf(most_here, s[kt][i]);
+      exponentials(kt);
+    };
+    const auto settle = [&](int kt) {
+      const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(most_here), __float_as_uint(most_here), false, false);
+      const float new_max = fmaxf(run_max, fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * c);
+      if (__builtin_expect(__ballot(new_max - run_max > 8.0f) != 0, 0)) {
+        const float alpha = __builtin_amdgcn_exp2f(fmaxf(run_max - new_max, -126.0f));
+        run_max = new_max;
+        run_sum *= alpha;
+#pragma unroll
+        for (int part = 0; part < kParts; ++part)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[part][i] *= alpha;
+        exponentials(kt);
+      }
+      run_sum += sum;
+    };
     const auto read_v = [&](int part, int step) {
       const unsigned char *const at = tile + v_rd[part] + 16 * step * (D * 2);
       const uintx2 lo = lds_read_tr(at), hi = lds_read_tr(at + 8 * (D * 2));
       return uintx4{lo[0], lo[1], hi[0], hi[1]};
     };
+    const auto products = [&](int kt) {
+#pragma unroll
+      for (int step = 2 * kt; step < 2 * kt + 2; ++step)
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) o[part] = T::mfma_32x32x16(read_v(part, step), pt[step], o[part]);
+    };
+
+    // A masked key's probability is zero, but zero times an infinity or a NaN in its v is NaN: a tile with such values takes the products of the
+    // finite ones, and the others are added, key by key, to the queries that see them.  (Keys behind the sequence are zeros.)
     bool bad = false;
-    if constexpr (cut && CAUSAL) {  // (keys behind the sequence are zeros)
+    if constexpr (cut && CAUSAL) {
 #pragma unroll
       for (int part = 0; part < kParts; ++part)
 #pragma unroll
@@ -236,21 +265,28 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(const P
         }
       bad = __ballot(bad) != 0;
     }
-    if (!(cut && CAUSAL) || !__builtin_expect(bad, 0)) {
+
+    if (ahead) __builtin_amdgcn_s_setprio(1);
+    scores(0);
+    scores(1);
+    if (ahead) __builtin_amdgcn_s_setprio(0);
+    probabilities(0);
+    settle(0);
+    if (__builtin_expect(bad, 0)) {
 #pragma unroll
-      for (int part = 0; part < kParts; ++part)
-#pragma unroll
-        for (int step = 0; step < 4; ++step) o[part] = T::mfma_32x32x16(read_v(part, step), pt[step], o[part]);
-    } else {
-      // A masked key's probability is zero, but zero times an infinity or a NaN in its v is NaN.  Finite values as ever; the others are
-      // added, key by key, to the queries that see them.
-#pragma unroll
-      for (int part = 0; part < kParts; ++part)
-#pragma unroll
-        for (int step = 0; step < 4; ++step) {
-          o[part] = T::mfma_32x32x16(finite_part<T>(read_v(part, step)), pt[step], o[part]);
-          __builtin_amdgcn_sched_barrier(0);  // (one operand at a time: registers are short)
+      for (int kt = 0; kt < 2; ++kt) {
+        if (kt == 1) {
+          probabilities(1);
+          settle(1);
         }
+#pragma unroll
+        for (int step = 2 * kt; step < 2 * kt + 2; ++step)
+#pragma unroll
+          for (int part = 0; part < kParts; ++part) {
+            o[part] = T::mfma_32x32x16(finite_part<T>(read_v(part, step)), pt[step], o[part]);
+            __builtin_amdgcn_sched_barrier(0);  // (one operand at a time: registers are short)
+          }
+      }
 #pragma unroll 1
       for (int r = 0; r < kKeys; ++r) {
         const bool sees = key0 + r < seen;
@@ -265,28 +301,70 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(const P
             for (int j = 0; j < 4; ++j) o[part][i + j] += sees && !(fabsf(x[j]) < INFINITY) ? x[j] : 0.f;
           }
       }
+      return;
     }
+    products(0);
+    probabilities(1);
+    settle(1);
+    products(1);
   };
 
+  // Group g works on tiles g, g + GROUPS, ...; all of them pass the same barriers.
   const std::integral_constant<bool, false> whole{};
   const std::integral_constant<bool, true> cut{};
-  const auto next = [&](int t) {  // tile t is there, and nobody reads tile t - 1 any more
+  const auto next = [&](int t) {  // tile t is there, and nobody reads the group's tile before it any more
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
     __syncthreads();
-    if (t + 1 < key_tiles) fetch(t + 1);
+    if (t + GROUPS < key_tiles) fetch(t + GROUPS);
   };
   const int whole_tiles = (CAUSAL ? min(q0 + 1, length) : length) / kKeys;  // that all queries of the workgroup see
-  fetch(0);
-  int t = 0;
-  for (; t + 2 <= whole_tiles; t += 2) {
+  if (group < key_tiles) fetch(group);
+  int t0 = 0;  // group 0's tile
+  for (; t0 + 2 * GROUPS <= whole_tiles; t0 += 2 * GROUPS) {
+    const int t = t0 + group;
     next(t);
     work_on(whole, lds, t * kKeys);
-    next(t + 1);
-    work_on(whole, lds + 2 * kTile, (t + 1) * kKeys);
+    next(t + GROUPS);
+    work_on(whole, lds + 2 * kTile, (t + GROUPS) * kKeys);
   }
-  for (; t < key_tiles; ++t) {
+  for (; t0 < key_tiles; t0 += GROUPS) {
+    const int t = t0 + group;
     next(t);
-    if (t * kKeys < most) work_on(cut, lds + (t & 1) * 2 * kTile, t * kKeys);
+    if (t * kKeys < most) work_on(cut, lds + (t / GROUPS & 1) * 2 * kTile, t * kKeys);
+  }
+
+  if constexpr (GROUPS > 1) {
+    // ---- the groups' states as one: the others leave theirs where their tiles were
+    static_assert(kParts * 16 * 64 * 4 * WAVES <= 4 * kTile, "a group's accumulators fit its tiles");
+    __syncthreads();
+    if (group > 0) {
+      floatx4 *const to = reinterpret_cast<floatx4 *>(lds) + wave * (kParts * 4 * 64) + lane;
+#pragma unroll
+      for (int part = 0; part < kParts; ++part)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[(part * 4 + i) * 64] = floatx4{o[part][4 * i], o[part][4 * i + 1], o[part][4 * i + 2], o[part][4 * i + 3]};
+      float *const st = states + ((group - 1) * WAVES + wave) * 128 + lane;
+      st[0] = run_max;
+      st[64] = run_sum;
+    }
+    __syncthreads();
+    if (group > 0) return;
+    for (int g = 1; g < GROUPS; ++g) {
+      const float *const st = states + ((g - 1) * WAVES + wave) * 128 + lane;
+      const float new_max = fmaxf(run_max, st[0]);
+      const float mine = __builtin_amdgcn_exp2f(fmaxf(run_max - new_max, -126.0f)), theirs = __builtin_amdgcn_exp2f(fmaxf(st[0] - new_max, -126.0f));
+      run_max = new_max;
+      run_sum = run_sum * mine + st[64] * theirs;
+      const floatx4 *const from = reinterpret_cast<const floatx4 *>(tiles_lds + g * 4 * kTile) + wave * (kParts * 4 * 64) + lane;
+#pragma unroll
+      for (int part = 0; part < kParts; ++part)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const floatx4 x = from[(part * 4 + i) * 64];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[part][4 * i + j] = o[part][4 * i + j] * mine + x[j] * theirs;
+        }
+    }
   }
 
   {
@@ -305,20 +383,33 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(const P
     }
 }
 
-template <typename T, int D, int WAVES>
+template <typename T, int D, int GROUPS>
 hipError_t launch(bool causal, const PromptArgs &a, hipStream_t stream) {
-  const long long tiles = (long long)a.tokens / (32 * WAVES) + a.sequences, blocks = tiles * a.heads;
-  if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+  const long long tiles = (long long)a.tokens / kTileQueries + a.sequences;
+  if (tiles * a.heads > 0x7fffffffLL) return hipErrorInvalidValue;
+  const unsigned blocks = (unsigned)(tiles * a.heads), threads = 64 * kWaves * GROUPS;
   if (causal)
-    hipLaunchKernelGGL((prompt_attention_kernel<T, D, WAVES, true>), dim3((unsigned)blocks), dim3(64 * WAVES), 0, stream, a, (int)tiles, (int)blocks);
+    hipLaunchKernelGGL((prompt_attention_kernel<T, D, kWaves, GROUPS, true>), dim3(blocks), dim3(threads), 0, stream, a, (int)tiles);
   else
-    hipLaunchKernelGGL((prompt_attention_kernel<T, D, WAVES, false>), dim3((unsigned)blocks), dim3(64 * WAVES), 0, stream, a, (int)tiles, (int)blocks);
+    hipLaunchKernelGGL((prompt_attention_kernel<T, D, kWaves, GROUPS, false>), dim3(blocks), dim3(threads), 0, stream, a, (int)tiles);
   return hipGetLastError();
+}
+
+// Two groups where one would leave half of the chip's 512 places for workgroups empty, or with a causal mask most of them while the last
+// tiles of long sequences run (lengths known on average only: a sequence of a few hundred tokens has nothing to split).
+bool two_groups(bool causal, const PromptArgs &a) {
+  const long long tiles = ((long long)a.tokens + kTileQueries - 1) / kTileQueries * a.heads, length = a.tokens / a.sequences;
+  return length >= 768 && (tiles <= 256 || (causal && tiles <= 512 && length >= 3000));
+}
+
+template <typename T, int D>
+hipError_t launch(bool causal, const PromptArgs &a, hipStream_t stream) {
+  return two_groups(causal, a) ? launch<T, D, 2>(causal, a, stream) : launch<T, D, 1>(causal, a, stream);
 }
 
 template <typename T>
 hipError_t launch(int d, bool causal, const PromptArgs &a, hipStream_t stream) {
-  return d == 128 ? launch<T, 128, 4>(causal, a, stream) : d == 64 ? launch<T, 64, 4>(causal, a, stream) : launch<T, 32, 4>(causal, a, stream);
+  return d == 128 ? launch<T, 128>(causal, a, stream) : d == 64 ? launch<T, 64>(causal, a, stream) : launch<T, 32>(causal, a, stream);
 }
 
 }  // namespace
