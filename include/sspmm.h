@@ -566,7 +566,7 @@ int sspmm_prompt_attention(int type, int sequences, int tokens, int heads, int k
  * written there is dropped, and what would be read is masked.
  *
  * sspmm_cache_write: tokens offsets[b] .. offsets[b + 1] - 1 of k and v to positions starts[b] on of row b.  A page has one scale per head for its
- * keys and one for its values: max |x| / 127 (int8), or the smallest power of two that brings it to 448 or less (e4m3), codes are rounded to
+ * keys and one for its values: max |x| times 1 / 127 in 32 bits (int8), or the smallest power of two that brings it to 448 or less (e4m3), codes are rounded to
  * nearest, ties to even.  Tokens in front of the new ones in their page are kept: the scale is then the larger of the page's and the new
  * tokens', and if it grows the kept codes are brought to it.  What lies behind the new ones in their page counts as unwritten.  A block that is
  * given an infinity or NaN has scale NaN until it is written from its page's first position again.  No two rows of a call may write to the same page.

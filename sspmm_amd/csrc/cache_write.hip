@@ -1,5 +1,5 @@
 // Keys and values of new tokens into the paged cache: one scale for the tokens of a page and head,
-//   scale = max |x| / 127 (int8) or the smallest power of two with max |x| / scale <= 448 (e4m3),  code = round(x / scale).
+//   scale = max |x| times 1 / 127 in 32 bits (int8) or the smallest power of two with max |x| / scale <= 448 (e4m3),  code = round(x / scale).
 // A page that already holds tokens keeps its scale unless the new ones need a larger one; its codes are then brought to it.
 #include "cache_kernels.h"
 
@@ -16,7 +16,7 @@ constexpr int kThreads = 256;
 template <int FORMAT>
 __device__ __forceinline__ float scale_for(uint32_t most) {  // most: the bits of the largest magnitude
   if (most >= 0x7f800000u) return NAN;
-  if (FORMAT == 0) return __uint_as_float(most) / 127.0f;
+  if (FORMAT == 0) return __uint_as_float(most) * (1.0f / 127.0f);
   if (most == 0) return 0.f;
   // 448 = 1.75 * 2^8.  (Below the normal numbers' range the exponent is out of the clamp's reach anyway.)
   const int e = (int)(most >> 23) - 8 + ((most & 0x7fffffu) > 0x600000u ? 1 : 0);

@@ -66,7 +66,7 @@ __device__ __forceinline__ uintx4 finite_part(uintx4 v) {
 // inside the lane, but for one exchange with the lane 32 apart, and what the matrix instruction leaves is, rounded to 16 bits, the operand P^T
 // of the second product V^T P^T, whose contraction slots are numbered accordingly: slots of lane half h in step t are keys
 // 16 t + 4 h + {0 .. 3, 8 .. 11}.  V^T comes from transpose reads.
-template <typename T, int D, int WAVES, int GROUPS, bool CAUSAL>
+template <typename T, int D, int WAVES, int GROUPS, bool CAUSAL, bool AHEAD>
 __global__ __launch_bounds__(64 * WAVES * GROUPS, 2) void prompt_attention_kernel(const PromptArgs p, int tiles) {
   constexpr int kQueries = 32 * WAVES, kPieces = D / 8, kTile = kKeys * D * 2;
   constexpr int kSteps = D / 16, kParts = D / 32;  // steps of the first product; parts of 32 features of the second
@@ -181,7 +181,6 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, 2) void prompt_attention_kerne
     v_rd[part] = kTile + r * (D * 2) + ((piece ^ swizzle_v<D>(r)) * 16) + (lane & 1) * 8;  // (8 rows on: the same swizzle)
   }
 
-  const bool ahead = D == 128 && key_tiles >= 64;
   floatx16 o[kParts];  // lane (n, half): features 32 part + 8 (i / 4) + 4 half + i % 4 of its query
 #pragma unroll
   for (int part = 0; part < kParts; ++part)
@@ -202,31 +201,22 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, 2) void prompt_attention_kerne
       for (int step = 0; step < kSteps; ++step)
         s[kt] = T::mfma_32x32x16(*reinterpret_cast<const uintx4 *>(tile + k_rd[step] + 32 * kt * (D * 2)), q[step], s[kt]);
     };
-    // The probabilities of 32 keys, by the reference point as it is.  That moves only when some query's maximum has grown by more than 2^8:
-    // until then probabilities are up to 2^8 too large, which either type holds, and the accumulators stay as they are.
-    float most_here = 0.f, sum = 0.f;
-    const auto exponentials = [&](int kt) {
-      sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        const float a = __builtin_amdgcn_exp2f(fmaf(s[kt][i], c, -run_max)), b = __builtin_amdgcn_exp2f(fmaf(s[kt][i + 1], c, -run_max));
-        sum += a + b;  // (of the exponentials, not of what 16 bits make of them)
-        pt[2 * kt + i / 8][(i % 8) / 2] = T::pack(a, b);
-      }
-    };
-    const auto probabilities = [&](int kt) {
+    // The reference point of the exponentials moves only when some query's maximum has grown by more than 2^8: until then probabilities are up
+    // to 2^8 too large, which either type holds, and the accumulators stay as they are.
+    const auto refer = [&]() {
       if constexpr (cut) {
         const int left = seen - key0 - 4 * half;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[kt][i] = 32 * kt + 8 * (i / 4) + i % 4 >= left ? -INFINITY : s[kt][i];
-      }
-      most_here = s[kt][0];
+        for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-      for (int i = 1; i < 16; ++i) most_here = fmaxf(most_here, s[kt][i]);
-      exponentials(kt);
-    };
-    const auto settle = [&](int kt) {
-      const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(most_here), __float_as_uint(most_here), false, false);
+          for (int i = 0; i < 16; ++i) s[kt][i] = 32 * kt + 8 * (i / 4) + i % 4 >= left ? -INFINITY : s[kt][i];
+      }
+      float most = s[0][0];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) most = fmaxf(most, s[kt][i]);
+      const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
       const float new_max = fmaxf(run_max, fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * c);
       if (__builtin_expect(__ballot(new_max - run_max > 8.0f) != 0, 0)) {
         const float alpha = __builtin_amdgcn_exp2f(fmaxf(run_max - new_max, -126.0f));
@@ -236,9 +226,15 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, 2) void prompt_attention_kerne
         for (int part = 0; part < kParts; ++part)
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[part][i] *= alpha;
-        exponentials(kt);
       }
-      run_sum += sum;
+    };
+    const auto exponentials = [&](int kt) {
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const float a = __builtin_amdgcn_exp2f(fmaf(s[kt][i], c, -run_max)), b = __builtin_amdgcn_exp2f(fmaf(s[kt][i + 1], c, -run_max));
+        run_sum += a + b;  // (of the exponentials, not of what 16 bits make of them)
+        pt[2 * kt + i / 8][(i % 8) / 2] = T::pack(a, b);
+      }
     };
     const auto read_v = [&](int part, int step) {
       const unsigned char *const at = tile + v_rd[part] + 16 * step * (D * 2);
@@ -266,19 +262,17 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, 2) void prompt_attention_kerne
       bad = __ballot(bad) != 0;
     }
 
-    if (ahead) __builtin_amdgcn_s_setprio(1);
+    // (the second half's exponentials run beside the first half's products)
+    if constexpr (AHEAD) __builtin_amdgcn_s_setprio(1);
     scores(0);
     scores(1);
-    if (ahead) __builtin_amdgcn_s_setprio(0);
-    probabilities(0);
-    settle(0);
+    refer();
+    exponentials(0);
     if (__builtin_expect(bad, 0)) {
+      if constexpr (AHEAD) __builtin_amdgcn_s_setprio(0);
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
-        if (kt == 1) {
-          probabilities(1);
-          settle(1);
-        }
+        if (kt == 1) exponentials(1);
 #pragma unroll
         for (int step = 2 * kt; step < 2 * kt + 2; ++step)
 #pragma unroll
@@ -304,8 +298,8 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, 2) void prompt_attention_kerne
       return;
     }
     products(0);
-    probabilities(1);
-    settle(1);
+    if constexpr (AHEAD) __builtin_amdgcn_s_setprio(0);
+    exponentials(1);
     products(1);
   };
 
@@ -383,15 +377,15 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, 2) void prompt_attention_kerne
     }
 }
 
-template <typename T, int D, int GROUPS>
+template <typename T, int D, int GROUPS, bool AHEAD>
 hipError_t launch(bool causal, const PromptArgs &a, hipStream_t stream) {
   const long long tiles = (long long)a.tokens / kTileQueries + a.sequences;
   if (tiles * a.heads > 0x7fffffffLL) return hipErrorInvalidValue;
   const unsigned blocks = (unsigned)(tiles * a.heads), threads = 64 * kWaves * GROUPS;
   if (causal)
-    hipLaunchKernelGGL((prompt_attention_kernel<T, D, kWaves, GROUPS, true>), dim3(blocks), dim3(threads), 0, stream, a, (int)tiles);
+    hipLaunchKernelGGL((prompt_attention_kernel<T, D, kWaves, GROUPS, true, AHEAD>), dim3(blocks), dim3(threads), 0, stream, a, (int)tiles);
   else
-    hipLaunchKernelGGL((prompt_attention_kernel<T, D, kWaves, GROUPS, false>), dim3(blocks), dim3(threads), 0, stream, a, (int)tiles);
+    hipLaunchKernelGGL((prompt_attention_kernel<T, D, kWaves, GROUPS, false, AHEAD>), dim3(blocks), dim3(threads), 0, stream, a, (int)tiles);
   return hipGetLastError();
 }
 
@@ -402,9 +396,14 @@ bool two_groups(bool causal, const PromptArgs &a) {
   return length >= 768 && (tiles <= 256 || (causal && tiles <= 512 && length >= 3000));
 }
 
+// Waves that are between a tile's scores and its first products go ahead of the others on their SIMD.  128 features, 8 heads of 16384 tokens
+// 555 -> 526 us, 16 of 8192 284 -> 272; 64 of 4096 273 -> 281, 32 of 2048 51.0 -> 52.2: for sequences of more than 6000 tokens.
 template <typename T, int D>
 hipError_t launch(bool causal, const PromptArgs &a, hipStream_t stream) {
-  return two_groups(causal, a) ? launch<T, D, 2>(causal, a, stream) : launch<T, D, 1>(causal, a, stream);
+  if (two_groups(causal, a)) return launch<T, D, 2, false>(causal, a, stream);
+  if constexpr (D == 128)
+    if (a.tokens / a.sequences > 6000) return launch<T, D, 1, true>(causal, a, stream);
+  return launch<T, D, 1, false>(causal, a, stream);
 }
 
 template <typename T>

@@ -190,7 +190,7 @@ def prompt_attention(q, k, v, offsets, scaling=None, causal=True, out=None):
 def cache_write(k, v, offsets, starts, page_table, keys, values, scales):
     """Tokens offsets[b] .. offsets[b + 1] - 1 of k and v [tokens, kv_heads, d] into the cache, at positions starts[b] on of row b of
     page_table [rows, slots].  The tokens of a page have one scale per head for their keys and one for their values: the largest magnitude
-    / 127 (int8), or the smallest power of two that brings it to 448 or less (e4m3).  Tokens before starts[b] in its page stay, at the
+    times 1 / 127 in 32 bits (int8), or the smallest power of two that brings it to 448 or less (e4m3).  Tokens before starts[b] in its page stay, at the
     larger of their scale and the new tokens'; what lies behind the last new token in its page counts as unwritten.  An infinity or NaN makes
     its block's scale NaN, until the page is written from its first position again.  Tokens for which the row has no page are dropped.  No
     two rows of a call may write to one page (fork_pages gives every row its own last page)."""

@@ -85,7 +85,7 @@ def check_step(got, q, table, lengths, keys, values, scales, scale, what=""):
 def scale_for(most, dtype):
     """The scale of a block whose largest magnitude is `most` (float32)."""
     if dtype is torch.int8:
-        s = most / 127.0
+        s = most * torch.tensor(1.0 / 127.0, dtype=torch.float32, device=most.device)
     else:
         mantissa, exponent = torch.frexp(most)
         e = (exponent - 9 + (mantissa > 0.875).int()).clamp(min=-126)
