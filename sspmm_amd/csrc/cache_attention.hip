@@ -73,7 +73,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_attention_kernel(const C
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const CachePool pool = p.pool;
   const int group = p.heads / pool.kv_heads, rows = p.queries * group, tiles = (rows + kRows - 1) / kRows;
-  const int split = blockIdx.x, head = blockIdx.y % pool.kv_heads, tile = blockIdx.y / pool.kv_heads;
+  const int split = blockIdx.y, head = blockIdx.x % pool.kv_heads, tile = blockIdx.x / pool.kv_heads;
   const int seq = longest_first(p.lengths, p.sequences);
   const int length = max(0, (int)min((long long)p.lengths[seq], (long long)pool.slots * pool.page_size));
   const int units = (length + UNIT - 1) / UNIT, pieces = p.splits * kWaves, piece = split * kWaves + wave;
@@ -357,7 +357,7 @@ Shape shape_of(int sequences, int queries, int heads, int kv_heads, long long lo
   s.tiles = (rows + 16 * s.row_tiles - 1) / (16 * s.row_tiles);
   const long long wide = (long long)sequences * kv_heads * s.tiles;
   const bool whole = wide >= 128 || longest <= 2048;
-  s.waves = whole ? 8 : 4;
+  s.waves = whole && wide <= 128 && longest > 512 ? 8 : 4;
   s.splits = whole ? 1 : (int)max(1ll, min(min((256 + wide - 1) / wide, (longest + 511) / 512), (long long)kMostSplits));
   return s;
 }
@@ -370,7 +370,7 @@ void launch(const CacheAttentionArgs &a, const Shape &s, const dim3 &grid, hipSt
 
 template <typename T, int FORMAT, int D>
 hipError_t launch(const CacheAttentionArgs &a, const Shape &s, hipStream_t stream) {
-  const dim3 grid(a.splits, a.pool.kv_heads * s.tiles, a.sequences);
+  const dim3 grid(a.pool.kv_heads * s.tiles, a.splits, a.sequences);
   if (a.pool.page_size == 32) {
     if (s.row_tiles == 1) launch<T, FORMAT, D, 1, 32>(a, s, grid, stream);
     else launch<T, FORMAT, D, 2, 32>(a, s, grid, stream);
