@@ -398,3 +398,75 @@ def test_refusals(built_library):
         with pytest.raises(ValueError):
             sspmm_amd.new_cache(4, 2, page, d)
     assert step(q[:0], table[:0], n[:0], keys, values, scales).shape == (0, 1, 4, 64)
+
+
+def test_more_rows_than_a_wave_has_lanes(built_library):
+    """Rows of all lengths, the longest of every 64 first; more queries than a tile of rows; writes of as many sequences."""
+    lengths = [(97 * i * i + 13 * i) % 700 for i in range(150)]
+    table, pages = _table(lengths, 64, seed=21)
+    pool = _filled(pages, 3, 64, 64, torch.int8, seed=22)
+    q = _randn((150, 1, 6, 64), 23).half()
+    got = sspmm_amd.cache_attention(q, table, _ints(lengths), *pool)
+    check_step(got, q, table, lengths, *pool, 0.125)
+    counts = [(3 * i) % 7 for i in range(150)]
+    starts = [max(0, n - c) for n, c in zip(lengths, counts)]
+    x = _randn((sum(counts), 2, 3, 64), 24).half()
+    k, v = x.unbind(1)
+    host = [t.cpu().clone() for t in pool]
+    write(k.cpu(), v.cpu(), offsets_of(counts).cpu(), starts, table.cpu(), *host)
+    sspmm_amd.cache_write(k, v, offsets_of(counts), _ints(starts), table, *pool)
+    for a, b in zip(pool, host):
+        assert torch.equal(a.cpu().view(torch.int8), b.view(torch.int8))
+
+
+@pytest.mark.parametrize("n,heads,kv", [(70, 4, 1), (129, 3, 3), (33, 16, 1)])
+def test_a_piece_of_a_prompt_over_the_cache(built_library, n, heads, kv):
+    """Many queries at once: a prompt's later part over what is in the cache, its own tokens among it."""
+    lengths, page, d = [n, 3 * n + 5, n - 3, 700], 64, 64
+    table, pages = _table(lengths, page, seed=25)
+    pool = _filled(pages, kv, page, d, torch.float8_e4m3fn, seed=26)
+    q = _randn((4, n, heads, d), 27).bfloat16()
+    got = sspmm_amd.cache_attention(q, table, _ints(lengths), *pool)
+    check_step(got, q, table, lengths, *pool, 0.125)
+
+
+@pytest.mark.parametrize("form", FORMATS)
+def test_a_captured_decoding_step(built_library, form):
+    """Pages, writing and attention of the next token in one graph, replayed token after token with the program's own work in between; the cache and
+    every result as in a program that calls them one by one."""
+    rows, kv, heads, d, page, pages = 3, 2, 4, 64, 32, 24
+    state = []
+    for _ in range(2):
+        keys, values, scales = sspmm_amd.new_cache(pages, kv, page, d, form)
+        state.append(dict(cache=(keys, values, scales), refs=_ints([0] * pages), table=torch.full((rows, 6), -1, dtype=torch.int32, device="cuda"),
+                          starts=_ints([0, 30, 63]), lengths=_ints([1, 31, 64]), out=torch.zeros(rows, 1, heads, d, device="cuda", dtype=torch.float16)))
+    offsets = offsets_of([1] * rows)
+    k, v, q = (torch.zeros(rows, n, d, device="cuda", dtype=torch.float16) for n in (kv, kv, heads))
+    for s in state:  # what came before
+        x = _randn((93, 2, kv, d), 50).half()
+        first = _ints([0, 0, 30, 93])
+        sspmm_amd.reserve_pages(s["refs"], s["table"], _ints([0, 0, 0]), first, page)
+        sspmm_amd.cache_write(x[:, 0], x[:, 1], first, _ints([0, 0, 0]), s["table"], *s["cache"])
+
+    def step(s):
+        sspmm_amd.reserve_pages(s["refs"], s["table"], s["starts"], offsets, page)
+        sspmm_amd.cache_write(k, v, offsets, s["starts"], s["table"], *s["cache"])
+        sspmm_amd.cache_attention(q[:, None], s["table"], s["lengths"], *s["cache"], out=s["out"])
+
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step(state[0])
+    for token in range(70):
+        for i, t in enumerate((k, v, q)):
+            t.copy_(_randn(t.shape, 100 + 3 * token + i) * 2.0 ** (token % 5))
+        g.replay()
+        step(state[1])
+        torch.cuda.synchronize()
+        assert torch.equal(state[0]["out"], state[1]["out"]), token
+        for s in state:
+            s["starts"] += 1
+            s["lengths"] += 1
+    for a, b in zip(state[0]["cache"] + (state[0]["table"], state[0]["refs"]), state[1]["cache"] + (state[1]["table"], state[1]["refs"])):
+        assert torch.equal(a.view(torch.int8), b.view(torch.int8))
+    check_step(state[0]["out"], q[:, None], state[0]["table"], [70, 100, 133], *state[0]["cache"], 0.125)

@@ -234,3 +234,49 @@ def test_refusals(built_library):
     with torch.no_grad():
         assert not call(q.clone().requires_grad_(), k, v, offsets).requires_grad
     assert call(q[:0], k[:0], v[:0], offsets_of([])).shape == (0, 4, 64)
+
+
+def test_few_workgroups_share_their_keys_between_groups(built_library):
+    """Long sequences and few heads: the other launch shape, with every width, empty and one-token sequences beside them."""
+    for d, dtype, causal in ((32, torch.float16, True), (64, torch.bfloat16, False), (128, torch.float16, False), (64, torch.float16, True)):
+        for lengths in ([2049, 1600], [1, 3333, 0], [1664]):
+            q, k, v = _projection(sum(lengths), 3, 1, d, dtype, seed=d)
+            print(d, dtype, causal, lengths, flush=True)
+            got = sspmm_amd.prompt_attention(q, k, v, offsets_of(lengths), causal=causal)
+            check_prompt(got, q, k, v, lengths, causal, d ** -0.5)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_masked_places_where_groups_share_the_keys(built_library, bad):
+    n = 1500
+    q, k, v = (t.clone() for t in _projection(n, 2, 1, 128, torch.bfloat16, seed=31))
+    at = 1210
+    v[at, 0, 5] = bad
+    got = sspmm_amd.prompt_attention(q, k, v, offsets_of([n]))
+    check_prompt(got, q, k, v, [n], True, 128 ** -0.5)
+    assert torch.isfinite(got[:at]).all() and not torch.isfinite(got[at:, :, 5]).any()
+
+
+def test_prompts_of_many_thousand_tokens(built_library):
+    """More than 6000 tokens with 128 features take a launch of their own."""
+    lengths = [8003, 6500]
+    q, k, v = _projection(sum(lengths), 8, 2, 128, torch.bfloat16, seed=32)
+    for causal in (True, False):
+        got = sspmm_amd.prompt_attention(q, k, v, offsets_of(lengths), causal=causal)
+        check_prompt(got, q, k, v, lengths, causal, 128 ** -0.5)
+
+
+def test_more_sequences_than_a_wave_has_lanes(built_library):
+    """The longest tiles of 64 sequences go first, then the next 64's: every tile of every sequence is found, whatever their order."""
+    for lengths in ([300] + [0] * 130 + [5, 257], list(range(0, 400, 3)), [128] * 65, [1] * 129 + [700]):
+        for causal in (True, False):
+            q, k, v = _projection(sum(lengths), 2, 2, 32, torch.float16, seed=len(lengths))
+            got = sspmm_amd.prompt_attention(q, k, v, offsets_of(lengths), causal=causal)
+            check_prompt(got, q, k, v, lengths, causal, 32 ** -0.5)
+
+
+def test_twice_the_same_bits(built_library):
+    q, k, v = _projection(3000, 8, 8, 64, torch.bfloat16, seed=33)
+    first = sspmm_amd.prompt_attention(q, k, v, offsets_of([1200, 1800]))
+    for _ in range(3):
+        assert torch.equal(sspmm_amd.prompt_attention(q, k, v, offsets_of([1200, 1800])), first)
