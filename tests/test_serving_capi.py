@@ -46,7 +46,7 @@ def test_cache_write(L):
 
 def test_cache_attention(L):
     #        type form seqs queries heads q seq row head table slots lengths pages kv page d keys values scales scale out seq row head workspace bytes stream
-    good = [0, 0, 2, 1, 4, A, 256, 256, 64, A, 64, A, 100, 2, 32, 64, A, A, A, 0.125, A, 256, 256, 64, A, 1 << 30, None]
+    good = [0, 0, 2, 1, 4, A, 256, 256, 64, A, 640, A, 100, 2, 32, 64, A, A, A, 0.125, A, 256, 256, 64, A, 1 << 30, None]
     run = _changed(good, L.sspmm_cache_attention)
     for i, v in ((0, 3), (1, 2), (2, -1), (2, 65536), (3, -1), (3, 1 << 19), (4, 3), (4, 0), (5, None), (5, A + 8), (6, 4), (6, -8), (7, 32), (8, 4), (9, None), (10, 0),
                  (10, 1 << 26), (11, None), (12, 0), (13, 3), (14, 48), (15, 96), (16, None), (17, None), (17, A + 8), (18, None), (19, 0.0), (19, float("inf")), (20, None), (21, 4),
@@ -54,10 +54,10 @@ def test_cache_attention(L):
         assert run((i, v)) == 1, (i, v)
     assert run((2, 0)) == 0 and run((3, 0)) == 0
     size = L.sspmm_cache_attention_workspace_bytes
-    need = size(2, 1, 4, 2, 64, 64, 32)
+    need = size(2, 1, 4, 2, 64, 640, 32)
     assert need > 0 and run((25, need - 1)) == 1
     assert size(2, 1, 3, 2, 64, 64, 32) == 0 and size(0, 1, 4, 2, 64, 64, 32) == 0 and size(2, 1, 4, 2, 65, 64, 32) == 0
-    assert size(60000, 1, 4, 2, 64, 64, 32) == 0  # enough rows for the chip: nothing is split
+    assert size(2, 1, 4, 2, 64, 64, 32) == 0 and size(60000, 1, 4, 2, 64, 640, 32) == 0  # short rows; enough rows for the chip: nothing is split
 
 
 def test_pages(L):
