@@ -41,15 +41,6 @@ __device__ __forceinline__ srd descriptor(const uint16_t *base, uint32_t bytes) 
   return srd{(int)(uint32_t)b, (int)((uint32_t)(b >> 32) & 0xffffu), (int)bytes, (int)kSrdWord3};
 }
 
-// Whether any of the eight values is infinite or NaN.
-template <typename T>
-__device__ __forceinline__ bool not_finite(uintx4 v) {
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) bad |= ((v[i] & T::kExponent) == T::kExponent) | (((v[i] >> 16) & T::kExponent) == T::kExponent);
-  return bad;
-}
-
 // The eight values with zeros in place of infinities and NaN.
 template <typename T>
 __device__ __forceinline__ uintx4 finite_part(uintx4 v) {
@@ -72,6 +63,7 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, 2) void prompt_attention_kerne
   constexpr int kSteps = D / 16, kParts = D / 32;  // steps of the first product; parts of 32 features of the second
   constexpr int kLoads = kTile / (64 * WAVES * 16);  // pieces of 16 bytes of a tile that a thread fetches
   __shared__ __align__(16) unsigned char tiles_lds[GROUPS * 4 * kTile];  // of each group K, V, K, V
+  __shared__ int not_finite;
   __shared__ float states[GROUPS > 1 ? (GROUPS - 1) * WAVES * 2 * 64 : 1];
   const int lane = threadIdx.x & 63, n = lane & 31, half = lane >> 5;
   const int group = GROUPS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * WAVES));
@@ -182,11 +174,8 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, 2) void prompt_attention_kerne
   }
 
   floatx16 o[kParts];  // lane (n, half): features 32 part + 8 (i / 4) + 4 half + i % 4 of its query
-#pragma unroll
-  for (int part = 0; part < kParts; ++part)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[part][i] = 0.f;
-  float run_max = -3.0e38f, run_sum = 0.f;  // of the scaled scores; this lane's share of the sum
+  float run_max, run_sum;  // of the scaled scores; this lane's share of the sum
+  bool again = false;
   const float c = p.scale_log2e;
 
   // Tile t, in `tile` of LDS.  cut: some query may not see all of its keys.
@@ -248,27 +237,13 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, 2) void prompt_attention_kerne
         for (int part = 0; part < kParts; ++part) o[part] = T::mfma_32x32x16(read_v(part, step), pt[step], o[part]);
     };
 
-    // A masked key's probability is zero, but zero times an infinity or a NaN in its v is NaN: a tile with such values takes the products of the
-    // finite ones, and the others are added, key by key, to the queries that see them.  (Keys behind the sequence are zeros.)
-    bool bad = false;
-    if constexpr (cut && CAUSAL) {
-#pragma unroll
-      for (int part = 0; part < kParts; ++part)
-#pragma unroll
-        for (int step = 0; step < 4; ++step) {
-          bad |= not_finite<T>(read_v(part, step));
-          if (step % 2 == 1) __builtin_amdgcn_sched_barrier(0);
-        }
-      bad = __ballot(bad) != 0;
-    }
-
     // (the second half's exponentials run beside the first half's products)
     if constexpr (AHEAD) __builtin_amdgcn_s_setprio(1);
     scores(0);
     scores(1);
     refer();
     exponentials(0);
-    if (__builtin_expect(bad, 0)) {
+    if (cut && CAUSAL && __builtin_expect(again, 0)) {
       if constexpr (AHEAD) __builtin_amdgcn_s_setprio(0);
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
@@ -312,19 +287,40 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, 2) void prompt_attention_kerne
     if (t + GROUPS < key_tiles) fetch(t + GROUPS);
   };
   const int whole_tiles = (CAUSAL ? min(q0 + 1, length) : length) / kKeys;  // that all queries of the workgroup see
-  if (group < key_tiles) fetch(group);
-  int t0 = 0;  // group 0's tile
-  for (; t0 + 2 * GROUPS <= whole_tiles; t0 += 2 * GROUPS) {
-    const int t = t0 + group;
-    next(t);
-    work_on(whole, lds, t * kKeys);
-    next(t + GROUPS);
-    work_on(whole, lds + 2 * kTile, (t + GROUPS) * kKeys);
-  }
-  for (; t0 < key_tiles; t0 += GROUPS) {
-    const int t = t0 + group;
-    next(t);
-    if (t * kKeys < most) work_on(cut, lds + (t / GROUPS & 1) * 2 * kTile, t * kKeys);
+  // A masked key's probability is zero, but zero times an infinity or a NaN in its v is NaN.  A workgroup that finds a result which is not finite
+  // goes over its keys again: the tiles at the mask's edge then take the products of the finite values, and the others are added, key by key, to
+  // the queries that see them.  (Looking at every such tile first: 512 tokens, 32 heads of 128 features 17.0 us instead of 15.1.)
+  if (CAUSAL && threadIdx.x == 0) not_finite = 0;
+  for (;; again = true) {
+#pragma unroll
+    for (int part = 0; part < kParts; ++part)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[part][i] = 0.f;
+    run_max = -3.0e38f;
+    run_sum = 0.f;
+    if (group < key_tiles) fetch(group);
+    int t0 = 0;  // group 0's tile
+    for (; t0 + 2 * GROUPS <= whole_tiles; t0 += 2 * GROUPS) {
+      const int t = t0 + group;
+      next(t);
+      work_on(whole, lds, t * kKeys);
+      next(t + GROUPS);
+      work_on(whole, lds + 2 * kTile, (t + GROUPS) * kKeys);
+    }
+    for (; t0 < key_tiles; t0 += GROUPS) {
+      const int t = t0 + group;
+      next(t);
+      if (t * kKeys < most) work_on(cut, lds + (t / GROUPS & 1) * 2 * kTile, t * kKeys);
+    }
+    if (!CAUSAL || again) break;
+    float zero = 0.f;
+#pragma unroll
+    for (int part = 0; part < kParts; ++part)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) zero = fmaf(o[part][i], 0.f, zero);
+    if (__ballot(zero != zero) != 0 && lane == 0) not_finite = 1;
+    __syncthreads();
+    if (__builtin_amdgcn_readfirstlane(not_finite) == 0) break;
   }
 
   if constexpr (GROUPS > 1) {
