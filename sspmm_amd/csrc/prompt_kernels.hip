@@ -52,22 +52,29 @@ __device__ __forceinline__ uintx4 finite_part(uintx4 v) {
   return v;
 }
 
-// A workgroup of WAVES waves owns 32 * WAVES consecutive queries of one sequence and head, 32 a wave.
+// A workgroup owns 128 consecutive queries of one sequence and head, 32 a wave, and passes over the keys they see in tiles of 64.
 // Scores are made transposed, K Q^T, so that a lane holds 32 of a tile's 64 scores of ONE query: maxima and sums are taken
 // inside the lane, but for one exchange with the lane 32 apart, and what the matrix instruction leaves is, rounded to 16 bits, the operand P^T
 // of the second product V^T P^T, whose contraction slots are numbered accordingly: slots of lane half h in step t are keys
-// 16 t + 4 h + {0 .. 3, 8 .. 11}.  V^T comes from transpose reads.
-template <typename T, int D, int WAVES, int GROUPS, bool CAUSAL, bool AHEAD>
-__global__ __launch_bounds__(64 * WAVES * GROUPS, 2) void prompt_attention_kernel(const PromptArgs p, int tiles) {
-  constexpr int kQueries = 32 * WAVES, kPieces = D / 8, kTile = kKeys * D * 2;
+// 16 t + 4 h + {0 .. 3, 8 .. 11}.  V^T comes from transpose reads.  Two buffers of K and V, one barrier a tile, two workgroups a CU (64 KB and up to 256
+// registers a lane with 128 features).
+//
+// Bound by the matrix instructions and the power they take: 16384 tokens, 8 heads of 128 features, 1.10 PFLOP/s causal and 1.14 not, where the library's
+// product of 8192^3 reaches 1.15 on the same card; the clock stands at 1.85 GHz then, the matrix units are busy 53 % of the cycles, the vector ones 37 %
+// (without the exponentials the launch takes 5 % less, with K and V from registers 33 %).  Tried without gain: all of K's operands asked for
+// ahead, K two tiles and V one and a half ahead with two barriers a tile, 256 queries a workgroup, 64 queries a workgroup (1.4 times as long).
+// Short prompts wait for their latencies: 512 tokens, 32 heads 15 us, eight tiles one after the other.
+template <typename T, int D, int GROUPS, bool CAUSAL, bool AHEAD>
+__global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void prompt_attention_kernel(const PromptArgs p, int tiles) {
+  constexpr int kPieces = D / 8, kTile = kKeys * D * 2;
   constexpr int kSteps = D / 16, kParts = D / 32;  // steps of the first product; parts of 32 features of the second
-  constexpr int kLoads = kTile / (64 * WAVES * 16);  // pieces of 16 bytes of a tile that a thread fetches
+  constexpr int kLoads = kTile / (64 * kWaves * 16);  // pieces of 16 bytes of a tile that a thread fetches
   __shared__ __align__(16) unsigned char tiles_lds[GROUPS * 4 * kTile];  // of each group K, V, K, V
   __shared__ int not_finite;
-  __shared__ float states[GROUPS > 1 ? (GROUPS - 1) * WAVES * 2 * 64 : 1];
+  __shared__ float states[GROUPS > 1 ? (GROUPS - 1) * kWaves * 2 * 64 : 1];
   const int lane = threadIdx.x & 63, n = lane & 31, half = lane >> 5;
-  const int group = GROUPS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * WAVES));
-  const int wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) % WAVES);
+  const int group = GROUPS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * kWaves));
+  const int wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) % kWaves);
   unsigned char *const lds = tiles_lds + group * 4 * kTile;
 
   // ---- which queries
@@ -95,7 +102,7 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, 2) void prompt_attention_kerne
       lo = max(0, min(p.offsets[b], p.tokens));
       hi = max(lo, min(p.offsets[b + 1], p.tokens));
     }
-    const int count = (int)(((long long)(hi - lo) + kQueries - 1) / kQueries);
+    const int count = (int)(((long long)(hi - lo) + kTileQueries - 1) / kTileQueries);
     const int all = (int)from_last_lane(wave_inclusive_sum((uint32_t)count));
     if (left >= all) {
       left -= all;
@@ -120,7 +127,7 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, 2) void prompt_attention_kerne
     const int at = __builtin_ctzll(__ballot(is));
     first = __builtin_amdgcn_readlane(lo, at);
     length = __builtin_amdgcn_readlane(hi, at) - first;
-    q0 = (CAUSAL ? x - 1 : left % x) * kQueries;
+    q0 = (CAUSAL ? x - 1 : left % x) * kTileQueries;
     break;
   }
   if (length < 0) return;  // (there are fewer tiles than the host could exclude)
@@ -129,7 +136,7 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, 2) void prompt_attention_kerne
   const int my = q0 + 32 * wave + n;  // this lane's query
   const int seen = CAUSAL ? min(my + 1, length) : length;  // keys it sees: those below
   const int most = CAUSAL ? min(q0 + 32 * wave + 32, length) : length;  // (no query of the wave sees one from here on)
-  const int last = CAUSAL ? min(q0 + kQueries, length) : length;
+  const int last = CAUSAL ? min(q0 + kTileQueries, length) : length;
   const int key_tiles = (last + kKeys - 1) / kKeys;
 
   // ---- queries: lane (n, half) holds features 16 s + 8 half .. + 7 of its query
@@ -148,7 +155,7 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, 2) void prompt_attention_kerne
   uint32_t k_at[kLoads], v_at[kLoads];
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
-    const int piece = (i * WAVES + wave) * 64 + lane, r = piece / kPieces, c = piece % kPieces;
+    const int piece = (i * kWaves + wave) * 64 + lane, r = piece / kPieces, c = piece % kPieces;
     k_at[i] = r * k_pitch + (c ^ swizzle_k<D>(r)) * 16;
     v_at[i] = r * v_pitch + (c ^ swizzle_v<D>(r)) * 16;
   }
@@ -158,9 +165,9 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, 2) void prompt_attention_kerne
     const srd sv = descriptor(v0 + (long long)t * kKeys * p.v_row, (rows - 1) * v_pitch + D * 2);
     const uint32_t to = lds_at + (t / GROUPS & 1) * 2 * kTile;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) load_to_lds(sk, k_at[i], to + i * WAVES * 1024);
+    for (int i = 0; i < kLoads; ++i) load_to_lds(sk, k_at[i], to + i * kWaves * 1024);
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) load_to_lds(sv, v_at[i], to + kTile + i * WAVES * 1024);
+    for (int i = 0; i < kLoads; ++i) load_to_lds(sv, v_at[i], to + kTile + i * kWaves * 1024);
   };
 
   // ---- where a lane's operands lie in a tile: of K in its first 32 rows by step, of V in the first 8 rows of a step by part
@@ -243,7 +250,7 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, 2) void prompt_attention_kerne
     scores(1);
     refer();
     exponentials(0);
-    if (cut && CAUSAL && __builtin_expect(again, 0)) {
+    if (cut && __builtin_expect(again, 0)) {
       if constexpr (AHEAD) __builtin_amdgcn_s_setprio(0);
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
@@ -256,8 +263,15 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, 2) void prompt_attention_kerne
             __builtin_amdgcn_sched_barrier(0);  // (one operand at a time: registers are short)
           }
       }
+      uint32_t others = 0;
 #pragma unroll 1
-      for (int r = 0; r < kKeys; ++r) {
+      for (int i = 0; i < kTile; i += 1024) {
+        const uintx4 v = *reinterpret_cast<const uintx4 *>(tile + kTile + i + lane * 16), finite = finite_part<T>(v);
+        others |= (v[0] ^ finite[0]) | (v[1] ^ finite[1]) | (v[2] ^ finite[2]) | (v[3] ^ finite[3]);
+      }
+      const int special = __ballot(others != 0) != 0 ? kKeys : 0;
+#pragma unroll 1
+      for (int r = 0; r < special; ++r) {
         const bool sees = key0 + r < seen;
 #pragma unroll
         for (int part = 0; part < kParts; ++part)
@@ -287,10 +301,10 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, 2) void prompt_attention_kerne
     if (t + GROUPS < key_tiles) fetch(t + GROUPS);
   };
   const int whole_tiles = (CAUSAL ? min(q0 + 1, length) : length) / kKeys;  // that all queries of the workgroup see
-  // A masked key's probability is zero, but zero times an infinity or a NaN in its v is NaN.  A workgroup that finds a result which is not finite
-  // goes over its keys again: the tiles at the mask's edge then take the products of the finite values, and the others are added, key by key, to
-  // the queries that see them.  (Looking at every such tile first: 512 tokens, 32 heads of 128 features 17.0 us instead of 15.1.)
-  if (CAUSAL && threadIdx.x == 0) not_finite = 0;
+  // A masked key's probability is zero, and so is what underflows, but zero times an infinity or a NaN in v is NaN.  A workgroup that finds a
+  // result which is not finite goes over its keys again: the products are of the finite values then, and the others are added, key by key,
+  // to the queries that see them.  (Looking at every tile at the mask's edge first: 512 tokens, 32 heads of 128 features 17.0 us instead of 15.1.)
+  if (threadIdx.x == 0) not_finite = 0;
   for (;; again = true) {
 #pragma unroll
     for (int part = 0; part < kParts; ++part)
@@ -300,7 +314,7 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, 2) void prompt_attention_kerne
     run_sum = 0.f;
     if (group < key_tiles) fetch(group);
     int t0 = 0;  // group 0's tile
-    for (; t0 + 2 * GROUPS <= whole_tiles; t0 += 2 * GROUPS) {
+    for (; !again && t0 + 2 * GROUPS <= whole_tiles; t0 += 2 * GROUPS) {
       const int t = t0 + group;
       next(t);
       work_on(whole, lds, t * kKeys);
@@ -312,7 +326,7 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, 2) void prompt_attention_kerne
       next(t);
       if (t * kKeys < most) work_on(cut, lds + (t / GROUPS & 1) * 2 * kTile, t * kKeys);
     }
-    if (!CAUSAL || again) break;
+    if (again) break;
     float zero = 0.f;
 #pragma unroll
     for (int part = 0; part < kParts; ++part)
@@ -325,7 +339,7 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, 2) void prompt_attention_kerne
 
   if constexpr (GROUPS > 1) {
     // ---- the groups' states as one: the others leave theirs where their tiles were
-    static_assert(kParts * 16 * 64 * 4 * WAVES <= 4 * kTile, "a group's accumulators fit its tiles");
+    static_assert(kParts * 16 * 64 * 4 * kWaves <= 4 * kTile, "a group's accumulators fit its tiles");
     __syncthreads();
     if (group > 0) {
       floatx4 *const to = reinterpret_cast<floatx4 *>(lds) + wave * (kParts * 4 * 64) + lane;
@@ -333,14 +347,14 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, 2) void prompt_attention_kerne
       for (int part = 0; part < kParts; ++part)
 #pragma unroll
         for (int i = 0; i < 4; ++i) to[(part * 4 + i) * 64] = floatx4{o[part][4 * i], o[part][4 * i + 1], o[part][4 * i + 2], o[part][4 * i + 3]};
-      float *const st = states + ((group - 1) * WAVES + wave) * 128 + lane;
+      float *const st = states + ((group - 1) * kWaves + wave) * 128 + lane;
       st[0] = run_max;
       st[64] = run_sum;
     }
     __syncthreads();
     if (group > 0) return;
     for (int g = 1; g < GROUPS; ++g) {
-      const float *const st = states + ((g - 1) * WAVES + wave) * 128 + lane;
+      const float *const st = states + ((g - 1) * kWaves + wave) * 128 + lane;
       const float new_max = fmaxf(run_max, st[0]);
       const float mine = __builtin_amdgcn_exp2f(fmaxf(run_max - new_max, -126.0f)), theirs = __builtin_amdgcn_exp2f(fmaxf(st[0] - new_max, -126.0f));
       run_max = new_max;
@@ -379,9 +393,9 @@ hipError_t launch(bool causal, const PromptArgs &a, hipStream_t stream) {
   if (tiles * a.heads > 0x7fffffffLL) return hipErrorInvalidValue;
   const unsigned blocks = (unsigned)(tiles * a.heads), threads = 64 * kWaves * GROUPS;
   if (causal)
-    hipLaunchKernelGGL((prompt_attention_kernel<T, D, kWaves, GROUPS, true, AHEAD>), dim3(blocks), dim3(threads), 0, stream, a, (int)tiles);
+    hipLaunchKernelGGL((prompt_attention_kernel<T, D, GROUPS, true, AHEAD>), dim3(blocks), dim3(threads), 0, stream, a, (int)tiles);
   else
-    hipLaunchKernelGGL((prompt_attention_kernel<T, D, kWaves, GROUPS, false, AHEAD>), dim3(blocks), dim3(threads), 0, stream, a, (int)tiles);
+    hipLaunchKernelGGL((prompt_attention_kernel<T, D, GROUPS, false, AHEAD>), dim3(blocks), dim3(threads), 0, stream, a, (int)tiles);
   return hipGetLastError();
 }
 

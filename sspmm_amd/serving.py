@@ -38,7 +38,7 @@ def new_cache(pages, kv_heads, page_size, head_dim, dtype=torch.int8, device="cu
 
 
 # Calls of a few microseconds: each entry asks for all it wants of its arguments in one expression, and goes through it again, name by name, for the
-# error only (16.0 -> 11.9 us of the host a step of the cache, 11.3 -> 8.8 a prompt).
+# error only (prompt_attention 11.3 -> 9.8 us of the host, 4.5 of which are the C call with its launch).
 
 def _ints(name, t, dim, device):
     if t.dtype is not torch.int32 or t.get_device() != device or device < 0 or not t.is_contiguous():

@@ -280,3 +280,17 @@ def test_twice_the_same_bits(built_library):
     first = sspmm_amd.prompt_attention(q, k, v, offsets_of([1200, 1800]))
     for _ in range(3):
         assert torch.equal(sspmm_amd.prompt_attention(q, k, v, offsets_of([1200, 1800])), first)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lengths,heads", [([200, 90], 2), ([1700], 1)])
+def test_infinities_beside_probabilities_that_underflow(built_library, causal, lengths, heads):
+    """A key whose probability is far below what 16 bits hold is seen all the same: what is infinite in its v is infinite in the result."""
+    n = sum(lengths)
+    q, k, v = (t.clone() for t in _projection(n, heads, heads, 64, torch.float16, seed=34))
+    q[:, :, 0], k[:, :, 0] = 8.0, 0.0
+    for at, what in ((3, float("inf")), (70, float("-inf")), (n - 2, float("nan"))):
+        k[at, :, 0] = -40.0  # 2^-58 beside the others
+        v[at, 0, 7 + at % 5] = what
+    got = sspmm_amd.prompt_attention(q, k, v, offsets_of(lengths), causal=causal)
+    check_prompt(got, q, k, v, lengths, causal, 0.125)
