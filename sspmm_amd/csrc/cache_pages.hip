@@ -134,7 +134,8 @@ struct Fork {
   int32_t child, parent, source, target, shared;  // child -1: nothing
 };
 
-// One workgroup.  Per row the last naming as a child holds; a row that is a child in the call cannot be a parent in it.
+// One workgroup.  Per row the last naming as a child holds; a row that becomes another's copy in the call cannot be a
+// parent in it; a row that is named its own parent stays as it is.
 __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(const PageTable t, int32_t *lengths, const int32_t *parents, const int32_t *children, int count,
                                                                  int page_size, int32_t *workspace) {
   __shared__ uint32_t share[kPlanWaves];
@@ -150,10 +151,10 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(const PageTable
   for (int i0 = 0; i0 < count; i0 += kPlanThreads) {
     const int i = i0 + tid;
     Fork f = {-1, -1, -1, -1, 0};
-    if (i < count && children[i] >= 0 && children[i] < t.rows && mark[children[i]] == i) {
+    if (i < count && children[i] >= 0 && children[i] < t.rows && mark[children[i]] == i && parents[i] != children[i]) {
       f.child = children[i];
       const int parent = parents[i];
-      if (parent >= 0 && parent < t.rows && mark[parent] < 0) {
+      if (parent >= 0 && parent < t.rows && (mark[parent] < 0 || parents[mark[parent]] == parent)) {
         const int length = (int)max(0ll, min((long long)lengths[parent], (long long)t.slots * page_size));
         f.parent = parent;
         f.shared = length / page_size;
@@ -217,7 +218,10 @@ __global__ __launch_bounds__(256) void fork_copy_kernel(const PageTable t, const
     } else if (s == f.shared && f.source >= 0) {
       page = f.target;
     }
-    t.table[(long long)f.child * t.slots + s] = page;
+    int32_t *const at = t.table + (long long)f.child * t.slots + s;
+    const int before = *at;
+    if (before >= 0 && before < t.pages) atomicSub(&t.refs[before], 1);  // (while the plan was made its pages were in use)
+    *at = page;
   }
 }
 

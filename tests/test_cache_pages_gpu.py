@@ -297,3 +297,32 @@ def test_refusals(built_library):
     sspmm_amd.fork_pages(refs, t, n, none, none, *cache)
     sspmm_amd.reserve_pages(refs, t[:0], none, offsets_of([]), 32)
     assert all(torch.equal(a, b) for a, b in zip((t, refs, n), before))
+
+
+@pytest.mark.parametrize("seed", [1, 2, 3, 4])
+def test_beams_that_take_the_places_of_others(built_library, seed):
+    """Children that hold pages give them back, whatever becomes of them; rows that are their own parents stay, and are parents of others."""
+    r = random.Random(seed)
+    pages, rows, slots, page = 160, 12, 8, 32
+    model, dev = Model(pages, rows, slots, page), Device(pages, rows, slots, page)
+    counts = [r.randint(0, slots * page) for _ in range(rows)]
+    model.reserve([0] * rows, counts)
+    sspmm_amd.reserve_pages(dev.refs, dev.table, dev.lengths, offsets_of(counts), page)
+    model.lengths = counts
+    dev.lengths.copy_(_ints(counts))
+    for step in range(12):
+        children = [r.randrange(-1, rows) for _ in range(r.randint(1, rows))]
+        parents = [c if r.random() < 0.3 else r.randrange(-1, rows) for c in children]
+        last = {c: i for i, c in enumerate(children) if c >= 0}
+        moved = [c for c, i in last.items() if parents[i] != c]
+        before = [list(model.table[c]) for c in moved]
+        pairs = sorted((last[c], c) for c in moved)
+        model.fork([parents[i] for i, _ in pairs], [c for _, c in pairs])
+        for row in before:
+            for p in row:
+                if p >= 0:
+                    model.refs[p] -= 1
+        sspmm_amd.fork_pages(dev.refs, dev.table, dev.lengths, _ints(parents), _ints(children), *dev.cache)
+        dev.same(model, "seed %d, step %d: %s of %s" % (seed, step, children, parents))
+        held = [p for row in model.table for p in row if p >= 0]
+        assert model.refs == [held.count(p) for p in range(pages)]
