@@ -76,6 +76,21 @@ __device__ __forceinline__ float wave_sum_all(float x) {
 // The value lane 63 holds, in every lane.
 __device__ __forceinline__ uint32_t from_last_lane(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, 63); }
 
+// The last of `count` numbers, base(0) <= base(1) <= ..., that is not above `id` (the first, if none is): 64 of them are asked at a time.
+template <typename Base>
+__device__ __forceinline__ int last_not_above(int count, int id, const Base &base) {
+  const int lane = threadIdx.x & 63;
+  int first = 0;
+  while (count > 1) {
+    const int step = (count + 63) / 64, at = lane * step;
+    const unsigned long long those = __ballot(at < count && base(first + at) <= id);
+    const int skip = those == 0 ? 0 : (63 - __builtin_clzll(those)) * step;
+    first += skip;
+    count = min(step, count - skip);
+  }
+  return first;
+}
+
 // Four consecutive fp16 values of a row of which `left` exist.  RAGGED: the row begins at any element, and what lies behind its
 // end is neither read nor written.
 typedef _Float16 four_halfs __attribute__((ext_vector_type(4)));

@@ -470,3 +470,61 @@ def test_a_captured_decoding_step(built_library, form):
     for a, b in zip(state[0]["cache"] + (state[0]["table"], state[0]["refs"]), state[1]["cache"] + (state[1]["table"], state[1]["refs"])):
         assert torch.equal(a.view(torch.int8), b.view(torch.int8))
     check_step(state[0]["out"], q[:, None], state[0]["table"], [70, 100, 133], *state[0]["cache"], 0.125)
+
+
+def test_thousands_of_rows_are_written(built_library):
+    """Rows found by way of more than 64 groups of 64, by their tokens (most of one) and by their pages: the bytes of a few rows at a time."""
+    g = torch.Generator()
+    g.manual_seed(6)
+    for most in (2, 90):
+        counts = torch.randint(0, most, (4500,), generator=g)
+        counts[700:900] = 0
+        starts = torch.randint(0, 40, (4500,), generator=g)
+        slots = -(-(most + 40) // 32)
+        offsets = torch.cat([torch.zeros(1, dtype=torch.long), counts.cumsum(0)]).int().cuda()
+        starts = starts.int().cuda()
+        table = torch.randperm(4500 * slots, generator=g).int().cuda().view(4500, slots)
+        k, v = (_randn((int(offsets[-1]), 2, 32), i).half() for i in (1, 2))
+        caches = [sspmm_amd.new_cache(4500 * slots, 2, 32, 32) for _ in range(2)]
+        sspmm_amd.cache_write(k, v, offsets, starts, table, *caches[0])
+        for b in range(0, 4500, 60):
+            sspmm_amd.cache_write(k, v, offsets[b:b + 61].clone(), starts[b:b + 60].clone(), table[b:b + 60].clone(), *caches[1])
+        for x, y in zip(*caches):
+            assert torch.equal(x, y)
+
+
+def test_thousands_of_small_probabilities(built_library):
+    """As with prompts: off by 2^-32 a key at most, and 2^-11 of the sum and of the result."""
+    n, page = 16384, 64
+    keys, values, scales = sspmm_amd.new_cache(n // page, 1, page, 64)
+    keys[..., 0] = -127
+    keys[0, 0, 0, 0] = 0
+    values.fill_(127)
+    values[0, :, :, 0] = 0
+    scales[:, 0], scales[:, 1] = 25.5 * math.log(2.0) / 127, 1.0 / 127
+    q = torch.zeros(1, 1, 1, 64, device="cuda", dtype=torch.float16)
+    q[..., 0] = 1.0
+    table = torch.arange(n // page, dtype=torch.int32, device="cuda").view(1, -1)
+    out = sspmm_amd.cache_attention(q, table, _ints([n]), keys, values, scales, scaling=1.0)
+    p = math.exp(-127 * scales[0, 0, 0].item())
+    want = (n - 1) * p / (1 + (n - 1) * p)
+    assert (out.double() - want).abs().max().item() <= (n - 1) * 2.0 ** -32 + want * 2.0 ** -10
+
+
+@pytest.mark.parametrize("lengths,heads,kv", [([700, 33, 0, 200], 8, 2), ([9000], 40, 2)])
+def test_attention_in_place(built_library, lengths, heads, kv):
+    table, pages = _table(lengths, 64, seed=3)
+    cache = _filled(pages, kv, 64, 64, torch.int8, seed=4)
+    q = _randn((len(lengths), 2, heads, 64), 5).half()
+    want = sspmm_amd.cache_attention(q, table, _ints(lengths), *cache)
+    assert sspmm_amd.cache_attention(q, table, _ints(lengths), *cache, out=q) is q
+    assert torch.equal(q, want)
+
+
+def test_attention_into_rows_that_overlap_is_refused(built_library):
+    table, pages = _table([40], 64, seed=3)
+    cache = _filled(pages, 1, 64, 64, torch.int8, seed=4)
+    q = _randn((1, 2, 4, 64), 5).half()
+    for out in (q[:, :, :1].expand(1, 2, 4, 64), q.view(-1)[:320].as_strided((1, 2, 4, 64), (512, 64, 64, 1))):
+        with pytest.raises(ValueError):
+            sspmm_amd.cache_attention(q, table, _ints([40]), *cache, out=out)
