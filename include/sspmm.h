@@ -552,7 +552,7 @@ int sspmm_attention_fm_ragged_f16(int batch, int heads, int seq, int head_dim, c
  * out_i = softmax over j of (q_i . k_j * scale) times v_j per sequence and head; sequence b is tokens offsets[b] .. offsets[b + 1] - 1
  * (device, sequences + 1 of them, ascending within 0 .. tokens; others are taken to the nearest of these).  causal: j <= i.  Token i,
  * head h of q is at q + i * q_row + h * q_head elements, and so on.  Tokens of no sequence are neither read nor written.  A row whose scores
- * are all -infinity is zeros.  Row strides below 2^23.
+ * are all -infinity is zeros.  Row strides below 2^23.  out may be q, and overlaps neither with k and v nor otherwise with q.
  */
 int sspmm_prompt_attention(int type, int sequences, int tokens, int heads, int kv_heads, int head_dim, const int32_t *offsets,
                            const sspmm_half_t *q, int64_t q_row, int64_t q_head, const sspmm_half_t *k, int64_t k_row, int64_t k_head,
@@ -564,6 +564,9 @@ int sspmm_prompt_attention(int type, int sequences, int tokens, int heads, int k
  * [pages, 2, kv_heads] (keys, values): element = code * scale.  page_size 32, 64 or 128; all of it dense, 16-byte aligned.
  * page_table [rows, slots]: the page of positions slot * page_size .. of a row; an entry outside 0 .. pages - 1 is no page: what would be
  * written there is dropped, and what would be read is masked.
+ *
+ * A page that several rows name is written for all of them: rows that share pages (fork, below) do not go back in front of the
+ * position where they parted.
  *
  * sspmm_cache_write: tokens offsets[b] .. offsets[b + 1] - 1 of k and v to positions starts[b] on of row b.  A page has one scale per head for its
  * keys and one for its values: max |x| times 1 / 127 in 32 bits (int8), or the smallest power of two that brings it to 448 or less (e4m3), codes are rounded to
@@ -578,7 +581,8 @@ int sspmm_cache_write(int type, int format, int sequences, int tokens, const int
 
 /*
  * out[b, i, h] = attention of q[b, i, h] ([sequences, queries, heads, head_dim]) over positions 0 .. lengths[b] - queries + i of row b: the
- * queries are the row's newest tokens, whose keys and values are in the cache already.  A query without any position is zeros.
+ * queries are the row's newest tokens, whose keys and values are in the cache already.  A query without any position is zeros.  out may
+ * be q, and does not overlap with it otherwise.  At most 65535 sequences, and 2^20 queries times heads.
  * workspace: sspmm_cache_attention_workspace_bytes of the same sizes, 16-byte aligned (may be 0 bytes).
  */
 size_t sspmm_cache_attention_workspace_bytes(int sequences, int queries, int heads, int kv_heads, int head_dim, int slots, int page_size);
@@ -594,9 +598,10 @@ int sspmm_cache_attention(int type, int format, int sequences, int queries, int 
  *   reserve   gives a page to every slot that holds positions starts[b] .. of row b's new tokens (offsets as above, one row of the table a
  *             sequence) and has none; when no page is free the rest go without
  *   release   the pages that the named rows hold lose a reference each, the rows' entries become -1, their lengths 0
- *   fork      row children[i], which holds no pages, becomes a copy of row parents[i]: full pages are shared, a last page that is not full is
- *             copied to a free one.  A child that finds none, or whose parent is no row or itself a child in the call, is left empty with
- *             length 0.  A row named several times as a child becomes its last naming.
+ *   fork      row children[i] becomes a copy of row parents[i]: full pages are shared, a last page that is not full is copied to one that was free
+ *             before the call, and the pages that the child held lose a reference each.  A child that finds no free page, or whose parent is no row
+ *             or becomes another row's copy in the call, is left empty with length 0.  A row that is its own parent stays as it is (and may be
+ *             another's parent).  A row named several times as a child becomes its last naming.
  *   compact   with n pages in use, the contents of those at n and behind go to the free ones below n, and the table and counts with them
  * Indices outside the table are passed over.  workspace: what the functions say (reserve: 0 where a workgroup's LDS holds it), 4-byte aligned.
  */

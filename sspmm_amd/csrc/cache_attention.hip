@@ -203,8 +203,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_attention_kernel(const C
           most = fmaxf(most, s[t][kt][i]);
         }
       most = max_over_rows(most);
-      // the reference point moves only when a row's maximum has grown by more than 2^8, which fp16 holds
-      const float new_max = fmaxf(run_max[t], most);
+      // The reference point moves only when a row's maximum has grown by more than 2^8, and lies 2^7 below it then: fp16 holds 2^15, but loses what is
+      // below 2^-25, and many keys of small probabilities are not nothing.
+      const float new_max = fmaxf(run_max[t], most - 7.0f);
       if (__ballot(new_max - run_max[t] > 8.0f) != 0) {
         const float alpha = __builtin_amdgcn_exp2f(fmaxf(run_max[t] - new_max, -126.0f));
         run_max[t] = new_max;

@@ -108,6 +108,16 @@ def _heads(heads, kv_heads, d):
         raise ValueError("the heads of q (%d) must be a multiple of those of keys and values (%d)" % (heads, kv_heads))
 
 
+def _apart(t):
+    """Whether t's elements lie at different places."""
+    reach = 0
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if stride <= reach:
+            return False
+        reach += stride * (size - 1)
+    return True
+
+
 def _out(out, q, places):
     """(out or a new tensor, its places): of q's shape, written where it lies."""
     if out is None:
@@ -117,8 +127,8 @@ def _out(out, q, places):
         raise ValueError("out must have q's shape and type and lie on its GPU")
     _no_gradients(out)
     at = places(out)
-    if at[-1] is not out:
-        raise ValueError("out must have its features side by side in 16-byte aligned rows")
+    if at[-1] is not out or not (out.is_contiguous() or _apart(out)):
+        raise ValueError("out must have its features side by side in 16-byte aligned rows that do not overlap")
     return out, at
 
 
@@ -156,7 +166,8 @@ def prompt_attention(q, k, v, offsets, scaling=None, causal=True, out=None):
     bfloat16, d = 32, 64 or 128, heads a multiple of kv_heads; sequence b is tokens offsets[b] .. offsets[b + 1] - 1 (int32 on the GPU,
     ascending).  causal: a token sees itself and those before it; otherwise all of its sequence.  Returns [tokens, heads, d]; tokens of no
     sequence are not written, in `out` either.  Views of a fused projection are read where they lie; what lies otherwise than the kernel reads
-    (features apart, rows not 16-byte aligned) is copied first.  scaling: 1 / sqrt(d) by default."""
+    (features apart, rows not 16-byte aligned) is copied first.  out may be q, and may not overlap with k and v.  scaling: 1 / sqrt(d) by
+    default."""
     dtype, device = q.dtype, q.get_device()
     kind = TYPES.get(dtype)
     if (kind is None or device < 0 or k.dtype is not dtype or v.dtype is not dtype or k.get_device() != device or v.get_device() != device or
@@ -193,7 +204,8 @@ def cache_write(k, v, offsets, starts, page_table, keys, values, scales):
     times 1 / 127 in 32 bits (int8), or the smallest power of two that brings it to 448 or less (e4m3).  Tokens before starts[b] in its page stay, at the
     larger of their scale and the new tokens'; what lies behind the last new token in its page counts as unwritten.  An infinity or NaN makes
     its block's scale NaN, until the page is written from its first position again.  Tokens for which the row has no page are dropped.  No
-    two rows of a call may write to one page (fork_pages gives every row its own last page)."""
+    two rows of a call may write to one page (fork_pages gives every row its own last page; a row that goes back in front of the position
+    where it was forked writes to pages that its relatives read, too)."""
     dtype, device = k.dtype, k.get_device()
     kind = TYPES.get(dtype)
     if kind is None or device < 0 or v.dtype is not dtype or v.get_device() != device or k.dim() != 3 or v.dim() != 3:
@@ -224,7 +236,8 @@ def cache_write(k, v, offsets, starts, page_table, keys, values, scales):
 def cache_attention(q, page_table, lengths, keys, values, scales, scaling=None, out=None):
     """Attention of the newest tokens of every row over the cache: q [rows, n, heads, d] are the last n of row b's lengths[b] tokens, whose keys
     and values are in the cache already, and query i sees positions 0 .. lengths[b] - n + i.  Returns [rows, n, heads, d]; a query that sees
-    nothing (a row shorter than n, or empty) is zeros.  Positions for which the row has no page are masked."""
+    nothing (a row shorter than n, or empty) is zeros.  Positions for which the row has no page are masked.  out may be q.  At most 65535 rows, and
+    2^20 of n * heads."""
     dtype, device = q.dtype, q.get_device()
     kind = TYPES.get(dtype)
     if kind is None or device < 0 or q.dim() != 4:
@@ -333,9 +346,10 @@ def _pool_of(pages, keys, values, scales, device):
 
 
 def fork_pages(page_refs, page_table, lengths, parents, children, keys, values, scales):
-    """Row children[i], which holds no pages, becomes a copy of row parents[i]: full pages are shared, a last page that is not full is copied to the
-    lowest free one, lengths follow.  A child for which no page is free, or whose parent is itself a child in the call, is left empty
-    with length 0.  Named twice as a child, a row becomes its last naming."""
+    """Row children[i] becomes a copy of row parents[i]: full pages are shared, a last page that is not full is copied to the lowest one that was free
+    before the call, lengths follow, and the pages that the child held lose a reference each.  A child for which no page is free, or
+    whose parent is no row or becomes another's copy in the call, is left empty with length 0.  A row that is its own parent stays as it is,
+    and may be another's parent.  Named twice as a child, a row becomes its last naming."""
     pages, rows, slots, device = _table(page_refs, page_table)
     _lengths(lengths, rows, device)
     if not (_listed(parents, 1, device) and _listed(children, 1, device)):

@@ -294,3 +294,64 @@ def test_infinities_beside_probabilities_that_underflow(built_library, causal, l
         v[at, 0, 7 + at % 5] = what
     got = sspmm_amd.prompt_attention(q, k, v, offsets_of(lengths), causal=causal)
     check_prompt(got, q, k, v, lengths, causal, 0.125)
+
+
+def _randn(shape, seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return torch.randn(shape, generator=g, device="cuda")
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_thousands_of_sequences(built_library, causal):
+    """Sequences that are found by way of more than 64 groups of 64, empty ones and tokens in front of the first among them: the bits of a few at a time."""
+    g = torch.Generator()
+    g.manual_seed(5)
+    counts = torch.randint(0, 4, (4500,), generator=g)
+    counts[1000:1200] = 0
+    counts[[64, 3000, 4499]] = 300
+    offsets = (torch.cat([torch.zeros(1, dtype=torch.long), counts.cumsum(0)]) + 200).int().cuda()
+    tokens = int(offsets[-1]) + 70
+    q, k, v = (_randn((tokens, h, 32), i).half() for i, h in ((1, 4), (2, 2), (3, 2)))
+    out = torch.full_like(q, 7.0)
+    sspmm_amd.prompt_attention(q, k, v, offsets, causal=causal, out=out)
+    want = torch.full_like(q, 7.0)
+    for b in range(0, 4500, 60):
+        sspmm_amd.prompt_attention(q, k, v, offsets[b:b + 61].clone(), causal=causal, out=want)
+    assert torch.equal(out, want)
+
+
+def test_thousands_of_small_probabilities_in_fp16(built_library):
+    """Probabilities below half of fp16's smallest number beside one of 1, together as large as what the result's type resolves: v is 1 there.  They are
+    rounded as multiples of 2^-24 / 2^7: off by 2^-32 each at most, and the sum and the result by 2^-11 of it."""
+    n = 16384
+    q = torch.zeros(n, 1, 64, device="cuda", dtype=torch.float16)
+    k, v = torch.zeros_like(q), torch.ones_like(q)
+    q[..., 0] = 1.0
+    k[1:, :, 0] = -25.5 * math.log(2.0)
+    v[0] = 0.0
+    out = sspmm_amd.prompt_attention(q, k, v, offsets_of([n]), scaling=1.0, causal=False)
+    p = math.exp(k[1, 0, 0].item())
+    want = (n - 1) * p / (1 + (n - 1) * p)
+    assert (out.double() - want).abs().max().item() <= (n - 1) * 2.0 ** -32 + want * 2.0 ** -10
+
+
+def test_in_place(built_library):
+    lengths, heads, kv, d = [700, 1, 130, 2000], 8, 2, 128
+    x = _randn((sum(lengths), (heads + 2 * kv) * d), 3).to(torch.bfloat16)
+    q, k, v = x[:, :heads * d].view(-1, heads, d), x[:, heads * d:(heads + kv) * d].view(-1, kv, d), x[:, (heads + kv) * d:].view(-1, kv, d)
+    for parts in (lengths, [2831]):  # (one sequence: two groups share the keys)
+        kept = x.clone()
+        want = sspmm_amd.prompt_attention(q, k, v, offsets_of(parts))
+        assert sspmm_amd.prompt_attention(q, k, v, offsets_of(parts), out=q) is q
+        assert torch.equal(q, want) and torch.equal(x[:, heads * d:], kept[:, heads * d:])
+        x.copy_(kept)
+
+
+def test_out_that_overlaps_itself_is_refused(built_library):
+    q, k, v = (_randn((16, 4, 64), i).half() for i in range(3))
+    narrow = torch.zeros(16, 1, 64, device="cuda", dtype=torch.float16)
+    close = torch.zeros(16 * 128 + 256, device="cuda", dtype=torch.float16).as_strided((16, 4, 64), (128, 64, 1))
+    for out in (narrow.expand(16, 4, 64), close):
+        with pytest.raises(ValueError):
+            sspmm_amd.prompt_attention(q, k, v, offsets_of([16]), out=out)
