@@ -13,7 +13,7 @@ struct PageTable {
   int32_t *refs, *table;
   int pages, rows, slots;
 };
-// A pool as bytes: of each page, key_bytes of keys, as many of values, and scale_floats.
+// A pool as bytes: of each page block_bytes of keys, as many of values, and scale_floats.
 struct PagePool {
   unsigned char *keys, *values;
   float *scales;
