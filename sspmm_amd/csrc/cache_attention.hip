@@ -1,6 +1,10 @@
 // Attention of the newest tokens of every sequence over its paged cache in 8 bits:
 //   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^((q . k_j) scale log2(e) - m),  k_j and v_j codes times their block's scale.
-// Bound by the cache's bytes, each read once: a wave's loads go from memory to the registers that the products read.
+// Bound by the cache's bytes, each read once: a wave's loads go from memory to the registers that the products read.  64 rows of 4000 tokens, 32 heads on
+// 8 of 128 features, int8 101 us, 5.2 TB/s (caches that are in no cache of the chip's); of 64 to 4063 tokens 52 us, 4.5 TB/s: with two workgroups a CU a unit of 64
+// keys is some 1.4 us of a wave's instructions (half of them make fp16 of the codes) behind 10 us of launch, look-ups and joining, which short rows
+// pay for (256 rows of 450 tokens 69 us, 3.4 TB/s).  Tried without gain: two units' loads ahead (52 -> 58 us, a wave has no time to spare for
+// them), units of 32 keys, three workgroups a CU (eleven spilled registers, 65 us), non-temporal loads.
 #include "cache_kernels.h"
 
 #include "lane_ops.h"
@@ -39,24 +43,28 @@ __device__ __forceinline__ uintx4 as_halfs(uint32_t lo, uint32_t hi) {
   return r;
 }
 
-// The sequence that a workgroup takes: of 64 consecutive ones the longest go first, where not all workgroups find a place at once.
+// The sequence that a workgroup takes: of 64 consecutive ones the longest go first, where there are more workgroups than CUs; but of those that become
+// the CUs' second ones the shortest, so that a CU that has begun on the longest gets the least beside it (64 rows of 64 to 4063 tokens, 8 heads of the
+// cache: 57.0 -> 52.3 us).
 __device__ __forceinline__ int longest_first(const int32_t *lengths, int sequences) {
-  const int z = blockIdx.z;
-  if (gridDim.x * gridDim.y * gridDim.z <= 256 || sequences == 1) return z;
+  const int z = blockIdx.z, each = gridDim.x * gridDim.y;
+  if (each * gridDim.z <= 256 || sequences == 1) return z;
   const int lane = threadIdx.x & 63, first = z & ~63, count = min(64, sequences - first);
+  const int round = 256 / each, end = min(2 * round, count);  // sequences in a round of the CUs, in both of the first
+  const int place = z >= round && z < end ? round + end - 1 - z : z - first;
   const int mine = lane < count ? lengths[first + lane] : -1;
   int rank = lane < count ? 0 : 64;
   for (int j = 0; j < count; ++j) {
     const int other = __builtin_amdgcn_readlane(mine, j);
     rank += other > mine || (other == mine && j < lane);
   }
-  return first + __builtin_ctzll(__ballot(rank == z - first));
+  return first + __builtin_ctzll(__ballot(rank == place));
 }
 
 __device__ __forceinline__ long long partial_floats(int rows, int d) { return (long long)rows * (d + 2); }
 
 // A workgroup owns 16 * TILES rows (queries x heads of one head of the cache; row i * group + j is query i, head j of the group) of one
-// sequence and one of its `splits` shares of the keys, a wave a quarter of those, UNIT keys at a time, all of them in one page.  Scores are
+// sequence and one of its `splits` shares of the keys, a wave its part of those, UNIT keys at a time, all of them in one page.  Scores are
 // made transposed, K Q^T: the lane of row m and group g holds keys UNIT / 4 * g .. of the unit, which is the operand of the second product
 // V^T P^T as it is, and the order in which values lie in a page.
 template <typename T, int FORMAT, int D, int TILES, int UNIT, int kWaves>
@@ -189,19 +197,34 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_attention_kernel(const C
     if (more) load_k(u + 1, page_next);
     const int key0 = u * UNIT, key = key0 + UNIT / 4 * g;
     const bool cut = !there || key0 + UNIT > length - p.queries + 1;  // uniform: some row does not see some key
-    uintx4 pt[TILES][kShares];
+    float v_scale_of[TILES];
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
       const float f = k_scale * c[t];
+#pragma unroll
+      for (int kt = 0; kt < kKeyTiles; ++kt) s[t][kt] *= f;
+      v_scale_of[t] = v_scale;
+    }
+    if (__builtin_expect(cut, 0)) {
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) {
+        const int left = there ? seen[t] - key : INT_MIN;
+#pragma unroll
+        for (int kt = 0; kt < kKeyTiles; ++kt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[t][kt][i] = 4 * kt + i >= left ? -INFINITY : s[t][kt][i];
+        // (a row that sees nothing of the page does not see that its scale is NaN either)
+        if (!there || key0 >= seen[t]) v_scale_of[t] = 0.f;
+      }
+    }
+    uintx4 pt[TILES][kShares];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
       float most = -INFINITY;
 #pragma unroll
       for (int kt = 0; kt < kKeyTiles; ++kt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[t][kt][i] *= f;
-          if (cut && (!there || key + 4 * kt + i >= seen[t])) s[t][kt][i] = -INFINITY;
-          most = fmaxf(most, s[t][kt][i]);
-        }
+        for (int i = 0; i < 4; ++i) most = fmaxf(most, s[t][kt][i]);
       most = max_over_rows(most);
       // The reference point moves only when a row's maximum has grown by more than 2^8, and lies 2^7 below it then: fp16 holds 2^15, but loses what is
       // below 2^-25, and many keys of small probabilities are not nothing.
@@ -226,10 +249,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_attention_kernel(const C
     // wanted at one place.  -verify-machineinstrs finds it; the build asks for that.)
 #pragma unroll
     for (int part = 0; part < kParts; ++part) asm volatile("" : "+v"(vv[part]));
-    if (FORMAT == 1 && key0 + UNIT > length) {  // (what lies behind the sequence may be NaN)
+    if (FORMAT == 1 && (!there || key0 + UNIT > length)) {  // (what lies behind the sequence, or in no page of it, may be NaN)
 #pragma unroll
       for (int w = 0; w < kValueWords; ++w) {
-        const int left = max(0, min(4, length - key - 4 * w));
+        const int left = there ? max(0, min(4, length - key - 4 * w)) : 0;
         const uint32_t mask = left == 4 ? 0xffffffffu : (1u << (8 * left)) - 1u;
 #pragma unroll
         for (int part = 0; part < kParts; ++part) vv[part][w] &= mask;
@@ -247,11 +270,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_attention_kernel(const C
 #pragma unroll
       for (int t = 0; t < TILES; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // (a row that sees nothing of the page does not see that its scale is NaN either)
-          const float x = fmaf(sum[t][i], v_scale, o[t][part][i]);
-          o[t][part][i] = cut && (!there || key0 >= seen[t]) ? o[t][part][i] : x;
-        }
+        for (int i = 0; i < 4; ++i) o[t][part][i] = fmaf(sum[t][i], v_scale_of[t], o[t][part][i]);
     }
     if (more) load_v(u + 1, page_next);
     page = page_next;
@@ -308,7 +327,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_attention_kernel(const C
 }
 
 // The splits' states of one row as one: their weights first, then D / 4 threads for the features and 1024 / D sets of them that take every so
-// manyth split.
+// manyth split.  A launch of its own, 4.5 us for 64 splits of 16 rows: three dependent loads and two barriers.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void cache_attention_join_kernel(const CacheAttentionArgs p, int row_tiles) {
   constexpr int kSets = 1024 / D;
@@ -348,6 +367,12 @@ __global__ __launch_bounds__(256) void cache_attention_join_kernel(const CacheAt
 }
 
 // Rows of the largest tiles, workgroups for the rows and heads, waves of one, and shares of the keys.
+//
+// Long rows that are few are split, as far as every CU has a workgroup, in shares of 512 keys or more; the join has to be earned: 128 workgroups (16 rows, 8 heads of
+// 128 features) split in two 2500 tokens 27.8 -> 24.3 us, 4000 38 -> 32, 8000 68 -> 56, 16 rows of 64 to 4000 33 -> 26; 192 workgroups of 4000 tokens 41 -> 50: up to
+// 128, and where rows have room for more than 2048 (one row of 131009 tokens, 4 heads: 64 splits best).
+// Eight waves a workgroup where there are few and nothing is split: eight rows of 3 to 1500 tokens, 12 heads of 64 features 13.0 -> 11.1 us; 64 rows of 2000, 8 heads
+// of 128 48 -> 56 us (one workgroup a CU has room), eight of 100 4.9 -> 6.1.
 struct Shape {
   int row_tiles, tiles, waves, splits;
 };
@@ -357,7 +382,7 @@ Shape shape_of(int sequences, int queries, int heads, int kv_heads, long long lo
   s.row_tiles = rows > 16 ? 2 : 1;
   s.tiles = (rows + 16 * s.row_tiles - 1) / (16 * s.row_tiles);
   const long long wide = (long long)sequences * kv_heads * s.tiles;
-  const bool whole = wide >= 128 || longest <= 2048;
+  const bool whole = wide > 128 || longest <= 2048;
   s.waves = whole && wide <= 128 && longest > 512 ? 8 : 4;
   s.splits = whole ? 1 : (int)max(1ll, min(min((256 + wide - 1) / wide, (longest + 511) / 512), (long long)kMostSplits));
   return s;
