@@ -552,7 +552,7 @@ int sspmm_attention_fm_ragged_f16(int batch, int heads, int seq, int head_dim, c
  * out_i = softmax over j of (q_i . k_j * scale) times v_j per sequence and head; sequence b is tokens offsets[b] .. offsets[b + 1] - 1
  * (device, sequences + 1 of them, ascending within 0 .. tokens; others are taken to the nearest of these).  causal: j <= i.  Token i,
  * head h of q is at q + i * q_row + h * q_head elements, and so on.  Tokens of no sequence are neither read nor written.  A row whose scores
- * are all -infinity is zeros.  Row strides below 2^23.  out may be q, and overlaps neither with k and v nor otherwise with q.
+ * are all -infinity is zeros.  Row strides below 2^23, (tokens / 128 + sequences) * heads below 2^23.  out may be q, and overlaps neither with k and v nor otherwise with q.
  */
 int sspmm_prompt_attention(int type, int sequences, int tokens, int heads, int kv_heads, int head_dim, const int32_t *offsets,
                            const sspmm_half_t *q, int64_t q_row, int64_t q_head, const sspmm_half_t *k, int64_t k_row, int64_t k_head,

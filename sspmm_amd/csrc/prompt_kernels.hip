@@ -394,7 +394,7 @@ template <typename T, int D, int GROUPS, bool AHEAD>
 hipError_t launch(bool causal, const PromptArgs &a, hipStream_t stream) {
   const long long tiles = (long long)a.tokens / kTileQueries + a.sequences;
   const unsigned threads = 64 * kWaves * GROUPS;
-  if (tiles * a.heads >= (1ll << 32) / threads) return hipErrorInvalidValue;  // (a launch has less than 2^32 threads)
+  if (tiles * a.heads >= 1 << 23) return hipErrorInvalidValue;  // (a launch has less than 2^32 threads)
   const unsigned blocks = (unsigned)(tiles * a.heads);
   if (causal)
     hipLaunchKernelGGL((prompt_attention_kernel<T, D, GROUPS, true, AHEAD>), dim3(blocks), dim3(threads), 0, stream, a, (int)tiles);

@@ -167,7 +167,7 @@ def prompt_attention(q, k, v, offsets, scaling=None, causal=True, out=None):
     ascending).  causal: a token sees itself and those before it; otherwise all of its sequence.  Returns [tokens, heads, d]; tokens of no
     sequence are not written, in `out` either.  Views of a fused projection are read where they lie; what lies otherwise than the kernel reads
     (features apart, rows not 16-byte aligned) is copied first.  out may be q, and may not overlap with k and v.  scaling: 1 / sqrt(d) by
-    default."""
+    default.  (tokens / 128 + sequences) * heads is below 2^23."""
     dtype, device = q.dtype, q.get_device()
     kind = TYPES.get(dtype)
     if (kind is None or device < 0 or k.dtype is not dtype or v.dtype is not dtype or k.get_device() != device or v.get_device() != device or

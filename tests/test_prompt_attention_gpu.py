@@ -355,3 +355,12 @@ def test_out_that_overlaps_itself_is_refused(built_library):
     for out in (narrow.expand(16, 4, 64), close):
         with pytest.raises(ValueError):
             sspmm_amd.prompt_attention(q, k, v, offsets_of([16]), out=out)
+
+
+def test_more_sequences_than_a_launch_holds_are_refused(built_library):
+    q, k, v = (torch.zeros(1, h, 32, device="cuda", dtype=torch.float16) for h in (32, 8, 8))
+    with pytest.raises(RuntimeError):
+        sspmm_amd.prompt_attention(q, k, v, torch.zeros(2 ** 18 + 1, dtype=torch.int32, device="cuda"))
+    offsets = torch.ones(2 ** 18 - 1, dtype=torch.int32, device="cuda")
+    offsets[0] = 0
+    assert not sspmm_amd.prompt_attention(q, k, v, offsets).any()
