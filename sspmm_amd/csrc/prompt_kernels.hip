@@ -404,19 +404,26 @@ hipError_t launch(bool causal, const PromptArgs &a, hipStream_t stream) {
 }
 
 // Two groups where one would leave half of the chip's 512 places for workgroups empty, or with a causal mask most of them while the last
-// tiles of long sequences run (lengths known on average only: a sequence of a few hundred tokens has nothing to split).
+// tiles of long sequences run (lengths known on average only: a sequence of a few hundred tokens has nothing to split).  One group and two, us: causal,
+// 128 features, 4096 tokens 16 heads 96 and 88, 8 heads 84 and 69, 1000 tokens 16 heads 27 and 25; 2048 tokens 32 heads 54 and 56; 8 x 512 tokens, 12 heads of 64 16
+// and 19.
+long long workgroups(const PromptArgs &a) { return ((long long)a.tokens + kTileQueries - 1) / kTileQueries * a.heads; }
 bool two_groups(bool causal, const PromptArgs &a) {
-  const long long tiles = ((long long)a.tokens + kTileQueries - 1) / kTileQueries * a.heads, length = a.tokens / a.sequences;
+  const long long tiles = workgroups(a), length = a.tokens / a.sequences;
   return length >= 768 && (tiles <= 256 || (causal && tiles <= 512 && length >= 3000));
 }
 
 // Waves that are between a tile's scores and its first products go ahead of the others on their SIMD.  128 features, 8 heads of 16384 tokens
-// 555 -> 526 us, 16 of 8192 284 -> 272; 64 of 4096 273 -> 281, 32 of 2048 51.0 -> 52.2: for sequences of more than 6000 tokens.
+// 542 -> 497 us, 16 of 8192 279 -> 259, 4 of 32768 1069 -> 975; 64 of 4096 273 -> 281, 32 of 2048 51.0 -> 52.2: for sequences of more than 6000 tokens.  Not
+// where little more than one round of workgroups has to be done, 512 places: 8 heads of 9000 tokens (568) 191 -> 200, 12000 (752) 286 -> 306, 12500 (784) 318 -> 327,
+// 13000 (816) 347 -> 345, 15000 (944) 465 -> 424.
+bool go_ahead(const PromptArgs &a) { return a.tokens / a.sequences > 6000 && (workgroups(a) <= 512 || workgroups(a) > 800); }
+
 template <typename T, int D>
 hipError_t launch(bool causal, const PromptArgs &a, hipStream_t stream) {
   if (two_groups(causal, a)) return launch<T, D, 2, false>(causal, a, stream);
   if constexpr (D == 128)
-    if (a.tokens / a.sequences > 6000) return launch<T, D, 1, true>(causal, a, stream);
+    if (go_ahead(a)) return launch<T, D, 1, true>(causal, a, stream);
   return launch<T, D, 1, false>(causal, a, stream);
 }
 

@@ -364,3 +364,13 @@ def test_more_sequences_than_a_launch_holds_are_refused(built_library):
     offsets = torch.ones(2 ** 18 - 1, dtype=torch.int32, device="cuda")
     offsets[0] = 0
     assert not sspmm_amd.prompt_attention(q, k, v, offsets).any()
+
+
+@pytest.mark.parametrize("tokens,heads,kv", [(6100, 4, 1), (6100, 12, 4), (6100, 20, 4)])
+def test_long_prompts_in_one_round_of_workgroups_and_more(built_library, tokens, heads, kv):
+    q, k, v = _projection(tokens, heads, kv, 128, torch.bfloat16, seed=heads)
+    for causal in (True, False):
+        got = sspmm_amd.prompt_attention(q, k, v, offsets_of([tokens]), causal=causal)
+        for h in (0, heads - 1):  # (each pair of a head of q and of k and v is a prompt of its own)
+            pair = slice(h, h + 1), slice(h * kv // heads, h * kv // heads + 1)
+            check_prompt(got[:, pair[0]], q[:, pair[0]], k[:, pair[1]], v[:, pair[1]], [tokens], causal, 1 / math.sqrt(128))
