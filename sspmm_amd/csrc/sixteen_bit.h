@@ -15,7 +15,7 @@ typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
 struct Fp16 {
   typedef _Float16 vec8 __attribute__((ext_vector_type(8)));
   typedef _Float16 vec2 __attribute__((ext_vector_type(2)));
-  static constexpr uint32_t kExponent = 0x7c00, kOne = 0x3c00, kInfinity = 0x7c00;
+  static constexpr uint32_t kExponent = 0x7c00;
   // two values rounded to nearest, ties to even, lo in the lower half
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     const vec2 h = {(_Float16)lo, (_Float16)hi};
@@ -31,7 +31,7 @@ struct Fp16 {
 struct Bf16 {
   typedef __bf16 vec8 __attribute__((ext_vector_type(8)));
   typedef __bf16 vec2 __attribute__((ext_vector_type(2)));
-  static constexpr uint32_t kExponent = 0x7f80, kOne = 0x3f80, kInfinity = 0x7f80;
+  static constexpr uint32_t kExponent = 0x7f80;
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     const vec2 h = {(__bf16)lo, (__bf16)hi};
     return __builtin_bit_cast(uint32_t, h);
