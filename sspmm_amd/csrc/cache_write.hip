@@ -69,8 +69,8 @@ __host__ __device__ __forceinline__ long long most_pages(const CacheWriteArgs &p
 // of the page and eight features, side by side with threads of other features (keys) or other places (values, which lie transposed in the page), so that
 // either's stores are whole lines and nothing passes through LDS.
 //
-// Bound by its bytes when there are many: 128 sequences of 1000 tokens, 8 heads of 128 features in bf16 191 us, 4.1 TB/s of reads and writes; 8100 tokens 14 us,
-// 3.5 TB/s; and by the chain of loads that finds a page, its scale and its tokens when there are few: 64 sequences of one token 5.6 us.
+// Bound by its bytes when there are many: 128 sequences of 1000 tokens, 8 heads of 128 features in bf16 191 us, 4.1 TB/s of reads and writes; 8084 tokens 12.6 us,
+// 3.9 TB/s; and by the chain of loads that finds a page, its scale and its tokens when there are few: 48 sequences of one token, 8 heads of 64 features 4.9 us.
 // A thread per item (64 to 256 a workgroup) instead of 256 always: 64 features, 4096 sequences of 64 tokens 504 -> 376 us, 8 of 1000 tokens 38 -> 31.
 // kMost: of these a thread takes, the page's places / 4 times D / 8 over the threads.
 template <typename T, int FORMAT, int D, int kThreads, int kMost>
