@@ -70,7 +70,7 @@ __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void prompt_attention_kern
   constexpr int kSteps = D / 16, kParts = D / 32;  // steps of the first product; parts of 32 features of the second
   constexpr int kLoads = kTile / (64 * kWaves * 16);  // pieces of 16 bytes of a tile that a thread fetches
   __shared__ __align__(16) unsigned char tiles_lds[GROUPS * 4 * kTile];  // of each group K, V, K, V
-  __shared__ int not_finite;
+  __shared__ int once_more;
   __shared__ float states[GROUPS > 1 ? (GROUPS - 1) * kWaves * 2 * 64 : 1];
   const int lane = threadIdx.x & 63, n = lane & 31, half = lane >> 5;
   const int group = GROUPS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * kWaves));
@@ -183,10 +183,31 @@ __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void prompt_attention_kern
 
   floatx16 o[kParts];  // lane (n, half): features 32 part + 8 (i / 4) + 4 half + i % 4 of its query
   float run_max, run_sum;  // of the scaled scores; this lane's share of the sum
-  bool again = false;
   const float c = p.scale_log2e;
   // fp16 loses what is below 2^-25, and many keys of small probabilities are not nothing: their largest is 2^7 or more there.
   constexpr float kHeadroom = __is_same(T, Fp16) ? 7.f : 0.f;
+
+  const auto read_v = [&](const unsigned char *tile, int part, int step) __attribute__((always_inline)) {
+    const unsigned char *const at = tile + v_rd[part] + 16 * step * (D * 2);
+    const uintx2 lo = lds_read_tr(at), hi = lds_read_tr(at + 8 * (D * 2));
+    return uintx4{lo[0], lo[1], hi[0], hi[1]};
+  };
+  const auto begin = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int part = 0; part < kParts; ++part)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[part][i] = 0.f;
+    run_max = -3.0e38f;
+    run_sum = 0.f;
+  };
+  const auto move_by = [&](float grown) __attribute__((always_inline)) {  // the reference point, by so many powers of two
+    const float alpha = __builtin_amdgcn_exp2f(fmaxf(-grown, -126.0f));
+    run_sum *= alpha;
+#pragma unroll
+    for (int part = 0; part < kParts; ++part)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[part][i] *= alpha;
+  };
 
   // Tile t, in `tile` of LDS.  cut: some query may not see all of its keys.
   const auto work_on = [&](auto cut_, const unsigned char *tile, int key0) {
@@ -218,13 +239,8 @@ __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void prompt_attention_kern
       const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
       const float new_max = fmaxf(run_max, fmaf(fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])), c, -kHeadroom));
       if (__builtin_expect(__ballot(new_max - run_max > 8.0f) != 0, 0)) {
-        const float alpha = __builtin_amdgcn_exp2f(fmaxf(run_max - new_max, -126.0f));
+        move_by(new_max - run_max);
         run_max = new_max;
-        run_sum *= alpha;
-#pragma unroll
-        for (int part = 0; part < kParts; ++part)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[part][i] *= alpha;
       }
     };
     const auto exponentials = [&](int kt) {
@@ -235,16 +251,11 @@ __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void prompt_attention_kern
         pt[2 * kt + i / 8][(i % 8) / 2] = T::pack(a, b);
       }
     };
-    const auto read_v = [&](int part, int step) {
-      const unsigned char *const at = tile + v_rd[part] + 16 * step * (D * 2);
-      const uintx2 lo = lds_read_tr(at), hi = lds_read_tr(at + 8 * (D * 2));
-      return uintx4{lo[0], lo[1], hi[0], hi[1]};
-    };
     const auto products = [&](int kt) {
 #pragma unroll
       for (int step = 2 * kt; step < 2 * kt + 2; ++step)
 #pragma unroll
-        for (int part = 0; part < kParts; ++part) o[part] = T::mfma_32x32x16(read_v(part, step), pt[step], o[part]);
+        for (int part = 0; part < kParts; ++part) o[part] = T::mfma_32x32x16(read_v(tile, part, step), pt[step], o[part]);
     };
 
     // (the second half's exponentials run beside the first half's products)
@@ -253,46 +264,70 @@ __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void prompt_attention_kern
     scores(1);
     refer();
     exponentials(0);
-    if (cut && __builtin_expect(again, 0)) {
-      if constexpr (AHEAD) __builtin_amdgcn_s_setprio(0);
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        if (kt == 1) exponentials(1);
-#pragma unroll
-        for (int step = 2 * kt; step < 2 * kt + 2; ++step)
-#pragma unroll
-          for (int part = 0; part < kParts; ++part) {
-            o[part] = T::mfma_32x32x16(finite_part<T>(read_v(part, step)), pt[step], o[part]);
-            __builtin_amdgcn_sched_barrier(0);  // (one operand at a time: registers are short)
-          }
-      }
-      uint32_t others = 0;
-#pragma unroll 1
-      for (int i = 0; i < kTile; i += 1024) {
-        const uintx4 v = *reinterpret_cast<const uintx4 *>(tile + kTile + i + lane * 16), finite = finite_part<T>(v);
-        others |= (v[0] ^ finite[0]) | (v[1] ^ finite[1]) | (v[2] ^ finite[2]) | (v[3] ^ finite[3]);
-      }
-      const int special = __ballot(others != 0) != 0 ? kKeys : 0;
-#pragma unroll 1
-      for (int r = 0; r < special; ++r) {
-        const bool sees = key0 + r < seen;
-#pragma unroll
-        for (int part = 0; part < kParts; ++part)
-#pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            const int piece = 4 * part + i / 4;
-            const uintx2 v = *reinterpret_cast<const uintx2 *>(tile + kTile + r * (D * 2) + ((piece ^ swizzle_v<D>(r)) * 16) + 8 * half);
-            const float x[4] = {T::lower(v[0]), T::upper(v[0]), T::lower(v[1]), T::upper(v[1])};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[part][i + j] += sees && !(fabsf(x[j]) < INFINITY) ? x[j] : 0.f;
-          }
-      }
-      return;
-    }
     products(0);
     if constexpr (AHEAD) __builtin_amdgcn_s_setprio(0);
     exponentials(1);
     products(1);
+  };
+
+  // The same for a workgroup that goes over its keys again, 32 of them at a time.  run_max is of the scores themselves here.
+  const auto work_again = [&](const unsigned char *tile, int key0) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (int kt = 0; kt < 2; ++kt) {
+      floatx16 s;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+      for (int step = 0; step < kSteps; ++step)
+        s = T::mfma_32x32x16(*reinterpret_cast<const uintx4 *>(tile + k_rd[step] + 32 * kt * (D * 2)), q[step], s);
+      const int left = seen - key0 - 32 * kt - 4 * half;
+      float most = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[i] = 8 * (i / 4) + i % 4 >= left ? -INFINITY : s[i];
+        most = fmaxf(most, s[i]);
+      }
+      const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
+      const float new_max = fmaxf(run_max, fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])));
+      const float grown = (new_max - run_max) * c;
+      if (__ballot(grown > 8.0f) != 0) {
+        move_by(grown);
+        run_max = new_max;
+      }
+      uintx4 pt[2];
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const float a = __builtin_amdgcn_exp2f(fmaf(s[i] - run_max, c, kHeadroom)), b = __builtin_amdgcn_exp2f(fmaf(s[i + 1] - run_max, c, kHeadroom));
+        run_sum += a + b;
+        pt[i / 8][(i % 8) / 2] = T::pack(a, b);
+      }
+#pragma unroll
+      for (int step = 0; step < 2; ++step)
+#pragma unroll
+        for (int part = 0; part < kParts; ++part)
+          o[part] = T::mfma_32x32x16(finite_part<T>(read_v(tile, part, 2 * kt + step)), pt[step], o[part]);
+    }
+    uint32_t others = 0;
+#pragma unroll 1
+    for (int i = 0; i < kTile; i += 1024) {
+      const uintx4 v = *reinterpret_cast<const uintx4 *>(tile + kTile + i + lane * 16), finite = finite_part<T>(v);
+      others |= (v[0] ^ finite[0]) | (v[1] ^ finite[1]) | (v[2] ^ finite[2]) | (v[3] ^ finite[3]);
+    }
+    const int special = __ballot(others != 0) != 0 ? kKeys : 0;
+#pragma unroll 1
+    for (int r = 0; r < special; ++r) {
+      const bool sees = key0 + r < seen;
+#pragma unroll
+      for (int part = 0; part < kParts; ++part)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const int piece = 4 * part + i / 4;
+          const uintx2 v = *reinterpret_cast<const uintx2 *>(tile + kTile + r * (D * 2) + ((piece ^ swizzle_v<D>(r)) * 16) + 8 * half);
+          const float x[4] = {T::lower(v[0]), T::upper(v[0]), T::lower(v[1]), T::upper(v[1])};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[part][i + j] += sees && !(fabsf(x[j]) < INFINITY) ? x[j] : 0.f;
+        }
+    }
   };
 
   // Group g works on tiles g, g + GROUPS, ...; all of them pass the same barriers.
@@ -307,37 +342,42 @@ __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void prompt_attention_kern
   // A masked key's probability is zero, and so is what underflows, but zero times an infinity or a NaN in v is NaN.  A workgroup that finds a
   // result which is not finite goes over its keys again: the products are of the finite values then, and the others are added, key by key,
   // to the queries that see them.  (Looking at every tile at the mask's edge first: 512 tokens, 32 heads of 128 features 17.0 us instead of 15.1.)
-  if (threadIdx.x == 0) not_finite = 0;
-  for (;; again = true) {
+  // So does one whose reference points lie beyond 2^24: an exponent is the score times c minus that, one rounding in all, but off by what the
+  // reference point was rounded by, for all keys of the query alike.  Half a power of two at most up to there; at 2^28 eight of them, and the largest probability
+  // may be infinite in fp16, or nothing.  The second time differences of scores are taken first.
+  if (threadIdx.x == 0) once_more = 0;
+  begin();
+  if (group < key_tiles) fetch(group);
+  int t0 = 0;  // group 0's tile
+  for (; t0 + 2 * GROUPS <= whole_tiles; t0 += 2 * GROUPS) {
+    const int t = t0 + group;
+    next(t);
+    work_on(whole, lds, t * kKeys);
+    next(t + GROUPS);
+    work_on(whole, lds + 2 * kTile, (t + GROUPS) * kKeys);
+  }
+  for (; t0 < key_tiles; t0 += GROUPS) {
+    const int t = t0 + group;
+    next(t);
+    if (t * kKeys < most) work_on(cut, lds + (t / GROUPS & 1) * 2 * kTile, t * kKeys);
+  }
+  float zero = 0.f;
 #pragma unroll
-    for (int part = 0; part < kParts; ++part)
+  for (int part = 0; part < kParts; ++part)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[part][i] = 0.f;
-    run_max = -3.0e38f;
-    run_sum = 0.f;
+    for (int i = 0; i < 16; ++i) zero = fmaf(o[part][i], 0.f, zero);
+  const bool far = seen > group * kKeys && !(fabsf(run_max) < 0x1p24f);  // (a query that sees none of the group's keys has no reference point)
+  if (__ballot(zero != zero || far) != 0 && lane == 0) once_more = 1;
+  __syncthreads();
+  const bool again = __builtin_amdgcn_readfirstlane(once_more) != 0;
+  if (__builtin_expect(again, 0)) {
+    begin();
     if (group < key_tiles) fetch(group);
-    int t0 = 0;  // group 0's tile
-    for (; !again && t0 + 2 * GROUPS <= whole_tiles; t0 += 2 * GROUPS) {
+    for (t0 = 0; t0 < key_tiles; t0 += GROUPS) {
       const int t = t0 + group;
       next(t);
-      work_on(whole, lds, t * kKeys);
-      next(t + GROUPS);
-      work_on(whole, lds + 2 * kTile, (t + GROUPS) * kKeys);
+      if (t * kKeys < most) work_again(lds + (t / GROUPS & 1) * 2 * kTile, t * kKeys);
     }
-    for (; t0 < key_tiles; t0 += GROUPS) {
-      const int t = t0 + group;
-      next(t);
-      if (t * kKeys < most) work_on(cut, lds + (t / GROUPS & 1) * 2 * kTile, t * kKeys);
-    }
-    if (again) break;
-    float zero = 0.f;
-#pragma unroll
-    for (int part = 0; part < kParts; ++part)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) zero = fmaf(o[part][i], 0.f, zero);
-    if (__ballot(zero != zero) != 0 && lane == 0) not_finite = 1;
-    __syncthreads();
-    if (__builtin_amdgcn_readfirstlane(not_finite) == 0) break;
   }
 
   if constexpr (GROUPS > 1) {
@@ -358,8 +398,9 @@ __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void prompt_attention_kern
     if (group > 0) return;
     for (int g = 1; g < GROUPS; ++g) {
       const float *const st = states + ((g - 1) * kWaves + wave) * 128 + lane;
-      const float new_max = fmaxf(run_max, st[0]);
-      const float mine = __builtin_amdgcn_exp2f(fmaxf(run_max - new_max, -126.0f)), theirs = __builtin_amdgcn_exp2f(fmaxf(st[0] - new_max, -126.0f));
+      const float new_max = fmaxf(run_max, st[0]), unit = again ? c : 1.f;
+      const float mine = __builtin_amdgcn_exp2f(fmaxf((run_max - new_max) * unit, -126.0f));
+      const float theirs = __builtin_amdgcn_exp2f(fmaxf((st[0] - new_max) * unit, -126.0f));
       run_max = new_max;
       run_sum = run_sum * mine + st[64] * theirs;
       const floatx4 *const from = reinterpret_cast<const floatx4 *>(tiles_lds + g * 4 * kTile) + wave * (kParts * 4 * 64) + lane;

@@ -374,3 +374,65 @@ def test_long_prompts_in_one_round_of_workgroups_and_more(built_library, tokens,
         for h in (0, heads - 1):  # (each pair of a head of q and of k and v is a prompt of its own)
             pair = slice(h, h + 1), slice(h * kv // heads, h * kv // heads + 1)
             check_prompt(got[:, pair[0]], q[:, pair[0]], k[:, pair[1]], v[:, pair[1]], [tokens], causal, 1 / math.sqrt(128))
+
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lengths,heads,kv,d,causal", [([70, 1, 200], 2, 1, 64, True), ([131], 3, 3, 32, False), ([900, 5], 1, 1, 128, True), ([6100], 6, 6, 128, False)])
+@pytest.mark.parametrize("scaling", [0.125, 1.0, 2.0 ** 40, 2.0e38])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_scores_far_beyond_what_32_bits_resolve(built_library, dtype, lengths, heads, kv, d, causal, scaling, sign):
+    """Scores of sign * 2^30 + 128 t, each exact in 32 bits, t a small whole number: softmax does not know of the 2^30.  Each probability is rounded to 16 bits (in
+    fp16 below the normal numbers: half of 2^-24 where the largest is 2^7), its exponent, 48 scaling log2(e) or next to nothing, to a few times 2^-24; the result
+    is rounded once."""
+    n = sum(lengths)
+    q, k = torch.zeros(n, heads, d, device="cuda", dtype=dtype), torch.zeros(n, kv, d, device="cuda", dtype=dtype)
+    q[..., 0], k[..., 0] = 2.0 ** 15, sign * 2.0 ** 15
+    t = torch.randint(0, 4, (n, kv), generator=torch.Generator().manual_seed(n)).cuda()
+    q[..., 1], k[..., 1] = 128.0, t.to(dtype)
+    q[::5] = 1.0  # queries of ordinary scores beside them: 0 .. 2^15 + 3
+    v = _randn((n, kv, d), 3).to(dtype)
+    got = sspmm_amd.prompt_attention(q, k, v, offsets_of(lengths), scaling=scaling, causal=causal)
+    half = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[dtype]
+    at = 0
+    for count in lengths:
+        part = slice(at, at + count)
+        visible = torch.ones(count, count, device="cuda", dtype=torch.bool)
+        visible = visible.tril() if causal else visible
+        far = torch.arange(at, at + count, device="cuda") % 5 != 0
+        for h in range(heads):
+            key = t[part, h * kv // heads]
+            most = torch.where(visible, key, -1).amax(1, keepdim=True)
+            p = torch.exp(128 * scaling * (key - most).double()).masked_fill(~visible, 0.0)
+            p /= p.sum(1, keepdim=True)
+            x = v[part, h * kv // heads].double()
+            off = (p @ x.abs()) * (half + 2.0 ** -16) + (p @ x).abs() * half + count * 2.0 ** -32 * x.abs().max() + 2.0 ** -25
+            check(got[part, h][far], (p @ x)[far], off[far] * 1.01, "sequence at %d, head %d" % (at, h))
+        at += count
+    assert torch.isfinite(got).all()
+
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [True, False])
+def test_large_queries_and_keys(built_library, dtype, causal):
+    """Normal values of size 12000: a query whose largest score is ahead of all others by more than both may be off, and 40, takes that key's v."""
+    n, d = 300, 64
+    q, k, v = (_randn((n, 2, d), i) for i in range(3))
+    q, k, v = (q * 12000).to(dtype), (k * 12000).to(dtype), v.to(dtype)
+    got = sspmm_amd.prompt_attention(q, k, v, offsets_of([n]), causal=causal)
+    assert torch.isfinite(got).all()
+    decided = 0
+    for h in range(2):
+        s = (q[:, h].double() @ k[:, h].double().t().contiguous()) / 8
+        size = (q[:, h].double().abs() @ k[:, h].double().abs().t().contiguous()).amax(1) / 8
+        if causal:
+            s = s.masked_fill(torch.ones(n, n, device="cuda", dtype=torch.bool).triu(1), float("-inf"))
+        two = s.topk(2, 1)
+        sure = two.values[:, 0] - two.values[:, 1] > 40 + 2 * size * (d + 8) * 2.0 ** -24
+        want = v[two.indices[:, 0], h].double()
+        half = 2.0 ** -11 if dtype is torch.float16 else 2.0 ** -8
+        off = want.abs() * (2 * half + 2.0 ** -17) + 1e-15
+        check(got[:, h][sure], want[sure], off[sure])
+        decided += int(sure.sum())
+    assert decided > n  # (of 2 n)
