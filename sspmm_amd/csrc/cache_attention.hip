@@ -61,6 +61,10 @@ __device__ __forceinline__ int longest_first(const int32_t *lengths, int sequenc
   return first + __builtin_ctzll(__ballot(rank == place));
 }
 
+// Sums of values are kept in units of 2^16: probabilities are up to 2^15 and values of bf16 as large as 32 bits hold, and the sum must not overflow where the
+// formula's does not.  (A scale may lose what is then below 32 bits' smallest number: 2^-127 of a value at most.)
+constexpr float kValueUnit = 0x1p-16f;
+
 __device__ __forceinline__ long long partial_floats(int rows, int d) { return (long long)rows * (d + 2); }
 
 // A workgroup owns 16 * TILES rows (queries x heads of one head of the cache; row i * group + j is query i, head j of the group) of one
@@ -145,7 +149,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_attention_kernel(const C
     pages_of = table[mine >> page_bits];
     const float *const scale = pool.scales + (long long)(usable(pages_of) ? pages_of : 0) * 2 * pool.kv_heads + head;
     k_scales = scale[0];
-    v_scales = scale[pool.kv_heads];
+    v_scales = scale[pool.kv_heads] * kValueUnit;
   };
   const auto load_k = [&](int u, int pg) {
     const unsigned char *const at = pool.keys + ((long long)(usable(pg) ? pg : 0) * pool.kv_heads + head) * block + place_of(u) * D;
@@ -318,7 +322,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_attention_kernel(const C
         partial[(long long)kRows * D + kRows + r] = total;
       }
     } else {
-      const float inv = total > 0.f || total != total ? 1.0f / total : 0.f;
+      const float inv = total > 0.f || total != total ? 1.0f / kValueUnit / total : 0.f;
       const int i = row / group, h = head * group + row % group;
       uint16_t *const to = p.out + (long long)seq * p.out_seq + (long long)i * p.out_row + (long long)h * p.out_head + d;
       *reinterpret_cast<uintx2 *>(to) = uintx2{T::pack(x[0] * inv, x[1] * inv), T::pack(x[2] * inv, x[3] * inv)};
@@ -360,7 +364,7 @@ __global__ __launch_bounds__(256) void cache_attention_join_kernel(const CacheAt
   __syncthreads();
   if (set != 0) return;
   for (int i = 1; i < kSets; ++i) x += *reinterpret_cast<const floatx4 *>(&part[i][d]);
-  const float inv = total > 0.f || total != total ? 1.0f / total : 0.f;
+  const float inv = total > 0.f || total != total ? 1.0f / kValueUnit / total : 0.f;
   const int i = row / group, h = head * group + row % group;
   uint16_t *const to = p.out + (long long)seq * p.out_seq + (long long)i * p.out_row + (long long)h * p.out_head + d;
   *reinterpret_cast<uintx2 *>(to) = uintx2{T::pack(x[0] * inv, x[1] * inv), T::pack(x[2] * inv, x[3] * inv)};

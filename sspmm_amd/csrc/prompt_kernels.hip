@@ -184,8 +184,9 @@ __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void prompt_attention_kern
   floatx16 o[kParts];  // lane (n, half): features 32 part + 8 (i / 4) + 4 half + i % 4 of its query
   float run_max, run_sum;  // of the scaled scores; this lane's share of the sum
   const float c = p.scale_log2e;
-  // fp16 loses what is below 2^-25, and many keys of small probabilities are not nothing: their largest is 2^7 or more there.
-  constexpr float kHeadroom = __is_same(T, Fp16) ? 7.f : 0.f;
+  // fp16 loses what is below 2^-25, and many keys of small probabilities are not nothing: their largest is 2^7 or more there.  bf16 does not, but its v may be as
+  // large as 32 bits hold: probabilities are 1 at most, so that sums overflow where the formula's do.
+  constexpr float kHeadroom = __is_same(T, Fp16) ? 7.f : -8.f;
 
   const auto read_v = [&](const unsigned char *tile, int part, int step) __attribute__((always_inline)) {
     const unsigned char *const at = tile + v_rd[part] + 16 * step * (D * 2);
@@ -222,7 +223,7 @@ __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void prompt_attention_kern
         s[kt] = T::mfma_32x32x16(*reinterpret_cast<const uintx4 *>(tile + k_rd[step] + 32 * kt * (D * 2)), q[step], s[kt]);
     };
     // The reference point of the exponentials moves only when some query's maximum has grown by more than 2^8: until then probabilities are up
-    // to 2^8 (fp16: 2^15) too large, which either type holds, and the accumulators stay as they are.
+    // to 2^8 times the first tile's largest, 2^15 in fp16 and 1 in bf16, and the accumulators stay as they are.
     const auto refer = [&]() {
       if constexpr (cut) {
         const int left = seen - key0 - 4 * half;

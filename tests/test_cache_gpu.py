@@ -528,3 +528,37 @@ def test_attention_into_rows_that_overlap_is_refused(built_library):
     for out in (q[:, :, :1].expand(1, 2, 4, 64), q.view(-1)[:320].as_strided((1, 2, 4, 64), (512, 64, 64, 1))):
         with pytest.raises(ValueError):
             sspmm_amd.cache_attention(q, table, _ints([40]), *cache, out=out)
+
+
+
+@pytest.mark.parametrize("form", FORMATS)
+def test_values_at_the_end_of_the_range(built_library, form):
+    """Values of up to 6e36 and keys whose scores grow by some powers of two along the row: probabilities are large numbers before they are divided by their sum."""
+    lengths, d, page = [700, 40, 5000], 64, 64
+    table, pages = _table(lengths, page, seed=31)
+    keys, values, scales = _filled(pages, 2, page, d, form, seed=32)
+    scales[:, 1] *= 6e36 / (127 if form is torch.int8 else 448) / scales[:, 1].max()
+    q = _randn((3, 2, 4, d), 33).bfloat16()
+    for rows in (slice(0, 2), slice(0, 3)):
+        got = sspmm_amd.cache_attention(q[rows], table[rows].contiguous(), _ints(lengths[rows]), keys, values, scales)
+        check_step(got, q[rows], table[rows], lengths[rows], keys, values, scales, 0.125)
+
+
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("size", [1e-36, 1e-30, 1e-6])
+def test_values_near_the_smallest(built_library, form, size):
+    """Tiny values come back as far as 32 bits hold them: a scale in units of 2^16 is off by half of 2^-149, which is 2^-134 of the scale, and 2^-127 with the largest
+    code; 2^-125 is allowed."""
+    lengths, d, page = [300, 40], 64, 64
+    table, pages = _table(lengths, page, seed=36)
+    keys, values, scales = _filled(pages, 2, page, d, form, seed=37)
+    scales[:, 1] *= size / scales[:, 1].max()
+    if form is torch.float8_e4m3fn:
+        scales[:, 1] = torch.ldexp(torch.ones(()), scales[:, 1].log2().round().cpu()).cuda()
+    q = _randn((2, 1, 4, d), 38).bfloat16()
+    got = sspmm_amd.cache_attention(q, table, _ints(lengths), keys, values, scales).double()
+    for b, n in enumerate(lengths):
+        k, v = row_of_cache(table[b], keys, values, scales, n)
+        for h in range(4):
+            want, off = attention(q[b, :, h], k[:, h // 2], v[:, h // 2], torch.tensor([n], device="cuda"), 0.125, torch.float16, torch.bfloat16)
+            check(got[b, :, h], want, off + 2.0 ** -125)

@@ -436,3 +436,16 @@ def test_large_queries_and_keys(built_library, dtype, causal):
         check(got[:, h][sure], want[sure], off[sure])
         decided += int(sure.sum())
     assert decided > n  # (of 2 n)
+
+
+
+def test_values_at_the_end_of_the_range(built_library):
+    """Means of values whose sum is still a number of 32 bits, where later tiles' scores are some powers of two larger than the first one's."""
+    n, d = 192, 64
+    q = torch.ones(n, 1, d, device="cuda", dtype=torch.bfloat16)
+    k = torch.zeros_like(q)
+    k[64:, :, 0] = 7.5
+    v = (1e36 * (1 + 0.5 * torch.rand(n, 1, d, generator=torch.Generator().manual_seed(4)))).cuda().bfloat16()
+    for causal in (True, False):
+        got = sspmm_amd.prompt_attention(q, k, v, offsets_of([n]), scaling=math.log(2.0), causal=causal)
+        check_prompt(got, q, k, v, [n], causal, math.log(2.0))
