@@ -234,11 +234,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_attention_kernel(const C
       // below 2^-25, and many keys of small probabilities are not nothing.
       const float new_max = fmaxf(run_max[t], most - 7.0f);
       if (__ballot(new_max - run_max[t] > 8.0f) != 0) {
-        const float alpha = __builtin_amdgcn_exp2f(fmaxf(run_max[t] - new_max, -126.0f));
+        const float down = half_way_down(new_max - run_max[t]);
         run_max[t] = new_max;
-        run_sum[t] *= alpha;
+        run_sum[t] = run_sum[t] * down * down;
 #pragma unroll
-        for (int part = 0; part < kParts; ++part) o[t][part] *= alpha;
+        for (int part = 0; part < kParts; ++part) o[t][part] = o[t][part] * down * down;
       }
 #pragma unroll
       for (int kt = 0; kt < kKeyTiles; ++kt)
@@ -295,9 +295,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_attention_kernel(const C
     float most = state[0][0][16 * t + m];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) most = fmaxf(most, state[w][0][16 * t + m]);
-    const float weight = __builtin_amdgcn_exp2f(fmaxf(run_max[t] - most, -126.0f));
+    const float down = half_way_down(most - run_max[t]);
 #pragma unroll
-    for (int part = 0; part < kParts; ++part) *reinterpret_cast<floatx4 *>(&sums[wave][16 * t + m][16 * part + 4 * g]) = o[t][part] * weight;
+    for (int part = 0; part < kParts; ++part) *reinterpret_cast<floatx4 *>(&sums[wave][16 * t + m][16 * part + 4 * g]) = o[t][part] * down * down;
   }
   __syncthreads();
   const int r0 = tile * kRows;
@@ -313,7 +313,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_attention_kernel(const C
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
       x += *reinterpret_cast<const floatx4 *>(&sums[w][r][d]);
-      total += state[w][1][r] * __builtin_amdgcn_exp2f(fmaxf(state[w][0][r] - most, -126.0f));
+      const float down = half_way_down(most - state[w][0][r]);
+      total += state[w][1][r] * down * down;
     }
     if (partial) {
       *reinterpret_cast<floatx4 *>(partial + (long long)r * D + d) = x;
@@ -330,7 +331,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_attention_kernel(const C
   }
 }
 
-// The splits' states of one row as one: their weights first, then D / 4 threads for the features and 1024 / D sets of them that take every so
+// The splits' states of one row as one: their weights (a factor to be taken twice) first, then D / 4 threads for the features and 1024 / D sets of them that take every so
 // manyth split.  A launch of its own, 4.5 us for 64 splits of 16 rows: three dependent loads and two barriers.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void cache_attention_join_kernel(const CacheAttentionArgs p, int row_tiles) {
@@ -350,16 +351,16 @@ __global__ __launch_bounds__(256) void cache_attention_join_kernel(const CacheAt
   if ((tid & 63) == 0) largest[tid >> 6] = most;
   __syncthreads();
   most = fmaxf(fmaxf(largest[0], largest[1]), fmaxf(largest[2], largest[3]));
-  const float weight = __builtin_amdgcn_exp2f(fmaxf(max_here - most, -126.0f));
-  if (mine) weights[tid] = weight;
-  const float sum = wave_sum_all(mine ? sum_here * weight : 0.f);
+  const float down = half_way_down(most - max_here);
+  if (mine) weights[tid] = down;
+  const float sum = wave_sum_all(mine ? sum_here * down * down : 0.f);
   if ((tid & 63) == 0) totals_of[tid >> 6] = sum;
   __syncthreads();
   const float total = (totals_of[0] + totals_of[1]) + (totals_of[2] + totals_of[3]);
   const int set = tid / (D / 4), d = (tid % (D / 4)) * 4;
   floatx4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-  for (int s = set; s < p.splits; s += kSets) x += *reinterpret_cast<const floatx4 *>(base + s * pitch + (long long)r * D + d) * weights[s];
+  for (int s = set; s < p.splits; s += kSets) x += *reinterpret_cast<const floatx4 *>(base + s * pitch + (long long)r * D + d) * weights[s] * weights[s];
   *reinterpret_cast<floatx4 *>(&part[set][d]) = x;
   __syncthreads();
   if (set != 0) return;

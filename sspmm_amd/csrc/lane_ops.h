@@ -139,6 +139,10 @@ __device__ __forceinline__ float sum_over_rows(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// The factor that, taken twice, brings a sum of exponentials or of what they weigh to a reference point x >= 0 powers of two above its own.  (One factor
+// ends at 2^-126, and 2^-126 of a value near the end of the range is a number like any other.  At 2^-252 nothing is left of it, and what is infinite stays so.)
+__device__ __forceinline__ float half_way_down(float x) { return __builtin_amdgcn_exp2f(-0.5f * fminf(x, 252.0f)); }
+
 // Sum of v over the lanes of the wave with the same lane % 4, in each of them.
 __device__ __forceinline__ float sum_over_quads(float v) {
   v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, false));  // rotated by 8 in each 16

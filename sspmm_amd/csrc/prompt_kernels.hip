@@ -202,12 +202,12 @@ __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void prompt_attention_kern
     run_sum = 0.f;
   };
   const auto move_by = [&](float grown) __attribute__((always_inline)) {  // the reference point, by so many powers of two
-    const float alpha = __builtin_amdgcn_exp2f(fmaxf(-grown, -126.0f));
-    run_sum *= alpha;
+    const float down = half_way_down(grown);
+    run_sum = run_sum * down * down;
 #pragma unroll
     for (int part = 0; part < kParts; ++part)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[part][i] *= alpha;
+      for (int i = 0; i < 16; ++i) o[part][i] = o[part][i] * down * down;
   };
 
   // Tile t, in `tile` of LDS.  cut: some query may not see all of its keys.
@@ -400,10 +400,9 @@ __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void prompt_attention_kern
     for (int g = 1; g < GROUPS; ++g) {
       const float *const st = states + ((g - 1) * kWaves + wave) * 128 + lane;
       const float new_max = fmaxf(run_max, st[0]), unit = again ? c : 1.f;
-      const float mine = __builtin_amdgcn_exp2f(fmaxf((run_max - new_max) * unit, -126.0f));
-      const float theirs = __builtin_amdgcn_exp2f(fmaxf((st[0] - new_max) * unit, -126.0f));
+      const float mine = half_way_down((new_max - run_max) * unit), theirs = half_way_down((new_max - st[0]) * unit);
       run_max = new_max;
-      run_sum = run_sum * mine + st[64] * theirs;
+      run_sum = run_sum * mine * mine + st[64] * theirs * theirs;
       const floatx4 *const from = reinterpret_cast<const floatx4 *>(tiles_lds + g * 4 * kTile) + wave * (kParts * 4 * 64) + lane;
 #pragma unroll
       for (int part = 0; part < kParts; ++part)
@@ -411,7 +410,7 @@ __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void prompt_attention_kern
         for (int i = 0; i < 4; ++i) {
           const floatx4 x = from[(part * 4 + i) * 64];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) o[part][4 * i + j] = o[part][4 * i + j] * mine + x[j] * theirs;
+          for (int j = 0; j < 4; ++j) o[part][4 * i + j] = o[part][4 * i + j] * mine * mine + x[j] * theirs * theirs;
         }
     }
   }

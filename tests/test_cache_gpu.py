@@ -562,3 +562,33 @@ def test_values_near_the_smallest(built_library, form, size):
         for h in range(4):
             want, off = attention(q[b, :, h], k[:, h // 2], v[:, h // 2], torch.tensor([n], device="cuda"), 0.125, torch.float16, torch.bfloat16)
             check(got[b, :, h], want, off + 2.0 ** -125)
+
+
+
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("splits", [False, True])
+@pytest.mark.parametrize("place,below", [(0, 100.0), (0, 140.0), (0, 200.0), (700, 140.0), (1100, 200.0), (1100, 500.0)])
+def test_large_values_of_small_probability(built_library, form, splits, place, below):
+    """v of 1e38 in a page whose keys' scores lie `below` powers of two under the others': its share is there as long as 2^-below of it is, and nothing else of it."""
+    page, d, n = 32, 64, 1200
+    slots = 2048 // page + (40 if splits else 0)
+    keys, values, scales = sspmm_amd.new_cache(n // page + 1, 1, page, d, form)
+    largest = 127.0 if form is torch.int8 else 448.0
+    table = torch.full((1, slots), -1, dtype=torch.int32, device="cuda")
+    table[0, :-(-n // page)] = torch.arange(-(-n // page))
+    values.view(torch.int8).copy_(torch.full(values.shape, largest, device="cuda").to(form).view(torch.int8))
+    scales[:, 1] = 1.0 / largest
+    low = place // page
+    keys.view(torch.int8)[low, :, :, 0] = torch.tensor(-largest, device="cuda").to(form).view(torch.int8)
+    scales[:, 0] = below / largest
+    scales[low, 1] = 1e38 / largest
+    q = torch.zeros(1, 1, 1, d, device="cuda", dtype=torch.bfloat16)
+    q[..., 0] = 1.0
+    got = sspmm_amd.cache_attention(q, table, _ints([n]), keys, values, scales, scaling=math.log(2.0))
+    big, p = scales[low, 1, 0].double() * largest, 2.0 ** (-largest * scales[low, 0, 0].double())
+    count = min(page, n - low * page)
+    want = ((n - count) + count * p * big) / (n - count + count * p)
+    # a probability's half step in fp16, what scaling and the scales of 32 bits are off by, the result's half step; behind larger ones the page's
+    # probabilities are nothing in fp16
+    off = want * (2.0 ** -11 + 2.0 ** -18 + below * 2.0 ** -21 + 2.0 ** -8) + (count * p * big / (n - count) if place else 0.0)
+    check(got.flatten(), want.expand(d), (off * 1.01).expand(d))

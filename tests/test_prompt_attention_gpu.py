@@ -449,3 +449,25 @@ def test_values_at_the_end_of_the_range(built_library):
     for causal in (True, False):
         got = sspmm_amd.prompt_attention(q, k, v, offsets_of([n]), scaling=math.log(2.0), causal=causal)
         check_prompt(got, q, k, v, [n], causal, math.log(2.0))
+
+
+
+@pytest.mark.parametrize("n,causal", [(200, True), (200, False), (1700, True), (1700, False)])
+@pytest.mark.parametrize("below", [100.0, 140.0, 200.0, 500.0])
+@pytest.mark.parametrize("first", [0, 64, 128])
+def test_large_values_of_small_probability(built_library, n, causal, below, first):
+    """v of 1e38 at 64 keys whose scores lie `below` powers of two under the others': their share is there as long as it is a number, and nothing else of them."""
+    d, large = 64, slice(first, first + 64)
+    q = torch.zeros(n, 1, d, device="cuda", dtype=torch.bfloat16)
+    k, v = torch.zeros_like(q), torch.ones_like(q)
+    q[..., 0], k[..., 0] = 1.0, below
+    k[large], v[large] = 0.0, 1e38
+    got = sspmm_amd.prompt_attention(q, k, v, offsets_of([n]), scaling=math.log(2.0), causal=causal)[:, 0]
+    big, p = v[first, 0, 0].double(), 2.0 ** -below
+    seen = torch.arange(1, n + 1, device="cuda")[:, None].double() if causal else torch.full((n, 1), n, device="cuda").double()
+    low = (seen - first).clamp(0, 64)
+    high = seen - low
+    want = (high + low * p * big) / (high + low * p)
+    # half a step of each probability (bf16), what scaling and its product with log2(e) are off by, the result's half step; a probability below 2^-126 may be nothing
+    off = want * (2.0 ** -8 + 2.0 ** -18 + below * 2.0 ** -22) + want * 2.0 ** -8 + torch.where(high > 0, low * p * big if below > 110 else 0.0, 0.0)
+    check(got, want.expand(-1, d), (off * 1.01).expand(-1, d))
