@@ -87,7 +87,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_attention_kernel(const C
   const int group = p.heads / pool.kv_heads, rows = p.queries * group, tiles = (rows + kRows - 1) / kRows;
   const int split = blockIdx.y, head = blockIdx.x % pool.kv_heads, tile = blockIdx.x / pool.kv_heads;
   const int seq = longest_first(p.lengths, p.sequences);
-  const int length = max(0, (int)min((long long)p.lengths[seq], (long long)pool.slots * pool.page_size));
+  // (tokens that the table has no slot for are nowhere, but the queries' positions count them)
+  const int all_length = max(0, p.lengths[seq]), length = (int)min((long long)all_length, (long long)pool.slots * pool.page_size);
   const int units = (length + UNIT - 1) / UNIT, pieces = p.splits * kWaves, piece = split * kWaves + wave;
   const int unit0 = (int)((long long)units * piece / pieces), unit1 = (int)((long long)units * (piece + 1) / pieces);
 
@@ -98,7 +99,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_attention_kernel(const C
 #pragma unroll
   for (int t = 0; t < TILES; ++t) {
     const int row = tile * kRows + 16 * t + m, r = row < rows ? row : 0, i = r / group;
-    seen[t] = length - p.queries + 1 + i;
+    seen[t] = all_length - p.queries + 1 + i;
     const uint16_t *const at = p.q + (long long)seq * p.q_seq + (long long)i * p.q_row + (long long)(head * group + r % group) * p.q_head;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
@@ -200,7 +201,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_attention_kernel(const C
     }
     if (more) load_k(u + 1, page_next);
     const int key0 = u * UNIT, key = key0 + UNIT / 4 * g;
-    const bool cut = !there || key0 + UNIT > length - p.queries + 1;  // uniform: some row does not see some key
+    const bool cut = !there || key0 + UNIT > all_length - p.queries + 1;  // uniform: some row does not see some key
     float v_scale_of[TILES];
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {

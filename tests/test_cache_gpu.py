@@ -592,3 +592,19 @@ def test_large_values_of_small_probability(built_library, form, splits, place, b
     # probabilities are nothing in fp16
     off = want * (2.0 ** -11 + 2.0 ** -18 + below * 2.0 ** -21 + 2.0 ** -8) + (count * p * big / (n - count) if place else 0.0)
     check(got.flatten(), want.expand(d), (off * 1.01).expand(d))
+
+
+
+def test_rows_longer_than_their_table(built_library):
+    """Tokens for which the table has no slot were dropped, and count all the same: query i sees positions 0 .. length - n + i, those behind the table masked."""
+    page, d, n = 32, 64, 4
+    pool = _filled(6, 1, page, d, torch.int8, seed=34)
+    table = _ints([[4, 0], [1, 2], [3, 5], [0, 1], [2, 3]])
+    lengths = [64, 65, 66, 90, 2 ** 31 - 1]
+    q = _randn((5, n, 2, d), 35).half()
+    got = sspmm_amd.cache_attention(q, table, _ints(lengths), *pool)
+    for b, length in enumerate(lengths):
+        k, v = row_of_cache(table[b], *pool, 64)
+        visible = torch.tensor([min(64, length - n + 1 + i) for i in range(n)], device="cuda")
+        for h in range(2):
+            check(got[b, :, h], *attention(q[b, :, h], k[:, 0], v[:, 0], visible, 0.125, torch.float16, torch.float16), "row %d" % b)
