@@ -98,7 +98,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_attention_kernel(const C
   int seen[TILES];  // keys that the row sees: those below
 #pragma unroll
   for (int t = 0; t < TILES; ++t) {
-    const int row = tile * kRows + 16 * t + m, r = row < rows ? row : 0, i = r / group;
+    // (Places behind the last row take that one's query: it lies in the workgroup's own tile, since out may be q and others write theirs while this reads, and
+    // its maxima move no reference point that it does not move itself.)
+    const int r = min(tile * kRows + 16 * t + m, rows - 1), i = r / group;
     seen[t] = all_length - p.queries + 1 + i;
     const uint16_t *const at = p.q + (long long)seq * p.q_seq + (long long)i * p.q_row + (long long)(head * group + r % group) * p.q_head;
 #pragma unroll

@@ -608,3 +608,17 @@ def test_rows_longer_than_their_table(built_library):
         visible = torch.tensor([min(64, length - n + 1 + i) for i in range(n)], device="cuda")
         for h in range(2):
             check(got[b, :, h], *attention(q[b, :, h], k[:, 0], v[:, 0], visible, 0.125, torch.float16, torch.float16), "row %d" % b)
+
+
+@pytest.mark.parametrize("n,heads,kv,lengths", [(70, 4, 4, [70, 500, 1000]), (33, 8, 8, [800] * 20), (21, 6, 2, [64, 1900, 40]), (17, 8, 4, [300] * 40), (49, 4, 4, [9000])])
+def test_in_place_with_several_tiles_of_queries(built_library, n, heads, kv, lengths):
+    """Queries that fill more than a workgroup's places, the last tile in part: written over q they are the bits that they are beside it, however often."""
+    table, pages = _table(lengths, 64, seed=39)
+    cache = _filled(pages, kv, 64, 64, torch.int8, seed=40)
+    q = (_randn((len(lengths), n, heads, 64), 41) * 2.0 ** torch.arange(n, device="cuda").view(1, n, 1, 1).remainder(5)).half()
+    want = sspmm_amd.cache_attention(q, table, _ints(lengths), *cache)
+    check_step(want, q, table, lengths, *cache, 0.125)
+    for _ in range(10):
+        x = q.clone()
+        assert sspmm_amd.cache_attention(x, table, _ints(lengths), *cache, out=x) is x
+        assert torch.equal(x, want)
