@@ -595,8 +595,9 @@ int sspmm_cache_attention(int type, int format, int sequences, int queries, int 
 /*
  * Pages.  page_refs[pages]: how many table entries name a page; it is free where that is not positive.  Free pages are taken lowest
  * first, in the order of rows and slots or of children.
- *   reserve   gives a page to every slot that holds positions starts[b] .. of row b's new tokens (offsets as above, one row of the table a
- *             sequence) and has none; when no page is free the rest go without
+ *   reserve   gives a page to every slot that begins with one of row b's new tokens, at positions starts[b] .. (offsets as above, one row of the
+ *             table a sequence), and has none; when no page is free the rest go without.  A slot that begins before starts[b] and has none has lost the
+ *             tokens in front: it stays without
  *   release   the pages that the named rows hold lose a reference each, the rows' entries become -1, their lengths 0
  *   fork      row children[i] becomes a copy of row parents[i]: full pages are shared, a last page that is not full is copied to one that was free
  *             before the call, and the pages that the child held lose a reference each.  A child that finds no free page, or whose parent is no row

@@ -59,14 +59,15 @@ __device__ uint32_t take_free_pages(int32_t *refs, int pages, uint32_t need, int
   return min(found, need);
 }
 
-// The slots of row b that hold positions starts[b] .. of its new tokens: first .. end - 1.
+// The slots of row b that begin with one of the new tokens, at positions starts[b] ..: first .. end - 1.  (A slot that they go on in has its page, or has lost the
+// tokens in front of them: a page given to it now would show what was in it before as theirs.)
 __device__ __forceinline__ void new_slots(const int32_t *starts, const int32_t *offsets, int b, int page_size, int slots, int *first, int *end) {
   const int start = starts[b];
   const long long n = (long long)offsets[b + 1] - offsets[b];
   *first = 0;
   *end = 0;
   if (start < 0 || n <= 0) return;
-  *first = start / page_size;
+  *first = start / page_size + (start % page_size != 0);
   *end = (int)min((long long)slots, (start + n + page_size - 1) / page_size);
 }
 

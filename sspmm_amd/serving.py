@@ -296,9 +296,10 @@ def _room(page_refs, entry, *sizes):
 
 
 def reserve_pages(page_refs, page_table, starts, offsets, page_size):
-    """Gives a page to every slot of page_table [rows, slots] that is to hold row b's new tokens, offsets[b + 1] - offsets[b] of them from
+    """Gives a page to every slot of page_table [rows, slots] that begins with one of row b's new tokens, offsets[b + 1] - offsets[b] of them from
     position starts[b] on, and has none (an entry below zero): the lowest free ones, in the order of rows and slots.  page_refs [pages]: how many entries
-    name a page, free where that is not positive.  When no page is free the rest stay without."""
+    name a page, free where that is not positive.  When no page is free the rest stay without, and a slot whose first position was given none stays
+    without until the row is released: its tokens are dropped, and masked."""
     pages, rows, slots, device = _table(page_refs, page_table)
     if not (_listed(starts, 1, device) and _listed(offsets, 1, device)):
         _ints("starts", starts, 1, device)

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import sspmm_amd
-from serving_util import check_prompt, check_step, offsets_of, row_of_cache
+from serving_util import attention, check, check_prompt, check_step, offsets_of, row_of_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -326,3 +326,48 @@ def test_beams_that_take_the_places_of_others(built_library, seed):
         dev.same(model, "seed %d, step %d: %s of %s" % (seed, step, children, parents))
         held = [p for row in model.table for p in row if p >= 0]
         assert model.refs == [held.count(p) for p in range(pages)]
+
+
+
+@pytest.mark.parametrize("form", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("old", [100.0, float("nan")])
+def test_a_page_that_was_missing_is_not_entered_in_the_middle(built_library, form, old):
+    """A row whose tokens found no free page goes on when another row's pages are free again: the positions that were dropped stay masked, nothing of the other row's
+    keys, values and scales is read or kept."""
+    page, kv, heads, d, pages = 32, 2, 4, 64, 3
+    g = torch.Generator(device="cuda")
+    g.manual_seed(41)
+    cache = sspmm_amd.new_cache(pages, kv, page, d, form)
+    refs, table, lengths = _ints([0] * pages), torch.full((3, 4), -1, dtype=torch.int32, device="cuda"), _ints([0, 0, 0])
+
+    def put(counts, size=1.0):
+        x = (torch.randn(sum(counts), 2, kv, d, generator=g, device="cuda") * size).half()
+        sspmm_amd.reserve_pages(refs, table, lengths, offsets_of(counts), page)
+        sspmm_amd.cache_write(x[:, 0], x[:, 1], offsets_of(counts), lengths, table, *cache)
+        lengths.add_(_ints(counts))
+        return x
+
+    def step(n):
+        q = torch.randn(3, n, heads, d, generator=g, device="cuda").half()
+        return q, sspmm_amd.cache_attention(q, table, lengths, *cache)
+
+    put([40, 20, 0], old if old == old else 1.0)
+    if old != old:
+        cache[2][table[0, :2].long()] = old
+    put([0, 0, 10])  # there is no page for these
+    assert refs.tolist() == [1, 1, 1] and (table[2] < 0).all()
+    sspmm_amd.release_pages(refs, table, lengths, _ints([0]))
+    put([0, 0, 5])  # positions 10 .. 14: their page has lost its front
+    assert (table[2] < 0).all() and refs.tolist() == [0, 0, 1]
+    assert not step(1)[1][2].any()
+    x = put([0, 0, 30])  # 15 .. 44: of these, 32 .. 44 lie in a page that begins with them
+    assert table[2].tolist() == [-1, 0, -1, -1] and refs.tolist() == [1, 0, 1]
+    k, v = row_of_cache(table[2, 1:], *cache, 13)
+    for i, got in enumerate((k, v)):
+        s = cache[2][0, i].double()[None, :, None]
+        want = x[17:, i].double()
+        assert ((got - want).abs() <= (s * 0.5 if form is torch.int8 else want.abs() * 2.0 ** -4 + s * 2.0 ** -10) * 1.001).all()
+    q, got = step(2)
+    for h in range(heads):
+        visible = torch.tensor([12, 13], device="cuda")
+        check(got[2, :, h], *attention(q[2, :, h], k[:, h // 2], v[:, h // 2], visible, 0.125, torch.float16, torch.float16))
