@@ -10,7 +10,7 @@ tokens after them are written to and read from.  They stand beside the attention
 
 Lists and tables are int32 tensors on the GPU, read when the kernels run: no call waits for the device, so a step can be captured in a
 graph.  What the device alone knows is not checked by the host: entries that name no token, row or page are passed over.
-Inference only, as all operators here: inputs that want gradients are refused.
+Inference only, as all operators here: inputs that want gradients, backward or forward, are refused.
 """
 import functools
 import math
@@ -19,6 +19,8 @@ import torch
 
 from . import _lib
 from .attention import FUSED_HEAD_WIDTHS as HEAD_WIDTHS
+
+_forward_ad = torch.autograd.forward_ad
 
 TYPES = {torch.float16: 0, torch.bfloat16: 1}
 CACHE_TYPES = {torch.int8: 0, torch.float8_e4m3fn: 1}
@@ -64,6 +66,10 @@ def _no_gradients(*tensors):
         for t in tensors:
             if t.requires_grad:
                 raise RuntimeError("an argument wants gradients, and this operator has no backward pass")
+    if _forward_ad._current_level >= 0:
+        for t in tensors:
+            if _forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("an argument carries forward-mode gradients, and this operator has no rule for them")
 
 
 def _tokens(t):
@@ -211,7 +217,7 @@ def cache_write(k, v, offsets, starts, page_table, keys, values, scales):
     if kind is None or device < 0 or v.dtype is not dtype or v.get_device() != device or k.dim() != 3 or v.dim() != 3:
         _activations("k", k, 3, dtype, device)
         _activations("v", v, 3, dtype, device)
-    _no_gradients(k, v)
+    _no_gradients(k, v, keys, values, scales)
     form, pages, kv, page_size, d = _cache(keys, values, scales, device)
     tokens = k.size(0)
     if k.shape != (tokens, kv, d) or v.shape != k.shape:
@@ -242,7 +248,7 @@ def cache_attention(q, page_table, lengths, keys, values, scales, scaling=None, 
     kind = TYPES.get(dtype)
     if kind is None or device < 0 or q.dim() != 4:
         _activations("q", q, 4, dtype, device)
-    _no_gradients(q)
+    _no_gradients(q, keys, values, scales)
     form, pages, kv, page_size, d = _cache(keys, values, scales, device)
     rows, n, heads, dq = q.shape
     if dq != d:
@@ -340,6 +346,7 @@ def release_pages(page_refs, page_table, lengths, rows):
 
 
 def _pool_of(pages, keys, values, scales, device):
+    _no_gradients(keys, values, scales)
     _, held, kv, page_size, d = _cache(keys, values, scales, device)
     if pages != held:
         raise ValueError("page_refs must have a count for each of the cache's %d pages" % held)

@@ -622,3 +622,46 @@ def test_in_place_with_several_tiles_of_queries(built_library, n, heads, kv, len
         x = q.clone()
         assert sspmm_amd.cache_attention(x, table, _ints(lengths), *cache, out=x) is x
         assert torch.equal(x, want)
+
+
+
+def test_whatever_wants_gradients_is_refused(built_library):
+    """Gradients backward and forward, of activations and of scales: none is dropped without a word."""
+    from torch.autograd import forward_ad
+    cache = sspmm_amd.new_cache(4, 2, 32, 64)
+    table, n, off, start = _ints([[0, 1]]), _ints([40]), offsets_of([3]), _ints([0])
+    q, k = _randn((1, 1, 4, 64), 1).half(), _randn((3, 2, 64), 2).half()
+
+    def calls(wrap):
+        keys, values, scales = cache
+        return (lambda: sspmm_amd.prompt_attention(wrap(k), k, k, off), lambda: sspmm_amd.prompt_attention(k, wrap(k), k, off),
+                lambda: sspmm_amd.prompt_attention(k, k, wrap(k), off), lambda: sspmm_amd.prompt_attention(k, k, k, off, out=wrap(k.clone())),
+                lambda: sspmm_amd.cache_attention(wrap(q), table, n, *cache), lambda: sspmm_amd.cache_attention(q, table, n, keys, values, wrap(scales)),
+                lambda: sspmm_amd.cache_attention(q, table, n, *cache, out=wrap(q.clone())),
+                lambda: sspmm_amd.cache_write(wrap(k), k, off, start, table, *cache), lambda: sspmm_amd.cache_write(k, wrap(k), off, start, table, *cache),
+                lambda: sspmm_amd.cache_write(k, k, off, start, table, keys, values, wrap(scales)))
+
+    for call in calls(lambda t: t.detach().clone().requires_grad_()):
+        with pytest.raises(RuntimeError, match="gradients"):
+            call()
+    with forward_ad.dual_level():
+        for call in calls(lambda t: forward_ad.make_dual(t, torch.ones_like(t))):
+            with pytest.raises(RuntimeError, match="gradients"):
+                call()
+        sspmm_amd.cache_write(k, k, off, start, table, *cache)  # (others than these, while a level is open, are as ever)
+        assert torch.isfinite(sspmm_amd.cache_attention(q, table, n, *cache)).all()
+    for f in (lambda x: sspmm_amd.prompt_attention(x, k, k, off), lambda x: sspmm_amd.prompt_attention(k, k, x, off)):
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(f, (k,), (torch.ones_like(k),))
+        with pytest.raises(RuntimeError):
+            torch.func.vjp(f, k)
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(f)(k.expand(2, 3, 2, 64))
+    refs, length = _ints([1, 1, 0, 0]), _ints([40])
+    for wanting in (cache[2].clone().requires_grad_(), None):
+        with forward_ad.dual_level():
+            scales = forward_ad.make_dual(cache[2], torch.ones_like(cache[2])) if wanting is None else wanting
+            for call in (lambda: sspmm_amd.fork_pages(refs, table, length, _ints([0]), _ints([0]), *cache[:2], scales),
+                         lambda: sspmm_amd.compact_pages(refs, table, *cache[:2], scales)):
+                with pytest.raises(RuntimeError, match="gradients"):
+                    call()

@@ -94,3 +94,19 @@ def test_python_entries_want_a_gpu(built_library):
             call()
     with pytest.raises(TypeError):
         sspmm_amd.new_cache(2, 1, 32, 64, torch.uint8, "cpu")
+
+
+def test_gradients_are_noticed(built_library):
+    """Backward and forward, before anything else is asked of an argument."""
+    from torch.autograd import forward_ad
+    from sspmm_amd import serving
+    t = torch.ones(3)
+    serving._no_gradients(t)
+    with pytest.raises(RuntimeError, match="gradients"):
+        serving._no_gradients(t, t.clone().requires_grad_())
+    with forward_ad.dual_level():
+        serving._no_gradients(t)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            serving._no_gradients(t, forward_ad.make_dual(t, t))
+    with torch.no_grad():
+        serving._no_gradients(t.clone().requires_grad_())
