@@ -33,8 +33,11 @@ __device__ __forceinline__ int swizzle_v(int r) {
 // the next one's loads (16001 tokens, 8 heads: 619 us with the builtin); the waits for these are the ones before the barriers below.
 typedef int srd __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void load_to_lds(srd from, uint32_t at, uint32_t to) {
-  // (m0 is nobody else's here.  The wait is what a vector instruction that wrote one of the scalars just before would need.)
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(at), "s"(from) : "memory");
+  // m0 is the compiler's (it takes no such clobber): it is put back, which the load, once issued, does not mind.  (The wait is what a vector instruction that wrote
+  // one of the scalars just before would need.)
+  uint32_t kept;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+               : "=&s"(kept) : "s"(to), "v"(at), "s"(from) : "memory");
 }
 __device__ __forceinline__ srd descriptor(const uint16_t *base, uint32_t bytes) {
   const uint64_t b = reinterpret_cast<uint64_t>(base);
