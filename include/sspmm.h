@@ -600,9 +600,9 @@ int sspmm_cache_attention(int type, int format, int sequences, int queries, int 
  *             tokens in front: it stays without
  *   release   the pages that the named rows hold lose a reference each, the rows' entries become -1, their lengths 0
  *   fork      row children[i] becomes a copy of row parents[i]: full pages are shared, a last page that is not full is copied to one that was free
- *             before the call, and the pages that the child held lose a reference each.  A child that finds no free page, or whose parent is no row
- *             or becomes another row's copy in the call, is left empty with length 0.  A row that is its own parent stays as it is (and may be
- *             another's parent).  A row named several times as a child becomes its last naming.
+ *             before the call, and the pages that the child held lose a reference each.  A child that finds no free page, or whose parent is no row,
+ *             has no page for its last tokens or becomes another row's copy in the call, is left empty with length 0.  A row that is its own parent
+ *             stays as it is (and may be another's parent).  A row named several times as a child becomes its last naming.
  *   compact   with n pages in use, the contents of those at n and behind go to the free ones below n, and the table and counts with them
  * Indices outside the table are passed over.  workspace: what the functions say (reserve: 0 where a workgroup's LDS holds it), 4-byte aligned.
  */

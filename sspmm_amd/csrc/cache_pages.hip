@@ -71,8 +71,9 @@ __device__ __forceinline__ void new_slots(const int32_t *starts, const int32_t *
   *end = (int)min((long long)slots, (start + n + page_size - 1) / page_size);
 }
 
-// Chains of a few loads and barriers, a microsecond or three whatever the sizes: 48 rows of one new token 1.9 us, five prompts 3.4.
-// One workgroup: a wave counts a row's slots without a page, ranks follow in the order of rows and slots, the list of free pages is made, and
+// Chains of loads and barriers, one workgroup, whose waves take their rows one after the other: 48 rows of one new token 3.0 us where all pages are there and 6.0
+// where one is given, five prompts 2.0 and 5.0 (127 pages); 256 rows 9.6 and 21, 4096 rows 138 and 275, and 356 where a quarter of a million pages in use come first.
+// A wave counts a row's slots without a page, ranks follow in the order of rows and slots, the list of free pages is made, and
 // the slots take theirs.  workspace: the ranks, then the list; null: in LDS.
 __global__ __launch_bounds__(kPlanThreads) void reserve_pages_kernel(const PageTable t, const int32_t *starts, const int32_t *offsets, int page_size,
                                                                      int32_t *workspace) {
@@ -192,7 +193,7 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(const PageTable
 }
 
 // A part of page `source` to page `target`.  Bound by memory: 131 MB of pages 65.7 us a call as one piece of 16 bytes of either side after the other, 63.3 with
-// four of them on their way and twice as many workgroups (the plan before it is 5 of these; 45 us and 5.8 TB/s where the last-level cache has the pool).
+// four of them on their way and twice as many workgroups (the plan before it is 5 of these; 42 us and 6.3 TB/s where the last-level cache has the pool).
 __device__ __forceinline__ void copy_page(const PagePool &pool, int source, int target, int part, int parts) {
   const long long pieces = pool.block_bytes / 16;
   const long long from = pieces * part / parts, upto = pieces * (part + 1) / parts;

@@ -59,12 +59,12 @@ __device__ __forceinline__ uintx4 finite_part(uintx4 v) {
 // Scores are made transposed, K Q^T, so that a lane holds 32 of a tile's 64 scores of ONE query: maxima and sums are taken
 // inside the lane, but for one exchange with the lane 32 apart, and what the matrix instruction leaves is, rounded to 16 bits, the operand P^T
 // of the second product V^T P^T, whose contraction slots are numbered accordingly: slots of lane half h in step t are keys
-// 16 t + 4 h + {0 .. 3, 8 .. 11}.  V^T comes from transpose reads.  Two buffers of K and V, one barrier a tile, two workgroups a CU (64 KB and up to 256
+// 16 t + 4 h + {0 .. 3, 8 .. 11}.  V^T comes from transpose reads.  Two buffers of K and V, one barrier a tile, two workgroups a CU (64 KB and up to 228
 // registers a lane with 128 features).
 //
-// Bound by the matrix instructions and the power they take: 16384 tokens, 8 heads of 128 features, 1.10 PFLOP/s causal and 1.14 not, where the library's
-// product of 8192^3 reaches 1.15 on the same card; the clock stands at 1.85 GHz then, the matrix units are busy 53 % of the cycles, the vector ones 37 %
-// (without the exponentials the launch takes 5 % less, with K and V from registers 33 %).  Tried without gain: all of K's operands asked for
+// Bound by the matrix instructions and the power they take: 16384 tokens, 8 heads of 128 features in bf16, 1.03 to 1.13 PFLOP/s causal and 1.05 to 1.17 not (three
+// cards), where the library's product of 8192^3 reaches 1.1 to 1.25 in its first launches and 1.39 in a long run of them; the clock stands at 1.85 GHz, the matrix
+// units are busy 53 % of the cycles, the vector ones 37 % (without the exponentials the launch takes 5 % less, with K and V from registers 33 %).  Tried without gain: all of K's operands asked for
 // ahead, K two tiles and V one and a half ahead with two barriers a tile, 256 queries a workgroup, 64 queries a workgroup (1.4 times as long).
 // Short prompts wait for their latencies: 512 tokens, 32 heads 15 us, eight tiles one after the other.
 template <typename T, int D, int GROUPS, bool CAUSAL, bool AHEAD>
@@ -449,18 +449,21 @@ hipError_t launch(bool causal, const PromptArgs &a, hipStream_t stream) {
 
 // Two groups where one would leave half of the chip's 512 places for workgroups empty, or with a causal mask most of them while the last
 // tiles of long sequences run (lengths known on average only: a sequence of a few hundred tokens has nothing to split).  One group and two, us: causal,
-// 128 features, 4096 tokens 16 heads 96 and 88, 8 heads 84 and 69, 1000 tokens 16 heads 27 and 25; 2048 tokens 32 heads 54 and 56; 8 x 512 tokens, 12 heads of 64 16
-// and 19.
+// 128 features, 4096 tokens 16 heads 108 and 82, 8 heads 74 and 60, 1000 tokens 16 heads 23.1 and 21.2; 2048 tokens 32 heads 58 and 59; not causal, 2048 tokens 8 heads
+// 39.9 and 33.9; 8 x 512 tokens, 12 heads of 64 15.6 and 16.6.
 long long workgroups(const PromptArgs &a) { return ((long long)a.tokens + kTileQueries - 1) / kTileQueries * a.heads; }
 bool two_groups(bool causal, const PromptArgs &a) {
   const long long tiles = workgroups(a), length = a.tokens / a.sequences;
   return length >= 768 && (tiles <= 256 || (causal && tiles <= 512 && length >= 3000));
 }
 
-// Waves that are between a tile's scores and its first products go ahead of the others on their SIMD.  128 features, 8 heads of 16384 tokens
-// 542 -> 497 us, 16 of 8192 279 -> 259, 4 of 32768 1069 -> 975; 64 of 4096 273 -> 281, 32 of 2048 51.0 -> 52.2: for sequences of more than 6000 tokens.  Not
-// where little more than one round of workgroups has to be done, 512 places: 8 heads of 9000 tokens (568) 191 -> 200, 12000 (752) 286 -> 306, 12500 (784) 318 -> 327,
-// 13000 (816) 347 -> 345, 15000 (944) 465 -> 424.
+// Waves that are between a tile's scores and its first products go ahead of the others on their SIMD.  128 features, causal, 8 heads of 16001 tokens
+// 551 -> 509 us, 16 of 8192 292 -> 276, 4 of 32768 1122 -> 1034, 12 of 20000 1195 -> 1180; 64 of 4096 273 -> 281, 32 of 2048 51.0 -> 52.2: for sequences of more than 6000
+// tokens.  Not where little more than one round of workgroups has to be done, 512 places: 8 heads of 9000 tokens (568) 201 -> 211, 4 of 20000 (628) 460 -> 481,
+// 12000 (752) 286 -> 306, 12500 (784) 329 -> 343, 13000 (816) 359 -> 365, 15000 (944) 465 -> 424.
+// Without a mask the bad stretch ends sooner: 8 heads of 6500 tokens (408) 191 -> 180, 8192 (512) 267 -> 259, 9000 416 -> 436, 4 of 20000 917 -> 961, 12500 722 -> 671, 13000
+// 757 -> 708, 16001 1011 -> 973, 32768 4143 -> 4037; 32 of 6500 (1632) 708 -> 729.  The mean length is what the host knows: 16001 tokens with two prompts of one token beside
+// them go without (545 us, with it 503).
 bool go_ahead(const PromptArgs &a) { return a.tokens / a.sequences > 6000 && (workgroups(a) <= 512 || workgroups(a) > 800); }
 
 template <typename T, int D>

@@ -356,8 +356,9 @@ def _pool_of(pages, keys, values, scales, device):
 def fork_pages(page_refs, page_table, lengths, parents, children, keys, values, scales):
     """Row children[i] becomes a copy of row parents[i]: full pages are shared, a last page that is not full is copied to the lowest one that was free
     before the call, lengths follow, and the pages that the child held lose a reference each.  A child for which no page is free, or
-    whose parent is no row or becomes another's copy in the call, is left empty with length 0.  A row that is its own parent stays as it is,
-    and may be another's parent.  Named twice as a child, a row becomes its last naming."""
+    whose parent is no row, has no page for its last tokens or becomes another's copy in the call, is left empty with length 0: rows do not change
+    places in one call, they are copied to rows that are not parents.  A row that is its own parent stays as it is, and may be another's
+    parent.  Named twice as a child, a row becomes its last naming."""
     pages, rows, slots, device = _table(page_refs, page_table)
     _lengths(lengths, rows, device)
     if not (_listed(parents, 1, device) and _listed(children, 1, device)):
