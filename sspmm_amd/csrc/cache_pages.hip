@@ -187,7 +187,7 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(const PageTable
     }
     if (f.source < 0) f.target = -1;
     if (f.parent < 0) f.shared = 0;
-    lengths[f.child] = f.parent < 0 ? 0 : (int)max(0ll, min((long long)lengths[f.parent], (long long)t.slots * page_size));
+    lengths[f.child] = f.parent < 0 ? 0 : max(0, lengths[f.parent]);  // (tokens behind the table count, as they do for the parent)
     forks[i] = f;
   }
 }

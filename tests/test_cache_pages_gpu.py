@@ -371,3 +371,26 @@ def test_a_page_that_was_missing_is_not_entered_in_the_middle(built_library, for
     for h in range(heads):
         visible = torch.tensor([12, 13], device="cuda")
         check(got[2, :, h], *attention(q[2, :, h], k[:, h // 2], v[:, h // 2], visible, 0.125, torch.float16, torch.float16))
+
+
+def test_a_fork_of_a_row_longer_than_its_table(built_library):
+    """The child's tokens behind the table count as the parent's do: the newest queries of either see the same positions."""
+    page, d, n = 32, 64, 4
+    cache = sspmm_amd.new_cache(4, 1, page, d)
+    refs, table, lengths = _ints([0] * 4), torch.full((3, 2), -1, dtype=torch.int32, device="cuda"), _ints([0, 0, -7])
+    g = torch.Generator(device="cuda")
+    g.manual_seed(43)
+    x = torch.randn(66, 2, 1, d, generator=g, device="cuda").half()
+    off = offsets_of([66, 0, 0])
+    sspmm_amd.reserve_pages(refs, table, lengths.clamp(min=0), off, page)
+    sspmm_amd.cache_write(x[:, 0], x[:, 1], off, lengths, table, *cache)
+    lengths += off.diff()
+    sspmm_amd.fork_pages(refs, table, lengths, _ints([0, 2]), _ints([1, 2]), *cache)
+    assert lengths.tolist() == [66, 66, -7] and refs.tolist() == [2, 2, 0, 0] and table[1].tolist() == table[0].tolist()
+    q = torch.randn(1, n, 2, d, generator=g, device="cuda").half().expand(3, n, 2, d)
+    got = sspmm_amd.cache_attention(q, table, lengths, *cache)
+    assert torch.equal(got[0], got[1]) and not got[2].any()
+    k, v = row_of_cache(table[0], *cache, 64)
+    for h in range(2):
+        visible = torch.tensor([63, 64, 64, 64], device="cuda")
+        check(got[1, :, h], *attention(q[1, :, h], k[:, 0], v[:, 0], visible, 0.125, torch.float16, torch.float16))
