@@ -1,0 +1,396 @@
+"""A decoding step's operators beside those of perf/operators.py, as timing cases.
+
+    own                 False: the plain forms, elementary torch operations; True: the package's operators
+    listed()            the named cases
+    draw(rng)           one more case of the same ranges
+    prepare(case, seed) what a program holds before the call
+    run(state)          one pass
+    work(case)          bytes and operations the pass cannot do without
+    exact(case, seed)   what run returns, from the definitions in 64 bits
+
+Three kinds of work:
+
+    prefix   attention of the newest tokens over the paged cache, for rows that share leading pages, as forks leave them: in a step the
+             sharing is looked for once, and every layer's attention uses it
+    cross    attention of packed queries over an encoder's packed states, sequence by sequence
+    sample   tokens drawn from logits with temperature, min-p, top-k and top-p, from given uniform numbers
+
+The cache: keys [pages, kv_heads, page_size, d] and values [pages, kv_heads, d, page_size] in 8 bits (int8 or e4m3), scales
+[pages, 2, kv_heads] (keys, values), page_table [rows, slots] (-1: no page).
+"""
+import math
+
+import torch
+
+own = False
+
+TYPES = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
+CACHE_TYPES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+FILTERS = ("none", "greedy", "top_k", "top_p", "min_p", "mixed")
+
+
+def _text(numbers):
+    return ",".join(str(n) for n in numbers)
+
+
+def _numbers(text):
+    return [int(n) for n in text.split(",")]
+
+
+def _groups(case):
+    """[(shared tokens, [tokens of its own for each row])] of a prefix case."""
+    return [(int(shared), _numbers(each)) for shared, each in (g.split("+") for g in case["groups"].split(";"))]
+
+
+def listed():
+    return [
+        # eight prompts, eight continuations each, half way through their answers
+        {"name": "prefix_branches", "kind": "prefix", "layers": 2, "queries": 1, "heads": 32, "kv_heads": 8, "d": 128, "page_size": 64, "type": "bf16", "cache": "int8",
+         "groups": ";".join("%d+%s" % (64 + (797 * i * i + 331 * i) % 4000, _text([1 + (53 * j * j + 29 * i * j + 17 * i) % 500 for j in range(8)])) for i in range(8))},
+        # a service's one long instruction in front of 64 conversations
+        {"name": "prefix_instruction", "kind": "prefix", "layers": 2, "queries": 1, "heads": 16, "kv_heads": 4, "d": 128, "page_size": 128, "type": "bf16", "cache": "e4m3",
+         "groups": "8000+" + _text([1 + (613 * i * i + 97 * i) % 1900 for i in range(64)])},
+        # sixteen answers about one very long document
+        {"name": "prefix_document", "kind": "prefix", "layers": 1, "queries": 1, "heads": 16, "kv_heads": 4, "d": 128, "page_size": 128, "type": "f16", "cache": "int8",
+         "groups": "100003+" + _text([1 + 37 * i for i in range(16)])},
+        # three drafted tokens a row, heads with keys of their own, small: two forked rows, one beside them that shares nothing
+        {"name": "prefix_drafted", "kind": "prefix", "layers": 1, "queries": 3, "heads": 12, "kv_heads": 12, "d": 64, "page_size": 32, "type": "f16", "cache": "int8",
+         "groups": "333+5,40;0+77"},
+        # the prompts of translations: a decoder's first tokens on the encoder's states (12 heads of 64 features, sources up to 512 tokens)
+        {"name": "cross_prompts", "kind": "cross", "lengths": "300,17,1,128,511,64,250,90", "sources": "512,512,77,400,512,9,333,130", "heads": 12, "kv_heads": 12, "d": 64,
+         "type": "f16"},
+        # one token each of 64 sequences
+        {"name": "cross_step", "kind": "cross", "lengths": _text([1] * 64), "sources": _text([50 + (797 * i * i + 331 * i) % 1950 for i in range(64)]), "heads": 32, "kv_heads": 8,
+         "d": 128, "type": "bf16"},
+        # a long text on a long source
+        {"name": "cross_long", "kind": "cross", "lengths": "4001", "sources": "16001", "heads": 16, "kv_heads": 2, "d": 128, "type": "bf16"},
+        # the smallest call; one of the three has no source
+        {"name": "cross_words", "kind": "cross", "lengths": "1,2,1", "sources": "19,0,40", "heads": 4, "kv_heads": 2, "d": 64, "type": "f16"},
+        # the draw of a full batch, every row with its user's settings
+        {"name": "sample_batch", "kind": "sample", "rows": 64, "vocab": 131072, "filters": "mixed", "type": "bf16"},
+        # one conversation
+        {"name": "sample_one", "kind": "sample", "rows": 1, "vocab": 32000, "filters": "top_p", "type": "f16"},
+        # logits in 32 bits, an odd vocabulary, more rows than the chip has compute units
+        {"name": "sample_wide", "kind": "sample", "rows": 384, "vocab": 100003, "filters": "top_k", "type": "f32"},
+    ]
+
+
+def _log(rng, low, high):
+    return int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+
+
+def draw(rng):
+    kind = rng.choice(("prefix", "cross", "sample"))
+    if kind == "sample":
+        rows, vocab = _log(rng, 1, 384), _log(rng, 500, 131072)
+        while rows * vocab > 38000000:
+            rows = rows // 2 + 1
+        return {"kind": kind, "rows": rows, "vocab": vocab, "filters": rng.choice(FILTERS), "type": rng.choice(sorted(TYPES))}
+    kv = rng.choice((1, 2, 3, 4, 8))
+    heads, d, kind_of = kv * rng.choice((1, 2, 3, 4, 8)), rng.choice((32, 64, 128)), rng.choice(("bf16", "f16"))
+    if kind == "cross":
+        most, n = rng.choice(((1, 64), (4, 64), (2000, 12))), 1
+        n = _log(rng, 1, most[1])
+        lengths, sources, left = [], [], 4.0e11 / (4 * d * heads)
+        for _ in range(n):
+            a, b = _log(rng, 1, most[0]) if most[0] > 1 else 1, 0 if rng.random() < 0.04 else _log(rng, 1, 16000 if n < 8 else 2000)
+            b = min(b, int(left / a))
+            lengths.append(a)
+            sources.append(b)
+            left -= a * b
+        while heads * len(lengths) * max(lengths) * max(sources) > 1.0e9:  # (the plain form holds this many scores)
+            if max(lengths) > 1:
+                lengths[lengths.index(max(lengths))] = max(lengths) // 2 + 1
+            else:
+                sources[sources.index(max(sources))] = max(sources) // 2 + 1
+        return {"kind": kind, "lengths": _text(lengths), "sources": _text(sources), "heads": heads, "kv_heads": kv, "d": d, "type": kind_of}
+    groups, left = [], 64
+    for _ in range(rng.choice((1, 1, 2, 3, 8))):
+        m = min(left, _log(rng, 1, 32))
+        if m:
+            shared = rng.choice((0, _log(rng, 1, 4000), _log(rng, 200, 50000 if m <= 8 and not groups else 8000)))
+            groups.append((shared, [_log(rng, 1, 1500) for _ in range(m)]))
+            left -= m
+    return {"kind": kind, "layers": rng.choice((1, 2)), "queries": rng.choice((1, 1, 1, 2, 4, 7)), "heads": heads, "kv_heads": kv, "d": d, "page_size": rng.choice((32, 64, 128)),
+            "type": kind_of, "cache": rng.choice(sorted(CACHE_TYPES)), "groups": ";".join("%d+%s" % (s, _text(each)) for s, each in groups)}
+
+
+def work(case):
+    if case["kind"] == "sample":
+        size = 4 if case["type"] == "f32" else 2
+        return {"bytes": case["rows"] * (case["vocab"] * size + 4 * 7), "flops": 10 * case["rows"] * case["vocab"]}
+    heads, kv, d = case["heads"], case["kv_heads"], case["d"]
+    if case["kind"] == "cross":
+        n, s = _numbers(case["lengths"]), _numbers(case["sources"])
+        return {"bytes": 2 * d * (2 * sum(n) * heads + 2 * sum(b for a, b in zip(n, s) if a) * kv), "flops": 4 * d * heads * sum(a * b for a, b in zip(n, s))}
+    page, q = case["page_size"], case["queries"]
+    tokens, blocks, seen, rows = 0, 0, 0, 0
+    for shared, each in _groups(case):
+        full = shared // page * page
+        tokens += full
+        blocks += full // page
+        for x in each:
+            rows += 1
+            tokens += shared + x - full
+            blocks += -(-(shared + x - full) // page)
+            seen += sum(max(0, shared + x - i) for i in range(q))
+    return {"bytes": case["layers"] * (tokens * kv * 2 * d + blocks * kv * 8 + 4 * rows * q * heads * d), "flops": case["layers"] * 4 * d * heads * seen}
+
+
+# ---- what a program has in hand
+
+
+def _offsets(lengths):
+    return torch.tensor([sum(lengths[:i]) for i in range(len(lengths) + 1)], dtype=torch.int32, device="cuda")
+
+
+def _values(g, shape, scale=1.0):
+    return torch.randn(shape, generator=g, device="cuda") * scale
+
+
+def _pool(case, g, pages):
+    """(keys, values, scales) of a pool whose tokens have been quantised block by block."""
+    kv, d, page = case["kv_heads"], case["d"], case["page_size"]
+    parts, scales = [], []
+    for shape in ((pages, kv, page, d), (pages, kv, d, page)):
+        # (features of different size, as projections leave them)
+        by = torch.exp(0.5 * torch.randn((kv, 1, d) if shape[2] == page else (kv, d, 1), generator=g, device="cuda"))
+        x = torch.randn(shape, generator=g, device="cuda") * by
+        most = x.abs().amax((2, 3))
+        if case["cache"] == "int8":
+            s = most / 127.0
+            parts.append((x / s[:, :, None, None]).round().clamp(-127, 127).to(torch.int8))
+        else:
+            s = torch.exp2(torch.ceil(torch.log2(most / 448.0)))
+            parts.append((x / s[:, :, None, None]).clamp(-448, 448).to(torch.float8_e4m3fn))
+        scales.append(s)
+    return parts[0], parts[1], torch.stack(scales, 1).contiguous()
+
+
+def _prepare_prefix(case, g):
+    groups, page = _groups(case), case["page_size"]
+    # (rows as forks leave them: the first of every group, then the second ones, ...)
+    rows = sorted((j, i) for i, (_, each) in enumerate(groups) for j in range(len(each)))
+    lengths = [groups[i][0] + groups[i][1][j] for j, i in rows]
+    need = sum(s // page for s, _ in groups) + sum(-(-n // page) - groups[i][0] // page for n, (_, i) in zip(lengths, rows))
+    at = torch.randperm(need + 5, generator=g, device="cuda").to(torch.int32)
+    table = torch.full((len(rows), max(-(-n // page) for n in lengths) + 1), -1, dtype=torch.int32, device="cuda")
+    taken, fronts = 0, []
+    for shared, _ in groups:
+        fronts.append(at[taken:taken + shared // page])
+        taken += shared // page
+    for row, (n, (_, i)) in enumerate(zip(lengths, rows)):
+        front, own_pages = fronts[i], -(-n // page) - fronts[i].numel()
+        table[row, :front.numel()] = front
+        table[row, front.numel():front.numel() + own_pages] = at[taken:taken + own_pages]
+        taken += own_pages
+    shape = (len(rows), case["queries"], case["heads"], case["d"])
+    return {"table": table, "lengths": torch.tensor(lengths, dtype=torch.int32, device="cuda"),
+            "layers": [(_values(g, shape, 1.5).to(TYPES[case["type"]]),) + _pool(case, g, need + 5) for _ in range(case["layers"])]}
+
+
+def _settings(case, g):
+    """(temperature, top_k, top_p, min_p) [rows] each, as users choose them."""
+    rows, what = case["rows"], case["filters"]
+    temperature = 0.6 + 0.7 * torch.rand(rows, generator=g, device="cuda")
+    top_k = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    top_p, min_p = torch.ones(rows, device="cuda"), torch.zeros(rows, device="cuda")
+    pick = torch.randint(0, 6, (rows,), generator=g, device="cuda")
+    uses = [torch.full_like(pick, what == name, dtype=torch.bool) if what != "mixed" else pick == i for i, name in enumerate(FILTERS)]
+    every = pick == 5 if what == "mixed" else torch.zeros_like(pick, dtype=torch.bool)  # (all three at once)
+    some_k = torch.tensor([1, 20, 50, 1000], dtype=torch.int32, device="cuda")[torch.randint(0, 4, (rows,), generator=g, device="cuda")]
+    some_p = torch.tensor([0.5, 0.9, 0.95, 0.99], device="cuda")[torch.randint(0, 4, (rows,), generator=g, device="cuda")]
+    temperature = torch.where(uses[1], 0.0, temperature)
+    top_k = torch.where(uses[2] | every, some_k, top_k)
+    top_p = torch.where(uses[3] | every, some_p, top_p)
+    min_p = torch.where(uses[4] | every, 0.05, min_p)
+    return temperature, top_k, top_p, min_p
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    state = {"case": case}
+    if case["kind"] == "prefix":
+        return state | _prepare_prefix(case, g)
+    if case["kind"] == "cross":
+        lengths, sources, heads, kv, d = _numbers(case["lengths"]), _numbers(case["sources"]), case["heads"], case["kv_heads"], case["d"]
+        kind_of = TYPES[case["type"]]
+        return state | {"q": _values(g, (sum(lengths), heads, d), 1.5).to(kind_of), "kv": _values(g, (sum(sources), 2 * kv * d)).to(kind_of),
+                        "offsets": _offsets(lengths), "source_offsets": _offsets(sources), "longest": max(lengths), "longest_source": max(sources)}
+    rows, vocab = case["rows"], case["vocab"]
+    # (what is common in a language is likely everywhere, a few tokens are likely here)
+    common = -0.8 * torch.log(1.0 + torch.randperm(vocab, generator=g, device="cuda"))
+    logits = 2.0 * torch.randn((rows, vocab), generator=g, device="cuda") + common
+    likely = torch.randint(0, vocab, (rows, 12), generator=g, device="cuda")
+    logits.scatter_add_(1, likely, 9.0 * torch.rand((rows, 12), generator=g, device="cuda"))
+    # (a grammar rules out a third of the vocabulary for every fourth row)
+    ruled = (torch.rand((rows, vocab), generator=g, device="cuda") < 0.33) & (torch.arange(rows, device="cuda") % 4 == 3)[:, None]
+    logits = logits.masked_fill_(ruled, float("-inf")).to(TYPES[case["type"]])
+    return state | {"logits": logits, "uniform": torch.rand(rows, generator=g, device="cuda"), "settings": _settings(case, g)}
+
+
+# ---- the operators in their plain form
+
+
+def _plain_step(q, table, lengths, keys, values, scales):
+    n, queries, heads, d = q.shape
+    kv, page = keys.size(1), keys.size(2)
+    at = table.long().clamp(min=0)
+    m = at.size(1) * page
+    K = keys.view(torch.int8)[at].view(keys.dtype).float() * scales[at][:, :, 0, :, None, None]  # [n, slots, kv, page, d]
+    K = K.permute(0, 2, 4, 1, 3).reshape(n, kv, d, m)
+    V = values.view(torch.int8)[at].view(values.dtype).float() * scales[at][:, :, 1, :, None, None]  # [n, slots, kv, d, page]
+    V = V.permute(0, 2, 1, 4, 3).reshape(n, kv, m, d)
+    g = heads // kv
+    Q = q.float().view(n, queries, kv, g, d).permute(0, 2, 1, 3, 4).reshape(n, kv, queries * g, d)
+    s = (Q @ K).view(n, kv, queries, g, m) * (1.0 / math.sqrt(d))
+    last = lengths.long()[:, None] - queries + torch.arange(queries, device=q.device)  # the newest key that a query sees
+    mask = (torch.arange(m, device=q.device) <= last[:, :, None])[:, None, :, None, :]
+    s = s.masked_fill(~mask, float("-inf"))
+    most = s.amax(-1, keepdim=True)
+    p = (s - torch.where(most == float("-inf"), 0.0, most)).exp()
+    total = p.sum(-1, keepdim=True)
+    out = (p.view(n, kv, queries * g, m) @ V).view(n, kv, queries, g, d)
+    out = torch.where(total > 0, out / total, 0.0)
+    return out.permute(0, 2, 1, 3, 4).reshape(n, queries, heads, d).to(q.dtype)
+
+
+def _plain_cross(q, k, v, offsets, source_offsets, longest, longest_source):
+    tokens, heads, d = q.shape
+    kv, n = k.size(1), offsets.numel() - 1
+    if longest_source == 0:
+        return torch.zeros_like(q)
+    off, at = offsets.long(), source_offsets.long()
+    pos, source = torch.arange(longest, device=q.device), torch.arange(longest_source, device=q.device)
+    rows = (off[:-1, None] + pos).clamp(max=tokens - 1)  # [n, longest]
+    states = (at[:-1, None] + source).clamp(max=k.size(0) - 1)
+    inside = source < (at[1:] - at[:-1])[:, None]
+    Q = q.float()[rows].view(n, longest, kv, heads // kv, d).permute(0, 2, 3, 1, 4).reshape(n, kv, heads // kv * longest, d)
+    K = k.float()[states].permute(0, 2, 3, 1).contiguous()
+    V = v.float()[states].permute(0, 2, 1, 3).contiguous()
+    s = (Q @ K).mul_(1.0 / math.sqrt(d)).masked_fill_(~inside[:, None, None, :], float("-inf"))
+    most = s.amax(-1, keepdim=True)
+    p = s.sub_(torch.where(most == float("-inf"), 0.0, most)).exp_()
+    total = p.sum(-1, keepdim=True)
+    out = torch.where(total > 0, (p @ V) / total, 0.0).view(n, kv, heads // kv, longest, d)
+    out = out.permute(0, 3, 1, 2, 4).reshape(n, longest, heads, d)
+    token = torch.arange(tokens, device=q.device)
+    of = torch.searchsorted(off[1:].contiguous(), token, right=True)
+    return out[of, token - off[of]].to(q.dtype)
+
+
+def _plain_sample(logits, uniform, temperature, top_k, top_p, min_p):
+    # (in 64 bits: running sums are compared with borders)
+    x = torch.nan_to_num(logits.double(), nan=float("-inf"), posinf=float("inf"), neginf=float("-inf"))
+    x, order = torch.sort(x, dim=-1, descending=True, stable=True)
+    greedy = temperature <= 0
+    w = torch.where(x == x[:, :1], 1.0, torch.exp((x - x[:, :1]) / torch.where(greedy, 1.0, temperature.double())[:, None]))
+    w = torch.where((x > float("-inf")) & (w >= min_p.double()[:, None]), w, 0.0)
+    place = torch.arange(x.size(1), device=x.device)
+    k = torch.where(greedy, 1, torch.where(top_k > 0, top_k.long(), x.size(1)))
+    w = torch.where(place < k[:, None], w, 0.0)
+    sums = w.cumsum(-1)
+    before = torch.nn.functional.pad(sums[:, :-1], (1, 0))
+    w = torch.where((before < top_p.double()[:, None] * sums[:, -1:]) | (place == 0) | (top_p >= 1)[:, None], w, 0.0)
+    sums = w.cumsum(-1)
+    total = sums[:, -1:]
+    first = (sums > uniform.double()[:, None] * total).int().argmax(-1, keepdim=True)
+    token = torch.where(total > 0, order.gather(1, first), -1)[:, 0]
+    return token.int(), torch.where(total > 0, w.gather(1, first) / total, 0.0)[:, 0].float()
+
+
+def run(state):
+    case = state["case"]
+    if case["kind"] == "prefix":
+        table, lengths = state["table"], state["lengths"]
+        if own:
+            import sspmm_amd
+            plan = sspmm_amd.plan_prefixes(table, lengths, case["queries"], case["heads"], case["kv_heads"], case["page_size"])
+            return [sspmm_amd.prefix_attention(q, table, plan, keys, values, scales) for q, keys, values, scales in state["layers"]]
+        return [_plain_step(q, table, lengths, keys, values, scales) for q, keys, values, scales in state["layers"]]
+    if case["kind"] == "cross":
+        k, v = state["kv"].view(-1, 2, case["kv_heads"], case["d"]).unbind(1)
+        if own:
+            import sspmm_amd
+            return sspmm_amd.cross_attention(state["q"], k, v, state["offsets"], state["source_offsets"])
+        return _plain_cross(state["q"], k, v, state["offsets"], state["source_offsets"], state["longest"], state["longest_source"])
+    if own:
+        import sspmm_amd
+        return sspmm_amd.sample_tokens(state["logits"], state["uniform"], *state["settings"], probabilities=True)
+    return _plain_sample(state["logits"], state["uniform"], *state["settings"])
+
+
+# ---- from the definitions, in 64 bits
+
+
+def _exact_head(q, k, v, visible):
+    """softmax(q k^T / sqrt(d)) v over the first visible[i] keys of each query, in 64 bits."""
+    out = torch.zeros_like(q)
+    if k.size(0) == 0:
+        return out
+    s = torch.mm(q, k.t().contiguous()) * q.size(1) ** -0.5
+    s[torch.arange(k.size(0), device=q.device)[None, :] >= visible[:, None]] = float("-inf")
+    some = visible > 0
+    out[some] = torch.mm(torch.softmax(s[some], -1), v)
+    return out
+
+
+def _exact_sample(logits, u, temperature, top_k, top_p, min_p):
+    """One row: (token, probability), its likely tokens one after the other."""
+    import numpy as np
+    logits = np.where(np.isnan(logits), -np.inf, logits)
+    order = np.lexsort((np.arange(logits.size), -logits))
+    x = logits[order]
+    x = x[x > -np.inf]
+    if x.size == 0:
+        return -1, 0.0
+    if temperature <= 0:
+        return int(order[0]), 1.0
+    w = np.ones_like(x)
+    below = x < x[0]
+    w[below] = np.exp((x[below] - x[0]) / temperature)
+    w = w[w >= min_p]
+    if top_k > 0:
+        w = w[:top_k]
+    if top_p < 1:
+        sums = np.cumsum(w)
+        w = w[:max(1, int(np.searchsorted(sums, top_p * sums[-1], side="left")) + 1)]
+    sums = np.cumsum(w)
+    at = min(int(np.searchsorted(sums, u * sums[-1], side="right")), w.size - 1)
+    return int(order[at]), float(w[at] / sums[-1])
+
+
+def exact(case, seed):
+    state = prepare(case, seed)
+    if case["kind"] == "sample":
+        columns = [state["uniform"].double().tolist()] + [t.double().tolist() for t in state["settings"]]
+        rows = state["logits"].double().cpu().numpy()
+        drawn = [_exact_sample(rows[i], u, t, int(k), p, m) for i, (u, t, k, p, m) in enumerate(zip(*columns))]
+        return torch.tensor([t for t, _ in drawn], dtype=torch.int32), torch.tensor([p for _, p in drawn], dtype=torch.float64)
+    heads, kv, d = case["heads"], case["kv_heads"], case["d"]
+    group = heads // kv
+    if case["kind"] == "cross":
+        q = state["q"].double()
+        k, v = state["kv"].double().view(-1, 2, kv, d).unbind(1)
+        out, i, j = torch.zeros_like(q), 0, 0
+        for n, m in zip(_numbers(case["lengths"]), _numbers(case["sources"])):
+            for h in range(heads):
+                out[i:i + n, h] = _exact_head(q[i:i + n, h], k[j:j + m, h // group], v[j:j + m, h // group], torch.full((n,), m, device=q.device))
+            i, j = i + n, j + m
+        return out
+    table, lengths, queries, page = state["table"], state["lengths"].tolist(), case["queries"], case["page_size"]
+    outs = []
+    for q, keys, values, scales in state["layers"]:
+        q = q.double()
+        out = torch.zeros_like(q)
+        for b, n in enumerate(lengths):
+            held = table[b, :-(-n // page)].long()
+            ends = torch.arange(n - queries + 1, n + 1, device=q.device).clamp(min=0).repeat_interleave(group)
+            for h in range(kv):
+                K = (keys.view(torch.int8)[held, h].view(keys.dtype).double() * scales[held, 0, h].double()[:, None, None]).reshape(-1, d)[:n]
+                V = (values.view(torch.int8)[held, h].view(values.dtype).double() * scales[held, 1, h].double()[:, None, None]).transpose(1, 2).reshape(-1, d)[:n]
+                rows = q[b, :, h * group:(h + 1) * group].reshape(queries * group, d)
+                out[b, :, h * group:(h + 1) * group] = _exact_head(rows, K, V, ends).view(queries, group, d)
+        outs.append(out)
+    return outs
