@@ -46,7 +46,7 @@ def listed():
     return [
         # eight prompts, eight continuations each, half way through their answers
         {"name": "prefix_branches", "kind": "prefix", "layers": 2, "queries": 1, "heads": 32, "kv_heads": 8, "d": 128, "page_size": 64, "type": "bf16", "cache": "int8",
-         "groups": ";".join("%d+%s" % (64 + (797 * i * i + 331 * i) % 4000, _text([1 + (53 * j * j + 29 * i * j + 17 * i) % 500 for j in range(8)])) for i in range(8))},
+         "groups": ";".join("%d+%s" % (64 + (797 * i * i + 331 * i) % 4000, _text([1 + (53 * j * j + 29 * i * j + 19 * i) % 500 for j in range(8)])) for i in range(8))},
         # a service's one long instruction in front of 64 conversations
         {"name": "prefix_instruction", "kind": "prefix", "layers": 2, "queries": 1, "heads": 16, "kv_heads": 4, "d": 128, "page_size": 128, "type": "bf16", "cache": "e4m3",
          "groups": "8000+" + _text([1 + (613 * i * i + 97 * i) % 1900 for i in range(64)])},
