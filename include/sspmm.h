@@ -545,6 +545,7 @@ int sspmm_attention_fm_ragged_f16(int batch, int heads, int seq, int head_dim, c
  * ---------------------------------------------------------------------------------------- */
 #define SSPMM_TYPE_F16 0
 #define SSPMM_TYPE_BF16 1
+#define SSPMM_TYPE_F32 2 /* of logits */
 #define SSPMM_CACHE_INT8 0
 #define SSPMM_CACHE_E4M3 1
 
@@ -618,6 +619,47 @@ int sspmm_fork_pages(int32_t *page_refs, int pages, int32_t *page_table, int row
                      float *scales, void *workspace, size_t workspace_bytes, void *hip_stream);
 int sspmm_compact_pages(int32_t *page_refs, int pages, int32_t *page_table, int rows, int slots, int kv_heads, int page_size, int head_dim,
                         void *keys, void *values, float *scales, void *workspace, size_t workspace_bytes, void *hip_stream);
+
+/*
+ * Attention of packed queries over packed states of other lengths, as a decoder's over its encoder's: query i of sequence b (rows offsets[b] ..
+ * offsets[b + 1] - 1 of q and out) sees rows source_offsets[b] .. source_offsets[b + 1] - 1 of k and v, all of them.  Both lists as offsets in
+ * sspmm_prompt_attention, the second within 0 .. source_tokens; a sequence without states, or whose scores are all -infinity, is zeros.  Strides, limits and out as there.
+ */
+int sspmm_cross_attention(int type, int sequences, int tokens, int source_tokens, int heads, int kv_heads, int head_dim, const int32_t *offsets,
+                          const int32_t *source_offsets, const sspmm_half_t *q, int64_t q_row, int64_t q_head, const sspmm_half_t *k, int64_t k_row,
+                          int64_t k_head, const sspmm_half_t *v, int64_t v_row, int64_t v_head, float scale, sspmm_half_t *out, int64_t out_row,
+                          int64_t out_head, void *hip_stream);
+
+/*
+ * sspmm_cache_attention for rows that share leading pages, as sspmm_fork_pages leaves them: pages that several rows name in the same slots from the first on are
+ * read once for all of these.  A plan says which, for the sizes it was made with and the table and lengths as they were then; the attention takes the
+ * lengths from it, and the pages from the table.  Rows that begin with the same page are compared with the lowest of them, and those that share enough pages with it
+ * (the number that saves most) are a group; whole pages in front of all queries are shared.  At most 1024 rows, 2^20 queries times heads and 2^22 rows times queries times heads; plan 16-byte aligned, sspmm_prefix_plan_bytes of it
+ * (0: sizes that no plan is made for).  A plan may be made anew in place, and is read by any number of calls.
+ */
+size_t sspmm_prefix_plan_bytes(int rows, int queries, int heads, int kv_heads);
+int sspmm_plan_prefixes(const int32_t *page_table, int rows, int slots, const int32_t *lengths, int page_size, int queries, int heads, int kv_heads, void *plan,
+                        size_t plan_bytes, void *hip_stream);
+/* workspace: sspmm_prefix_attention_workspace_bytes of the same sizes, 16-byte aligned */
+size_t sspmm_prefix_attention_workspace_bytes(int rows, int queries, int heads, int kv_heads, int head_dim);
+int sspmm_prefix_attention(int type, int format, int rows, int queries, int heads, const sspmm_half_t *q, int64_t q_seq, int64_t q_row, int64_t q_head,
+                           const int32_t *page_table, int slots, const void *plan, size_t plan_bytes, int pages, int kv_heads, int page_size, int head_dim,
+                           const void *keys, const void *values, const float *scales, float scale, sspmm_half_t *out, int64_t out_seq, int64_t out_row,
+                           int64_t out_head, void *workspace, size_t workspace_bytes, void *hip_stream);
+
+/*
+ * One token of each row of logits [rows, vocab] (fp16, bf16 or fp32, row i at logits + i * row_stride elements, aligned to an element; row_stride may be 0), drawn with
+ * uniform[i] in [0, 1).  With the weights w = exp((l - max l) / temperature): kept are those with w >= min_p; of these the top_k first in the order of falling
+ * logits, equal ones by rising index; of these the shortest run, at least one, whose weights reach top_p of the sum of all of these.  The token is the first in that order
+ * at which the running sum of the weights exceeds uniform * their sum.  temperature <= 0 (or NaN): the largest logit's first index; top_k <= 0, top_p >= 1 (or NaN), min_p <= 0
+ * (or NaN): everything is kept.  NaN logits are taken as -infinity, which is never drawn; infinite ones share the draw.  A row that is all -infinity gives -1.
+ * Weights are whole multiples of 2^-b of the largest's, vocab * 2^b <= 2^62, b <= 52: the result does not depend on the order of the sums.
+ * temperature, top_k, top_p, min_p: one value a row, or NULL and the value beside it for all.  probabilities (may be NULL): weight over sum, of the token (0 with -1).
+ * vocab 1 .. 2^24.
+ */
+int sspmm_sample_tokens(int type, int rows, int vocab, const void *logits, int64_t row_stride, const float *uniform, const float *temperature, float temperature_all,
+                        const int32_t *top_k, int top_k_all, const float *top_p, float top_p_all, const float *min_p, float min_p_all, int32_t *tokens,
+                        float *probabilities, void *hip_stream);
 
 /* ------------------------------------------------------------------------------------------
  * Coordinate list -> CSR, the step between a Matrix Market file and the RowMerge in the

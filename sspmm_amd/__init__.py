@@ -12,8 +12,8 @@ from .spmm import spmm, bspmm, sorted_row_swizzle  # noqa: F401
 from .plan import Plan, PlanInfo  # noqa: F401
 from .svc import svc, svc_batched, stack_csr, SvcBatch, SvcResult  # noqa: F401
 from .attention import sddmm, bsddmm, csr_softmax, bcsr_softmax, sparse_attention, fused_sparse_attention, sparse_attention_packed  # noqa: F401
-from .serving import (cache_attention, cache_write, compact_pages, fork_pages, new_cache, prompt_attention, release_pages,  # noqa: F401
-                      reserve_pages)
+from .serving import (cache_attention, cache_write, compact_pages, cross_attention, fork_pages, new_cache, plan_prefixes,  # noqa: F401
+                      prefix_attention, PrefixPlan, prompt_attention, release_pages, reserve_pages, sample_tokens)
 from .reorder import minhash_order, permute_csr, svc_reordered  # noqa: F401
 from .layers import SparseLinear, SparseEncoderLayer  # noqa: F401
 from .formats import Cvse, read_smtx, write_smtx, read_cvse, write_cvse, cvse_text  # noqa: F401

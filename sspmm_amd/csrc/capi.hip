@@ -10,8 +10,10 @@
 #include "coo_kernels.h"
 #include "layer_kernels.h"
 #include "plan.h"
+#include "prefix_kernels.h"
 #include "prompt_kernels.h"
 #include "reorder_kernels.h"
+#include "sample_kernels.h"
 #include "spmm_kernels.h"
 #include "svc_kernels.h"
 
@@ -77,6 +79,11 @@ bool pool_fits(int pages, int kv_heads, int page_size, int head_dim, const void 
   return pages >= 1 && pages <= (1 << 30) && kv_heads >= 1 && kv_heads <= 65535 && (page_size == 32 || page_size == 64 || page_size == 128) &&
          (head_dim == 32 || head_dim == 64 || head_dim == 128) && keys && values && scales && reinterpret_cast<uintptr_t>(keys) % 16 == 0 &&
          reinterpret_cast<uintptr_t>(values) % 16 == 0 && reinterpret_cast<uintptr_t>(scales) % 4 == 0;
+}
+// (a plan's tiles and the attention's states stay far below what 32 bits count)
+bool plan_fits(int rows, int queries, int heads, int kv_heads) {
+  return rows > 0 && rows <= sspmm::kMostPlanRows && queries > 0 && kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && (int64_t)queries * heads <= 1 << 20 &&
+         (int64_t)rows * queries * heads <= 1 << 22;
 }
 bool workspace_fits(const void *p, size_t bytes, size_t need) { return p && bytes >= need && reinterpret_cast<uintptr_t>(p) % 4 == 0; }
 bool table_fits(const void *refs, int pages, const void *table, int rows, int slots) {
@@ -809,6 +816,7 @@ int sspmm_prompt_attention(int type, int sequences, int tokens, int heads, int k
   a.v = v;
   a.out = out;
   a.offsets = offsets;
+  a.key_tokens = tokens;
   a.q_row = q_row;
   a.q_head = q_head;
   a.k_row = k_row;
@@ -823,6 +831,40 @@ int sspmm_prompt_attention(int type, int sequences, int tokens, int heads, int k
   a.kv_heads = kv_heads;
   a.scale_log2e = scale * 1.4426950408889634f;
   return (int)sspmm::launch_prompt_attention(type, head_dim, causal != 0, a, static_cast<hipStream_t>(hip_stream));
+}
+
+int sspmm_cross_attention(int type, int sequences, int tokens, int source_tokens, int heads, int kv_heads, int head_dim, const int32_t *offsets,
+                          const int32_t *source_offsets, const sspmm_half_t *q, int64_t q_row, int64_t q_head, const sspmm_half_t *k, int64_t k_row,
+                          int64_t k_head, const sspmm_half_t *v, int64_t v_row, int64_t v_head, float scale, sspmm_half_t *out, int64_t out_row,
+                          int64_t out_head, void *hip_stream) {
+  if (type != SSPMM_TYPE_F16 && type != SSPMM_TYPE_BF16) return kInvalid;
+  if (sequences < 0 || tokens < 0 || source_tokens < 0 || !heads_fit(heads, kv_heads, head_dim) || !scale_fits(scale)) return kInvalid;
+  if (sequences == 0 || tokens == 0) return 0;
+  if (!offsets || !source_offsets || !operand_fits(q, q_row, q_head, head_dim) || !operand_fits(out, out_row, out_head, head_dim)) return kInvalid;
+  if (source_tokens > 0 && (!operand_fits(k, k_row, k_head, head_dim) || !operand_fits(v, v_row, v_head, head_dim))) return kInvalid;
+  if (tokens > (1 << 30) || source_tokens > (1 << 30)) return kInvalid;
+  sspmm::PromptArgs a{};
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.out = out;
+  a.offsets = offsets;
+  a.key_offsets = source_offsets;
+  a.q_row = q_row;
+  a.q_head = q_head;
+  a.k_row = k_row;
+  a.k_head = k_head;
+  a.v_row = v_row;
+  a.v_head = v_head;
+  a.out_row = out_row;
+  a.out_head = out_head;
+  a.sequences = sequences;
+  a.tokens = tokens;
+  a.key_tokens = source_tokens;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.scale_log2e = scale * 1.4426950408889634f;
+  return (int)sspmm::launch_prompt_attention(type, head_dim, false, a, static_cast<hipStream_t>(hip_stream));
 }
 
 int sspmm_cache_write(int type, int format, int sequences, int tokens, const int32_t *offsets, const int32_t *starts,
@@ -886,6 +928,77 @@ int sspmm_cache_attention(int type, int format, int sequences, int queries, int 
   const size_t need = 4 * sspmm::cache_attention_workspace(sequences, queries, heads, kv_heads, head_dim, (long long)slots * page_size);
   if (workspace_bytes < need || (need > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16))) return kInvalid;
   return (int)sspmm::launch_cache_attention(type, format, a, static_cast<hipStream_t>(hip_stream));
+}
+
+size_t sspmm_prefix_plan_bytes(int rows, int queries, int heads, int kv_heads) {
+  return plan_fits(rows, queries, heads, kv_heads) ? 4 * sspmm::prefix_plan_ints(sspmm::prefix_shape(rows, queries, heads, kv_heads), rows) : 0;
+}
+
+int sspmm_plan_prefixes(const int32_t *page_table, int rows, int slots, const int32_t *lengths, int page_size, int queries, int heads, int kv_heads, void *plan,
+                        size_t plan_bytes, void *hip_stream) {
+  if (rows == 0 || queries == 0) return 0;
+  if (!plan_fits(rows, queries, heads, kv_heads) || slots < 1 || (page_size != 32 && page_size != 64 && page_size != 128) || !page_table || !lengths) return kInvalid;
+  if ((int64_t)slots * page_size > (1ll << 31) - 256 || !plan || reinterpret_cast<uintptr_t>(plan) % 16) return kInvalid;
+  if (plan_bytes < sspmm_prefix_plan_bytes(rows, queries, heads, kv_heads)) return kInvalid;
+  return (int)sspmm::launch_plan_prefixes(sspmm::prefix_shape(rows, queries, heads, kv_heads), page_table, rows, slots, lengths, page_size, queries,
+                                          static_cast<int32_t *>(plan), static_cast<hipStream_t>(hip_stream));
+}
+
+size_t sspmm_prefix_attention_workspace_bytes(int rows, int queries, int heads, int kv_heads, int head_dim) {
+  if (!plan_fits(rows, queries, heads, kv_heads) || !heads_fit(heads, kv_heads, head_dim)) return 0;
+  return 4 * sspmm::prefix_attention_floats(sspmm::prefix_shape(rows, queries, heads, kv_heads), kv_heads, head_dim);
+}
+
+int sspmm_prefix_attention(int type, int format, int rows, int queries, int heads, const sspmm_half_t *q, int64_t q_seq, int64_t q_row, int64_t q_head,
+                           const int32_t *page_table, int slots, const void *plan, size_t plan_bytes, int pages, int kv_heads, int page_size, int head_dim,
+                           const void *keys, const void *values, const float *scales, float scale, sspmm_half_t *out, int64_t out_seq, int64_t out_row,
+                           int64_t out_head, void *workspace, size_t workspace_bytes, void *hip_stream) {
+  if ((type != SSPMM_TYPE_F16 && type != SSPMM_TYPE_BF16) || (format != SSPMM_CACHE_INT8 && format != SSPMM_CACHE_E4M3)) return kInvalid;
+  if (rows < 0 || queries < 0 || slots < 1 || !heads_fit(heads, kv_heads, head_dim) || !scale_fits(scale)) return kInvalid;
+  if (rows == 0 || queries == 0) return 0;
+  if (!plan_fits(rows, queries, heads, kv_heads) || (int64_t)slots * page_size > (1ll << 31) - 256) return kInvalid;
+  if (!page_table || !plan || reinterpret_cast<uintptr_t>(plan) % 16 || plan_bytes < sspmm_prefix_plan_bytes(rows, queries, heads, kv_heads)) return kInvalid;
+  if (!pool_fits(pages, kv_heads, page_size, head_dim, keys, values, scales)) return kInvalid;
+  if (!operand_fits(q, q_row, q_head, head_dim) || !operand_fits(out, out_row, out_head, head_dim) || q_seq % 8 || q_seq < 0 || out_seq % 8 || out_seq < 0)
+    return kInvalid;
+  if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < sspmm_prefix_attention_workspace_bytes(rows, queries, heads, kv_heads, head_dim))
+    return kInvalid;
+  sspmm::PrefixAttentionArgs a{};
+  a.pool = {static_cast<unsigned char *>(const_cast<void *>(keys)), static_cast<unsigned char *>(const_cast<void *>(values)), const_cast<float *>(scales),
+            page_table, pages, kv_heads, page_size, head_dim, slots};
+  a.q = q;
+  a.out = out;
+  a.q_seq = q_seq;
+  a.q_row = q_row;
+  a.q_head = q_head;
+  a.out_seq = out_seq;
+  a.out_row = out_row;
+  a.out_head = out_head;
+  a.plan = static_cast<const int32_t *>(plan);
+  a.rows = rows;
+  a.queries = queries;
+  a.heads = heads;
+  a.scale_log2e = scale * 1.4426950408889634f;
+  a.partial = static_cast<float *>(workspace);
+  a.shape = sspmm::prefix_shape(rows, queries, heads, kv_heads);
+  return (int)sspmm::launch_prefix_attention(type, format, a, static_cast<hipStream_t>(hip_stream));
+}
+
+int sspmm_sample_tokens(int type, int rows, int vocab, const void *logits, int64_t row_stride, const float *uniform, const float *temperature, float temperature_all,
+                        const int32_t *top_k, int top_k_all, const float *top_p, float top_p_all, const float *min_p, float min_p_all, int32_t *tokens,
+                        float *probabilities, void *hip_stream) {
+  if ((type != SSPMM_TYPE_F16 && type != SSPMM_TYPE_BF16 && type != SSPMM_TYPE_F32) || rows < 0 || vocab < 1 || vocab > 1 << 24 || row_stride < 0) return kInvalid;
+  if (rows == 0) return 0;
+  if (rows >= 1 << 22) return kInvalid;  // (a launch has less than 2^32 threads)
+  if (!logits || reinterpret_cast<uintptr_t>(logits) % (type == SSPMM_TYPE_F32 ? 4 : 2) || !uniform || !tokens) return kInvalid;
+  uintptr_t bits = 0;
+  for (const void *x : {(const void *)uniform, (const void *)temperature, (const void *)top_k, (const void *)top_p, (const void *)min_p, (const void *)tokens,
+                        (const void *)probabilities})
+    bits |= reinterpret_cast<uintptr_t>(x);
+  if (bits % 4) return kInvalid;
+  const sspmm::SampleArgs a = {logits, row_stride, rows, vocab, uniform, temperature, top_p, min_p, top_k, temperature_all, top_p_all, min_p_all, top_k_all, tokens,
+                               probabilities};
+  return (int)sspmm::launch_sample_tokens(type, a, static_cast<hipStream_t>(hip_stream));
 }
 
 size_t sspmm_reserve_pages_workspace_bytes(int pages, int rows, int slots) {

@@ -1,0 +1,584 @@
+// Attention of the newest tokens over the paged cache in 8 bits, for rows that share leading pages: what a group of rows shares is read once for all of them.
+//   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^((q . k_j) scale log2(e) - m),  k_j and v_j codes times their block's scale.
+// A plan says which rows share what.  Rows with the same first page are compared with the lowest of them; of these the rows that share S pages or more are a
+// group, with the S that saves most, S times the rows but one.  The queries of a group's rows lie one behind the other in tiles of 32 (queries x heads of one head of the cache) over
+// the shared pages, and every row's in tiles of their own over the rest.  All tiles, one behind the other, are as many units of keys, which the workgroups of a head of
+// the cache share evenly: a workgroup goes from tile to tile where its share does, and leaves a state (maximum, sum, weighted values) for each.  A second
+// launch makes one of the states of a row's queries.
+#include "prefix_kernels.h"
+
+#include "cache_codes.h"
+
+#include <limits.h>
+
+namespace sspmm {
+
+namespace {
+
+typedef unsigned long long u64;
+
+constexpr int kUnit = 32;   // keys of a unit, all of them in one page
+constexpr int kRows = 32;   // of a tile
+constexpr int kWaves = 4;   // of a workgroup, which share a tile's units
+constexpr int kLeastUnits = 16;  // of a workgroup's share, as far as there are
+
+// ---- the plan: 32-bit words, in this order
+//   header   tiles, workgroups that have a share (0: there are no units)
+//   starts   tiles + 1 numbers of 64 bits: units in front of a tile
+//   tiles    kTileWords each
+//   rows     kRowWords each
+//   order    the rows, group after group
+//   leaders, shared pages (of the first launch)
+constexpr int kHeaderWords = 4, kTileWords = 8, kRowWords = 4;
+struct Tile {
+  int row;       // of the table
+  int member;    // place in the order of the first row whose queries it holds
+  int first;     // its first query among theirs
+  int count;     // queries
+  int unit;      // its first unit, of the row
+  int end;       // positions of the row from here on are not the tile's
+  int all_seen;  // every query sees the keys below
+  int states;    // queries of the tiles in front
+};
+static_assert(sizeof(Tile) == 4 * kTileWords, "");
+struct RowPlan {
+  int shared_tile;  // the group's first tile, or -1
+  int place;        // in the group
+  int own_tile;
+  int length;       // tokens, also those that the table has no slot for
+};
+static_assert(sizeof(RowPlan) == 4 * kRowWords, "");
+struct PrefixPlan {
+  int32_t *header;
+  long long *starts;
+  Tile *tiles;
+  RowPlan *rows;
+  int32_t *order, *leaders, *shared;
+  __host__ __device__ PrefixPlan(int32_t *at, long long most_tiles, int n) {
+    header = at;
+    starts = reinterpret_cast<long long *>(at + kHeaderWords);
+    tiles = reinterpret_cast<Tile *>(starts + ((most_tiles + 2) & ~1ll));
+    rows = reinterpret_cast<RowPlan *>(tiles + most_tiles);
+    order = reinterpret_cast<int32_t *>(rows + n);
+    leaders = order + n;
+    shared = leaders + n;
+  }
+  __host__ __device__ long long words(int n) const { return shared + n - header; }
+};
+
+// Pages that lie whole in front of the row's first query.
+__device__ __forceinline__ int full_pages(int length, int queries, int page_size, int slots) {
+  return (int)min((long long)slots, max(0ll, (long long)length - queries + 1) / page_size);
+}
+
+// A wave a row: the lowest row that begins with the same page, and the pages that the two share.
+__global__ __launch_bounds__(64) void plan_prefixes_compare_kernel(PrefixPlan plan, const int32_t *table, int rows, int slots, const int32_t *lengths, int page_size, int queries) {
+  const int row = blockIdx.x, lane = threadIdx.x;
+  const int32_t *const own = table + (long long)row * slots;
+  const int first = own[0], full = full_pages(lengths[row], queries, page_size, slots);
+  int leader = -1, shared = 0;
+  if (first >= 0 && full > 0) {
+    for (int at = 0; at < rows && leader < 0; at += 64) {
+      const int r = at + lane;
+      const bool same = r < rows && table[(long long)r * slots] == first && full_pages(lengths[r], queries, page_size, slots) > 0;
+      const u64 those = __ballot(same);
+      if (those) leader = at + __builtin_ctzll(those);
+    }
+    const int32_t *const other = table + (long long)leader * slots;
+    const int most = min(full, full_pages(lengths[leader], queries, page_size, slots));
+    for (shared = 0; shared < most; shared += 64) {
+      const int s = shared + lane;
+      const u64 differ = __ballot(!(s < most && own[s] >= 0 && own[s] == other[s]));
+      if (differ) {
+        shared += __builtin_ctzll(differ);
+        break;
+      }
+    }
+    shared = min(shared, most);
+  }
+  if (lane == 0) {
+    plan.leaders[row] = leader;
+    plan.shared[row] = shared;
+  }
+}
+
+// Sum of v over the threads in front of the own one, and over all.
+__device__ __forceinline__ u64 sum_before(u64 v, u64 (&waves)[kMostPlanRows / 64], u64 &all) {
+  const int wave = threadIdx.x >> 6;
+  const u64 upto = wave_inclusive_sum(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) waves[wave] = upto;
+  __syncthreads();
+  u64 before = upto - v;
+  all = 0;
+  for (int i = 0; i < kMostPlanRows / 64; ++i) {
+    before += i < wave ? waves[i] : 0;
+    all += waves[i];
+  }
+  return before;
+}
+
+// One workgroup, a thread a row.
+__global__ __launch_bounds__(kMostPlanRows) void plan_prefixes_kernel(PrefixPlan plan, int rows, int slots, const int32_t *lengths, int page_size, int queries, PrefixShape shape) {
+  __shared__ int leaders[kMostPlanRows], shared[kMostPlanRows], base[kMostPlanRows], group_tile[kMostPlanRows];
+  __shared__ u64 best[kMostPlanRows], waves[kMostPlanRows / 64];
+  const int r = threadIdx.x;
+  const bool there = r < rows;
+  const int leader = there ? plan.leaders[r] : -1, mine = there ? plan.shared[r] : 0;
+  leaders[r] = leader;
+  shared[r] = mine;
+  best[r] = 0;
+  __syncthreads();
+  // ---- the pages that a group shares: of its rows' numbers the one that saves most
+  if (leader >= 0) {
+    int as_many = 0;
+    for (int i = 0; i < rows; ++i) as_many += leaders[i] == leader && shared[i] >= mine;
+    const u64 saved = (u64)mine * (u64)(as_many - 1);
+    if (saved) atomicMax(&best[leader], saved << 26 | (u64)mine);  // (fewer than 2^26 slots)
+  }
+  __syncthreads();
+  const u64 chosen = leader >= 0 ? best[leader] : 0;
+  const int pages = (int)(chosen & ((1u << 26) - 1)), own_pages = chosen && mine >= pages ? pages : 0;
+  const bool member = own_pages > 0, leads = member && leader == r;
+  // ---- order: a group's rows stand where its leader would
+  __syncthreads();
+  shared[r] = own_pages;
+  __syncthreads();
+  int place = 0, members = 0;
+  if (member)
+    for (int i = 0; i < rows; ++i) {
+      const bool one = leaders[i] == leader && shared[i] > 0;
+      members += one;
+      place += one && i < r;
+    }
+  u64 all;
+  const u64 at = sum_before(there ? (leads ? members : member ? 0 : 1) : 0, waves, all);
+  base[r] = (int)at;
+  __syncthreads();
+  const int in_order = member ? base[leader] + place : (int)at;
+  if (there) plan.order[in_order] = r;
+  // ---- tiles: the group's at its leader, and every row's own
+  const int length = there ? max(0, lengths[r]) : 0, end = (int)min((long long)length, (long long)slots * page_size);
+  const int from = own_pages * page_size;
+  const long long stacked = leads ? (long long)members * shape.row_queries : 0;
+  const int group_tiles = (int)((stacked + kRows - 1) / kRows), own_tiles = there ? (shape.row_queries + kRows - 1) / kRows : 0;
+  const int group_units = from / kUnit, own_units = (end - from + kUnit - 1) / kUnit;
+  const int tile = (int)sum_before((u64)(group_tiles + own_tiles), waves, all);
+  const int tiles = (int)all;
+  u64 units;
+  long long start = (long long)sum_before((u64)group_tiles * group_units + (u64)own_tiles * own_units, waves, units);
+  int states = (int)sum_before(there ? (u64)(stacked + shape.row_queries) : 0, waves, all);
+  group_tile[r] = tile;
+  __syncthreads();
+  if (there) {
+    for (int i = 0; i < group_tiles; ++i, start += group_units) {
+      plan.starts[tile + i] = start;
+      const int count = (int)min((long long)kRows, stacked - (long long)i * kRows);
+      plan.tiles[tile + i] = {r, in_order, i * kRows, count, 0, from, INT_MAX, states};
+      states += count;
+    }
+    const int own = tile + group_tiles;
+    for (int i = 0; i < own_tiles; ++i, start += own_units) {
+      plan.starts[own + i] = start;
+      const int count = min(kRows, shape.row_queries - i * kRows);
+      plan.tiles[own + i] = {r, in_order, i * kRows, count, from / kUnit, end, length - queries + 1, states};
+      states += count;
+    }
+    plan.rows[r] = {member ? group_tile[leader] : -1, place, own, length};
+  }
+  if (r == 0) {
+    plan.starts[tiles] = (long long)units;
+    plan.header[0] = tiles;
+    plan.header[1] = (int)min((u64)shape.workgroups, (units + kLeastUnits - 1) / kLeastUnits);
+  }
+}
+
+// Share i of the units begins at floor(i units / shares), for as many shares as units at most.
+__device__ __forceinline__ long long share_start(long long units, int shares, int i) { return units * i / shares; }
+__device__ __forceinline__ int share_of(long long units, int shares, long long unit) { return (int)(((unit + 1) * shares - 1) / units); }
+// The rows where a share leaves its state of a tile: D values each, and behind all of these a maximum and a sum each.  From one state to the next either
+// the tile is another, and the tiles' queries are counted on, or the share is: no two overlap.
+__device__ __forceinline__ long long state_row(const Tile &tile, int share) { return (long long)tile.states + (long long)share * kRows; }
+
+template <typename T, int FORMAT, int D, int TILES, int UNIT>
+struct CacheRows {
+  static constexpr int kKeyTiles = UNIT / 16, kParts = D / 16, kSteps = D / 32, kShares = UNIT / 32;
+  static constexpr int kKeyWords = D >= 64 ? 4 : 2;  // of a load of K: 16 bytes, or 8 where a group's share of a row is no more
+  static constexpr int kKeyLoads = D / (16 * kKeyWords);  // of a row by a lane
+  static constexpr int kValueWords = UNIT / 16;
+  typedef uint32_t KeyWords __attribute__((ext_vector_type(kKeyWords)));
+  typedef uint32_t ValueWords __attribute__((ext_vector_type(kValueWords)));
+
+  uintx4 q[TILES][kSteps];
+  float c[TILES];
+  int seen[TILES];  // keys that the row sees: those below
+  floatx4 o[TILES][kParts];  // features 16 part + 4 g + i of row m
+  float run_max[TILES], run_sum[TILES];
+
+  // Row m of tile t: its features at `at`.  bf16 goes to fp16 by way of a power of two for the row, which leaves its largest magnitude in 2^14 .. 2^15
+  __device__ __forceinline__ void load_query(int t, const uint16_t *at, int sees, float scale_log2e) {
+    const int g = (threadIdx.x & 63) >> 4;
+    seen[t] = sees;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int d = D >= 64 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 8 * g;
+      q[t][s] = *reinterpret_cast<const uintx4 *>(at + d);
+    }
+    c[t] = scale_log2e;
+    if constexpr (!__is_same(T, Fp16)) {
+      float most = 0.f;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) most = fmaxf(most, fmaxf(fabsf(T::lower(q[t][s][j])), fabsf(T::upper(q[t][s][j]))));
+      most = max_over_rows(most);
+      const int e = max((int)(__float_as_uint(most) >> 23) - 127 - 14, -126);
+      const bool usual = most < INFINITY;  // (else as they are)
+      const float up = usual ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.f;
+      c[t] *= usual ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.f;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q[t][s][j] = Fp16::pack(T::lower(q[t][s][j]) * up, T::upper(q[t][s][j]) * up);
+    }
+  }
+
+  // Units unit0 .. unit1 - 1 of the sequence whose pages `table` lists, `length` positions of which are something.  all_seen: every row sees the keys below.
+  __device__ __forceinline__ void attend(const CachePool &pool, const int32_t *table, int head, int unit0, int unit1, int all_seen, int length) {
+    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+      run_max[t] = -3.0e38f;
+      run_sum[t] = 0.f;
+#pragma unroll
+      for (int part = 0; part < kParts; ++part) o[t][part] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    const long long block = (long long)pool.page_size * D;
+    KeyWords kk[kKeyTiles][kKeyLoads];
+    ValueWords vv[kParts];
+    const int page_units = pool.page_size / UNIT, page_bits = 31 - __builtin_clz(page_units);  // (1 or 2)
+    const auto place_of = [&](int u) { return (u & (page_units - 1)) * UNIT; };  // in its page
+    const auto usable = [&](int pg) { return pg >= 0 && pg < pool.pages; };
+    // Pages and scales of 64 units at a time, one a lane, so that no unit waits for them.
+    int pages_of = 0;
+    float k_scales = 0.f, v_scales = 0.f;
+    const auto look_up = [&](int u) {
+      const int mine = min(u + lane, unit1 - 1);
+      pages_of = table[mine >> page_bits];
+      const float *const scale = pool.scales + (long long)(usable(pages_of) ? pages_of : 0) * 2 * pool.kv_heads + head;
+      k_scales = scale[0];
+      v_scales = scale[pool.kv_heads] * kValueUnit;
+    };
+    const auto load_k = [&](int u, int pg) {
+      const unsigned char *const at = pool.keys + ((long long)(usable(pg) ? pg : 0) * pool.kv_heads + head) * block + place_of(u) * D;
+#pragma unroll
+      for (int kt = 0; kt < kKeyTiles; ++kt) {
+        const unsigned char *const row = at + (UNIT / 4 * (m >> 2) + 4 * kt + (m & 3)) * D + 4 * kKeyWords * g;
+#pragma unroll
+        for (int i = 0; i < kKeyLoads; ++i) {
+          kk[kt][i] = *reinterpret_cast<const KeyWords *>(row + 64 * i);
+        }
+      }
+    };
+    const auto load_v = [&](int u, int pg) {
+      const unsigned char *const at = pool.values + ((long long)(usable(pg) ? pg : 0) * pool.kv_heads + head) * block + place_of(u) + UNIT / 4 * g;
+#pragma unroll
+      for (int part = 0; part < kParts; ++part) {
+        const unsigned char *const row = at + (16 * part + m) * pool.page_size;
+        vv[part] = *reinterpret_cast<const ValueWords *>(row);
+      }
+    };
+
+    int page = 0;
+    if (unit0 < unit1) {
+      look_up(unit0);
+      page = __builtin_amdgcn_readlane(pages_of, 0);
+      load_k(unit0, page);
+      load_v(unit0, page);
+    }
+    for (int u = unit0; u < unit1; ++u) {
+      const bool more = u + 1 < unit1, there = usable(page);
+      const int at = (u - unit0) & 63;
+      const float k_scale = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(k_scales), at));
+      const float v_scale = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v_scales), at));
+      if (at == 63 && more) look_up(u + 1);
+      const int page_next = __builtin_amdgcn_readlane(pages_of, (at + 1) & 63);
+      floatx4 s[TILES][kKeyTiles];
+#pragma unroll
+      for (int kt = 0; kt < kKeyTiles; ++kt) {
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) s[t][kt] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int step = 0; step < kSteps; ++step) {
+          const int i = D >= 64 ? step / 2 : 0, w = D >= 64 ? 2 * (step % 2) : 0;
+          const uintx4 k = as_halfs<FORMAT>(kk[kt][i][w], kk[kt][i][w + 1]);
+#pragma unroll
+          for (int t = 0; t < TILES; ++t) s[t][kt] = mfma(k, q[t][step], s[t][kt]);
+        }
+      }
+      if (more) load_k(u + 1, page_next);
+      const int key0 = u * UNIT, key = key0 + UNIT / 4 * g;
+      const bool cut = !there || key0 + UNIT > all_seen;  // uniform: some row does not see some key
+      float v_scale_of[TILES];
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) {
+        const float f = k_scale * c[t];
+#pragma unroll
+        for (int kt = 0; kt < kKeyTiles; ++kt) s[t][kt] *= f;
+        v_scale_of[t] = v_scale;
+      }
+      if (__builtin_expect(cut, 0)) {
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+          const int left = there ? seen[t] - key : INT_MIN;
+#pragma unroll
+          for (int kt = 0; kt < kKeyTiles; ++kt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[t][kt][i] = 4 * kt + i >= left ? -INFINITY : s[t][kt][i];
+          // (a row that sees nothing of the page does not see that its scale is NaN either)
+          if (!there || key0 >= seen[t]) v_scale_of[t] = 0.f;
+        }
+      }
+      uintx4 pt[TILES][kShares];
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) {
+        float most = -INFINITY;
+#pragma unroll
+        for (int kt = 0; kt < kKeyTiles; ++kt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) most = fmaxf(most, s[t][kt][i]);
+        most = max_over_rows(most);
+        // The reference point moves only when a row's maximum has grown by more than 2^8, and lies 2^7 below it then: fp16 holds 2^15, but loses what is
+        // below 2^-25, and many keys of small probabilities are not nothing.
+        const float new_max = fmaxf(run_max[t], most - 7.0f);
+        if (__ballot(new_max - run_max[t] > 8.0f) != 0) {
+          const float down = half_way_down(new_max - run_max[t]);
+          run_max[t] = new_max;
+          run_sum[t] = run_sum[t] * down * down;
+#pragma unroll
+          for (int part = 0; part < kParts; ++part) o[t][part] = o[t][part] * down * down;
+        }
+#pragma unroll
+        for (int kt = 0; kt < kKeyTiles; ++kt)
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            const float a = __builtin_amdgcn_exp2f(s[t][kt][i] - run_max[t]), b = __builtin_amdgcn_exp2f(s[t][kt][i + 1] - run_max[t]);
+            run_sum[t] += a + b;
+            pt[t][kt / 2][2 * (kt % 2) + i / 2] = Fp16::pack(a, b);
+          }
+      }
+      // (Nothing: but the compiler of ROCm 7.2 loses half of such a pair of words between here and there, and reuses its register, unless both are
+      // wanted at one place.  -verify-machineinstrs finds it; the build asks for that.)
+#pragma unroll
+      for (int part = 0; part < kParts; ++part) asm volatile("" : "+v"(vv[part]));
+      if (FORMAT == 1 && (!there || key0 + UNIT > length)) {  // (what lies behind the sequence, or in no page of it, may be NaN)
+#pragma unroll
+        for (int w = 0; w < kValueWords; ++w) {
+          const int left = there ? max(0, min(4, length - key - 4 * w)) : 0;
+          const uint32_t mask = left == 4 ? 0xffffffffu : (1u << (8 * left)) - 1u;
+#pragma unroll
+          for (int part = 0; part < kParts; ++part) vv[part][w] &= mask;
+        }
+      }
+#pragma unroll
+      for (int part = 0; part < kParts; ++part) {
+        floatx4 sum[TILES];
+#pragma unroll
+        for (int w = 0; w < kShares; ++w) {
+          const uintx4 v = as_halfs<FORMAT>(vv[part][2 * w], vv[part][2 * w + 1]);
+#pragma unroll
+          for (int t = 0; t < TILES; ++t) sum[t] = mfma(v, pt[t][w], w == 0 ? floatx4{0.f, 0.f, 0.f, 0.f} : sum[t]);
+        }
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[t][part][i] = fmaf(sum[t][i], v_scale_of[t], o[t][part][i]);
+      }
+      if (more) load_v(u + 1, page_next);
+      page = page_next;
+    }
+  }
+
+  // The waves' sums of this workgroup to one reference point for each row, and that and the sums of the exponentials beside them.  Ends with a barrier.
+  template <int WAVES>
+  __device__ __forceinline__ void join(int wave, float (&state)[WAVES][2][16 * TILES], float (&sums)[WAVES][16 * TILES][D]) {
+    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+      run_sum[t] = sum_over_rows(run_sum[t]);
+      if (g == 0) {
+        state[wave][0][16 * t + m] = run_max[t];
+        state[wave][1][16 * t + m] = run_sum[t];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+      float most = state[0][0][16 * t + m];
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) most = fmaxf(most, state[w][0][16 * t + m]);
+      const float down = half_way_down(most - run_max[t]);
+#pragma unroll
+      for (int part = 0; part < kParts; ++part) *reinterpret_cast<floatx4 *>(&sums[wave][16 * t + m][16 * part + 4 * g]) = o[t][part] * down * down;
+    }
+    __syncthreads();
+  }
+  // Features d .. d + 3 of row r over all waves, after that: their sum, its reference point and the sum of its exponentials.
+  template <int WAVES>
+  __device__ __forceinline__ floatx4 joined(const float (&state)[WAVES][2][16 * TILES], const float (&sums)[WAVES][16 * TILES][D], int r, int d, float &most,
+                                            float &total) const {
+    most = state[0][0][r];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) most = fmaxf(most, state[w][0][r]);
+    floatx4 x = {0.f, 0.f, 0.f, 0.f};
+    total = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      x += *reinterpret_cast<const floatx4 *>(&sums[w][r][d]);
+      const float down = half_way_down(most - state[w][0][r]);
+      total += state[w][1][r] * down * down;
+    }
+    return x;
+  }
+};
+
+// A tile's units unit0 .. unit1 - 1 by the workgroup, and its state of them.
+template <typename T, int FORMAT, int D, int TILES>
+__device__ __forceinline__ void attend_tile(const PrefixAttentionArgs &p, const PrefixPlan &plan, const Tile &tile, int head, int unit0, int unit1, float *values, float *sums_to, float *lds) {
+  typedef float States[kWaves][2][16 * TILES];
+  typedef float Sums[kWaves][16 * TILES][D];
+  States &state = *reinterpret_cast<States *>(lds + sizeof(Sums) / 4);
+  Sums &sums = *reinterpret_cast<Sums *>(lds);
+  const int m = threadIdx.x & 15, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = p.heads / p.pool.kv_heads, row_queries = p.queries * group;
+  CacheRows<T, FORMAT, D, TILES, kUnit> w;
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) {
+    // (places behind the last query take that one's: its maxima move no reference point that it does not move itself)
+    const int at = tile.first + min(16 * t + m, tile.count - 1), row = plan.order[tile.member + at / row_queries], r = at % row_queries, i = r / group;
+    w.load_query(t, p.q + (long long)row * p.q_seq + (long long)i * p.q_row + (long long)(head * group + r % group) * p.q_head, plan.rows[row].length - p.queries + 1 + i,
+                 p.scale_log2e);
+  }
+  const int units = unit1 - unit0;
+  w.attend(p.pool, p.pool.table + (long long)tile.row * p.pool.slots, head, unit0 + units * wave / kWaves, unit0 + units * (wave + 1) / kWaves, tile.all_seen, tile.end);
+  w.template join<kWaves>(wave, state, sums);
+  for (int at = threadIdx.x; at < 16 * TILES * D / 4; at += 64 * kWaves) {
+    const int r = at / (D / 4), d = (at % (D / 4)) * 4;
+    if (r >= tile.count) continue;
+    float most, total;
+    const floatx4 x = w.joined(state, sums, r, d, most, total);
+    *reinterpret_cast<floatx4 *>(values + r * D + d) = x;
+    if (d == 0) {
+      sums_to[2 * r] = most;
+      sums_to[2 * r + 1] = total;
+    }
+  }
+  __syncthreads();
+}
+
+template <typename T, int FORMAT, int D>
+__global__ __launch_bounds__(64 * kWaves, 2) void prefix_attention_kernel(const PrefixAttentionArgs p) {
+  __shared__ __align__(16) float lds[kWaves * kRows * (D + 2)];
+  const PrefixPlan plan(const_cast<int32_t *>(p.plan), p.shape.tiles, p.rows);
+  const int head = blockIdx.x, share = blockIdx.y, shares = plan.header[1], tiles = plan.header[0];
+  if (share >= shares) return;
+  const long long units = plan.starts[tiles];
+  long long at = share_start(units, shares, share);
+  const long long end = share_start(units, shares, share + 1);
+  // (the last tile that begins here or before; those without units are passed over)
+  int i = last_not_above(tiles, 0, [&](int t) { return plan.starts[t] > at ? 1 : 0; });
+  for (; at < end; ++i) {
+    const long long begin = plan.starts[i], behind = min(plan.starts[i + 1], end);
+    if (behind <= at) continue;
+    const Tile tile = plan.tiles[i];
+    const int unit0 = tile.unit + (int)(at - begin), unit1 = tile.unit + (int)(behind - begin);
+    const long long row = head * p.shape.state_rows + state_row(tile, share);
+    float *const values = p.partial + row * D, *const sums = p.partial + p.pool.kv_heads * p.shape.state_rows * D + 2 * row;
+    if (tile.count > 16) attend_tile<T, FORMAT, D, 2>(p, plan, tile, head, unit0, unit1, values, sums, lds);
+    else attend_tile<T, FORMAT, D, 1>(p, plan, tile, head, unit0, unit1, values, sums, lds);
+    at = behind;
+  }
+}
+
+// D / 4 threads a query and head: its states of the shared pages, then those of the rest.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void prefix_attention_join_kernel(const PrefixAttentionArgs p) {
+  constexpr int kThreads = D / 4;
+  const PrefixPlan plan(const_cast<int32_t *>(p.plan), p.shape.tiles, p.rows);
+  const int kv = p.pool.kv_heads, group = p.heads / kv, row_queries = p.queries * group;
+  const long long n = (long long)blockIdx.x * (256 / kThreads) + threadIdx.x / kThreads;
+  if (n >= (long long)p.rows * p.queries * p.heads) return;
+  const int d = (threadIdx.x % kThreads) * 4;
+  const int h = (int)(n % p.heads), i = (int)(n / p.heads % p.queries), b = (int)(n / p.heads / p.queries);
+  const int head = h / group, r = i * group + h % group;
+  const RowPlan row = plan.rows[b];
+  const int shares = plan.header[1], tiles = plan.header[0];
+  const long long units = plan.starts[tiles];
+  const float *const values = p.partial + head * p.shape.state_rows * D, *const sums = p.partial + (kv * D + 2 * head) * p.shape.state_rows;
+  float most = -3.0e38f, total = 0.f;
+  floatx4 x = {0.f, 0.f, 0.f, 0.f};
+  for (int part = 0; part < 2; ++part) {
+    const int query = part == 0 ? row.place * row_queries + r : r;
+    if (part == 0 && row.shared_tile < 0) continue;
+    const int tile = (part == 0 ? row.shared_tile : row.own_tile) + query / kRows, place = query % kRows;
+    const long long begin = plan.starts[tile], end = plan.starts[tile + 1];
+    if (begin == end) continue;
+    const int last = share_of(units, shares, end - 1);
+    const Tile what = plan.tiles[tile];
+    for (int share = share_of(units, shares, begin); share <= last; ++share) {
+      const long long at = state_row(what, share) + place;
+      const float theirs = sums[2 * at], sum = sums[2 * at + 1], new_most = fmaxf(most, theirs);
+      const float down = half_way_down(new_most - most), their_down = half_way_down(new_most - theirs);
+      total = total * down * down + sum * their_down * their_down;
+      x = x * down * down + *reinterpret_cast<const floatx4 *>(values + at * D + d) * their_down * their_down;
+      most = new_most;
+    }
+  }
+  const float inv = total > 0.f || total != total ? 1.0f / kValueUnit / total : 0.f;
+  uint16_t *const to = p.out + (long long)b * p.out_seq + (long long)i * p.out_row + (long long)h * p.out_head + d;
+  *reinterpret_cast<uintx2 *>(to) = uintx2{T::pack(x[0] * inv, x[1] * inv), T::pack(x[2] * inv, x[3] * inv)};
+}
+
+template <typename T, int FORMAT, int D>
+hipError_t launch(const PrefixAttentionArgs &a, hipStream_t stream) {
+  hipLaunchKernelGGL((prefix_attention_kernel<T, FORMAT, D>), dim3(a.pool.kv_heads, a.shape.workgroups), dim3(64 * kWaves), 0, stream, a);
+  const long long n = (long long)a.rows * a.queries * a.heads, each = 256 / (D / 4);
+  hipLaunchKernelGGL((prefix_attention_join_kernel<T, D>), dim3((unsigned)((n + each - 1) / each)), dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+template <typename T, int FORMAT>
+hipError_t launch(const PrefixAttentionArgs &a, hipStream_t stream) {
+  return a.pool.d == 128 ? launch<T, FORMAT, 128>(a, stream) : a.pool.d == 64 ? launch<T, FORMAT, 64>(a, stream) : launch<T, FORMAT, 32>(a, stream);
+}
+
+}  // namespace
+
+PrefixShape prefix_shape(int rows, int queries, int heads, int kv_heads) {
+  PrefixShape s;
+  s.row_queries = queries * (heads / kv_heads);
+  // own tiles; shared ones, full but for one in a group of two rows or more
+  s.tiles = (long long)rows * ((s.row_queries + kRows - 1) / kRows) + (long long)rows * s.row_queries / kRows + rows / 2;
+  s.workgroups = max(1, 512 / kv_heads);
+  s.state_rows = 2ll * rows * s.row_queries + (long long)s.workgroups * kRows;
+  return s;
+}
+size_t prefix_plan_ints(const PrefixShape &shape, int rows) { return (size_t)PrefixPlan(nullptr, shape.tiles, rows).words(rows); }
+size_t prefix_attention_floats(const PrefixShape &shape, int kv_heads, int d) {
+  return (size_t)kv_heads * (size_t)shape.state_rows * (d + 2);
+}
+
+hipError_t launch_plan_prefixes(const PrefixShape &shape, const int32_t *table, int rows, int slots, const int32_t *lengths, int page_size, int queries, int32_t *plan,
+                                hipStream_t stream) {
+  const PrefixPlan at(plan, shape.tiles, rows);
+  hipLaunchKernelGGL(plan_prefixes_compare_kernel, dim3(rows), dim3(64), 0, stream, at, table, rows, slots, lengths, page_size, queries);
+  hipLaunchKernelGGL(plan_prefixes_kernel, dim3(1), dim3(kMostPlanRows), 0, stream, at, rows, slots, lengths, page_size, queries, shape);
+  return hipGetLastError();
+}
+
+hipError_t launch_prefix_attention(int type, int format, const PrefixAttentionArgs &a, hipStream_t stream) {
+  if (type == 0) return format == 0 ? launch<Fp16, 0>(a, stream) : launch<Fp16, 1>(a, stream);
+  return format == 0 ? launch<Bf16, 0>(a, stream) : launch<Bf16, 1>(a, stream);
+}
+
+}  // namespace sspmm

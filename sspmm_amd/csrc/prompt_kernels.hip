@@ -1,6 +1,7 @@
 // Attention over whole prompts that lie one behind the other: for every sequence and head
 //   out_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = 2^((q_i . k_j) scale log2(e) - m_i),  j <= i (causal) or all j of the sequence,
-// with heads / kv_heads query heads on each head of k and v.  One pass over the keys with a running m_i and sum.
+// with heads / kv_heads query heads on each head of k and v.  One pass over the keys with a running m_i and sum.  CROSS: the keys are another sequence's,
+// of another length, all of which the queries see.
 #include "prompt_kernels.h"
 
 #include "lane_ops.h"
@@ -67,7 +68,7 @@ __device__ __forceinline__ uintx4 finite_part(uintx4 v) {
 // units are busy 53 % of the cycles, the vector ones 37 % (without the exponentials the launch takes 5 % less, with K and V from registers 33 %).  Tried without gain: all of K's operands asked for
 // ahead, K two tiles and V one and a half ahead with two barriers a tile, 256 queries a workgroup, 64 queries a workgroup (1.4 times as long).
 // Short prompts wait for their latencies: 512 tokens, 32 heads 15 us, eight tiles one after the other.
-template <typename T, int D, int GROUPS, bool CAUSAL, bool AHEAD>
+template <typename T, int D, int GROUPS, bool CAUSAL, bool CROSS, bool AHEAD>
 __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void prompt_attention_kernel(const PromptArgs p, int tiles) {
   constexpr int kPieces = D / 8, kTile = kKeys * D * 2;
   constexpr int kSteps = D / 16, kParts = D / 32;  // steps of the first product; parts of 32 features of the second
@@ -100,6 +101,7 @@ __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void prompt_attention_kern
   // keys go first: level x (a causal tile has about as many keys as places before it in its sequence, another as many as its sequence) is
   // the largest at which more tiles than those before this one are of x or more.
   int first = 0, length = -1, q0 = 0;  // the sequence's first row and rows, the workgroup's first query in it
+  int key_first = 0, keys = 0;  // its first key's row, and keys
   const auto base = [&](int chunk) { return max(0, min(p.offsets[64 * chunk], p.tokens)) / kTileQueries + 64 * chunk; };
   const int chunk = last_not_above((p.sequences + 63) / 64, tile, base);
   int left = tile - base(chunk);
@@ -133,14 +135,21 @@ __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void prompt_attention_kern
     first = __builtin_amdgcn_readlane(lo, at);
     length = __builtin_amdgcn_readlane(hi, at) - first;
     q0 = (CAUSAL ? x - 1 : left % x) * kTileQueries;
+    if constexpr (CROSS) {
+      key_first = max(0, min(p.key_offsets[64 * chunk + at], p.key_tokens));
+      keys = max(key_first, min(p.key_offsets[64 * chunk + at + 1], p.key_tokens)) - key_first;
+    } else {
+      key_first = first;
+      keys = length;
+    }
   }
   if (length < 0) return;
 
   const int kv_head = head / (p.heads / p.kv_heads);
   const int my = q0 + 32 * wave + n;  // this lane's query
-  const int seen = CAUSAL ? min(my + 1, length) : length;  // keys it sees: those below
-  const int most = CAUSAL ? min(q0 + 32 * wave + 32, length) : length;  // (no query of the wave sees one from here on)
-  const int last = CAUSAL ? min(q0 + kTileQueries, length) : length;
+  const int seen = CAUSAL ? min(my + 1, keys) : keys;  // keys it sees: those below
+  const int most = CAUSAL ? min(q0 + 32 * wave + 32, keys) : keys;  // (no query of the wave sees one from here on)
+  const int last = CAUSAL ? min(q0 + kTileQueries, keys) : keys;
   const int key_tiles = (last + kKeys - 1) / kKeys;
 
   // ---- queries: lane (n, half) holds features 16 s + 8 half .. + 7 of its query
@@ -152,8 +161,8 @@ __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void prompt_attention_kern
   }
 
   // ---- tiles come from memory straight into LDS; rows behind the sequence are zeros
-  const uint16_t *const k0 = p.k + (long long)first * p.k_row + (long long)kv_head * p.k_head;
-  const uint16_t *const v0 = p.v + (long long)first * p.v_row + (long long)kv_head * p.v_head;
+  const uint16_t *const k0 = p.k + (long long)key_first * p.k_row + (long long)kv_head * p.k_head;
+  const uint16_t *const v0 = p.v + (long long)key_first * p.v_row + (long long)kv_head * p.v_head;
   const uint32_t k_pitch = (uint32_t)p.k_row * 2, v_pitch = (uint32_t)p.v_row * 2;
   const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)lds + wave * 1024;
   uint32_t k_at[kLoads], v_at[kLoads];
@@ -164,7 +173,7 @@ __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void prompt_attention_kern
     v_at[i] = r * v_pitch + (c ^ swizzle_v<D>(r)) * 16;
   }
   const auto fetch = [&](int t) {
-    const int rows = min(kKeys, length - t * kKeys);
+    const int rows = min(kKeys, keys - t * kKeys);
     const srd sk = descriptor(k0 + (long long)t * kKeys * p.k_row, (rows - 1) * k_pitch + D * 2);
     const srd sv = descriptor(v0 + (long long)t * kKeys * p.v_row, (rows - 1) * v_pitch + D * 2);
     const uint32_t to = lds_at + (t / GROUPS & 1) * 2 * kTile;
@@ -342,7 +351,7 @@ __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void prompt_attention_kern
     __syncthreads();
     if (t + GROUPS < key_tiles) fetch(t + GROUPS);
   };
-  const int whole_tiles = (CAUSAL ? min(q0 + 1, length) : length) / kKeys;  // that all queries of the workgroup see
+  const int whole_tiles = (CAUSAL ? min(q0 + 1, keys) : keys) / kKeys;  // that all queries of the workgroup see
   // A masked key's probability is zero, and so is what underflows, but zero times an infinity or a NaN in v is NaN.  A workgroup that finds a
   // result which is not finite goes over its keys again: the products are of the finite values then, and the others are added, key by key,
   // to the queries that see them.  (Looking at every tile at the mask's edge first: 512 tokens, 32 heads of 128 features 17.0 us instead of 15.1.)
@@ -440,10 +449,12 @@ hipError_t launch(bool causal, const PromptArgs &a, hipStream_t stream) {
   const unsigned threads = 64 * kWaves * GROUPS;
   if (tiles * a.heads >= 1 << 23) return hipErrorInvalidValue;  // (a launch has less than 2^32 threads)
   const unsigned blocks = (unsigned)(tiles * a.heads);
-  if (causal)
-    hipLaunchKernelGGL((prompt_attention_kernel<T, D, GROUPS, true, AHEAD>), dim3(blocks), dim3(threads), 0, stream, a, (int)tiles);
+  if (a.key_offsets)
+    hipLaunchKernelGGL((prompt_attention_kernel<T, D, GROUPS, false, true, AHEAD>), dim3(blocks), dim3(threads), 0, stream, a, (int)tiles);
+  else if (causal)
+    hipLaunchKernelGGL((prompt_attention_kernel<T, D, GROUPS, true, false, AHEAD>), dim3(blocks), dim3(threads), 0, stream, a, (int)tiles);
   else
-    hipLaunchKernelGGL((prompt_attention_kernel<T, D, GROUPS, false, AHEAD>), dim3(blocks), dim3(threads), 0, stream, a, (int)tiles);
+    hipLaunchKernelGGL((prompt_attention_kernel<T, D, GROUPS, false, false, AHEAD>), dim3(blocks), dim3(threads), 0, stream, a, (int)tiles);
   return hipGetLastError();
 }
 
@@ -453,7 +464,7 @@ hipError_t launch(bool causal, const PromptArgs &a, hipStream_t stream) {
 // 39.9 and 33.9; 8 x 512 tokens, 12 heads of 64 15.6 and 16.6.
 long long workgroups(const PromptArgs &a) { return ((long long)a.tokens + kTileQueries - 1) / kTileQueries * a.heads; }
 bool two_groups(bool causal, const PromptArgs &a) {
-  const long long tiles = workgroups(a), length = a.tokens / a.sequences;
+  const long long tiles = workgroups(a), length = a.key_tokens / a.sequences;  // (keys)
   return length >= 768 && (tiles <= 256 || (causal && tiles <= 512 && length >= 3000));
 }
 
@@ -464,7 +475,7 @@ bool two_groups(bool causal, const PromptArgs &a) {
 // Without a mask the bad stretch ends sooner: 8 heads of 6500 tokens (408) 191 -> 180, 8192 (512) 267 -> 259, 9000 416 -> 436, 4 of 20000 917 -> 961, 12500 722 -> 671, 13000
 // 757 -> 708, 16001 1011 -> 973, 32768 4143 -> 4037; 32 of 6500 (1632) 708 -> 729.  The mean length is what the host knows: 16001 tokens with two prompts of one token beside
 // them go without (545 us, with it 503).
-bool go_ahead(const PromptArgs &a) { return a.tokens / a.sequences > 6000 && (workgroups(a) <= 512 || workgroups(a) > 800); }
+bool go_ahead(const PromptArgs &a) { return a.key_tokens / a.sequences > 6000 && (workgroups(a) <= 512 || workgroups(a) > 800); }
 
 template <typename T, int D>
 hipError_t launch(bool causal, const PromptArgs &a, hipStream_t stream) {

@@ -7,6 +7,10 @@ tokens after them are written to and read from.  They stand beside the attention
     reserve_pages(page_refs, page_table, starts, offsets, page_size)  # pages for the new tokens
     cache_write(k, v, offsets, starts, page_table, keys, values, scales)
     out = cache_attention(q, page_table, lengths, keys, values, scales)  # the newest tokens of every row
+    plan = plan_prefixes(page_table, lengths, queries, heads, kv_heads, page_size)  # or, of rows that share pages, once a step
+    out = prefix_attention(q, page_table, plan, keys, values, scales)    # and in every layer
+    out = cross_attention(q, k, v, offsets, source_offsets)              # on an encoder's states
+    tokens = sample_tokens(logits, uniform, temperature, top_k, top_p, min_p)
 
 Lists and tables are int32 tensors on the GPU, read when the kernels run: no call waits for the device, so a step can be captured in a
 graph.  What the device alone knows is not checked by the host: entries that name no token, row or page are passed over.
@@ -204,6 +208,42 @@ def prompt_attention(q, k, v, offsets, scaling=None, causal=True, out=None):
     return out
 
 
+def cross_attention(q, k, v, offsets, source_offsets, scaling=None, out=None):
+    """softmax(q k^T * scaling) v of packed queries over packed states of other lengths, a decoder's over its encoder's: q [tokens, heads, d], k and v
+    [source_tokens, kv_heads, d]; the queries of sequence b, offsets[b] .. offsets[b + 1] - 1, see all of source_offsets[b] .. source_offsets[b + 1] - 1 and
+    nothing else.  Types, head widths, strides, scaling and out as in prompt_attention; single tokens are sequences of one.  A sequence without states is
+    zeros; tokens of no sequence are not written."""
+    dtype, device = q.dtype, q.get_device()
+    kind = TYPES.get(dtype)
+    if (kind is None or device < 0 or k.dtype is not dtype or v.dtype is not dtype or k.get_device() != device or v.get_device() != device or
+            q.dim() != 3 or k.dim() != 3 or v.dim() != 3):
+        for name, t in (("q", q), ("k", k), ("v", v)):
+            _activations(name, t, 3, dtype, device)
+    _no_gradients(q, k, v)
+    tokens, heads, d = q.shape
+    shape = k.shape
+    source_tokens, kv = shape[0], shape[1]
+    if shape != v.shape or shape[2] != d:
+        raise ValueError("k and v must both be [source_tokens, kv_heads, d] with q's d")
+    _heads(heads, kv, d)
+    if not (_listed(offsets, 1, device) and _listed(source_offsets, 1, device)):
+        _ints("offsets", offsets, 1, device)
+        _ints("source_offsets", source_offsets, 1, device)
+    sequences = offsets.numel() - 1
+    if sequences < 0 or source_offsets.numel() != sequences + 1:
+        raise ValueError("offsets and source_offsets must both hold one value more than there are sequences")
+    scale = _scaling(scaling, d)
+    out, (to, out_row, out_head, _) = _out(out, q, _tokens)
+    if tokens == 0:
+        return out
+    (q_at, q_row, q_head, q_), (k_at, k_row, k_head, k_), (v_at, v_row, v_head, v_) = _tokens(q), _tokens(k), _tokens(v)
+    rc = _lib.call(_lib.lib().sspmm_cross_attention, q.device, kind, sequences, tokens, source_tokens, heads, kv, d, offsets.data_ptr(), source_offsets.data_ptr(),
+                   q_at, q_row, q_head, k_at, k_row, k_head, v_at, v_row, v_head, scale, to, out_row, out_head)
+    if rc:
+        _lib.check(rc, "sspmm_cross_attention")
+    return out
+
+
 def cache_write(k, v, offsets, starts, page_table, keys, values, scales):
     """Tokens offsets[b] .. offsets[b + 1] - 1 of k and v [tokens, kv_heads, d] into the cache, at positions starts[b] on of row b of
     page_table [rows, slots].  The tokens of a page have one scale per head for their keys and one for their values: the largest magnitude
@@ -275,6 +315,141 @@ def cache_attention(q, page_table, lengths, keys, values, scales, scaling=None, 
     if rc:
         _lib.check(rc, "sspmm_cache_attention")
     return out
+
+
+class PrefixPlan:
+    """Which rows of a page table share their leading pages, as plan_prefixes found it on the device, for calls of prefix_attention with the sizes it names."""
+    __slots__ = ("rows", "slots", "queries", "heads", "kv_heads", "page_size", "data")
+
+    def __init__(self, rows, slots, queries, heads, kv_heads, page_size, data):
+        self.rows, self.slots, self.queries, self.heads, self.kv_heads, self.page_size, self.data = rows, slots, queries, heads, kv_heads, page_size, data
+
+
+def plan_prefixes(page_table, lengths, queries, heads, kv_heads, page_size, plan=None):
+    """Which rows of page_table [rows, slots] share leading pages, once a step for the prefix_attention of all layers: a PrefixPlan for `queries` newest tokens of
+    every row.  Rows that begin with the same page are compared with the lowest of them; those that share at least the number of pages that saves most
+    are a group.  `plan`: one of the same sizes, made anew in place (for a step captured in a graph whose plan is made outside).  At most 1024 rows, 2^20 of
+    queries * heads and 2^22 of rows * queries * heads."""
+    device = page_table.get_device()
+    if device < 0:
+        raise TypeError("page_table must be on a GPU")
+    if not (_listed(page_table, 2, device) and _listed(lengths, 1, device)):
+        _ints("page_table", page_table, 2, device)
+        _ints("lengths", lengths, 1, device)
+    rows, slots = page_table.shape
+    if lengths.numel() != rows:
+        raise ValueError("lengths must have a value for every row of page_table")
+    if slots < 1 or page_size not in PAGE_SIZES:
+        raise ValueError("page_table must have a slot, and pages 32, 64 or 128 tokens")
+    size = _workspace_bytes("sspmm_prefix_plan_bytes", rows, queries, heads, kv_heads)
+    if size == 0 and rows and queries:
+        raise ValueError("a plan is for up to 1024 rows, 2^20 queries * heads and 2^22 rows * queries * heads, heads a multiple of kv_heads")
+    if plan is None:
+        plan = PrefixPlan(rows, slots, queries, heads, kv_heads, page_size, page_table.new_empty(size >> 2))
+    elif ((plan.rows, plan.slots, plan.queries, plan.heads, plan.kv_heads, plan.page_size) != (rows, slots, queries, heads, kv_heads, page_size) or
+          plan.data.get_device() != device):
+        raise ValueError("plan is of other sizes, or on another GPU")
+    if rows and queries:
+        rc = _lib.call(_lib.lib().sspmm_plan_prefixes, page_table.device, page_table.data_ptr(), rows, slots, lengths.data_ptr(), page_size, queries, heads, kv_heads,
+                       plan.data.data_ptr(), size)
+        if rc:
+            _lib.check(rc, "sspmm_plan_prefixes")
+    return plan
+
+
+def prefix_attention(q, page_table, plan, keys, values, scales, scaling=None, out=None):
+    """cache_attention for rows that share leading pages, as fork_pages leaves them: a page that a group of rows shares is read once for all of them.  q
+    [rows, n, heads, d], page_table and the cache as there; plan: plan_prefixes of this table and the rows' lengths, which are taken from it."""
+    dtype, device = q.dtype, q.get_device()
+    kind = TYPES.get(dtype)
+    if kind is None or device < 0 or q.dim() != 4:
+        _activations("q", q, 4, dtype, device)
+    _no_gradients(q, keys, values, scales)
+    form, pages, kv, page_size, d = _cache(keys, values, scales, device)
+    rows, n, heads, dq = q.shape
+    if dq != d:
+        raise ValueError("q must have the cache's %d features a head" % d)
+    _heads(heads, kv, d)
+    if not _listed(page_table, 2, device):
+        _ints("page_table", page_table, 2, device)
+    if plan.data.get_device() != device:
+        raise TypeError("plan must be on the other arguments' GPU")
+    slots = page_table.size(1)
+    if (plan.rows, plan.slots, plan.queries, plan.heads, plan.kv_heads, plan.page_size) != (rows, slots, n, heads, kv, page_size) or page_table.size(0) != rows:
+        raise ValueError("plan is for %d rows of %d slots, %d queries, %d heads on %d, pages of %d" %
+                         (plan.rows, plan.slots, plan.queries, plan.heads, plan.kv_heads, plan.page_size))
+    scale = _scaling(scaling, d)
+    out, (to, out_seq, out_row, out_head, _) = _out(out, q, _queries)
+    if rows == 0 or n == 0:
+        return out
+    q_at, q_seq, q_row, q_head, q_ = _queries(q)
+    size = _workspace_bytes("sspmm_prefix_attention_workspace_bytes", rows, n, heads, kv, d)
+    room = scales.new_empty(size >> 2)
+    rc = _lib.call(_lib.lib().sspmm_prefix_attention, q.device, kind, form, rows, n, heads, q_at, q_seq, q_row, q_head, page_table.data_ptr(), slots,
+                   plan.data.data_ptr(), 4 * plan.data.numel(), pages, kv, page_size, d, keys.data_ptr(), values.data_ptr(), scales.data_ptr(), scale, to, out_seq,
+                   out_row, out_head, room.data_ptr(), size)
+    if rc:
+        _lib.check(rc, "sspmm_prefix_attention")
+    return out
+
+
+LOGIT_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+MOST_TOKENS = 1 << 24  # of a vocabulary
+
+
+def _setting(name, value, dtype, rows, device, fits):
+    """(address or None, the value for all rows) of one of sample_tokens' settings."""
+    if isinstance(value, torch.Tensor):
+        if value.dtype is not dtype or value.get_device() != device or not value.is_contiguous() or value.dim() != 1:
+            raise TypeError("%s must be a number, or a contiguous %s tensor of one dimension on the logits' GPU" % (name, str(dtype).split(".")[1]))
+        if value.numel() != rows:
+            raise ValueError("%s must have a value for each of the %d rows" % (name, rows))
+        _no_gradients(value)
+        return value.data_ptr(), 0
+    if not fits(value):
+        raise ValueError("%s cannot be %r" % (name, value))
+    return None, value
+
+
+def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, probabilities=False):
+    """A token of each row of logits [rows, vocab] (float16, bfloat16 or float32), drawn with uniform [rows] (float32, in [0, 1)): int32 [rows].
+
+    With the weights w = exp((l - max l) / temperature), kept are those with w >= min_p; of these the top_k first in the order of falling logits, equal ones by
+    rising index; of these the shortest run, at least one, whose weights reach top_p of the sum of all of these.  The token is the first in that order at which
+    the running sum of the weights exceeds uniform times their sum.  Each setting is a number or a tensor with one for every row (float32, top_k int32).
+    temperature 0: the largest logit, its first index; top_k 0, top_p 1, min_p 0: everything is kept (of tensors, which the host does not look at, also temperature and
+    top_k below 0, and NaN: temperature as 0, the others as what keeps everything).  Logits of -infinity, and NaN, are never drawn; of +infinity they share the draw; a row without any other gives -1.
+    probabilities: (tokens, float32 [rows] of the probabilities with which they were drawn).
+
+    Weights are whole multiples of 2^-b of the largest, vocab * 2^b <= 2^62 (at most 52), so that no order of sums changes a token.  Rows may lie apart, at any element;
+    other strides are copied first.  At most 2^24 tokens in a vocabulary."""
+    kind, device = LOGIT_TYPES.get(logits.dtype), logits.get_device()
+    if kind is None or device < 0:
+        raise TypeError("logits must be a float16, bfloat16 or float32 tensor on a GPU")
+    if logits.dim() != 2:
+        raise ValueError("logits must be [rows, vocab]")
+    _no_gradients(logits, uniform)
+    rows, vocab = logits.shape
+    if not 1 <= vocab <= MOST_TOKENS:
+        raise ValueError("a vocabulary has 1 to 2^24 tokens, got %d" % vocab)
+    if uniform.dtype is not torch.float32 or uniform.get_device() != device or not uniform.is_contiguous():
+        raise TypeError("uniform must be a contiguous float32 tensor on the logits' GPU")
+    if uniform.shape != (rows,):
+        raise ValueError("uniform must have a number for each of the %d rows" % rows)
+    t_at, t_all = _setting("temperature", temperature, torch.float32, rows, device, lambda x: 0.0 <= x < math.inf)
+    k_at, k_all = _setting("top_k", top_k, torch.int32, rows, device, lambda x: 0 <= x < 1 << 31)
+    p_at, p_all = _setting("top_p", top_p, torch.float32, rows, device, lambda x: 0.0 <= x <= 1.0)
+    m_at, m_all = _setting("min_p", min_p, torch.float32, rows, device, lambda x: 0.0 <= x <= 1.0)
+    tokens = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    chances = torch.empty(rows, dtype=torch.float32, device=logits.device) if probabilities else None
+    if rows:
+        if logits.stride(1) != 1 and vocab > 1:
+            logits = logits.contiguous()
+        rc = _lib.call(_lib.lib().sspmm_sample_tokens, logits.device, kind, rows, vocab, logits.data_ptr(), logits.stride(0), uniform.data_ptr(), t_at, t_all, k_at, k_all,
+                       p_at, p_all, m_at, m_all, tokens.data_ptr(), chances.data_ptr() if probabilities else None)
+        if rc:
+            _lib.check(rc, "sspmm_sample_tokens")
+    return (tokens, chances) if probabilities else tokens
 
 
 def _table(page_refs, page_table):
