@@ -3,8 +3,12 @@
 // reach top_p of all of theirs.  The token is the first in that order at which the running sum of the weights exceeds u times their sum.
 //
 // Weights are whole numbers, in units of 2^-unit_bits of the largest: sums of them are exact in any order, so that atomics and lanes give the same token every
-// time.  Vocabularies of 2^17 leave 45 bits; what weighs less than half a unit is never drawn.  No row is sorted: a row is put into bins by z, which is to say
-// by weight, and where a count or a sum ends inside a bin that bin alone is split by its logits until one logit is left.
+// time.  Vocabularies of 2^17 leave 45 bits; what weighs less than half a unit is never drawn.
+//
+// No row is sorted.  With a top_k of some hundred, the largest logit of every thread's share gives a logit that enough others reach; those that reach it become a list
+// in LDS, and the draw is the list's.  Else the row is put into bins by z, which is to say by weight; where a sum ends is then known up to a bin, and the logits of the few
+// bins that matter become the list.  A bin is split by its logits until one logit is left, and equal logits by their indices.  Where the list has no room, the row
+// in memory stands in its place.
 #include "sample_kernels.h"
 
 #include "lane_ops.h"
@@ -14,8 +18,12 @@ namespace sspmm {
 
 namespace {
 
+typedef unsigned long long u64;
+
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kBins = 4096, kFine = 1024;  // of the whole row, and of a range of logits
+constexpr int kBins = 2048, kFine = 1024;  // of a row or its list, and of a range of logits
+constexpr int kList = 4096;                // logits of a list
+constexpr int kMostTopK = 1200;            // that the threads' two largest each give a bound for
 
 struct F32 {};
 
@@ -46,91 +54,171 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   const uint32_t u = __float_as_uint(x + 0.f);
   return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
+__device__ __forceinline__ float logit_of(uint32_t key) { return __uint_as_float(key ^ ((uint32_t)((int32_t)~key >> 31) | 0x80000000u)); }
 
-typedef unsigned long long u64;
-
-// What a workgroup knows of its row.
-struct Row {
-  float most;            // the largest logit
-  double per_logit;      // 1 / T
-  double farthest;       // largest z of a token that is kept
-  double unit;           // weight of the largest
-  // (monotone in x, so that bins and ranges of logits never cross)
-  __device__ __forceinline__ bool candidate(float x, double &z) const {
-    z = x == most ? 0.0 : ((double)most - (double)x) * per_logit;
-    return x > -INFINITY && (x == most || most < INFINITY) && z <= farthest;
+// What a row is drawn with.
+struct Setting {
+  float temperature, top_p, min_p;
+  int top_k;  // 0: all
+  int unit_bits;
+  bool greedy;
+  __device__ __forceinline__ Setting(const SampleArgs &p, int r) {
+    temperature = p.temperature ? p.temperature[r] : p.temperature_all;
+    top_p = p.top_p ? p.top_p[r] : p.top_p_all;
+    min_p = p.min_p ? p.min_p[r] : p.min_p_all;
+    top_k = p.top_k ? p.top_k[r] : p.top_k_all;
+    if (top_k < 0 || top_k >= p.vocab) top_k = 0;
+    greedy = !(temperature > 0.f) || top_k == 1;
+    if (greedy) top_k = 1;
+    unit_bits = min(50, 30 + __builtin_clz(max(p.vocab - 1, 1)));  // vocab << unit_bits is no more than 2^62
   }
-  __device__ __forceinline__ u64 weight(double z) const { return (u64)(exp(-z) * unit + 0.5); }
+  __device__ __forceinline__ bool few() const { return top_k > 0 && top_k <= kMostTopK; }
 };
 
-struct Shared {
+struct Weights {
+  double most, per_logit, farthest;  // the largest logit; log2(e) / T; largest y = z log2(e) of a token that is kept
+  int unit_bits;
+  float to_bin;
+  bool infinite;
+  __device__ __forceinline__ Weights(const Setting &s, float largest) {
+    most = (double)largest;
+    per_logit = 1.4426950408889634 / (double)s.temperature;
+    unit_bits = s.unit_bits;
+    farthest = s.min_p > 0.f ? -log2((double)fminf(s.min_p, 1.f)) : 1100.0;
+    to_bin = (float)kBins / (float)(unit_bits + 1);
+    infinite = largest == INFINITY;
+  }
+  // (monotone in x, so that bins and ranges of logits never cross; -infinity and NaN are 1100, whose weight is nothing)
+  __device__ __forceinline__ double distance(float x) const { return fmin((most - (double)x) * per_logit, 1100.0); }
+  // 2^-y in units: y = n - f, 2^f = 1 + f g(f), g a polynomial through its Chebyshev points in -1/2 .. 1/2, off by 2^-44.  Adding 2^52 leaves the whole number
+  // in the lower bits.  (Some twenty instructions, at the rate of those in 32 bits.)
+  __device__ __forceinline__ u64 units(double y) const {
+    const double n = rint(y), f = n - y;
+    double g = 0x1.b638808b9c3c7p-24;
+    g = fma(g, f, 0x1.63d136362c015p-20);
+    g = fma(g, f, 0x1.ffcb9515bca86p-17);
+    g = fma(g, f, 0x1.4308ac85aafa8p-13);
+    g = fma(g, f, 0x1.5d87fe86fe84ep-10);
+    g = fma(g, f, 0x1.3b2ab7181b74fp-7);
+    g = fma(g, f, 0x1.c6b08d7047e52p-5);
+    g = fma(g, f, 0x1.ebfbdff823cedp-3);
+    g = fma(g, f, 0x1.62e42fefa39efp-1);
+    const double w = ldexp(fma(g, f, 1.0), unit_bits - (int)n) + 0x1p52;
+    return (u64)__double_as_longlong(w) - 0x4330000000000000ull;
+  }
+  // of any logit; y for its bin
+  __device__ __forceinline__ u64 of(float x, double &y) const {
+    y = (double)x == most ? 0.0 : infinite ? 1100.0 : distance(x);
+    return y <= farthest ? units(y) : 0;
+  }
+  __device__ __forceinline__ int bin(double y) const { return min((int)((float)y * to_bin), kBins - 1); }
+  // A logit that no logit of bin b and those before it is below (or, from the side of 0, above), whatever was rounded on the way.
+  __device__ __forceinline__ float lowest(int b) const {
+    if (b >= kBins - 1 || infinite) return -INFINITY;
+    const double x = most - (double)(b + 1) / (double)to_bin * 1.000001 / per_logit;
+    return (float)(x - (fabs(x) * 0x1p-22 + 1e-44));
+  }
+  __device__ __forceinline__ float highest(int b) const {
+    if (b == 0 || infinite) return INFINITY;
+    const double x = most - (double)b / (double)to_bin * 0.999999 / per_logit;
+    return (float)(x + (fabs(x) * 0x1p-22 + 1e-44));
+  }
+};
+
+struct Bins {
   u64 weights[kBins];
   uint32_t counts[kBins];
   u64 fine_weights[kFine];
   uint32_t fine_counts[kFine];
+};
+struct Shared {
+  Bins bins;
+  uint32_t keys[kList], indices[kList];
   u64 wave_weights[kWaves];
   uint32_t wave_counts[kWaves];
-  uint32_t low, high;
-  int found, token;
+  uint32_t low, high, listed;
+  int at, token;
   u64 before_weight, at_weight;
   uint32_t before_count, at_count;
 };
 
-// A place in the order: the logit, what lies before its first token, its tokens and the weight of each.
-struct Place {
-  uint32_t key, before_count, tokens;
-  u64 before_weight, weight;
-};
-
+// A row in memory, or a part of it.
 template <typename T>
-struct Reader {
+struct RowReader {
   typedef Elements<T> E;
-  const unsigned char *blocks;  // 16-byte aligned, at or before the row's first element
-  int lead, vocab, first, end;  // elements before the row in its first block, of the row; the wave's blocks
-  __device__ __forceinline__ Reader(const void *row, int vocab_) : vocab(vocab_) {
-    const uintptr_t at = reinterpret_cast<uintptr_t>(row);
-    blocks = reinterpret_cast<const unsigned char *>(at & ~(uintptr_t)15);
-    lead = (int)(at & 15) / E::kBytes;
-    const int all = (lead + vocab + E::kCount - 1) / E::kCount, each = (all + kThreads - 1) / kThreads * 64;
-    first = min(all, (int)(threadIdx.x >> 6) * each);
-    end = min(all, first + each);
+  const unsigned char *row;  // aligned to an element
+  int first, end;            // whole blocks of 16 aligned bytes in it, counted from the one that holds its first element
+  int lead, from, to;        // elements in front of the row in that block; the part's elements
+  // the part of a row in the blocks first_block .. end_block - 1 as they are counted here
+  __device__ __forceinline__ RowReader(const void *row_, int vocab, int first_block, int end_block) {
+    row = static_cast<const unsigned char *>(row_);
+    lead = (int)(reinterpret_cast<uintptr_t>(row_) & 15) / E::kBytes;
+    from = max(0, first_block * E::kCount - lead);
+    to = min((long long)vocab, (long long)end_block * E::kCount - lead);
+    first = (from + lead + E::kCount - 1) / E::kCount;
+    end = max(first, (to + lead) / E::kCount);
   }
-  // The elements of block b; those outside the row are -infinity, and so is NaN.
-  __device__ __forceinline__ void read(int b, float (&x)[E::kCount]) const {
-    const int at = b * E::kCount - lead;
-    if (at >= 0 && at + E::kCount <= vocab) {
-      E::take(*reinterpret_cast<const uintx4 *>(blocks + (long long)b * 16), x);
-    } else {
-#pragma unroll
-      for (int i = 0; i < E::kCount; ++i)
-        x[i] = at + i >= 0 && at + i < vocab ? E::one(blocks + (long long)b * 16 + i * E::kBytes) : -INFINITY;
-    }
-#pragma unroll
-    for (int i = 0; i < E::kCount; ++i) x[i] = x[i] == x[i] ? x[i] : -INFINITY;
+  static __device__ __forceinline__ int blocks(const void *row, int vocab) {
+    return ((int)(reinterpret_cast<uintptr_t>(row) & 15) / E::kBytes + vocab + E::kCount - 1) / E::kCount;
   }
-  // f(x) of every element of the wave's share, in any order
-  template <typename F>
+  __device__ __forceinline__ float one(int i) const { return E::one(row + (long long)i * E::kBytes); }
+  // f(logit, index) of every element, in any order
+  template <int UNROLL = 1, typename F>
   __device__ __forceinline__ void each(const F &f) const {
-    for (int b = first + (threadIdx.x & 63); b < end; b += 64) {
+    const unsigned char *const blocks = row - lead * E::kBytes;
+#pragma unroll UNROLL
+    for (int b = first + (int)threadIdx.x; b < end; b += kThreads) {
       float x[E::kCount];
-      read(b, x);
+      E::take(*reinterpret_cast<const uintx4 *>(blocks + (long long)b * 16), x);
 #pragma unroll
-      for (int i = 0; i < E::kCount; ++i) f(x[i]);
+      for (int i = 0; i < E::kCount; ++i) f(x[i], b * E::kCount - lead + i);
     }
+    // (what lies in front of the whole blocks and behind them, an element a thread)
+    const int tid = threadIdx.x, head_end = min(to, first * E::kCount - lead), tail = max(head_end, end * E::kCount - lead);
+    const int i = from + tid < head_end ? from + tid : tail + tid - (head_end - from);
+    if (i < head_end || (i >= tail && i < to)) f(one(i), i);
   }
 };
 
-// Counts and weights of BINS bins become sums of those up to and with each.  Ends with a barrier.
+struct ListReader {
+  const uint32_t *keys, *indices;
+  int count;
+  template <int UNROLL = 1, typename F>
+  __device__ __forceinline__ void each(const F &f) const {
+    for (int i = threadIdx.x; i < count; i += kThreads) f(logit_of(keys[i]), (int)indices[i]);
+  }
+};
+
+// Sum of v over the threads in front of the own one; and, in `all`, over all.  Two barriers.
+template <typename V>
+__device__ __forceinline__ V sum_before(V v, V (&waves)[kWaves], V &all) {
+  const int wave = threadIdx.x >> 6;
+  const V upto = wave_inclusive_sum(v);
+  if ((threadIdx.x & 63) == 63) waves[wave] = upto;
+  __syncthreads();
+  V before = upto - v;
+  all = 0;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    const V w = waves[i];
+    before += i < wave ? w : 0;
+    all += w;
+  }
+  __syncthreads();
+  return before;
+}
+
+// Counts and weights of the bins become sums of those up to and with each.  Ends with a barrier.
 template <int BINS>
 __device__ __forceinline__ void running_sums(u64 (&weights)[BINS], uint32_t (&counts)[BINS], Shared &s) {
-  constexpr int kEach = BINS / kThreads;
+  constexpr int kOwn = BINS / kThreads;
   const int tid = threadIdx.x, wave = tid >> 6;
-  u64 w[kEach], w_sum = 0;
-  uint32_t c[kEach], c_sum = 0;
+  u64 w[kOwn], w_sum = 0;
+  uint32_t c[kOwn], c_sum = 0;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    w[i] = w_sum += weights[tid * kEach + i];
-    c[i] = c_sum += counts[tid * kEach + i];
+  for (int i = 0; i < kOwn; ++i) {
+    w[i] = w_sum += weights[tid * kOwn + i];
+    c[i] = c_sum += counts[tid * kOwn + i];
   }
   u64 w_before = wave_inclusive_sum(w_sum);
   uint32_t c_before = wave_inclusive_sum(c_sum);
@@ -141,26 +229,27 @@ __device__ __forceinline__ void running_sums(u64 (&weights)[BINS], uint32_t (&co
   w_before -= w_sum;
   c_before -= c_sum;
   __syncthreads();
-  for (int i = 0; i < wave; ++i) {
-    w_before += s.wave_weights[i];
-    c_before += s.wave_counts[i];
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    w_before += i < wave ? s.wave_weights[i] : 0;
+    c_before += i < wave ? s.wave_counts[i] : 0;
   }
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    weights[tid * kEach + i] = w_before + w[i];
-    counts[tid * kEach + i] = c_before + c[i];
+  for (int i = 0; i < kOwn; ++i) {
+    weights[tid * kOwn + i] = w_before + w[i];
+    counts[tid * kOwn + i] = c_before + c[i];
   }
   __syncthreads();
 }
 
-// The first bin up to whose end there are `amount` tokens, or as much weight: into s.found, with what lies before it and in it.  Ends with a barrier.
+// The first bin up to whose end there are `amount` tokens, or as much weight: into s.at, with what lies before it and in it.  Ends with a barrier.
 template <int BINS>
 __device__ __forceinline__ void find(const u64 (&weights)[BINS], const uint32_t (&counts)[BINS], bool by_count, u64 amount, Shared &s) {
   for (int b = threadIdx.x; b < BINS; b += kThreads) {
     const u64 w0 = b ? weights[b - 1] : 0, w1 = weights[b];
     const uint32_t c0 = b ? counts[b - 1] : 0, c1 = counts[b];
     if (by_count ? c0 < amount && amount <= c1 : w0 < amount && amount <= w1) {
-      s.found = b;
+      s.at = b;
       s.before_weight = w0;
       s.before_count = c0;
       s.at_weight = w1 - w0;
@@ -170,60 +259,71 @@ __device__ __forceinline__ void find(const u64 (&weights)[BINS], const uint32_t 
   __syncthreads();
 }
 
+// A place in the order: the logit, what lies before its first token, its tokens and the weight of each.
+struct Place {
+  uint32_t key, before_count, tokens;
+  u64 before_weight, weight;
+};
+
 // The logit at which the running count, or the running sum of the weights, reaches `amount` (at least one, and no more than there is).
-template <typename T>
-__device__ Place locate(const Reader<T> &reader, const Row &row, float to_bin, bool by_count, u64 amount, Shared &s) {
+template <typename Reader>
+__device__ __forceinline__ Place locate(const Reader &reader, const Weights &weights, bool by_count, u64 amount, Shared &s) {
+  __syncthreads();
   if (threadIdx.x == 0) {
     s.low = 0xffffffffu;
     s.high = 0;
   }
-  find(s.weights, s.counts, by_count, amount, s);
-  const int bin = s.found;
+  find(s.bins.weights, s.bins.counts, by_count, amount, s);
+  const int bin = s.at;
   Place place;
   place.before_count = s.before_count;
   place.before_weight = s.before_weight;
-  place.tokens = s.at_count;
   u64 inside = s.at_weight;
-  uint32_t low = 0xffffffffu, high = 0;
-  reader.each([&](float x) {
-    double z;
-    if (row.candidate(x, z) && min((int)((float)z * to_bin), kBins - 1) == bin) {
-      low = min(low, key_of(x));
-      high = max(high, key_of(x));
+  uint32_t low = 0xffffffffu, high = 0, count = 0;
+  const float from = weights.lowest(bin), to = weights.highest(bin);
+  reader.template each<2>([&](float x, int) {
+    if (x >= from && x <= to) {
+      double y;
+      if (weights.of(x, y) && weights.bin(y) == bin) {
+        low = min(low, key_of(x));
+        high = max(high, key_of(x));
+        ++count;
+      }
     }
   });
   if (low <= high) {
     atomicMin(&s.low, low);
     atomicMax(&s.high, high);
   }
-  __syncthreads();
+  sum_before(count, s.wave_counts, place.tokens);  // (two barriers)
   low = s.low;
   high = s.high;
-  __syncthreads();
   while (low < high) {
     const int shift = max(0, 22 - (int)__builtin_clz(high - low));  // (high - low) >> shift is below kFine
     for (int b = threadIdx.x; b < kFine; b += kThreads) {
-      s.fine_weights[b] = 0;
-      s.fine_counts[b] = 0;
+      s.bins.fine_weights[b] = 0;
+      s.bins.fine_counts[b] = 0;
     }
     __syncthreads();
-    reader.each([&](float x) {
-      double z;
+    reader.each([&](float x, int) {
       const uint32_t key = key_of(x);
-      if (key >= low && key <= high && row.candidate(x, z)) {
-        const uint32_t b = (high - key) >> shift;
-        atomicAdd(&s.fine_counts[b], 1u);
-        atomicAdd(&s.fine_weights[b], row.weight(z));
+      if (key >= low && key <= high) {
+        double y;
+        const u64 w = weights.of(x, y);
+        if (w) {
+          atomicAdd(&s.bins.fine_counts[(high - key) >> shift], 1u);
+          atomicAdd(&s.bins.fine_weights[(high - key) >> shift], w);
+        }
       }
     });
     __syncthreads();
-    running_sums(s.fine_weights, s.fine_counts, s);
-    find(s.fine_weights, s.fine_counts, by_count, by_count ? amount - place.before_count : amount - place.before_weight, s);
+    running_sums(s.bins.fine_weights, s.bins.fine_counts, s);
+    find(s.bins.fine_weights, s.bins.fine_counts, by_count, by_count ? amount - place.before_count : amount - place.before_weight, s);
     place.before_count += s.before_count;
     place.before_weight += s.before_weight;
     place.tokens = s.at_count;
     inside = s.at_weight;
-    const uint32_t from = high - ((uint32_t)s.found << shift), rest = (1u << shift) - 1u;
+    const uint32_t from = high - ((uint32_t)s.at << shift), rest = (1u << shift) - 1u;
     high = from;
     low = max(low, from - min(from, rest));
     __syncthreads();
@@ -233,112 +333,238 @@ __device__ Place locate(const Reader<T> &reader, const Row &row, float to_bin, b
   return place;
 }
 
-// The index of the token number `which` among those of one logit.
-template <typename T>
-__device__ int index_of(const Reader<T> &reader, uint32_t key, uint32_t which, Shared &s) {
-  constexpr int kCount = Elements<T>::kCount;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint32_t mine = 0;
-  reader.each([&](float x) { mine += x > -INFINITY && key_of(x) == key; });
-  mine = wave_inclusive_sum(mine);
-  if (lane == 63) s.wave_counts[wave] = mine;
-  __syncthreads();
-  uint32_t before = 0;
-  for (int i = 0; i < wave; ++i) before += s.wave_counts[i];
-  if (which >= before && which < before + s.wave_counts[wave]) {
-    uint32_t left = which - before;
-    for (int b = reader.first; b < reader.end; b += 64) {
-      float x[kCount];
-      uint32_t here = 0;
-      if (b + lane < reader.end) {
-        reader.read(b + lane, x);
-#pragma unroll
-        for (int i = 0; i < kCount; ++i) here += x[i] > -INFINITY && key_of(x[i]) == key;
-      }
-      const uint32_t upto = wave_inclusive_sum(here), all = from_last_lane(upto);
-      if (left < all) {
-        uint32_t skip = left - (upto - here);  // (of this lane's)
-        if (left >= upto - here && left < upto) {
-#pragma unroll
-          for (int i = 0; i < kCount; ++i)
-            if (x[i] > -INFINITY && key_of(x[i]) == key && skip-- == 0) s.token = (b + lane) * kCount - reader.lead + i;
-        }
-        break;
-      }
-      left -= all;
+// The index of the token number `which` among those of one logit: the range of indices is split as ranges of logits are.
+template <typename Reader>
+__device__ __forceinline__ int index_of(const Reader &reader, uint32_t key, uint32_t which, int vocab, Shared &s) {
+  uint32_t low = 0, high = (uint32_t)vocab - 1;
+  while (low < high) {
+    const int shift = max(0, 22 - (int)__builtin_clz(high - low));
+    s.bins.fine_counts[threadIdx.x] = 0;
+    __syncthreads();
+    reader.each([&](float x, int i) {
+      if (key_of(x) == key && (uint32_t)i >= low && (uint32_t)i <= high) atomicAdd(&s.bins.fine_counts[((uint32_t)i - low) >> shift], 1u);
+    });
+    __syncthreads();
+    uint32_t all;
+    const uint32_t own = s.bins.fine_counts[threadIdx.x], before = sum_before(own, s.wave_counts, all);
+    if (which >= before && which < before + own) {
+      s.at = threadIdx.x;
+      s.before_count = before;
     }
+    __syncthreads();
+    which -= s.before_count;
+    const uint32_t from = low + ((uint32_t)s.at << shift);
+    high = min(high, from + ((1u << shift) - 1u));
+    low = from;
+    __syncthreads();
+  }
+  return (int)low;
+}
+
+// The reader's logits into the bins, whose sums are what s.bins then holds.  counted: tokens, too.
+template <typename Reader>
+__device__ __forceinline__ void fill_bins(const Reader &reader, const Weights &weights, bool counted, Shared &s) {
+  for (int b = threadIdx.x; b < kBins; b += kThreads) {
+    s.bins.weights[b] = 0;
+    s.bins.counts[b] = 0;
   }
   __syncthreads();
-  return s.token;
+  if (counted)
+    reader.each([&](float x, int) {
+      double y;
+      const u64 w = weights.of(x, y);
+      if (w) {
+        const int b = weights.bin(y);
+        atomicAdd(&s.bins.counts[b], 1u);
+        atomicAdd(&s.bins.weights[b], w);
+      }
+    });
+  else
+    reader.each([&](float x, int) {
+      double y;
+      const u64 w = weights.of(x, y);
+      if (w) atomicAdd(&s.bins.weights[weights.bin(y)], w);
+    });
+  __syncthreads();
+}
+
+__device__ __forceinline__ u64 top_p_amount(float top_p, u64 total) { return min(max((u64)ceil((double)fmaxf(top_p, 0.f) * (double)total), (u64)1), total); }
+__device__ __forceinline__ u64 drawn_amount(float u, u64 total) { return min((u64)((double)u * (double)total) + 1, total); }
+
+// The draw, with the row's sums in s.bins; of the bins in which the sums that it asks for end, the reader has the logits.
+template <typename Reader>
+__device__ __forceinline__ void draw(const Reader &reader, const Setting &setting, const Weights &weights, float u, int vocab, Shared &s, int &token, float &probability) {
+  u64 total = s.bins.weights[kBins - 1];
+  if (setting.top_k > 0 && (uint32_t)setting.top_k < s.bins.counts[kBins - 1]) {
+    const Place place = locate(reader, weights, true, (u64)setting.top_k, s);
+    total = place.before_weight + (u64)((uint32_t)setting.top_k - place.before_count) * place.weight;
+  }
+  if (setting.top_p < 1.f) {
+    const u64 amount = top_p_amount(setting.top_p, total);
+    const Place place = locate(reader, weights, false, amount, s);
+    // (the first of its tokens that reaches the amount is the last one kept)
+    total = place.before_weight + (amount - place.before_weight + place.weight - 1) / place.weight * place.weight;
+  }
+  const u64 amount = drawn_amount(u, total);
+  const Place place = locate(reader, weights, false, amount, s);
+  token = index_of(reader, place.key, (uint32_t)((amount - place.before_weight - 1) / place.weight), vocab, s);
+  probability = (float)((double)place.weight / (double)total);
+}
+
+// Logits from `from` to `to` and their indices onto the list, as far as it has room; s.listed counts all.
+__device__ __forceinline__ void list(float x, int i, Shared &s) {
+  const uint32_t at = atomicAdd(&s.listed, 1u);
+  if (at < kList) {
+    s.keys[at] = key_of(x);
+    s.indices[at] = (uint32_t)i;
+  }
+}
+
+// The logits of the bins in which what draw() asks for may end, as far as the sums in s.bins say, become the list.  Ends with a barrier.
+template <typename T>
+__device__ __forceinline__ void list_ends(const RowReader<T> &reader, const Setting &setting, const Weights &weights, float u, Shared &s) {
+  float from[3], to[3];
+  int ranges = 0;
+  u64 least = s.bins.weights[kBins - 1], most = least;  // that the kept tokens weigh
+  const auto ends = [&](bool by_count, u64 first, u64 last) {  // bins in which sums of first .. last end
+    find(s.bins.weights, s.bins.counts, by_count, first, s);
+    const int low = s.at;
+    least = s.before_weight + 1;
+    __syncthreads();
+    find(s.bins.weights, s.bins.counts, by_count, last, s);
+    const int high = s.at;
+    most = s.before_weight + s.at_weight;
+    __syncthreads();
+    from[ranges] = weights.lowest(high);
+    to[ranges] = weights.highest(low);
+    ++ranges;
+  };
+  if (threadIdx.x == 0) s.listed = 0;
+  if (setting.top_k > 0 && (uint32_t)setting.top_k < s.bins.counts[kBins - 1]) ends(true, (u64)setting.top_k, (u64)setting.top_k);
+  if (setting.top_p < 1.f) ends(false, top_p_amount(setting.top_p, least), top_p_amount(setting.top_p, most));
+  ends(false, drawn_amount(u, least), drawn_amount(u, most));
+  for (int i = ranges; i < 3; ++i) {
+    from[i] = INFINITY;
+    to[i] = -INFINITY;
+  }
+  reader.template each<2>([&](float x, int i) {
+    const bool a = x >= from[0] && x <= to[0], b = x >= from[1] && x <= to[1], c = x >= from[2] && x <= to[2];
+    if (a || b || c) list(x, i, s);
+  });
+  __syncthreads();
+}
+
+// The largest of the reader's logits, -infinity if there is none.
+template <typename Reader>
+__device__ __forceinline__ float largest_of(const Reader &reader, Shared &s) {
+  float most = -INFINITY;
+  reader.template each<4>([&](float x, int) { most = fmaxf(most, x); });
+  most = wave_max_all(most);
+  if ((threadIdx.x & 63) == 0) s.wave_counts[threadIdx.x >> 6] = __float_as_uint(most);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) most = fmaxf(most, __uint_as_float(s.wave_counts[i]));
+  __syncthreads();
+  return most;
+}
+
+// The first `wanted` of the reader's logits, and others, onto the list: those that a logit reaches which so many of the threads' largest, or two largest, reach.  Its number, or
+// 0 where the list has all.  Ends with a barrier.
+template <typename T>
+__device__ __forceinline__ uint32_t list_first(const RowReader<T> &reader, uint32_t wanted, float &largest, Shared &s) {
+  const int tid = threadIdx.x;
+  const bool two = wanted > kThreads / 4;
+  float first = -INFINITY, second = -INFINITY;
+  if (two)
+    reader.template each<2>([&](float x, int) {
+      x = x == x ? x : -INFINITY;
+      second = fmaxf(second, fminf(first, x));
+      first = fmaxf(first, x);
+    });
+  else
+    reader.template each<4>([&](float x, int) { first = fmaxf(first, x); });
+  // ---- bins of equal width from the smallest of these to the largest
+  if (tid == 0) {
+    s.low = s.high = 0;
+    s.at = kFine;
+    s.listed = 0;
+  }
+  s.bins.fine_counts[tid] = 0;
+  __syncthreads();
+  const float most = wave_max_all(first), least = -wave_max_all(first > -INFINITY ? -first : -INFINITY);
+  if ((tid & 63) == 0) {
+    atomicMax(&s.high, key_of(most));
+    atomicMax(&s.low, ~key_of(least));
+  }
+  __syncthreads();
+  const float top = logit_of(s.high), bottom = logit_of(~s.low);
+  const float scale = (float)(kFine - 1) / fmaxf(top - bottom, 1e-30f);
+  const auto bin = [&](float x) { return (int)fminf(fmaxf((top - x) * scale, 0.f), (float)(kFine - 1)); };
+  if (first > -INFINITY) atomicAdd(&s.bins.fine_counts[bin(first)], 1u);
+  if (second > -INFINITY) atomicAdd(&s.bins.fine_counts[bin(second)], 1u);
+  __syncthreads();
+  uint32_t all;
+  const uint32_t own = s.bins.fine_counts[tid], before = sum_before(own, s.wave_counts, all);
+  if (before < wanted && wanted <= before + own) s.at = tid;
+  if (tid == 0) s.low = 0xffffffffu;
+  __syncthreads();
+  const int last = s.at;
+  if (last < kFine) {
+    if (first > -INFINITY && bin(first) <= last) atomicMin(&s.low, key_of(first));
+    if (second > -INFINITY && bin(second) <= last) atomicMin(&s.low, key_of(second));
+  }
+  __syncthreads();
+  const uint32_t from = last < kFine ? s.low : 0;
+  const float reaches = last < kFine ? logit_of(from) : -INFINITY;
+  reader.template each<2>([&](float x, int i) {
+    if (x >= reaches && x > -INFINITY) list(x, i, s);
+  });
+  __syncthreads();
+  largest = top;
+  return from;
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_tokens_kernel(const SampleArgs p) {
+__device__ __forceinline__ const unsigned char *row_at(const SampleArgs &p, int r) {
+  return static_cast<const unsigned char *>(p.logits) + (long long)r * p.stride * Elements<T>::kBytes;
+}
+
+// A workgroup a row.
+template <typename T>
+__global__ __launch_bounds__(kThreads, 4) void sample_tokens_kernel(const SampleArgs p) {
   __shared__ Shared s;
-  const int r = blockIdx.x, tid = threadIdx.x, wave = tid >> 6;
-  const Reader<T> reader(static_cast<const unsigned char *>(p.logits) + (long long)r * p.stride * Elements<T>::kBytes, p.vocab);
-  const float temperature = p.temperature ? p.temperature[r] : p.temperature_all;
-  const float top_p = p.top_p ? p.top_p[r] : p.top_p_all, min_p = p.min_p ? p.min_p[r] : p.min_p_all;
-  const int top_k = p.top_k ? p.top_k[r] : p.top_k_all;
+  const int r = blockIdx.x;
+  const unsigned char *const row = row_at<T>(p, r);
+  const RowReader<T> reader(row, p.vocab, 0, RowReader<T>::blocks(row, p.vocab));
+  const Setting setting(p, r);
   const float u = fminf(fmaxf(p.uniform[r], 0.f), 0x1.fffffep-1f);  // (NaN: 0)
-
-  for (int b = tid; b < kBins; b += kThreads) {
-    s.weights[b] = 0;
-    s.counts[b] = 0;
-  }
-  float most = -INFINITY;
-  reader.each([&](float x) { most = fmaxf(most, x); });
-  most = wave_max_all(most);
-  if ((tid & 63) == 0) s.wave_counts[wave] = __float_as_uint(most);
-  __syncthreads();
-  for (int i = 0; i < kWaves; ++i) most = fmaxf(most, __uint_as_float(s.wave_counts[i]));
-  __syncthreads();
-
   int token = -1;
-  float probability = 0.f;
-  if (most == -INFINITY) {  // (nothing may be drawn)
-  } else if (!(temperature > 0.f) || top_k == 1) {
-    token = index_of(reader, key_of(most), 0, s);
-    probability = 1.f;
-  } else {
-    const int unit_bits = min(52, 31 + __builtin_clz(max(p.vocab - 1, 1)) - 1);  // vocab << unit_bits is no more than 2^62
-    Row row;
-    row.most = most;
-    row.per_logit = 1.0 / (double)temperature;
-    row.unit = (double)(1ull << unit_bits);
-    const double all = (unit_bits + 1) * 0.6931471805599453;
-    row.farthest = min_p > 0.f ? fmin(all, -log((double)fminf(min_p, 1.f))) : all;
-    const float to_bin = (float)(kBins / all);
-    reader.each([&](float x) {
-      double z;
-      if (row.candidate(x, z)) {
-        const int b = min((int)((float)z * to_bin), kBins - 1);
-        atomicAdd(&s.counts[b], 1u);
-        atomicAdd(&s.weights[b], row.weight(z));
+  float probability = 0.f, most;
+  if (setting.few()) list_first(reader, (uint32_t)setting.top_k, most, s);
+  else most = largest_of(reader, s);
+  if (most > -INFINITY) {
+    const Weights weights(setting, most);
+    if (!setting.few()) {
+      fill_bins(reader, weights, setting.top_k > 0, s);
+      running_sums(s.bins.weights, s.bins.counts, s);
+      list_ends(reader, setting, weights, u, s);
+    }
+    const bool fits = s.listed <= kList;
+    const ListReader listed = {s.keys, s.indices, (int)s.listed};
+    if (setting.greedy) {
+      token = fits ? index_of(listed, key_of(most), 0, p.vocab, s) : index_of(reader, key_of(most), 0, p.vocab, s);
+      probability = 1.f;
+    } else {
+      if (setting.few()) {
+        if (fits) fill_bins(listed, weights, true, s);
+        else fill_bins(reader, weights, true, s);
+        running_sums(s.bins.weights, s.bins.counts, s);
       }
-    });
-    __syncthreads();
-    running_sums(s.weights, s.counts, s);
-    u64 total = s.weights[kBins - 1];
-    // sums of `amount` and more end at the place's first tokens that reach it
-    const auto upto = [&](const Place &place, u64 amount) {
-      const u64 n = (amount - place.before_weight + place.weight - 1) / place.weight;
-      return place.before_weight + min(n, (u64)place.tokens) * place.weight;
-    };
-    if (top_k > 0 && (uint32_t)top_k < s.counts[kBins - 1]) {
-      const Place place = locate(reader, row, to_bin, true, (u64)top_k, s);
-      total = place.before_weight + (u64)((uint32_t)top_k - place.before_count) * place.weight;
+      if (fits) draw(listed, setting, weights, u, p.vocab, s, token, probability);
+      else draw(reader, setting, weights, u, p.vocab, s, token, probability);
     }
-    if (top_p < 1.f) {
-      const u64 amount = min(max((u64)ceil((double)fmaxf(top_p, 0.f) * (double)total), (u64)1), total);
-      total = upto(locate(reader, row, to_bin, false, amount, s), amount);
-    }
-    const u64 amount = min((u64)((double)u * (double)total) + 1, total);
-    const Place place = locate(reader, row, to_bin, false, amount, s);
-    token = index_of(reader, place.key, (uint32_t)((amount - place.before_weight - 1) / place.weight), s);
-    probability = (float)((double)place.weight / (double)total);
   }
-  if (tid == 0) {
+  if (threadIdx.x == 0) {
     p.tokens[r] = token;
     if (p.probabilities) p.probabilities[r] = probability;
   }
