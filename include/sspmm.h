@@ -655,11 +655,12 @@ int sspmm_prefix_attention(int type, int format, int rows, int queries, int head
  * (or NaN): everything is kept.  NaN logits are taken as -infinity, which is never drawn; infinite ones share the draw.  A row that is all -infinity gives -1.
  * Weights are whole multiples of 2^-b of the largest's, vocab * 2^b <= 2^62, b <= 52: the result does not depend on the order of the sums.
  * temperature, top_k, top_p, min_p: one value a row, or NULL and the value beside it for all.  probabilities (may be NULL): weight over sum, of the token (0 with -1).
- * vocab 1 .. 2^24.
+ * vocab 1 .. 2^24.  workspace: sspmm_sample_tokens_workspace_bytes of the same sizes (0 where a workgroup takes a row), 16-byte aligned.
  */
+size_t sspmm_sample_tokens_workspace_bytes(int rows, int vocab);
 int sspmm_sample_tokens(int type, int rows, int vocab, const void *logits, int64_t row_stride, const float *uniform, const float *temperature, float temperature_all,
                         const int32_t *top_k, int top_k_all, const float *top_p, float top_p_all, const float *min_p, float min_p_all, int32_t *tokens,
-                        float *probabilities, void *hip_stream);
+                        float *probabilities, void *workspace, size_t workspace_bytes, void *hip_stream);
 
 /* ------------------------------------------------------------------------------------------
  * Coordinate list -> CSR, the step between a Matrix Market file and the RowMerge in the

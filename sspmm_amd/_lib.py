@@ -79,7 +79,9 @@ SIGNATURES = {
     "sspmm_prefix_attention_workspace_bytes": (ctypes.c_size_t, [_int] * 5),
     "sspmm_prefix_attention": (_int, [_int] * 5 + [_vp, _i64, _i64, _i64, _vp, _int, _vp, ctypes.c_size_t] + [_int] * 4 +
                                [_vp] * 3 + [ctypes.c_float, _vp, _i64, _i64, _i64, _vp, ctypes.c_size_t, _vp]),
-    "sspmm_sample_tokens": (_int, [_int] * 3 + [_vp, _i64, _vp, _vp, ctypes.c_float, _vp, _int, _vp, ctypes.c_float, _vp, ctypes.c_float] + [_vp] * 3),
+    "sspmm_sample_tokens": (_int, [_int] * 3 + [_vp, _i64, _vp, _vp, ctypes.c_float, _vp, _int, _vp, ctypes.c_float, _vp, ctypes.c_float, _vp, _vp, _vp,
+                                                                                                        ctypes.c_size_t, _vp]),
+    "sspmm_sample_tokens_workspace_bytes": (ctypes.c_size_t, [_int, _int]),
     "sspmm_reserve_pages_workspace_bytes": (ctypes.c_size_t, [_int] * 3),
     "sspmm_fork_pages_workspace_bytes": (ctypes.c_size_t, [_int] * 2),
     "sspmm_compact_pages_workspace_bytes": (ctypes.c_size_t, [_int]),

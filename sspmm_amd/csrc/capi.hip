@@ -984,20 +984,26 @@ int sspmm_prefix_attention(int type, int format, int rows, int queries, int head
   return (int)sspmm::launch_prefix_attention(type, format, a, static_cast<hipStream_t>(hip_stream));
 }
 
+static bool logits_fit(int rows, int vocab) { return rows > 0 && rows < 1 << 22 && vocab > 0 && vocab <= 1 << 24; }  // (a launch has less than 2^32 threads)
+
+size_t sspmm_sample_tokens_workspace_bytes(int rows, int vocab) { return logits_fit(rows, vocab) ? sspmm::sample_workspace_bytes(rows, vocab) : 0; }
+
 int sspmm_sample_tokens(int type, int rows, int vocab, const void *logits, int64_t row_stride, const float *uniform, const float *temperature, float temperature_all,
                         const int32_t *top_k, int top_k_all, const float *top_p, float top_p_all, const float *min_p, float min_p_all, int32_t *tokens,
-                        float *probabilities, void *hip_stream) {
+                        float *probabilities, void *workspace, size_t workspace_bytes, void *hip_stream) {
   if ((type != SSPMM_TYPE_F16 && type != SSPMM_TYPE_BF16 && type != SSPMM_TYPE_F32) || rows < 0 || vocab < 1 || vocab > 1 << 24 || row_stride < 0) return kInvalid;
   if (rows == 0) return 0;
-  if (rows >= 1 << 22) return kInvalid;  // (a launch has less than 2^32 threads)
+  if (!logits_fit(rows, vocab)) return kInvalid;
   if (!logits || reinterpret_cast<uintptr_t>(logits) % (type == SSPMM_TYPE_F32 ? 4 : 2) || !uniform || !tokens) return kInvalid;
   uintptr_t bits = 0;
   for (const void *x : {(const void *)uniform, (const void *)temperature, (const void *)top_k, (const void *)top_p, (const void *)min_p, (const void *)tokens,
                         (const void *)probabilities})
     bits |= reinterpret_cast<uintptr_t>(x);
   if (bits % 4) return kInvalid;
+  const size_t need = sspmm::sample_workspace_bytes(rows, vocab);
+  if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)) return kInvalid;
   const sspmm::SampleArgs a = {logits, row_stride, rows, vocab, uniform, temperature, top_p, min_p, top_k, temperature_all, top_p_all, min_p_all, top_k_all, tokens,
-                               probabilities};
+                               probabilities, static_cast<unsigned char *>(workspace), 0};
   return (int)sspmm::launch_sample_tokens(type, a, static_cast<hipStream_t>(hip_stream));
 }
 

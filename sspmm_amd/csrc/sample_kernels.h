@@ -20,9 +20,12 @@ struct SampleArgs {
   int top_k_all;
   int32_t *tokens;
   float *probabilities;  // may be null
+  unsigned char *workspace;  // sample_workspace_bytes, 8-byte aligned
+  int parts;  // (the launch's own)
 };
+size_t sample_workspace_bytes(int rows, int vocab);
 // type: 0 fp16, 1 bf16, 2 fp32
-hipError_t launch_sample_tokens(int type, const SampleArgs &args, hipStream_t stream);
+hipError_t launch_sample_tokens(int type, SampleArgs args, hipStream_t stream);
 
 }  // namespace sspmm
 #endif

@@ -20,10 +20,10 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kBins = 2048, kFine = 1024;  // of a row or its list, and of a range of logits
-constexpr int kList = 4096;                // logits of a list
-constexpr int kMostTopK = 1200;            // that the threads' two largest each give a bound for
+constexpr int kThreads = 512, kWaves = kThreads / 64;
+constexpr int kBins = 1024, kFine = 512;    // of a row or its list, and of a range of logits
+constexpr int kList = 7168;                // logits of a list
+constexpr int kMostTopK = 1200;            // that the threads' four large ones each give a bound for
 
 struct F32 {};
 
@@ -162,7 +162,7 @@ struct RowReader {
     return ((int)(reinterpret_cast<uintptr_t>(row) & 15) / E::kBytes + vocab + E::kCount - 1) / E::kCount;
   }
   __device__ __forceinline__ float one(int i) const { return E::one(row + (long long)i * E::kBytes); }
-  // f(logit, index) of every element, in any order
+  // f(logit, index, place in its block) of every element, in any order
   template <int UNROLL = 1, typename F>
   __device__ __forceinline__ void each(const F &f) const {
     const unsigned char *const blocks = row - lead * E::kBytes;
@@ -171,12 +171,12 @@ struct RowReader {
       float x[E::kCount];
       E::take(*reinterpret_cast<const uintx4 *>(blocks + (long long)b * 16), x);
 #pragma unroll
-      for (int i = 0; i < E::kCount; ++i) f(x[i], b * E::kCount - lead + i);
+      for (int i = 0; i < E::kCount; ++i) f(x[i], b * E::kCount - lead + i, i);
     }
     // (what lies in front of the whole blocks and behind them, an element a thread)
     const int tid = threadIdx.x, head_end = min(to, first * E::kCount - lead), tail = max(head_end, end * E::kCount - lead);
     const int i = from + tid < head_end ? from + tid : tail + tid - (head_end - from);
-    if (i < head_end || (i >= tail && i < to)) f(one(i), i);
+    if (i < head_end || (i >= tail && i < to)) f(one(i), i, 0);
   }
 };
 
@@ -185,7 +185,7 @@ struct ListReader {
   int count;
   template <int UNROLL = 1, typename F>
   __device__ __forceinline__ void each(const F &f) const {
-    for (int i = threadIdx.x; i < count; i += kThreads) f(logit_of(keys[i]), (int)indices[i]);
+    for (int i = threadIdx.x; i < count; i += kThreads) f(logit_of(keys[i]), (int)indices[i], 0);
   }
 };
 
@@ -281,7 +281,7 @@ __device__ __forceinline__ Place locate(const Reader &reader, const Weights &wei
   u64 inside = s.at_weight;
   uint32_t low = 0xffffffffu, high = 0, count = 0;
   const float from = weights.lowest(bin), to = weights.highest(bin);
-  reader.template each<2>([&](float x, int) {
+  reader.template each<2>([&](float x, int, int) {
     if (x >= from && x <= to) {
       double y;
       if (weights.of(x, y) && weights.bin(y) == bin) {
@@ -299,13 +299,13 @@ __device__ __forceinline__ Place locate(const Reader &reader, const Weights &wei
   low = s.low;
   high = s.high;
   while (low < high) {
-    const int shift = max(0, 22 - (int)__builtin_clz(high - low));  // (high - low) >> shift is below kFine
+    const int shift = max(0, 23 - (int)__builtin_clz(high - low));  // (high - low) >> shift is below kFine
     for (int b = threadIdx.x; b < kFine; b += kThreads) {
       s.bins.fine_weights[b] = 0;
       s.bins.fine_counts[b] = 0;
     }
     __syncthreads();
-    reader.each([&](float x, int) {
+    reader.each([&](float x, int, int) {
       const uint32_t key = key_of(x);
       if (key >= low && key <= high) {
         double y;
@@ -338,10 +338,10 @@ template <typename Reader>
 __device__ __forceinline__ int index_of(const Reader &reader, uint32_t key, uint32_t which, int vocab, Shared &s) {
   uint32_t low = 0, high = (uint32_t)vocab - 1;
   while (low < high) {
-    const int shift = max(0, 22 - (int)__builtin_clz(high - low));
+    const int shift = max(0, 23 - (int)__builtin_clz(high - low));
     s.bins.fine_counts[threadIdx.x] = 0;
     __syncthreads();
-    reader.each([&](float x, int i) {
+    reader.each([&](float x, int i, int) {
       if (key_of(x) == key && (uint32_t)i >= low && (uint32_t)i <= high) atomicAdd(&s.bins.fine_counts[((uint32_t)i - low) >> shift], 1u);
     });
     __syncthreads();
@@ -370,7 +370,7 @@ __device__ __forceinline__ void fill_bins(const Reader &reader, const Weights &w
   }
   __syncthreads();
   if (counted)
-    reader.each([&](float x, int) {
+    reader.each([&](float x, int, int) {
       double y;
       const u64 w = weights.of(x, y);
       if (w) {
@@ -380,7 +380,7 @@ __device__ __forceinline__ void fill_bins(const Reader &reader, const Weights &w
       }
     });
   else
-    reader.each([&](float x, int) {
+    reader.each([&](float x, int, int) {
       double y;
       const u64 w = weights.of(x, y);
       if (w) atomicAdd(&s.bins.weights[weights.bin(y)], w);
@@ -411,7 +411,7 @@ __device__ __forceinline__ void draw(const Reader &reader, const Setting &settin
   probability = (float)((double)place.weight / (double)total);
 }
 
-// Logits from `from` to `to` and their indices onto the list, as far as it has room; s.listed counts all.
+// A logit onto the list, as far as it has room; s.listed counts all.
 __device__ __forceinline__ void list(float x, int i, Shared &s) {
   const uint32_t at = atomicAdd(&s.listed, 1u);
   if (at < kList) {
@@ -420,13 +420,16 @@ __device__ __forceinline__ void list(float x, int i, Shared &s) {
   }
 }
 
-// The logits of the bins in which what draw() asks for may end, as far as the sums in s.bins say, become the list.  Ends with a barrier.
-template <typename T>
-__device__ __forceinline__ void list_ends(const RowReader<T> &reader, const Setting &setting, const Weights &weights, float u, Shared &s) {
+// Ranges of logits.
+struct Ranges {
   float from[3], to[3];
-  int ranges = 0;
+};
+
+// Those of the bins in which what draw() asks for may end, as far as the sums in s.bins say.  Ends with a barrier.
+__device__ __forceinline__ Ranges ends_of(const Setting &setting, const Weights &weights, float u, Shared &s) {
+  Ranges r = {{INFINITY, INFINITY, INFINITY}, {-INFINITY, -INFINITY, -INFINITY}};
   u64 least = s.bins.weights[kBins - 1], most = least;  // that the kept tokens weigh
-  const auto ends = [&](bool by_count, u64 first, u64 last) {  // bins in which sums of first .. last end
+  const auto ends = [&](float &from, float &to, bool by_count, u64 first, u64 last) {  // bins in which sums of first .. last end
     find(s.bins.weights, s.bins.counts, by_count, first, s);
     const int low = s.at;
     least = s.before_weight + 1;
@@ -435,20 +438,22 @@ __device__ __forceinline__ void list_ends(const RowReader<T> &reader, const Sett
     const int high = s.at;
     most = s.before_weight + s.at_weight;
     __syncthreads();
-    from[ranges] = weights.lowest(high);
-    to[ranges] = weights.highest(low);
-    ++ranges;
+    from = weights.lowest(high);
+    to = weights.highest(low);
   };
+  if (setting.top_k > 0 && (uint32_t)setting.top_k < s.bins.counts[kBins - 1]) ends(r.from[0], r.to[0], true, (u64)setting.top_k, (u64)setting.top_k);
+  if (setting.top_p < 1.f) ends(r.from[1], r.to[1], false, top_p_amount(setting.top_p, least), top_p_amount(setting.top_p, most));
+  ends(r.from[2], r.to[2], false, drawn_amount(u, least), drawn_amount(u, most));
+  return r;
+}
+
+// The reader's logits in these ranges become the list.  Ends with a barrier.
+template <typename Reader>
+__device__ __forceinline__ void list_ranges(const Reader &reader, const Ranges &r, Shared &s) {
   if (threadIdx.x == 0) s.listed = 0;
-  if (setting.top_k > 0 && (uint32_t)setting.top_k < s.bins.counts[kBins - 1]) ends(true, (u64)setting.top_k, (u64)setting.top_k);
-  if (setting.top_p < 1.f) ends(false, top_p_amount(setting.top_p, least), top_p_amount(setting.top_p, most));
-  ends(false, drawn_amount(u, least), drawn_amount(u, most));
-  for (int i = ranges; i < 3; ++i) {
-    from[i] = INFINITY;
-    to[i] = -INFINITY;
-  }
-  reader.template each<2>([&](float x, int i) {
-    const bool a = x >= from[0] && x <= to[0], b = x >= from[1] && x <= to[1], c = x >= from[2] && x <= to[2];
+  __syncthreads();
+  reader.template each<4>([&](float x, int i, int) {
+    const bool a = x >= r.from[0] && x <= r.to[0], b = x >= r.from[1] && x <= r.to[1], c = x >= r.from[2] && x <= r.to[2];
     if (a || b || c) list(x, i, s);
   });
   __syncthreads();
@@ -458,7 +463,7 @@ __device__ __forceinline__ void list_ends(const RowReader<T> &reader, const Sett
 template <typename Reader>
 __device__ __forceinline__ float largest_of(const Reader &reader, Shared &s) {
   float most = -INFINITY;
-  reader.template each<4>([&](float x, int) { most = fmaxf(most, x); });
+  reader.template each<4>([&](float x, int, int) { most = fmaxf(most, x); });
   most = wave_max_all(most);
   if ((threadIdx.x & 63) == 0) s.wave_counts[threadIdx.x >> 6] = __float_as_uint(most);
   __syncthreads();
@@ -468,21 +473,25 @@ __device__ __forceinline__ float largest_of(const Reader &reader, Shared &s) {
   return most;
 }
 
-// The first `wanted` of the reader's logits, and others, onto the list: those that a logit reaches which so many of the threads' largest, or two largest, reach.  Its number, or
+// The first `wanted` of the reader's logits, and others, onto the list: those that reach a logit which so many of the threads' largest reach.  Its number, or
 // 0 where the list has all.  Ends with a barrier.
 template <typename T>
 __device__ __forceinline__ uint32_t list_first(const RowReader<T> &reader, uint32_t wanted, float &largest, Shared &s) {
   const int tid = threadIdx.x;
-  const bool two = wanted > kThreads / 4;
-  float first = -INFINITY, second = -INFINITY;
-  if (two)
-    reader.template each<2>([&](float x, int) {
+  constexpr int kPairs = 2;  // (the largest and the one behind it, of the even and of the odd places of all blocks)
+  const bool one = wanted <= kThreads / 4;
+  float large[2 * kPairs];
+#pragma unroll
+  for (float &x : large) x = -INFINITY;
+  if (one)
+    reader.template each<4>([&](float x, int, int) { large[0] = fmaxf(large[0], x); });
+  else
+    reader.template each<2>([&](float x, int, int place) {
       x = x == x ? x : -INFINITY;
+      float &first = large[2 * (place % kPairs)], &second = large[2 * (place % kPairs) + 1];
       second = fmaxf(second, fminf(first, x));
       first = fmaxf(first, x);
     });
-  else
-    reader.template each<4>([&](float x, int) { first = fmaxf(first, x); });
   // ---- bins of equal width from the smallest of these to the largest
   if (tid == 0) {
     s.low = s.high = 0;
@@ -491,7 +500,14 @@ __device__ __forceinline__ uint32_t list_first(const RowReader<T> &reader, uint3
   }
   s.bins.fine_counts[tid] = 0;
   __syncthreads();
-  const float most = wave_max_all(first), least = -wave_max_all(first > -INFINITY ? -first : -INFINITY);
+  float most = -INFINITY, least = INFINITY;  // of the finite ones
+#pragma unroll
+  for (float x : large) {
+    most = fmaxf(most, x);
+    least = x > -INFINITY ? fminf(least, x) : least;
+  }
+  most = wave_max_all(most);
+  least = -wave_max_all(-least);
   if ((tid & 63) == 0) {
     atomicMax(&s.high, key_of(most));
     atomicMax(&s.low, ~key_of(least));
@@ -500,8 +516,9 @@ __device__ __forceinline__ uint32_t list_first(const RowReader<T> &reader, uint3
   const float top = logit_of(s.high), bottom = logit_of(~s.low);
   const float scale = (float)(kFine - 1) / fmaxf(top - bottom, 1e-30f);
   const auto bin = [&](float x) { return (int)fminf(fmaxf((top - x) * scale, 0.f), (float)(kFine - 1)); };
-  if (first > -INFINITY) atomicAdd(&s.bins.fine_counts[bin(first)], 1u);
-  if (second > -INFINITY) atomicAdd(&s.bins.fine_counts[bin(second)], 1u);
+#pragma unroll
+  for (float x : large)
+    if (x > -INFINITY) atomicAdd(&s.bins.fine_counts[bin(x)], 1u);
   __syncthreads();
   uint32_t all;
   const uint32_t own = s.bins.fine_counts[tid], before = sum_before(own, s.wave_counts, all);
@@ -510,13 +527,14 @@ __device__ __forceinline__ uint32_t list_first(const RowReader<T> &reader, uint3
   __syncthreads();
   const int last = s.at;
   if (last < kFine) {
-    if (first > -INFINITY && bin(first) <= last) atomicMin(&s.low, key_of(first));
-    if (second > -INFINITY && bin(second) <= last) atomicMin(&s.low, key_of(second));
+#pragma unroll
+    for (float x : large)
+      if (x > -INFINITY && bin(x) <= last) atomicMin(&s.low, key_of(x));
   }
   __syncthreads();
   const uint32_t from = last < kFine ? s.low : 0;
   const float reaches = last < kFine ? logit_of(from) : -INFINITY;
-  reader.template each<2>([&](float x, int i) {
+  reader.template each<2>([&](float x, int i, int) {
     if (x >= reaches && x > -INFINITY) list(x, i, s);
   });
   __syncthreads();
@@ -529,6 +547,35 @@ __device__ __forceinline__ const unsigned char *row_at(const SampleArgs &p, int 
   return static_cast<const unsigned char *>(p.logits) + (long long)r * p.stride * Elements<T>::kBytes;
 }
 
+__device__ __forceinline__ void result(const SampleArgs &p, int r, int token, float probability) {
+  if (threadIdx.x == 0) {
+    p.tokens[r] = token;
+    if (p.probabilities) p.probabilities[r] = probability;
+  }
+}
+__device__ __forceinline__ float uniform_of(const SampleArgs &p, int r) { return fminf(fmaxf(p.uniform[r], 0.f), 0x1.fffffep-1f); }  // (NaN: 0)
+
+// The row's token, and it is written: from the list in s, of some bins of those in s.bins (binned) or of the row's first logits; or where there were too many for it, from the row itself.
+template <typename T>
+__device__ __forceinline__ void finish(const SampleArgs &p, const Setting &setting, int r, const RowReader<T> &reader, float most, bool binned, bool fits, Shared &s) {
+  const Weights weights(setting, most);
+  const ListReader listed = {s.keys, s.indices, (int)s.listed};
+  int token;
+  float probability = 1.f;
+  if (setting.greedy) {
+    token = fits ? index_of(listed, key_of(most), 0, p.vocab, s) : index_of(reader, key_of(most), 0, p.vocab, s);
+  } else {
+    if (!binned) {
+      if (fits) fill_bins(listed, weights, true, s);
+      else fill_bins(reader, weights, true, s);
+      running_sums(s.bins.weights, s.bins.counts, s);
+    }
+    if (fits) draw(listed, setting, weights, uniform_of(p, r), p.vocab, s, token, probability);
+    else draw(reader, setting, weights, uniform_of(p, r), p.vocab, s, token, probability);
+  }
+  result(p, r, token, probability);
+}
+
 // A workgroup a row.
 template <typename T>
 __global__ __launch_bounds__(kThreads, 4) void sample_tokens_kernel(const SampleArgs p) {
@@ -537,48 +584,224 @@ __global__ __launch_bounds__(kThreads, 4) void sample_tokens_kernel(const Sample
   const unsigned char *const row = row_at<T>(p, r);
   const RowReader<T> reader(row, p.vocab, 0, RowReader<T>::blocks(row, p.vocab));
   const Setting setting(p, r);
-  const float u = fminf(fmaxf(p.uniform[r], 0.f), 0x1.fffffep-1f);  // (NaN: 0)
-  int token = -1;
-  float probability = 0.f, most;
+  float most;
   if (setting.few()) list_first(reader, (uint32_t)setting.top_k, most, s);
   else most = largest_of(reader, s);
-  if (most > -INFINITY) {
-    const Weights weights(setting, most);
-    if (!setting.few()) {
-      fill_bins(reader, weights, setting.top_k > 0, s);
-      running_sums(s.bins.weights, s.bins.counts, s);
-      list_ends(reader, setting, weights, u, s);
-    }
-    const bool fits = s.listed <= kList;
-    const ListReader listed = {s.keys, s.indices, (int)s.listed};
-    if (setting.greedy) {
-      token = fits ? index_of(listed, key_of(most), 0, p.vocab, s) : index_of(reader, key_of(most), 0, p.vocab, s);
-      probability = 1.f;
-    } else {
-      if (setting.few()) {
-        if (fits) fill_bins(listed, weights, true, s);
-        else fill_bins(reader, weights, true, s);
-        running_sums(s.bins.weights, s.bins.counts, s);
-      }
-      if (fits) draw(listed, setting, weights, u, p.vocab, s, token, probability);
-      else draw(reader, setting, weights, u, p.vocab, s, token, probability);
-    }
+  if (most == -INFINITY) {  // (nothing may be drawn)
+    result(p, r, -1, 0.f);
+    return;
   }
-  if (threadIdx.x == 0) {
-    p.tokens[r] = token;
-    if (p.probabilities) p.probabilities[r] = probability;
+  if (!setting.few()) {
+    const Weights weights(setting, most);
+    fill_bins(reader, weights, setting.top_k > 0, s);
+    running_sums(s.bins.weights, s.bins.counts, s);
+    list_ranges(reader, ends_of(setting, weights, uniform_of(p, r), s), s);
+  }
+  finish(p, setting, r, reader, most, !setting.few(), s.listed <= kList, s);
+}
+
+// ---- The same where rows are few: p.parts workgroups a row, four launches.  What they leave for each other:
+constexpr int kMostParts = 8;  // (the third launch's workgroups go over all parts' bins)
+struct Part {
+  float most;
+  uint32_t from;   // its list has the logits whose numbers are this and more
+  uint32_t count;  // of its list, or more than kList
+};
+struct Between {
+  Part *parts;          // [rows, parts]
+  u64 *weights;         // [rows, parts, kBins]
+  uint32_t *counts;     // the same
+  uint32_t *keys, *indices;  // [rows, parts, kList]
+  __host__ __device__ Between(unsigned char *at, long long rows_, int parts_) {
+    weights = reinterpret_cast<u64 *>(at);
+    counts = reinterpret_cast<uint32_t *>(weights + rows_ * parts_ * kBins);
+    keys = counts + rows_ * parts_ * kBins;
+    indices = keys + rows_ * parts_ * kList;
+    parts = reinterpret_cast<Part *>(indices + rows_ * parts_ * kList);
+  }
+  __host__ __device__ size_t bytes(long long rows_, int parts_) const {
+    return reinterpret_cast<unsigned char *>(parts + rows_ * parts_) - reinterpret_cast<unsigned char *>(weights);
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ RowReader<T> part_of(const SampleArgs &p, int r, int part) {
+  const unsigned char *const row = row_at<T>(p, r);
+  const long long blocks = RowReader<T>::blocks(row, p.vocab);
+  return RowReader<T>(row, p.vocab, (int)(blocks * part / p.parts), (int)(blocks * (part + 1) / p.parts));
+}
+template <typename T>
+__device__ __forceinline__ RowReader<T> all_of(const SampleArgs &p, int r) {
+  const unsigned char *const row = row_at<T>(p, r);
+  return RowReader<T>(row, p.vocab, 0, RowReader<T>::blocks(row, p.vocab));
+}
+// (a lane a part)
+__device__ __forceinline__ Part part_here(const SampleArgs &p, const Part *parts) {
+  const int lane = threadIdx.x & 63;
+  return lane < p.parts ? parts[lane] : Part{-INFINITY, 0, 0};
+}
+__device__ __forceinline__ float largest_of_parts(const SampleArgs &p, const Part *parts) { return wave_max_all(part_here(p, parts).most); }
+
+// The list in s to memory.
+__device__ __forceinline__ void leave_list(const Between &b, long long at, const Shared &s) {
+  const int count = min((int)s.listed, kList);
+  for (int i = threadIdx.x; i < count; i += kThreads) {
+    b.keys[at * kList + i] = s.keys[i];
+    b.indices[at * kList + i] = s.indices[i];
+  }
+}
+// The parts' lists as one in s, but for logits that some part's list does not hold; false if some part's, or all together, are too many, or fewer than `wanted`.  Ends with a barrier.
+__device__ __forceinline__ bool take_lists(const SampleArgs &p, const Between &b, int r, uint32_t wanted, Shared &s) {
+  if (threadIdx.x == 0) s.listed = 0;
+  __syncthreads();
+  const Part mine = part_here(p, b.parts + (long long)r * p.parts);
+  const uint32_t from = from_last_lane(wave_inclusive_max(mine.from));
+  bool fits = from_last_lane(wave_inclusive_max(mine.count)) <= (uint32_t)kList;
+  const uint32_t behind = wave_inclusive_sum(min(mine.count, (uint32_t)kList)), all = from_last_lane(behind);
+  const long long first = (long long)r * p.parts * kList;
+#pragma unroll 2
+  for (uint32_t i = threadIdx.x; i < all; i += kThreads) {
+    int part = 0;
+    uint32_t before = 0;
+#pragma unroll
+    for (int j = 0; j < kMostParts - 1; ++j) {
+      const uint32_t end = (uint32_t)__builtin_amdgcn_readlane((int)behind, j);
+      part += i >= end;
+      before = i >= end ? end : before;
+    }
+    const long long at = first + (long long)part * kList + (i - before);
+    const uint32_t key = b.keys[at], index = b.indices[at];
+    if (key >= from) list(logit_of(key), (int)index, s);
+  }
+  __syncthreads();
+  return fits && s.listed <= kList && (from == 0 || s.listed >= wanted);
+}
+
+// The row's sums from its parts' bins.  Ends with a barrier.
+__device__ __forceinline__ void take_bins(const SampleArgs &p, const Between &b, int r, bool counted, Shared &s) {
+  const long long first = (long long)r * p.parts * kBins;
+  for (int i = threadIdx.x; i < kBins; i += kThreads) {
+    u64 weight = 0;
+    uint32_t count = 0;
+#pragma unroll
+    for (int j = 0; j < kMostParts; ++j) {
+      const long long at = first + (long long)min(j, p.parts - 1) * kBins + i;
+      const u64 w = b.weights[at];
+      weight += j < p.parts ? w : 0;
+      if (counted) count += j < p.parts ? b.counts[at] : 0;
+    }
+    s.bins.weights[i] = weight;
+    s.bins.counts[i] = count;
+  }
+  __syncthreads();
+  running_sums(s.bins.weights, s.bins.counts, s);
+}
+
+// First: every part's largest, and where top_k is small a list of its first.
+template <typename T>
+__global__ __launch_bounds__(kThreads, 4) void sample_first_kernel(const SampleArgs p) {
+  __shared__ Shared s;
+  const int part = blockIdx.x, r = blockIdx.y;
+  const Between b(p.workspace, p.rows, p.parts);
+  const RowReader<T> reader = part_of<T>(p, r, part);
+  const Setting setting(p, r);
+  const long long at = (long long)r * p.parts + part;
+  Part mine = {-INFINITY, 0, 0};
+  if (setting.few()) {
+    // (twice a part's share and some, of logits in any order)
+    mine.from = list_first(reader, (uint32_t)min(setting.top_k, 2 * setting.top_k / p.parts + 64), mine.most, s);
+    mine.count = s.listed;
+    leave_list(b, at, s);
+  } else {
+    mine.most = largest_of(reader, s);
+  }
+  if (threadIdx.x == 0) b.parts[at] = mine;
+}
+
+// Second: the draw from these lists, and else every part's bins.
+template <typename T>
+__global__ __launch_bounds__(kThreads, 4) void sample_bins_kernel(const SampleArgs p) {
+  __shared__ Shared s;
+  const int part = blockIdx.x, r = blockIdx.y;
+  const Between b(p.workspace, p.rows, p.parts);
+  const Setting setting(p, r);
+  if (setting.few() && part > 0) return;
+  const Part *const parts = b.parts + (long long)r * p.parts;
+  const float most = largest_of_parts(p, parts);
+  if (most == -INFINITY) {
+    if (part == 0) result(p, r, -1, 0.f);
+    return;
+  }
+  if (setting.few()) {
+    const bool fits = take_lists(p, b, r, (uint32_t)setting.top_k, s);
+    finish(p, setting, r, all_of<T>(p, r), most, false, fits, s);
+    return;
+  }
+  const bool counted = setting.top_k > 0;
+  fill_bins(part_of<T>(p, r, part), Weights(setting, most), counted, s);
+  const long long own = ((long long)r * p.parts + part) * kBins;
+  for (int i = threadIdx.x; i < kBins; i += kThreads) {
+    b.weights[own + i] = s.bins.weights[i];
+    if (counted) b.counts[own + i] = s.bins.counts[i];
   }
 }
 
+// Third: from all parts' bins the ranges of logits that matter, and every part's list of its own in these.
+template <typename T>
+__global__ __launch_bounds__(kThreads, 4) void sample_ends_kernel(const SampleArgs p) {
+  __shared__ Shared s;
+  const int part = blockIdx.x, r = blockIdx.y;
+  const Between b(p.workspace, p.rows, p.parts);
+  const Setting setting(p, r);
+  const long long at = (long long)r * p.parts + part;
+  const float most = largest_of_parts(p, b.parts + (long long)r * p.parts);
+  if (setting.few() || most == -INFINITY) return;
+  take_bins(p, b, r, setting.top_k > 0, s);
+  list_ranges(part_of<T>(p, r, part), ends_of(setting, Weights(setting, most), uniform_of(p, r), s), s);
+  leave_list(b, at, s);
+  if (threadIdx.x == 0) b.parts[at].count = s.listed;
+}
+
+// Fourth: the draw from those.
+template <typename T>
+__global__ __launch_bounds__(kThreads, 4) void sample_draw_kernel(const SampleArgs p) {
+  __shared__ Shared s;
+  const int r = blockIdx.x;
+  const Between b(p.workspace, p.rows, p.parts);
+  const Setting setting(p, r);
+  const float most = largest_of_parts(p, b.parts + (long long)r * p.parts);
+  if (setting.few() || most == -INFINITY) return;
+  take_bins(p, b, r, setting.top_k > 0, s);
+  const bool fits = take_lists(p, b, r, 0, s);
+  finish(p, setting, r, all_of<T>(p, r), most, true, fits, s);
+}
+
+// Rows that are too few for the chip's 512 places for workgroups are taken in parts of 8192 logits or more.
+int parts_of(int rows, int vocab) { return max(1, min(min(kMostParts, 512 / rows), vocab / 8192)); }
+
 template <typename T>
 hipError_t launch(const SampleArgs &a, hipStream_t stream) {
-  hipLaunchKernelGGL((sample_tokens_kernel<T>), dim3(a.rows), dim3(kThreads), 0, stream, a);
+  if (a.parts == 1) {
+    hipLaunchKernelGGL((sample_tokens_kernel<T>), dim3(a.rows), dim3(kThreads), 0, stream, a);
+  } else {
+    const dim3 grid(a.parts, a.rows);
+    hipLaunchKernelGGL((sample_first_kernel<T>), grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((sample_bins_kernel<T>), grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((sample_ends_kernel<T>), grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((sample_draw_kernel<T>), dim3(a.rows), dim3(kThreads), 0, stream, a);
+  }
   return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t launch_sample_tokens(int type, const SampleArgs &args, hipStream_t stream) {
+size_t sample_workspace_bytes(int rows, int vocab) {
+  const int parts = parts_of(rows, vocab);
+  return parts == 1 ? 0 : Between(nullptr, rows, parts).bytes(rows, parts);
+}
+
+hipError_t launch_sample_tokens(int type, SampleArgs args, hipStream_t stream) {
+  args.parts = parts_of(args.rows, args.vocab);
   return type == 0 ? launch<Fp16>(args, stream) : type == 1 ? launch<Bf16>(args, stream) : launch<F32>(args, stream);
 }
 

@@ -445,8 +445,11 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     if rows:
         if logits.stride(1) != 1 and vocab > 1:
             logits = logits.contiguous()
+        size = _workspace_bytes("sspmm_sample_tokens_workspace_bytes", rows, vocab)
+        room = uniform.new_empty(size >> 2) if size else None
         rc = _lib.call(_lib.lib().sspmm_sample_tokens, logits.device, kind, rows, vocab, logits.data_ptr(), logits.stride(0), uniform.data_ptr(), t_at, t_all, k_at, k_all,
-                       p_at, p_all, m_at, m_all, tokens.data_ptr(), chances.data_ptr() if probabilities else None)
+                       p_at, p_all, m_at, m_all, tokens.data_ptr(), chances.data_ptr() if probabilities else None,
+                       None if room is None else room.data_ptr(), size)
         if rc:
             _lib.check(rc, "sspmm_sample_tokens")
     return (tokens, chances) if probabilities else tokens

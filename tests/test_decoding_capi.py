@@ -56,11 +56,14 @@ def test_plan_and_prefix_attention(L):
 
 
 def test_sample_tokens(L):
-    #        type rows vocab logits stride uniform temperature all top_k all top_p all min_p all tokens probabilities stream
-    good = [0, 2, 100, A, 100, A, A, 1.0, A, 0, A, 1.0, A, 0.0, A, A, None]
+    size = L.sspmm_sample_tokens_workspace_bytes
+    need = size(2, 100000)
+    assert need > 0 and size(2, 1000) == 0 and size(1000, 100000) == 0 and size(0, 100000) == 0 and size(2, 0) == 0
+    #        type rows vocab logits stride uniform temperature all top_k all top_p all min_p all tokens probabilities workspace bytes stream
+    good = [0, 2, 100000, A, 100000, A, A, 1.0, A, 0, A, 1.0, A, 0.0, A, A, A, need, None]
     run = _changed(good, L.sspmm_sample_tokens)
     for i, v in ((0, 3), (0, -1), (1, -1), (1, 1 << 22), (2, 0), (2, (1 << 24) + 1), (3, None), (3, A + 1), (4, -1), (5, None), (5, A + 2), (6, A + 1), (8, A + 2), (10, A + 2), (12, A + 2),
-                 (14, None), (14, A + 2), (15, A + 2)):
+                 (14, None), (14, A + 2), (15, A + 2), (16, None), (16, A + 8), (17, need - 1)):
         assert run((i, v)) == 1, (i, v)
     assert run((0, 2), (3, A + 2)) == 1 and run((1, 0), (3, None)) == 0
 
