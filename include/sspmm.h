@@ -624,11 +624,13 @@ int sspmm_compact_pages(int32_t *page_refs, int pages, int32_t *page_table, int 
  * Attention of packed queries over packed states of other lengths, as a decoder's over its encoder's: query i of sequence b (rows offsets[b] ..
  * offsets[b + 1] - 1 of q and out) sees rows source_offsets[b] .. source_offsets[b + 1] - 1 of k and v, all of them.  Both lists as offsets in
  * sspmm_prompt_attention, the second within 0 .. source_tokens; a sequence without states, or whose scores are all -infinity, is zeros.  Strides, limits and out as there.
+ * workspace: sspmm_cross_attention_workspace_bytes of the same sizes, 16-byte aligned (may be 0 bytes).
  */
+size_t sspmm_cross_attention_workspace_bytes(int sequences, int tokens, int source_tokens, int heads, int kv_heads, int head_dim);
 int sspmm_cross_attention(int type, int sequences, int tokens, int source_tokens, int heads, int kv_heads, int head_dim, const int32_t *offsets,
                           const int32_t *source_offsets, const sspmm_half_t *q, int64_t q_row, int64_t q_head, const sspmm_half_t *k, int64_t k_row,
                           int64_t k_head, const sspmm_half_t *v, int64_t v_row, int64_t v_head, float scale, sspmm_half_t *out, int64_t out_row,
-                          int64_t out_head, void *hip_stream);
+                          int64_t out_head, void *workspace, size_t workspace_bytes, void *hip_stream);
 
 /*
  * sspmm_cache_attention for rows that share leading pages, as sspmm_fork_pages leaves them: pages that several rows name in the same slots from the first on are

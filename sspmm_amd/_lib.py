@@ -73,7 +73,8 @@ SIGNATURES = {
     "sspmm_cache_attention_workspace_bytes": (ctypes.c_size_t, [_int] * 7),
     "sspmm_cache_attention": (_int, [_int] * 5 + [_vp, _i64, _i64, _i64, _vp, _int, _vp] + [_int] * 4 + [_vp] * 3 + [ctypes.c_float, _vp, _i64, _i64, _i64,
                                                                                                                _vp, ctypes.c_size_t, _vp]),
-    "sspmm_cross_attention": (_int, [_int] * 7 + [_vp, _vp] + [_vp, _i64, _i64] * 3 + [ctypes.c_float, _vp, _i64, _i64, _vp]),
+    "sspmm_cross_attention": (_int, [_int] * 7 + [_vp, _vp] + [_vp, _i64, _i64] * 3 + [ctypes.c_float, _vp, _i64, _i64, _vp, ctypes.c_size_t, _vp]),
+    "sspmm_cross_attention_workspace_bytes": (ctypes.c_size_t, [_int] * 6),
     "sspmm_prefix_plan_bytes": (ctypes.c_size_t, [_int] * 4),
     "sspmm_plan_prefixes": (_int, [_vp, _int, _int, _vp] + [_int] * 4 + [_vp, ctypes.c_size_t, _vp]),
     "sspmm_prefix_attention_workspace_bytes": (ctypes.c_size_t, [_int] * 5),

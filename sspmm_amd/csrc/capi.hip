@@ -833,10 +833,15 @@ int sspmm_prompt_attention(int type, int sequences, int tokens, int heads, int k
   return (int)sspmm::launch_prompt_attention(type, head_dim, causal != 0, a, static_cast<hipStream_t>(hip_stream));
 }
 
+size_t sspmm_cross_attention_workspace_bytes(int sequences, int tokens, int source_tokens, int heads, int kv_heads, int head_dim) {
+  if (sequences <= 0 || tokens <= 0 || source_tokens < 0 || tokens > (1 << 30) || source_tokens > (1 << 30) || !heads_fit(heads, kv_heads, head_dim)) return 0;
+  return 4 * sspmm::cross_attention_workspace(sequences, tokens, source_tokens, heads, kv_heads, head_dim);
+}
+
 int sspmm_cross_attention(int type, int sequences, int tokens, int source_tokens, int heads, int kv_heads, int head_dim, const int32_t *offsets,
                           const int32_t *source_offsets, const sspmm_half_t *q, int64_t q_row, int64_t q_head, const sspmm_half_t *k, int64_t k_row,
                           int64_t k_head, const sspmm_half_t *v, int64_t v_row, int64_t v_head, float scale, sspmm_half_t *out, int64_t out_row,
-                          int64_t out_head, void *hip_stream) {
+                          int64_t out_head, void *workspace, size_t workspace_bytes, void *hip_stream) {
   if (type != SSPMM_TYPE_F16 && type != SSPMM_TYPE_BF16) return kInvalid;
   if (sequences < 0 || tokens < 0 || source_tokens < 0 || !heads_fit(heads, kv_heads, head_dim) || !scale_fits(scale)) return kInvalid;
   if (sequences == 0 || tokens == 0) return 0;
@@ -864,7 +869,9 @@ int sspmm_cross_attention(int type, int sequences, int tokens, int source_tokens
   a.heads = heads;
   a.kv_heads = kv_heads;
   a.scale_log2e = scale * 1.4426950408889634f;
-  return (int)sspmm::launch_prompt_attention(type, head_dim, false, a, static_cast<hipStream_t>(hip_stream));
+  const size_t need = 4 * sspmm::cross_attention_workspace(sequences, tokens, source_tokens, heads, kv_heads, head_dim);
+  if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)) return kInvalid;
+  return (int)sspmm::launch_cross_attention(type, head_dim, a, static_cast<float *>(workspace), static_cast<hipStream_t>(hip_stream));
 }
 
 int sspmm_cache_write(int type, int format, int sequences, int tokens, const int32_t *offsets, const int32_t *starts,

@@ -23,5 +23,9 @@ struct PromptArgs {
 // d: 32, 64 or 128; type: 0 fp16, 1 bf16; causal only without key_offsets
 hipError_t launch_prompt_attention(int type, int d, bool causal, const PromptArgs &args, hipStream_t stream);
 
+// The attention with key_offsets: by the above, or by workgroups that share out a sequence's keys where it has few queries.
+size_t cross_attention_workspace(int sequences, int tokens, int key_tokens, int heads, int kv_heads, int d);  // floats
+hipError_t launch_cross_attention(int type, int d, const PromptArgs &args, float *workspace, hipStream_t stream);
+
 }  // namespace sspmm
 #endif

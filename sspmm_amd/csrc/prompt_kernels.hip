@@ -45,17 +45,6 @@ __device__ __forceinline__ srd descriptor(const uint16_t *base, uint32_t bytes) 
   return srd{(int)(uint32_t)b, (int)((uint32_t)(b >> 32) & 0xffffu), (int)bytes, (int)kSrdWord3};
 }
 
-// The eight values with zeros in place of infinities and NaN.
-template <typename T>
-__device__ __forceinline__ uintx4 finite_part(uintx4 v) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if ((v[i] & T::kExponent) == T::kExponent) v[i] &= 0xffff0000u;
-    if (((v[i] >> 16) & T::kExponent) == T::kExponent) v[i] &= 0xffffu;
-  }
-  return v;
-}
-
 // A workgroup owns 128 consecutive queries of one sequence and head, 32 a wave, and passes over the keys they see in tiles of 64.
 // Scores are made transposed, K Q^T, so that a lane holds 32 of a tile's 64 scores of ONE query: maxima and sums are taken
 // inside the lane, but for one exchange with the lane 32 apart, and what the matrix instruction leaves is, rounded to 16 bits, the operand P^T

@@ -26,6 +26,9 @@ struct Fp16 {
   static __device__ __forceinline__ floatx16 mfma_32x32x16(uintx4 a, uintx4 b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(vec8, a), __builtin_bit_cast(vec8, b), c, 0, 0, 0);
   }
+  static __device__ __forceinline__ floatx4 mfma_16x16x32(uintx4 a, uintx4 b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vec8, a), __builtin_bit_cast(vec8, b), c, 0, 0, 0);
+  }
 };
 
 struct Bf16 {
@@ -41,7 +44,21 @@ struct Bf16 {
   static __device__ __forceinline__ floatx16 mfma_32x32x16(uintx4 a, uintx4 b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(vec8, a), __builtin_bit_cast(vec8, b), c, 0, 0, 0);
   }
+  static __device__ __forceinline__ floatx4 mfma_16x16x32(uintx4 a, uintx4 b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vec8, a), __builtin_bit_cast(vec8, b), c, 0, 0, 0);
+  }
 };
+
+// The eight values with zeros in place of infinities and NaN.
+template <typename T>
+__device__ __forceinline__ uintx4 finite_part(uintx4 v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if ((v[i] & T::kExponent) == T::kExponent) v[i] &= 0xffff0000u;
+    if (((v[i] >> 16) & T::kExponent) == T::kExponent) v[i] &= 0xffffu;
+  }
+  return v;
+}
 
 }  // namespace sspmm
 #endif

@@ -237,8 +237,11 @@ def cross_attention(q, k, v, offsets, source_offsets, scaling=None, out=None):
     if tokens == 0:
         return out
     (q_at, q_row, q_head, q_), (k_at, k_row, k_head, k_), (v_at, v_row, v_head, v_) = _tokens(q), _tokens(k), _tokens(v)
+    size = _workspace_bytes("sspmm_cross_attention_workspace_bytes", sequences, tokens, source_tokens, heads, kv, d)
+    room = offsets.new_empty(size >> 2) if size else None
     rc = _lib.call(_lib.lib().sspmm_cross_attention, q.device, kind, sequences, tokens, source_tokens, heads, kv, d, offsets.data_ptr(), source_offsets.data_ptr(),
-                   q_at, q_row, q_head, k_at, k_row, k_head, v_at, v_row, v_head, scale, to, out_row, out_head)
+                   q_at, q_row, q_head, k_at, k_row, k_head, v_at, v_row, v_head, scale, to, out_row, out_head,
+                   None if room is None else room.data_ptr(), size)
     if rc:
         _lib.check(rc, "sspmm_cross_attention")
     return out

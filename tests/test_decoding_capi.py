@@ -23,12 +23,15 @@ def _changed(good, call):
 
 
 def test_cross_attention(L):
-    #        type seqs tokens sources heads kv d offsets source_offsets q row head k row head v row head scale out row head stream
-    good = [0, 1, 8, 9, 4, 2, 64, A, A, A, 256, 64, A, 128, 64, A, 128, 64, 0.125, A, 256, 64, None]
+    size = L.sspmm_cross_attention_workspace_bytes
+    need = size(1, 2, 20000, 4, 2, 64)
+    assert need > 0 and size(1, 4000, 20000, 4, 2, 64) == 0 and size(0, 2, 20000, 4, 2, 64) == 0 and size(1, 2, 20000, 4, 3, 64) == 0 and size(1, 2, -1, 4, 2, 64) == 0
+    #        type seqs tokens sources heads kv d offsets source_offsets q row head k row head v row head scale out row head workspace bytes stream
+    good = [0, 1, 2, 20000, 4, 2, 64, A, A, A, 256, 64, A, 128, 64, A, 128, 64, 0.125, A, 256, 64, A, need, None]
     run = _changed(good, L.sspmm_cross_attention)
     for i, v in ((0, 2), (0, -1), (1, -1), (2, -1), (2, (1 << 30) + 1), (3, -1), (3, (1 << 30) + 1), (4, 3), (4, 0), (5, 0), (6, 48), (6, 256), (7, None), (8, None), (9, None),
                  (9, A + 8), (10, 252), (10, 56), (10, 1 << 23), (11, 4), (11, -8), (12, None), (13, 1 << 23), (15, None), (16, 32), (18, 0.0), (18, -1.0),
-                 (18, float("nan")), (18, float("inf")), (18, 3.0e38), (19, None), (19, A + 2), (20, 60), (21, 3)):
+                 (18, float("nan")), (18, float("inf")), (18, 3.0e38), (19, None), (19, A + 2), (20, 60), (21, 3), (22, None), (22, A + 8), (23, need - 1)):
         assert run((i, v)) == 1, (i, v)
     assert run((1, 0), (7, None), (8, None)) == 0 and run((2, 0), (9, None)) == 0
 
