@@ -14,6 +14,7 @@ namespace {
 
 constexpr int kUnit = 32;  // keys of a unit
 constexpr int kWaves = 4;
+constexpr int kMostSplits = 64;
 
 // Pieces of 16 bytes of V's row r lie at place piece ^ swizzle(r): the transpose reads take 32 bytes of each of eight consecutive rows at a time, which then fall on all banks.
 template <int D>
@@ -245,7 +246,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cross_step_kernel(const Prompt
   }
 }
 
-// The shares' states of a tile's rows as one: D / 4 threads a row.
+// The shares' states of a tile's rows as one where they are few: D / 4 threads a row.
 template <typename T, int D, int TILES>
 __global__ __launch_bounds__(256) void cross_join_kernel(const PromptArgs p, int splits, const float *partial) {
   constexpr int kRows = 16 * TILES;
@@ -276,28 +277,74 @@ __global__ __launch_bounds__(256) void cross_join_kernel(const PromptArgs p, int
   }
 }
 
+// Where they are many, a workgroup a row: their weights (a factor to be taken twice) first, a share a lane, then D / 4 threads for the features and 1024 / D sets of them that take
+// every so manyth share.  (16 tokens on 16000 keys, 16 heads on 2, 64 shares: 59 us by the one above, 23 by this; 64 tokens on 1500 keys each, two shares: 86 and 95.)
+template <typename T, int D, int TILES>
+__global__ __launch_bounds__(256) void cross_join_many_kernel(const PromptArgs p, int splits, const float *partial) {
+  constexpr int kRows = 16 * TILES, kSets = 1024 / D;
+  __shared__ float weights[kMostSplits];
+  __shared__ __align__(16) float part[kSets][D];
+  const int group = p.heads / p.kv_heads, r = blockIdx.x % kRows, head = blockIdx.x / kRows % p.kv_heads, number = blockIdx.x / kRows / p.kv_heads;
+  Tile tile;
+  if (!tile_of<kRows>(p, group, number, tile) || tile.row0 + r >= tile.rows) return;
+  const float *const from = partial + ((long long)number * p.kv_heads + head) * splits * state_floats(kRows, D);
+  const int tid = threadIdx.x, lane = tid & 63, set = tid / (D / 4), d = (tid % (D / 4)) * 4;
+  const float *const own = from + (long long)lane * state_floats(kRows, D) + (long long)kRows * D + r;
+  const float max_here = lane < splits ? own[0] : -3.0e38f, sum_here = lane < splits ? own[kRows] : 0.f;
+  const float down = half_way_down((wave_max_all(max_here) - max_here) * p.scale_log2e);
+  const float total = wave_sum_all(sum_here * down * down);
+  if (tid < splits) weights[tid] = down;
+  __syncthreads();
+  floatx4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = set; s < splits; s += kSets) x += *reinterpret_cast<const floatx4 *>(from + s * state_floats(kRows, D) + (long long)r * D + d) * weights[s] * weights[s];
+  *reinterpret_cast<floatx4 *>(&part[set][d]) = x;
+  __syncthreads();
+  if (set != 0) return;
+  for (int i = 1; i < kSets; ++i) x += *reinterpret_cast<const floatx4 *>(&part[i][d]);
+  const float inv = total > 0.f || total != total ? 1.0f / total : 0.f;
+  const int row = tile.row0 + r, i = row / group, h = head * group + row % group;
+  uint16_t *const out = p.out + (long long)(tile.first + i) * p.out_row + (long long)h * p.out_head + d;
+  *reinterpret_cast<uintx2 *>(out) = uintx2{T::pack(x[0] * inv, x[1] * inv), T::pack(x[2] * inv, x[3] * inv)};
+}
+
 // Rows of the tiles (0: the prompts' kernel), how many there may be, and shares of the keys.
+//
+// The prompts' kernel takes 128 queries of a head a workgroup, and goes over a sequence's keys at 18 ns a key with 128 features (11 with 64, 8 with 32), as
+// long as there is one workgroup a CU; this one reads k and v once for 32 rows or 16, at 4.8 TB/s, and some 4 us more where shares are joined.  The shorter estimate is taken,
+// of the mean lengths, which are what the host knows.  us, this kernel and that: 64 sequences of a token on 1500 keys, 32 heads on 8 of 128 features, 78 and 235; 16 of
+// 16 tokens 40 and 64, 8 of 32 33 and 31, 8 of 64 40 and 32; one of 64 on 16000 keys, 16 heads on 2, 36 and 207; two of 100 on 4000, 8 heads of 64, 17 and 40; 8 of 32
+// on 512, 12 heads of 64, 14 and 10; 32 of one 16 and 14.
+// Shares are of 256 keys or more (of 128: four of one token on 8000 keys 46 us instead of 42), as many as fill the 512 places for workgroups, or a few times as many where the last round
+// of them would leave more than a tenth of the places empty.
 struct Shape {
   int row_tiles, splits;
   long long tiles;
 };
-Shape shape_of(int sequences, int tokens, int key_tokens, int heads, int kv_heads) {
+Shape shape_of(int sequences, int tokens, int key_tokens, int heads, int kv_heads, int d) {
   const int group = heads / kv_heads;
-  const long long rows = (long long)tokens * group, mean = (rows + sequences - 1) / sequences, keys = key_tokens / sequences;
-  Shape s = {0, 1, 0};
-  if (mean > 64) return s;
+  const long long rows = (long long)tokens * group, live = min((long long)sequences, (long long)tokens), mean = (rows + live - 1) / live, keys = key_tokens / sequences;
+  Shape s;
   s.row_tiles = mean > 16 ? 2 : 1;
   s.tiles = rows / (16 * s.row_tiles) + sequences;
-  const long long wide = max(1ll, min((long long)sequences, rows)) * ((mean + 16 * s.row_tiles - 1) / (16 * s.row_tiles)) * kv_heads;
-  s.splits = (int)max(1ll, min(min((2048 + wide - 1) / wide, keys / 256), 64ll));
+  const long long wide = live * ((mean + 16 * s.row_tiles - 1) / (16 * s.row_tiles)) * kv_heads;
+  long long splits = (512 + wide - 1) / wide;
+  const long long most = max(splits, 1536 / wide);
+  while (splits < most && 10 * 512 * ((wide * splits + 511) / 512) > 11 * wide * splits) ++splits;
+  s.splits = (int)max(1ll, min(min(splits, keys / 256), (long long)kMostSplits));
+  const double theirs = (double)keys * (d == 128 ? 18e-3 : d == 64 ? 11e-3 : 8e-3) *
+                        max(1.0, (double)live * ((tokens + live * 128 - 1) / (live * 128)) * heads / 256);
+  const double ours = (double)wide * keys * d * 4 / 4.8e6 + (s.splits > 1 ? 4 : 0);
+  if (theirs < ours || s.tiles * kv_heads * max(s.splits, 32) >= 1 << 23) s.row_tiles = 0;  // (a launch has less than 2^32 threads)
   return s;
 }
 
 template <typename T, int D, int TILES>
 hipError_t launch(const PromptArgs &a, const Shape &s, float *workspace, hipStream_t stream) {
-  if (s.tiles * a.kv_heads * s.splits >= 1 << 23) return hipErrorInvalidValue;  // (a launch has less than 2^32 threads)
   hipLaunchKernelGGL((cross_step_kernel<T, D, TILES>), dim3((unsigned)(s.tiles * a.kv_heads * s.splits)), dim3(64 * kWaves), 0, stream, a, s.splits, workspace);
-  if (s.splits > 1)
+  if (s.splits > 8)
+    hipLaunchKernelGGL((cross_join_many_kernel<T, D, TILES>), dim3((unsigned)(s.tiles * a.kv_heads * 16 * TILES)), dim3(256), 0, stream, a, s.splits, workspace);
+  else if (s.splits > 1)
     hipLaunchKernelGGL((cross_join_kernel<T, D, TILES>), dim3((unsigned)(s.tiles * a.kv_heads)), dim3(256), 0, stream, a, s.splits, workspace);
   return hipGetLastError();
 }
@@ -313,12 +360,12 @@ hipError_t launch(int d, const PromptArgs &a, const Shape &s, float *workspace, 
 }  // namespace
 
 size_t cross_attention_workspace(int sequences, int tokens, int key_tokens, int heads, int kv_heads, int d) {
-  const Shape s = shape_of(sequences, tokens, key_tokens, heads, kv_heads);
-  return s.splits <= 1 ? 0 : (size_t)s.tiles * kv_heads * s.splits * (size_t)(16 * s.row_tiles) * (d + 2);
+  const Shape s = shape_of(sequences, tokens, key_tokens, heads, kv_heads, d);
+  return s.row_tiles == 0 || s.splits <= 1 ? 0 : (size_t)s.tiles * kv_heads * s.splits * (size_t)(16 * s.row_tiles) * (d + 2);
 }
 
 hipError_t launch_cross_attention(int type, int d, const PromptArgs &a, float *workspace, hipStream_t stream) {
-  const Shape s = shape_of(a.sequences, a.tokens, a.key_tokens, a.heads, a.kv_heads);
+  const Shape s = shape_of(a.sequences, a.tokens, a.key_tokens, a.heads, a.kv_heads, d);
   if (s.row_tiles == 0) return launch_prompt_attention(type, d, false, a, stream);
   return type == 0 ? launch<Fp16>(d, a, s, workspace, stream) : launch<Bf16>(d, a, s, workspace, stream);
 }

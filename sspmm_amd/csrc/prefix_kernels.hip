@@ -20,6 +20,8 @@ typedef unsigned long long u64;
 constexpr int kUnit = 32;   // keys of a unit, all of them in one page
 constexpr int kRows = 32;   // of a tile
 constexpr int kWaves = 4;   // of a workgroup, which share a tile's units
+constexpr int kMostWorkgroups = 512;    // of all heads of the cache: two a CU
+constexpr int kMostStates = 2 * kMostWorkgroups;  // of a query: each share may leave one of the shared pages and one of the rest
 constexpr int kLeastUnits = 16;  // of a workgroup's share, as far as there are
 
 // ---- the plan: 32-bit words, in this order
@@ -501,40 +503,61 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefix_attention_kernel(const 
   }
 }
 
-// D / 4 threads a query and head: its states of the shared pages, then those of the rest.
+// A workgroup a query and head: its states of the shared pages and of the rest as one.  Their weights (a factor to be taken twice) first, then D / 4 threads for the
+// features and 1024 / D sets of them that take every so manyth state.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void prefix_attention_join_kernel(const PrefixAttentionArgs p) {
-  constexpr int kThreads = D / 4;
+  constexpr int kSets = 1024 / D;
+  __shared__ float weights[kMostStates];
+  __shared__ __align__(16) float part[kSets][D];
+  __shared__ float largest[4], totals[4];
   const PrefixPlan plan(const_cast<int32_t *>(p.plan), p.shape.tiles, p.rows);
   const int kv = p.pool.kv_heads, group = p.heads / kv, row_queries = p.queries * group;
-  const long long n = (long long)blockIdx.x * (256 / kThreads) + threadIdx.x / kThreads;
-  if (n >= (long long)p.rows * p.queries * p.heads) return;
-  const int d = (threadIdx.x % kThreads) * 4;
-  const int h = (int)(n % p.heads), i = (int)(n / p.heads % p.queries), b = (int)(n / p.heads / p.queries);
-  const int head = h / group, r = i * group + h % group;
+  const int h = blockIdx.x % p.heads, i = blockIdx.x / p.heads % p.queries, b = blockIdx.x / p.heads / p.queries;
+  const int head = h / group, r = i * group + h % group, tid = threadIdx.x;
   const RowPlan row = plan.rows[b];
   const int shares = plan.header[1], tiles = plan.header[0];
   const long long units = plan.starts[tiles];
   const float *const values = p.partial + head * p.shape.state_rows * D, *const sums = p.partial + (kv * D + 2 * head) * p.shape.state_rows;
-  float most = -3.0e38f, total = 0.f;
-  floatx4 x = {0.f, 0.f, 0.f, 0.f};
-  for (int part = 0; part < 2; ++part) {
-    const int query = part == 0 ? row.place * row_queries + r : r;
-    if (part == 0 && row.shared_tile < 0) continue;
-    const int tile = (part == 0 ? row.shared_tile : row.own_tile) + query / kRows, place = query % kRows;
-    const long long begin = plan.starts[tile], end = plan.starts[tile + 1];
+  // ---- where they lie: every kRows rows from first[0] on, and from first[1] on
+  long long first[2] = {0, 0};
+  int count[2] = {0, 0};
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int query = j == 0 ? row.place * row_queries + r : r, at = (j == 0 ? row.shared_tile : row.own_tile) + query / kRows;
+    if (j == 0 && row.shared_tile < 0) continue;
+    const long long begin = plan.starts[at], end = plan.starts[at + 1];
     if (begin == end) continue;
-    const int last = share_of(units, shares, end - 1);
-    const Tile what = plan.tiles[tile];
-    for (int share = share_of(units, shares, begin); share <= last; ++share) {
-      const long long at = state_row(what, share) + place;
-      const float theirs = sums[2 * at], sum = sums[2 * at + 1], new_most = fmaxf(most, theirs);
-      const float down = half_way_down(new_most - most), their_down = half_way_down(new_most - theirs);
-      total = total * down * down + sum * their_down * their_down;
-      x = x * down * down + *reinterpret_cast<const floatx4 *>(values + at * D + d) * their_down * their_down;
-      most = new_most;
-    }
+    const int from = share_of(units, shares, begin);
+    first[j] = state_row(plan.tiles[at], from) + query % kRows;
+    count[j] = share_of(units, shares, end - 1) - from + 1;
   }
+  const int states = count[0] + count[1];
+  const auto place = [&](int s) { return s < count[0] ? first[0] + (long long)s * kRows : first[1] + (long long)(s - count[0]) * kRows; };
+  float most = -3.0e38f;
+  for (int s = tid; s < states; s += 256) most = fmaxf(most, sums[2 * place(s)]);
+  most = wave_max_all(most);
+  if ((tid & 63) == 0) largest[tid >> 6] = most;
+  __syncthreads();
+  most = fmaxf(fmaxf(largest[0], largest[1]), fmaxf(largest[2], largest[3]));
+  float total = 0.f;
+  for (int s = tid; s < states; s += 256) {
+    const float down = half_way_down(most - sums[2 * place(s)]);
+    weights[s] = down;
+    total += sums[2 * place(s) + 1] * down * down;
+  }
+  total = wave_sum_all(total);
+  if ((tid & 63) == 0) totals[tid >> 6] = total;
+  __syncthreads();
+  total = (totals[0] + totals[1]) + (totals[2] + totals[3]);
+  const int set = tid / (D / 4), d = (tid % (D / 4)) * 4;
+  floatx4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = set; s < states; s += kSets) x += *reinterpret_cast<const floatx4 *>(values + place(s) * D + d) * weights[s] * weights[s];
+  *reinterpret_cast<floatx4 *>(&part[set][d]) = x;
+  __syncthreads();
+  if (set != 0) return;
+  for (int j = 1; j < min(kSets, states); ++j) x += *reinterpret_cast<const floatx4 *>(&part[j][d]);
   const float inv = total > 0.f || total != total ? 1.0f / kValueUnit / total : 0.f;
   uint16_t *const to = p.out + (long long)b * p.out_seq + (long long)i * p.out_row + (long long)h * p.out_head + d;
   *reinterpret_cast<uintx2 *>(to) = uintx2{T::pack(x[0] * inv, x[1] * inv), T::pack(x[2] * inv, x[3] * inv)};
@@ -543,8 +566,7 @@ __global__ __launch_bounds__(256) void prefix_attention_join_kernel(const Prefix
 template <typename T, int FORMAT, int D>
 hipError_t launch(const PrefixAttentionArgs &a, hipStream_t stream) {
   hipLaunchKernelGGL((prefix_attention_kernel<T, FORMAT, D>), dim3(a.pool.kv_heads, a.shape.workgroups), dim3(64 * kWaves), 0, stream, a);
-  const long long n = (long long)a.rows * a.queries * a.heads, each = 256 / (D / 4);
-  hipLaunchKernelGGL((prefix_attention_join_kernel<T, D>), dim3((unsigned)((n + each - 1) / each)), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((prefix_attention_join_kernel<T, D>), dim3((unsigned)(a.rows * a.queries * a.heads)), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 template <typename T, int FORMAT>
@@ -559,7 +581,7 @@ PrefixShape prefix_shape(int rows, int queries, int heads, int kv_heads) {
   s.row_queries = queries * (heads / kv_heads);
   // own tiles; shared ones, full but for one in a group of two rows or more
   s.tiles = (long long)rows * ((s.row_queries + kRows - 1) / kRows) + (long long)rows * s.row_queries / kRows + rows / 2;
-  s.workgroups = max(1, 512 / kv_heads);
+  s.workgroups = max(1, kMostWorkgroups / kv_heads);
   s.state_rows = 2ll * rows * s.row_queries + (long long)s.workgroups * kRows;
   return s;
 }
