@@ -10,10 +10,10 @@ constexpr int kMostPlanRows = 1024;
 
 // What the sizes alone say of a plan and of the workspace of the attention that follows it.
 struct PrefixShape {
-  long long tiles;       // no plan has more
-  long long state_rows;  // of the states that the workgroups of a head of the cache leave
-  int workgroups;        // for each head of the cache
-  int row_queries;       // queries x heads of a group, of a row
+  long long tiles, jobs;  // no plan has more
+  long long state_rows;   // of the states that the jobs leave, for each head of the cache
+  int target;             // jobs, about, of many units
+  int row_queries;        // queries x heads of a group, of a row
 };
 PrefixShape prefix_shape(int rows, int queries, int heads, int kv_heads);
 size_t prefix_plan_ints(const PrefixShape &shape, int rows);

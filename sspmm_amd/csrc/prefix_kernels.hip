@@ -2,9 +2,8 @@
 //   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^((q . k_j) scale log2(e) - m),  k_j and v_j codes times their block's scale.
 // A plan says which rows share what.  Rows with the same first page are compared with the lowest of them; of these the rows that share S pages or more are a
 // group, with the S that saves most, S times the rows but one.  The queries of a group's rows lie one behind the other in tiles of 32 (queries x heads of one head of the cache) over
-// the shared pages, and every row's in tiles of their own over the rest.  All tiles, one behind the other, are as many units of keys, which the workgroups of a head of
-// the cache share evenly: a workgroup goes from tile to tile where its share does, and leaves a state (maximum, sum, weighted values) for each.  A second
-// launch makes one of the states of a row's queries.
+// the shared pages, and every row's in tiles of their own over the rest. A tile's keys are cut into jobs of about one size, a workgroup each for every head of the cache, which leaves
+// a state (maximum, sum, weighted values); a second launch makes one of the states of a row's queries.
 #include "prefix_kernels.h"
 
 #include "cache_codes.h"
@@ -17,56 +16,59 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kUnit = 32;   // keys of a unit, all of them in one page
 constexpr int kRows = 32;   // of a tile
-constexpr int kWaves = 4;   // of a workgroup, which share a tile's units
-constexpr int kMostWorkgroups = 512;    // of all heads of the cache: two a CU
-constexpr int kMostStates = 2 * kMostWorkgroups;  // of a query: each share may leave one of the shared pages and one of the rest
-constexpr int kLeastUnits = 16;  // of a workgroup's share, as far as there are
+constexpr int kWaves = 4;   // of a workgroup, which share a job's units
+constexpr int kPlaces = 512;     // for workgroups, two a CU
+constexpr int kJobKeys = 1280;   // that a workgroup goes over in the time that it takes to begin and to end
+constexpr int kLeastKeys = 256;  // of a job, as far as there are
+constexpr int kMostStates = 2 * (kPlaces + 1);  // of a query
 
 // ---- the plan: 32-bit words, in this order
-//   header   tiles, workgroups that have a share (0: there are no units)
-//   starts   tiles + 1 numbers of 64 bits: units in front of a tile
-//   tiles    kTileWords each
-//   rows     kRowWords each
-//   order    the rows, group after group
+//   header  jobs, 0, 0, 0
+//   jobs    those of the shared pages first, of all tiles of a group the same keys side by side; then the rows' own, the longest rows first
+//   rows    by their number
+//   order   the rows, group after group, and their lengths
 //   leaders, shared pages (of the first launch)
-constexpr int kHeaderWords = 4, kTileWords = 8, kRowWords = 4;
-struct Tile {
-  int row;       // of the table
-  int member;    // place in the order of the first row whose queries it holds
-  int first;     // its first query among theirs
-  int count;     // queries
-  int unit;      // its first unit, of the row
-  int end;       // positions of the row from here on are not the tile's
-  int all_seen;  // every query sees the keys below
-  int states;    // queries of the tiles in front
+constexpr int kHeaderWords = 4;
+struct Job {
+  int row;           // of the table
+  int unit0, unit1;  // of the row
+  int end;           // positions of the row from here on are not the job's
+  int all_seen;      // every query sees the keys below
+  int member;        // place in the order of the row whose queries come first in the tile's group
+  int first, count;  // its first query among theirs, and queries
+  int states;        // the first row of its state
+  int unused[3];
 };
-static_assert(sizeof(Tile) == 4 * kTileWords, "");
 struct RowPlan {
-  int shared_tile;  // the group's first tile, or -1
-  int place;        // in the group
-  int own_tile;
-  int length;       // tokens, also those that the table has no slot for
+  // A tile's jobs leave as many rows as it has queries, one job's behind the other's, and one tile's behind the other's.
+  int shared_states, shared_jobs;  // of the first tile of the group: its jobs' first row; jobs of a tile, 0: there is no group
+  int shared_queries, place;       // of the group; the row's place in it
+  int own_states, own_jobs;
+  int unused[2];
 };
-static_assert(sizeof(RowPlan) == 4 * kRowWords, "");
+struct Ordered {
+  int row, length;  // tokens, also those that the table has no slot for
+};
 struct PrefixPlan {
   int32_t *header;
-  long long *starts;
-  Tile *tiles;
+  Job *jobs;
   RowPlan *rows;
-  int32_t *order, *leaders, *shared;
-  __host__ __device__ PrefixPlan(int32_t *at, long long most_tiles, int n) {
+  Ordered *order;
+  int32_t *leaders, *shared;
+  __host__ __device__ PrefixPlan(int32_t *at, const PrefixShape &s, int n) {
     header = at;
-    starts = reinterpret_cast<long long *>(at + kHeaderWords);
-    tiles = reinterpret_cast<Tile *>(starts + ((most_tiles + 2) & ~1ll));
-    rows = reinterpret_cast<RowPlan *>(tiles + most_tiles);
-    order = reinterpret_cast<int32_t *>(rows + n);
-    leaders = order + n;
+    jobs = reinterpret_cast<Job *>(at + kHeaderWords);
+    rows = reinterpret_cast<RowPlan *>(jobs + s.jobs);
+    order = reinterpret_cast<Ordered *>(rows + n);
+    leaders = reinterpret_cast<int32_t *>(order + n);
     shared = leaders + n;
   }
   __host__ __device__ long long words(int n) const { return shared + n - header; }
 };
+
+// Keys of a unit, all of them in one page.
+__host__ __device__ constexpr int unit_of(int page_size) { return page_size == 32 ? 32 : 64; }
 
 // Pages that lie whole in front of the row's first query.
 __device__ __forceinline__ int full_pages(int length, int queries, int page_size, int slots) {
@@ -88,12 +90,22 @@ __global__ __launch_bounds__(64) void plan_prefixes_compare_kernel(PrefixPlan pl
     }
     const int32_t *const other = table + (long long)leader * slots;
     const int most = min(full, full_pages(lengths[leader], queries, page_size, slots));
-    for (shared = 0; shared < most; shared += 64) {
-      const int s = shared + lane;
-      const u64 differ = __ballot(!(s < most && own[s] >= 0 && own[s] == other[s]));
-      if (differ) {
-        shared += __builtin_ctzll(differ);
-        break;
+    constexpr int kAtOnce = 8;
+    bool more = true;
+    for (shared = 0; more && shared < most;) {
+      bool same[kAtOnce];
+      const int from = shared;
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int s = from + 64 * i + lane, at = min(s, most - 1);
+        const int mine = own[at];
+        same[i] = s < most && mine >= 0 && mine == other[at];
+      }
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const u64 differ = __ballot(!same[i]);
+        if (more) shared += differ ? __builtin_ctzll(differ) : 64;
+        more = more && differ == 0;
       }
     }
     shared = min(shared, most);
@@ -106,35 +118,35 @@ __global__ __launch_bounds__(64) void plan_prefixes_compare_kernel(PrefixPlan pl
 
 // Sum of v over the threads in front of the own one, and over all.
 __device__ __forceinline__ u64 sum_before(u64 v, u64 (&waves)[kMostPlanRows / 64], u64 &all) {
-  const int wave = threadIdx.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const u64 upto = wave_inclusive_sum(v);
   __syncthreads();
-  if ((threadIdx.x & 63) == 63) waves[wave] = upto;
+  if (lane == 63) waves[wave] = upto;
   __syncthreads();
-  u64 before = upto - v;
-  all = 0;
-  for (int i = 0; i < kMostPlanRows / 64; ++i) {
-    before += i < wave ? waves[i] : 0;
-    all += waves[i];
-  }
-  return before;
+  const u64 sums = wave_inclusive_sum(lane < (int)(blockDim.x >> 6) ? waves[lane] : 0);
+  const auto of = [&](int i) { return (u64)(uint32_t)__builtin_amdgcn_readlane((int)sums, i) | (u64)(uint32_t)__builtin_amdgcn_readlane((int)(sums >> 32), i) << 32; };
+  all = of(63);
+  return upto - v + (wave ? of(wave - 1) : 0);
 }
 
-// One workgroup, a thread a row.
+// One workgroup, a thread a row (and more threads than that).
 __global__ __launch_bounds__(kMostPlanRows) void plan_prefixes_kernel(PrefixPlan plan, int rows, int slots, const int32_t *lengths, int page_size, int queries, PrefixShape shape) {
-  __shared__ int leaders[kMostPlanRows], shared[kMostPlanRows], base[kMostPlanRows], group_tile[kMostPlanRows];
+  __shared__ int2 found[kMostPlanRows];  // leader, shared pages
+  __shared__ int base[kMostPlanRows];
+  __shared__ int in_orders[kMostPlanRows], lengths_of[kMostPlanRows], group_queries[kMostPlanRows];
+  __shared__ int by_rank[kMostPlanRows], shared_job[kMostPlanRows], own_job[kMostPlanRows], shared_states[kMostPlanRows], own_states[kMostPlanRows];
   __shared__ u64 best[kMostPlanRows], waves[kMostPlanRows / 64];
   const int r = threadIdx.x;
   const bool there = r < rows;
   const int leader = there ? plan.leaders[r] : -1, mine = there ? plan.shared[r] : 0;
-  leaders[r] = leader;
-  shared[r] = mine;
+  found[r] = {leader, mine};
   best[r] = 0;
   __syncthreads();
   // ---- the pages that a group shares: of its rows' numbers the one that saves most
   if (leader >= 0) {
     int as_many = 0;
-    for (int i = 0; i < rows; ++i) as_many += leaders[i] == leader && shared[i] >= mine;
+#pragma unroll 8
+    for (int i = 0; i < rows; ++i) as_many += (found[i].x == leader) & (found[i].y >= mine);
     const u64 saved = (u64)mine * (u64)(as_many - 1);
     if (saved) atomicMax(&best[leader], saved << 26 | (u64)mine);  // (fewer than 2^26 slots)
   }
@@ -144,63 +156,95 @@ __global__ __launch_bounds__(kMostPlanRows) void plan_prefixes_kernel(PrefixPlan
   const bool member = own_pages > 0, leads = member && leader == r;
   // ---- order: a group's rows stand where its leader would
   __syncthreads();
-  shared[r] = own_pages;
+  found[r].y = own_pages;
   __syncthreads();
   int place = 0, members = 0;
   if (member)
+#pragma unroll 8
     for (int i = 0; i < rows; ++i) {
-      const bool one = leaders[i] == leader && shared[i] > 0;
+      const int one = (found[i].x == leader) & (found[i].y > 0);
       members += one;
-      place += one && i < r;
+      place += one & (i < r);
     }
   u64 all;
   const u64 at = sum_before(there ? (leads ? members : member ? 0 : 1) : 0, waves, all);
   base[r] = (int)at;
   __syncthreads();
   const int in_order = member ? base[leader] + place : (int)at;
-  if (there) plan.order[in_order] = r;
-  // ---- tiles: the group's at its leader, and every row's own
   const int length = there ? max(0, lengths[r]) : 0, end = (int)min((long long)length, (long long)slots * page_size);
-  const int from = own_pages * page_size;
-  const long long stacked = leads ? (long long)members * shape.row_queries : 0;
-  const int group_tiles = (int)((stacked + kRows - 1) / kRows), own_tiles = there ? (shape.row_queries + kRows - 1) / kRows : 0;
-  const int group_units = from / kUnit, own_units = (end - from + kUnit - 1) / kUnit;
-  const int tile = (int)sum_before((u64)(group_tiles + own_tiles), waves, all);
-  const int tiles = (int)all;
-  u64 units;
-  long long start = (long long)sum_before((u64)group_tiles * group_units + (u64)own_tiles * own_units, waves, units);
-  int states = (int)sum_before(there ? (u64)(stacked + shape.row_queries) : 0, waves, all);
-  group_tile[r] = tile;
+  if (there) plan.order[in_order] = {r, length};
+  // ---- jobs: the groups' tiles in the order of their leaders, then every row's own
+  const int from = own_pages * page_size, unit = unit_of(page_size);
+  const int stacked = leads ? members * shape.row_queries : 0;  // queries of the group
+  const int group_tiles = (stacked + kRows - 1) / kRows, own_tiles = there ? (shape.row_queries + kRows - 1) / kRows : 0;
+  const int group_units = from / unit, own_units = (end - from + unit - 1) / unit;
+  u64 units, all_tiles, shared_jobs, jobs, states;
+  sum_before((u64)group_tiles * group_units + (u64)own_tiles * own_units, waves, units);
+  sum_before((u64)(group_units ? group_tiles : 0) + (u64)(own_units ? own_tiles : 0), waves, all_tiles);
+  // Units of a job, at most: as few as leave no more jobs than there are places, so that all run at once, found by halving; or, with too many tiles for that, so many that
+  // the last jobs' time and what beginning and ending take of all together are least.
+  const int least = kLeastKeys / unit;
+  int size = max(least, (int)sqrtf((float)units * (float)(kJobKeys / unit) / (float)shape.target));
+  if (4 * all_tiles <= 3 * (u64)shape.target) {
+    // (jobs of n units in all tiles are fewer than n / size + tiles)
+    u64 low = max((u64)least, (units + shape.target - 1) / shape.target), high = max(low, (units + shape.target - all_tiles - 1) / (shape.target - all_tiles));
+    while (low < high) {
+      const u64 step = (high - low + 3) / 4;
+      u64 mine = 0, counts;
+      for (int i = 0; i < 3; ++i) {  // three sizes at a time; a thread's jobs matter up to the places
+        const u64 at = low + i * step, jobs = (u64)group_tiles * ((group_units + at - 1) / at) + (u64)own_tiles * ((own_units + at - 1) / at);
+        mine |= min(jobs, (u64)2 * kPlaces) << 21 * i;
+      }
+      sum_before(mine, waves, counts);
+      int few = 0;  // sizes that are too small
+      for (int i = 0; i < 3; ++i) few += (counts >> 21 * i & ((1u << 21) - 1)) > (u64)shape.target;
+      if (few < 3) high = min(high, low + few * step);
+      if (few > 0) low = min(high, low + (few - 1) * step + 1);
+    }
+    size = (int)high;
+  }
+  const int group_cuts = (group_units + size - 1) / size, own_cuts = (own_units + size - 1) / size;  // jobs of a tile
+  shared_job[r] = (int)sum_before((u64)group_tiles * group_cuts, waves, shared_jobs);
+  lengths_of[r] = there ? own_units : -1;
   __syncthreads();
-  if (there) {
-    for (int i = 0; i < group_tiles; ++i, start += group_units) {
-      plan.starts[tile + i] = start;
-      const int count = (int)min((long long)kRows, stacked - (long long)i * kRows);
-      plan.tiles[tile + i] = {r, in_order, i * kRows, count, 0, from, INT_MAX, states};
-      states += count;
-    }
-    const int own = tile + group_tiles;
-    for (int i = 0; i < own_tiles; ++i, start += own_units) {
-      plan.starts[own + i] = start;
-      const int count = min(kRows, shape.row_queries - i * kRows);
-      plan.tiles[own + i] = {r, in_order, i * kRows, count, from / kUnit, end, length - queries + 1, states};
-      states += count;
-    }
-    plan.rows[r] = {member ? group_tile[leader] : -1, place, own, length};
+  int rank = there ? 0 : r;
+  if (there)
+#pragma unroll 8
+    for (int i = 0; i < rows; ++i) rank += (lengths_of[i] > own_units) | ((lengths_of[i] == own_units) & (i < r));
+  by_rank[rank] = r;
+  __syncthreads();
+  // (own_job and by_rank are of the r'th longest row)
+  const int ranked_units = there ? lengths_of[by_rank[r]] : 0, ranked_cuts = (ranked_units + size - 1) / size;
+  own_job[r] = (int)(shared_jobs + sum_before((u64)own_tiles * ranked_cuts, waves, jobs));
+  // (rows of states are below 2^25)
+  const u64 states_before = sum_before((u64)stacked * group_cuts | (there ? (u64)shape.row_queries * own_cuts : 0) << 32, waves, states);
+  shared_states[r] = (int)(uint32_t)states_before;
+  own_states[r] = (int)(uint32_t)states + (int)(states_before >> 32);
+  group_queries[r] = stacked;
+  in_orders[r] = in_order;
+  lengths_of[r] = length;
+  __syncthreads();
+  if (there) plan.rows[r] = {member ? shared_states[leader] : 0, member ? group_cuts : 0, member ? group_queries[leader] : 0, place, own_states[r], own_cuts, {0, 0}};
+  const int all_jobs = (int)(shared_jobs + jobs);
+  for (int j = r; j < all_jobs; j += blockDim.x) {
+    const bool of_group = j < (int)shared_jobs;
+    const int *const first_job = of_group ? shared_job : own_job;
+    int at = 0;  // the last whose first job is not behind j
+    for (int step = kMostPlanRows / 2; step > 0; step /= 2)
+      if (at + step < rows && first_job[at + step] <= j) at += step;
+    const int row = of_group ? at : by_rank[at], which = j - first_job[at];
+    const int start = found[row].y * page_size, stop = (int)min((long long)lengths_of[row], (long long)slots * page_size);
+    const int row_units = of_group ? start / unit : (stop - start + unit - 1) / unit, cuts = (row_units + size - 1) / size;
+    const int tiles = ((of_group ? group_queries[row] : shape.row_queries) + kRows - 1) / kRows;
+    const int tile = which % tiles, cut = which / tiles, first = tile * kRows;
+    const int count = min(kRows, (of_group ? group_queries[row] : shape.row_queries) - first);
+    const int unit0 = of_group ? 0 : start / unit;
+    plan.jobs[j] = {row, unit0 + (int)((long long)row_units * cut / cuts), unit0 + (int)((long long)row_units * (cut + 1) / cuts), of_group ? start : stop,
+                    of_group ? INT_MAX : lengths_of[row] - queries + 1, in_orders[row], first, count,
+                    (of_group ? shared_states[row] : own_states[row]) + first * cuts + cut * count, {0, 0, 0}};
   }
-  if (r == 0) {
-    plan.starts[tiles] = (long long)units;
-    plan.header[0] = tiles;
-    plan.header[1] = (int)min((u64)shape.workgroups, (units + kLeastUnits - 1) / kLeastUnits);
-  }
+  if (r == 0) plan.header[0] = all_jobs;
 }
-
-// Share i of the units begins at floor(i units / shares), for as many shares as units at most.
-__device__ __forceinline__ long long share_start(long long units, int shares, int i) { return units * i / shares; }
-__device__ __forceinline__ int share_of(long long units, int shares, long long unit) { return (int)(((unit + 1) * shares - 1) / units); }
-// The rows where a share leaves its state of a tile: D values each, and behind all of these a maximum and a sum each.  From one state to the next either
-// the tile is another, and the tiles' queries are counted on, or the share is: no two overlap.
-__device__ __forceinline__ long long state_row(const Tile &tile, int share) { return (long long)tile.states + (long long)share * kRows; }
 
 template <typename T, int FORMAT, int D, int TILES, int UNIT>
 struct CacheRows {
@@ -217,8 +261,8 @@ struct CacheRows {
   floatx4 o[TILES][kParts];  // features 16 part + 4 g + i of row m
   float run_max[TILES], run_sum[TILES];
 
-  // Row m of tile t: its features at `at`.  bf16 goes to fp16 by way of a power of two for the row, which leaves its largest magnitude in 2^14 .. 2^15
-  __device__ __forceinline__ void load_query(int t, const uint16_t *at, int sees, float scale_log2e) {
+  // Row m of tile t: its features at `at`.
+  __device__ __forceinline__ void load_query(int t, const uint16_t *at, int sees) {
     const int g = (threadIdx.x & 63) >> 4;
     seen[t] = sees;
 #pragma unroll
@@ -226,6 +270,9 @@ struct CacheRows {
       const int d = D >= 64 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 8 * g;
       q[t][s] = *reinterpret_cast<const uintx4 *>(at + d);
     }
+  }
+  // bf16 goes to fp16 by way of a power of two for the row, which leaves its largest magnitude in 2^14 .. 2^15
+  __device__ __forceinline__ void convert_query(int t, float scale_log2e) {
     c[t] = scale_log2e;
     if constexpr (!__is_same(T, Fp16)) {
       float most = 0.f;
@@ -246,7 +293,10 @@ struct CacheRows {
   }
 
   // Units unit0 .. unit1 - 1 of the sequence whose pages `table` lists, `length` positions of which are something.  all_seen: every row sees the keys below.
-  __device__ __forceinline__ void attend(const CachePool &pool, const int32_t *table, int head, int unit0, int unit1, int all_seen, int length) {
+  // query(): asks for the queries, once the first unit's page has been asked for.
+  template <typename Query>
+  __device__ __forceinline__ void attend(const CachePool &pool, const int32_t *table, int head, int unit0, int unit1, int all_seen, int length, float scale_log2e,
+                                         const Query &query) {
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
@@ -265,9 +315,8 @@ struct CacheRows {
     // Pages and scales of 64 units at a time, one a lane, so that no unit waits for them.
     int pages_of = 0;
     float k_scales = 0.f, v_scales = 0.f;
-    const auto look_up = [&](int u) {
-      const int mine = min(u + lane, unit1 - 1);
-      pages_of = table[mine >> page_bits];
+    const auto ask_pages = [&](int u) { pages_of = table[min(u + lane, unit1 - 1) >> page_bits]; };
+    const auto ask_scales = [&]() {
       const float *const scale = pool.scales + (long long)(usable(pages_of) ? pages_of : 0) * 2 * pool.kv_heads + head;
       k_scales = scale[0];
       v_scales = scale[pool.kv_heads] * kValueUnit;
@@ -293,18 +342,25 @@ struct CacheRows {
     };
 
     int page = 0;
+    if (unit0 < unit1) ask_pages(unit0);
+    query();
     if (unit0 < unit1) {
-      look_up(unit0);
       page = __builtin_amdgcn_readlane(pages_of, 0);
       load_k(unit0, page);
+      ask_scales();
       load_v(unit0, page);
     }
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) convert_query(t, scale_log2e);
     for (int u = unit0; u < unit1; ++u) {
       const bool more = u + 1 < unit1, there = usable(page);
       const int at = (u - unit0) & 63;
       const float k_scale = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(k_scales), at));
       const float v_scale = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v_scales), at));
-      if (at == 63 && more) look_up(u + 1);
+      if (at == 63 && more) {
+        ask_pages(u + 1);
+        ask_scales();
+      }
       const int page_next = __builtin_amdgcn_readlane(pages_of, (at + 1) & 63);
       floatx4 s[TILES][kKeyTiles];
 #pragma unroll
@@ -445,29 +501,34 @@ struct CacheRows {
   }
 };
 
-// A tile's units unit0 .. unit1 - 1 by the workgroup, and its state of them.
-template <typename T, int FORMAT, int D, int TILES>
-__device__ __forceinline__ void attend_tile(const PrefixAttentionArgs &p, const PrefixPlan &plan, const Tile &tile, int head, int unit0, int unit1, float *values, float *sums_to, float *lds) {
+// A job by the workgroup.
+template <typename T, int FORMAT, int D, int TILES, int UNIT>
+__device__ __forceinline__ void work_on(const PrefixAttentionArgs &p, const PrefixPlan &plan, const Job &job, int head, float *lds) {
   typedef float States[kWaves][2][16 * TILES];
   typedef float Sums[kWaves][16 * TILES][D];
   States &state = *reinterpret_cast<States *>(lds + sizeof(Sums) / 4);
   Sums &sums = *reinterpret_cast<Sums *>(lds);
   const int m = threadIdx.x & 15, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int group = p.heads / p.pool.kv_heads, row_queries = p.queries * group;
-  CacheRows<T, FORMAT, D, TILES, kUnit> w;
+  CacheRows<T, FORMAT, D, TILES, UNIT> w;
+  const auto query = [&]() __attribute__((always_inline)) {
 #pragma unroll
-  for (int t = 0; t < TILES; ++t) {
-    // (places behind the last query take that one's: its maxima move no reference point that it does not move itself)
-    const int at = tile.first + min(16 * t + m, tile.count - 1), row = plan.order[tile.member + at / row_queries], r = at % row_queries, i = r / group;
-    w.load_query(t, p.q + (long long)row * p.q_seq + (long long)i * p.q_row + (long long)(head * group + r % group) * p.q_head, plan.rows[row].length - p.queries + 1 + i,
-                 p.scale_log2e);
-  }
-  const int units = unit1 - unit0;
-  w.attend(p.pool, p.pool.table + (long long)tile.row * p.pool.slots, head, unit0 + units * wave / kWaves, unit0 + units * (wave + 1) / kWaves, tile.all_seen, tile.end);
+    for (int t = 0; t < TILES; ++t) {
+      // (places behind the last query take that one's: its maxima move no reference point that it does not move itself)
+      const int at = job.first + min(16 * t + m, job.count - 1), r = at % row_queries, i = r / group;
+      const Ordered row = plan.order[job.member + at / row_queries];
+      w.load_query(t, p.q + (long long)row.row * p.q_seq + (long long)i * p.q_row + (long long)(head * group + r % group) * p.q_head, row.length - p.queries + 1 + i);
+    }
+  };
+  const int units = job.unit1 - job.unit0;
+  w.attend(p.pool, p.pool.table + (long long)job.row * p.pool.slots, head, job.unit0 + units * wave / kWaves, job.unit0 + units * (wave + 1) / kWaves, job.all_seen, job.end,
+           p.scale_log2e, query);
   w.template join<kWaves>(wave, state, sums);
+  const long long row = head * p.shape.state_rows + job.states;
+  float *const values = p.partial + row * D, *const sums_to = p.partial + p.pool.kv_heads * p.shape.state_rows * D + 2 * row;
   for (int at = threadIdx.x; at < 16 * TILES * D / 4; at += 64 * kWaves) {
     const int r = at / (D / 4), d = (at % (D / 4)) * 4;
-    if (r >= tile.count) continue;
+    if (r >= job.count) break;
     float most, total;
     const floatx4 x = w.joined(state, sums, r, d, most, total);
     *reinterpret_cast<floatx4 *>(values + r * D + d) = x;
@@ -476,31 +537,24 @@ __device__ __forceinline__ void attend_tile(const PrefixAttentionArgs &p, const 
       sums_to[2 * r + 1] = total;
     }
   }
-  __syncthreads();
 }
 
-template <typename T, int FORMAT, int D>
+template <typename T, int FORMAT, int D, int UNIT>
 __global__ __launch_bounds__(64 * kWaves, 2) void prefix_attention_kernel(const PrefixAttentionArgs p) {
   __shared__ __align__(16) float lds[kWaves * kRows * (D + 2)];
-  const PrefixPlan plan(const_cast<int32_t *>(p.plan), p.shape.tiles, p.rows);
-  const int head = blockIdx.x, share = blockIdx.y, shares = plan.header[1], tiles = plan.header[0];
-  if (share >= shares) return;
-  const long long units = plan.starts[tiles];
-  long long at = share_start(units, shares, share);
-  const long long end = share_start(units, shares, share + 1);
-  // (the last tile that begins here or before; those without units are passed over)
-  int i = last_not_above(tiles, 0, [&](int t) { return plan.starts[t] > at ? 1 : 0; });
-  for (; at < end; ++i) {
-    const long long begin = plan.starts[i], behind = min(plan.starts[i + 1], end);
-    if (behind <= at) continue;
-    const Tile tile = plan.tiles[i];
-    const int unit0 = tile.unit + (int)(at - begin), unit1 = tile.unit + (int)(behind - begin);
-    const long long row = head * p.shape.state_rows + state_row(tile, share);
-    float *const values = p.partial + row * D, *const sums = p.partial + p.pool.kv_heads * p.shape.state_rows * D + 2 * row;
-    if (tile.count > 16) attend_tile<T, FORMAT, D, 2>(p, plan, tile, head, unit0, unit1, values, sums, lds);
-    else attend_tile<T, FORMAT, D, 1>(p, plan, tile, head, unit0, unit1, values, sums, lds);
-    at = behind;
+  const PrefixPlan plan(const_cast<int32_t *>(p.plan), p.shape, p.rows);
+  const int kv = p.pool.kv_heads, jobs = plan.header[0];
+  int number = blockIdx.x / kv, head = blockIdx.x % kv;
+  if (kv < 8 && 8 % kv == 0) {
+    // Workgroup ids go round-robin to the 8 XCDs: a head's jobs go to 8 / kv of them, one after the other, so that tiles that read the same keys do so through one L2.
+    const int parts = 8 / kv, each = (jobs + parts - 1) / parts, xcd = blockIdx.x & 7;
+    head = xcd % kv;
+    number = (int)(blockIdx.x >> 3) < each ? xcd / kv * each + (int)(blockIdx.x >> 3) : jobs;
   }
+  if (number >= jobs) return;
+  const Job job = plan.jobs[number];
+  if (job.count > 16) work_on<T, FORMAT, D, 2, UNIT>(p, plan, job, head, lds);
+  else work_on<T, FORMAT, D, 1, UNIT>(p, plan, job, head, lds);
 }
 
 // A workgroup a query and head: its states of the shared pages and of the rest as one.  Their weights (a factor to be taken twice) first, then D / 4 threads for the
@@ -508,32 +562,22 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefix_attention_kernel(const 
 template <typename T, int D>
 __global__ __launch_bounds__(256) void prefix_attention_join_kernel(const PrefixAttentionArgs p) {
   constexpr int kSets = 1024 / D;
-  __shared__ float weights[kMostStates];
+  __shared__ float weights[kMostStates];  // (jobs of two tiles)
   __shared__ __align__(16) float part[kSets][D];
   __shared__ float largest[4], totals[4];
-  const PrefixPlan plan(const_cast<int32_t *>(p.plan), p.shape.tiles, p.rows);
+  const PrefixPlan plan(const_cast<int32_t *>(p.plan), p.shape, p.rows);
   const int kv = p.pool.kv_heads, group = p.heads / kv, row_queries = p.queries * group;
   const int h = blockIdx.x % p.heads, i = blockIdx.x / p.heads % p.queries, b = blockIdx.x / p.heads / p.queries;
   const int head = h / group, r = i * group + h % group, tid = threadIdx.x;
   const RowPlan row = plan.rows[b];
-  const int shares = plan.header[1], tiles = plan.header[0];
-  const long long units = plan.starts[tiles];
   const float *const values = p.partial + head * p.shape.state_rows * D, *const sums = p.partial + (kv * D + 2 * head) * p.shape.state_rows;
-  // ---- where they lie: every kRows rows from first[0] on, and from first[1] on
-  long long first[2] = {0, 0};
-  int count[2] = {0, 0};
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int query = j == 0 ? row.place * row_queries + r : r, at = (j == 0 ? row.shared_tile : row.own_tile) + query / kRows;
-    if (j == 0 && row.shared_tile < 0) continue;
-    const long long begin = plan.starts[at], end = plan.starts[at + 1];
-    if (begin == end) continue;
-    const int from = share_of(units, shares, begin);
-    first[j] = state_row(plan.tiles[at], from) + query % kRows;
-    count[j] = share_of(units, shares, end - 1) - from + 1;
-  }
-  const int states = count[0] + count[1];
-  const auto place = [&](int s) { return s < count[0] ? first[0] + (long long)s * kRows : first[1] + (long long)(s - count[0]) * kRows; };
+  // ---- where they lie
+  const int shared_query = row.place * row_queries + r, shared_first = shared_query / kRows * kRows, own_first = r / kRows * kRows;
+  const int shared_step = min(kRows, row.shared_queries - shared_first), own_step = min(kRows, row_queries - own_first);
+  const long long shared_at = (long long)row.shared_states + shared_first * row.shared_jobs + shared_query % kRows;
+  const long long own_at = (long long)row.own_states + own_first * row.own_jobs + r % kRows;
+  const int states = row.shared_jobs + row.own_jobs;
+  const auto place = [&](int s) { return s < row.shared_jobs ? shared_at + (long long)s * shared_step : own_at + (long long)(s - row.shared_jobs) * own_step; };
   float most = -3.0e38f;
   for (int s = tid; s < states; s += 256) most = fmaxf(most, sums[2 * place(s)]);
   most = wave_max_all(most);
@@ -565,7 +609,9 @@ __global__ __launch_bounds__(256) void prefix_attention_join_kernel(const Prefix
 
 template <typename T, int FORMAT, int D>
 hipError_t launch(const PrefixAttentionArgs &a, hipStream_t stream) {
-  hipLaunchKernelGGL((prefix_attention_kernel<T, FORMAT, D>), dim3(a.pool.kv_heads, a.shape.workgroups), dim3(64 * kWaves), 0, stream, a);
+  const dim3 grid((unsigned)((a.shape.jobs * a.pool.kv_heads + 7) / 8 * 8 + 8));  // (each XCD may have one more)
+  if (unit_of(a.pool.page_size) == 32) hipLaunchKernelGGL((prefix_attention_kernel<T, FORMAT, D, 32>), grid, dim3(64 * kWaves), 0, stream, a);
+  else hipLaunchKernelGGL((prefix_attention_kernel<T, FORMAT, D, 64>), grid, dim3(64 * kWaves), 0, stream, a);
   hipLaunchKernelGGL((prefix_attention_join_kernel<T, D>), dim3((unsigned)(a.rows * a.queries * a.heads)), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
@@ -581,20 +627,22 @@ PrefixShape prefix_shape(int rows, int queries, int heads, int kv_heads) {
   s.row_queries = queries * (heads / kv_heads);
   // own tiles; shared ones, full but for one in a group of two rows or more
   s.tiles = (long long)rows * ((s.row_queries + kRows - 1) / kRows) + (long long)rows * s.row_queries / kRows + rows / 2;
-  s.workgroups = max(1, kMostWorkgroups / kv_heads);
-  s.state_rows = 2ll * rows * s.row_queries + (long long)s.workgroups * kRows;
+  s.target = max(1, kPlaces / kv_heads);
+  s.jobs = s.tiles + s.target;  // (a tile of n units has fewer than n / size + 1)
+  // a job's queries, 32 at most, are a tile's, and all tiles' no more than twice the rows'
+  s.state_rows = 2ll * rows * s.row_queries + (long long)s.target * kRows;
   return s;
 }
-size_t prefix_plan_ints(const PrefixShape &shape, int rows) { return (size_t)PrefixPlan(nullptr, shape.tiles, rows).words(rows); }
+size_t prefix_plan_ints(const PrefixShape &shape, int rows) { return (size_t)PrefixPlan(nullptr, shape, rows).words(rows); }
 size_t prefix_attention_floats(const PrefixShape &shape, int kv_heads, int d) {
   return (size_t)kv_heads * (size_t)shape.state_rows * (d + 2);
 }
 
 hipError_t launch_plan_prefixes(const PrefixShape &shape, const int32_t *table, int rows, int slots, const int32_t *lengths, int page_size, int queries, int32_t *plan,
                                 hipStream_t stream) {
-  const PrefixPlan at(plan, shape.tiles, rows);
+  const PrefixPlan at(plan, shape, rows);
   hipLaunchKernelGGL(plan_prefixes_compare_kernel, dim3(rows), dim3(64), 0, stream, at, table, rows, slots, lengths, page_size, queries);
-  hipLaunchKernelGGL(plan_prefixes_kernel, dim3(1), dim3(kMostPlanRows), 0, stream, at, rows, slots, lengths, page_size, queries, shape);
+  hipLaunchKernelGGL(plan_prefixes_kernel, dim3(1), dim3(max(256, (rows + 63) / 64 * 64)), 0, stream, at, rows, slots, lengths, page_size, queries, shape);
   return hipGetLastError();
 }
 

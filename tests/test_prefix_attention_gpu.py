@@ -57,10 +57,10 @@ def _tables(groups, page, seed=0):
 
 
 def _units(plan):
-    """Units of all tiles, which is what the workgroups of a head of the cache go over."""
+    """Units of all jobs, which is what the workgroups of a head of the cache go over."""
     words = plan.data
-    tiles = int(words[0])
-    return int(words[4:].view(torch.int64)[tiles])
+    jobs = words[4:4 + 12 * int(words[0])].view(-1, 12)
+    return int((jobs[:, 2] - jobs[:, 1]).sum())
 
 
 def _run(groups, n, heads, kv, page, d, dtype, form, seed=0):
