@@ -321,34 +321,26 @@ struct CacheRows {
       k_scales = scale[0];
       v_scales = scale[pool.kv_heads] * kValueUnit;
     };
-    const auto load_k = [&](int u, int pg) {
-      const unsigned char *const at = pool.keys + ((long long)(usable(pg) ? pg : 0) * pool.kv_heads + head) * block + place_of(u) * D;
+    // A page's keys and values at unit u; a tile of 16 keys, or 16 features, of them.
+    const auto keys_at = [&](int u, int pg) { return pool.keys + ((long long)(usable(pg) ? pg : 0) * pool.kv_heads + head) * block + place_of(u) * D; };
+    const auto values_at = [&](int u, int pg) { return pool.values + ((long long)(usable(pg) ? pg : 0) * pool.kv_heads + head) * block + place_of(u) + UNIT / 4 * g; };
+    const auto load_k = [&](const unsigned char *at, int kt) {
+      const unsigned char *const row = at + (UNIT / 4 * (m >> 2) + 4 * kt + (m & 3)) * D + 4 * kKeyWords * g;
 #pragma unroll
-      for (int kt = 0; kt < kKeyTiles; ++kt) {
-        const unsigned char *const row = at + (UNIT / 4 * (m >> 2) + 4 * kt + (m & 3)) * D + 4 * kKeyWords * g;
-#pragma unroll
-        for (int i = 0; i < kKeyLoads; ++i) {
-          kk[kt][i] = *reinterpret_cast<const KeyWords *>(row + 64 * i);
-        }
-      }
+      for (int i = 0; i < kKeyLoads; ++i) kk[kt][i] = *reinterpret_cast<const KeyWords *>(row + 64 * i);
     };
-    const auto load_v = [&](int u, int pg) {
-      const unsigned char *const at = pool.values + ((long long)(usable(pg) ? pg : 0) * pool.kv_heads + head) * block + place_of(u) + UNIT / 4 * g;
-#pragma unroll
-      for (int part = 0; part < kParts; ++part) {
-        const unsigned char *const row = at + (16 * part + m) * pool.page_size;
-        vv[part] = *reinterpret_cast<const ValueWords *>(row);
-      }
-    };
+    const auto load_v = [&](const unsigned char *at, int part) { vv[part] = *reinterpret_cast<const ValueWords *>(at + (16 * part + m) * pool.page_size); };
 
     int page = 0;
     if (unit0 < unit1) ask_pages(unit0);
     query();
     if (unit0 < unit1) {
       page = __builtin_amdgcn_readlane(pages_of, 0);
-      load_k(unit0, page);
+#pragma unroll
+      for (int kt = 0; kt < kKeyTiles; ++kt) load_k(keys_at(unit0, page), kt);
       ask_scales();
-      load_v(unit0, page);
+#pragma unroll
+      for (int part = 0; part < kParts; ++part) load_v(values_at(unit0, page), part);
     }
 #pragma unroll
     for (int t = 0; t < TILES; ++t) convert_query(t, scale_log2e);
@@ -362,6 +354,8 @@ struct CacheRows {
         ask_scales();
       }
       const int page_next = __builtin_amdgcn_readlane(pages_of, (at + 1) & 63);
+      // (the next unit's loads follow upon the last use of a register; behind the last unit, its own once more)
+      const unsigned char *const keys_next = keys_at(more ? u + 1 : u, more ? page_next : page), *const values_next = values_at(more ? u + 1 : u, more ? page_next : page);
       floatx4 s[TILES][kKeyTiles];
 #pragma unroll
       for (int kt = 0; kt < kKeyTiles; ++kt) {
@@ -374,8 +368,8 @@ struct CacheRows {
 #pragma unroll
           for (int t = 0; t < TILES; ++t) s[t][kt] = mfma(k, q[t][step], s[t][kt]);
         }
+        load_k(keys_next, kt);
       }
-      if (more) load_k(u + 1, page_next);
       const int key0 = u * UNIT, key = key0 + UNIT / 4 * g;
       const bool cut = !there || key0 + UNIT > all_seen;  // uniform: some row does not see some key
       float v_scale_of[TILES];
@@ -452,8 +446,8 @@ struct CacheRows {
         for (int t = 0; t < TILES; ++t)
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[t][part][i] = fmaf(sum[t][i], v_scale_of[t], o[t][part][i]);
+        load_v(values_next, part);
       }
-      if (more) load_v(u + 1, page_next);
       page = page_next;
     }
   }
