@@ -2,8 +2,9 @@
 // w_i >= min_p, of these the top_k first in the order of falling logits (equal ones in the order of their indices), of these the shortest run whose weights
 // reach top_p of all of theirs.  The token is the first in that order at which the running sum of the weights exceeds u times their sum.
 //
-// Weights are whole numbers, in units of 2^-unit_bits of the largest: sums of them are exact in any order, so that atomics and lanes give the same token every
-// time.  Vocabularies of 2^17 leave 45 bits; what weighs less than half a unit is never drawn.
+// Weights are 2^-(n / 16) times whole numbers, n the nearest to 16 z log2(e): the whole numbers, in units of 2^-unit_bits, are summed for each n, in bins, and a bin's sum is
+// brought to units of the largest's weight as a whole. Sums of whole numbers are exact in any order, so that atomics and lanes give the same token every time.
+// Vocabularies of 2^17 leave 45 bits.
 //
 // No row is sorted.  With a top_k of some hundred, the largest logit of every thread's share gives a logit that enough others reach; those that reach it become a list
 // in LDS, and the draw is the list's.  Else the row is put into bins by z, which is to say by weight; where a sum ends is then known up to a bin, and the logits of the few
@@ -21,8 +22,8 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr int kThreads = 512, kWaves = kThreads / 64;
-constexpr int kBins = 1024, kFine = 512;    // of a row or its list, and of a range of logits
-constexpr int kList = 7168;                // logits of a list
+constexpr int kBins = 1024, kFine = 512;  // of a row or its list (the last one for what weighs nothing), and of a range of logits
+constexpr int kList = 6144;               // logits of a list
 constexpr int kMostTopK = 1200;            // that the threads' four large ones each give a bound for
 
 struct F32 {};
@@ -76,57 +77,58 @@ struct Setting {
 };
 
 struct Weights {
-  double most, per_logit, farthest;  // the largest logit; log2(e) / T; largest y = z log2(e) of a token that is kept
-  int unit_bits;
-  float to_bin;
-  bool infinite;
+  double most, per_logit, farthest;  // the largest logit; 16 log2(e) / T; largest 16 z log2(e) of a token that is kept
+  double unit;                       // 2^unit_bits
+  bool infinite, everything;
   __device__ __forceinline__ Weights(const Setting &s, float largest) {
     most = (double)largest;
-    per_logit = 1.4426950408889634 / (double)s.temperature;
-    unit_bits = s.unit_bits;
-    farthest = s.min_p > 0.f ? -log2((double)fminf(s.min_p, 1.f)) : 1100.0;
-    to_bin = (float)kBins / (float)(unit_bits + 1);
+    per_logit = 16.0 * 1.4426950408889634 / (double)s.temperature;
+    unit = (double)(1ull << s.unit_bits);
+    everything = !(s.min_p > 0.f);
+    farthest = everything ? (double)(kBins - 1) : -16.0 * log2((double)fminf(s.min_p, 1.f));
     infinite = largest == INFINITY;
   }
-  // (monotone in x, so that bins and ranges of logits never cross; -infinity and NaN are 1100, whose weight is nothing)
-  __device__ __forceinline__ double distance(float x) const { return fmin((most - (double)x) * per_logit, 1100.0); }
-  // 2^-y in units: y = n - f, 2^f = 1 + f g(f), g a polynomial through its Chebyshev points in -1/2 .. 1/2, off by 2^-44.  Adding 2^52 leaves the whole number
-  // in the lower bits.  (Some twenty instructions, at the rate of those in 32 bits.)
-  __device__ __forceinline__ u64 units(double y) const {
-    const double n = rint(y), f = n - y;
-    double g = 0x1.b638808b9c3c7p-24;
-    g = fma(g, f, 0x1.63d136362c015p-20);
-    g = fma(g, f, 0x1.ffcb9515bca86p-17);
-    g = fma(g, f, 0x1.4308ac85aafa8p-13);
-    g = fma(g, f, 0x1.5d87fe86fe84ep-10);
-    g = fma(g, f, 0x1.3b2ab7181b74fp-7);
-    g = fma(g, f, 0x1.c6b08d7047e52p-5);
-    g = fma(g, f, 0x1.ebfbdff823cedp-3);
-    g = fma(g, f, 0x1.62e42fefa39efp-1);
-    const double w = ldexp(fma(g, f, 1.0), unit_bits - (int)n) + 0x1p52;
-    return (u64)__double_as_longlong(w) - 0x4330000000000000ull;
+  // 16 z log2(e).  (Monotone in x, so that bins and ranges of logits never cross; -infinity, NaN and what is farther than 2^-63 go to the last bin.)
+  __device__ __forceinline__ double distance(float x) const {
+    const double y = fmin((most - (double)x) * per_logit, (double)(kBins - 1));
+    return everything || y <= farthest ? y : (double)(kBins - 1);
   }
-  // of any logit; y for its bin
-  __device__ __forceinline__ u64 of(float x, double &y) const {
-    y = (double)x == most ? 0.0 : infinite ? 1100.0 : distance(x);
-    return y <= farthest ? units(y) : 0;
+  // Its bin, and in it 2^(n - y) / 16) in units: with f = n - y, 1 + f g(f), g a polynomial through its Chebyshev points in -1/2 .. 1/2, off by 2^-46.  Adding 2^52 leaves the
+  // whole number in the lower bits.
+  __device__ __forceinline__ int units(double y, u64 &w) const {
+    const double shifted = y + 0x1.8p52, n = shifted - 0x1.8p52, f = n - y;
+    double g = 0x1.5d893e591a8aap-30 * unit;
+    g = fma(g, f, 0x1.3b2c4ac7da6fep-23 * unit);
+    g = fma(g, f, 0x1.c6b08d6faa1acp-17 * unit);
+    g = fma(g, f, 0x1.ebfbdff6988c8p-11 * unit);
+    g = fma(g, f, 0x1.62e42fefa39efp-5 * unit);
+    w = (u64)__double_as_longlong(fma(g, f, unit + 0x1p52)) - 0x4330000000000000ull;
+    return (int)(uint32_t)__double_as_longlong(shifted);
   }
-  __device__ __forceinline__ int bin(double y) const { return min((int)((float)y * to_bin), kBins - 1); }
+  // The same of any logit (where the largest is infinite, it alone weighs something).
+  __device__ __forceinline__ int of(float x, u64 &w) const {
+    const double y = distance(x);
+    return units(infinite ? ((double)x == most ? 0.0 : (double)(kBins - 1)) : y, w);
+  }
+  // A bin's units as units of the largest's weight.
+  __device__ __forceinline__ double share(int bin) const { return exp2(-(double)bin / 16.0); }
+  __device__ __forceinline__ u64 whole(int bin, u64 inside) const { return (u64)rint((double)inside * share(bin)); }
   // A logit that no logit of bin b and those before it is below (or, from the side of 0, above), whatever was rounded on the way.
   __device__ __forceinline__ float lowest(int b) const {
-    if (b >= kBins - 1 || infinite) return -INFINITY;
-    const double x = most - (double)(b + 1) / (double)to_bin * 1.000001 / per_logit;
+    if (infinite) return -INFINITY;
+    const double x = most - ((double)b + 0.5) * 1.000001 / per_logit;
     return (float)(x - (fabs(x) * 0x1p-22 + 1e-44));
   }
   __device__ __forceinline__ float highest(int b) const {
     if (b == 0 || infinite) return INFINITY;
-    const double x = most - (double)b / (double)to_bin * 0.999999 / per_logit;
+    const double x = most - ((double)b - 0.5) * 0.999999 / per_logit;
     return (float)(x + (fabs(x) * 0x1p-22 + 1e-44));
   }
 };
 
 struct Bins {
-  u64 weights[kBins];
+  u64 inside[kBins];   // units of the bin
+  u64 weights[kBins];  // units of the largest, of this bin and those before
   uint32_t counts[kBins];
   u64 fine_weights[kFine];
   uint32_t fine_counts[kFine];
@@ -208,16 +210,16 @@ __device__ __forceinline__ V sum_before(V v, V (&waves)[kWaves], V &all) {
   return before;
 }
 
-// Counts and weights of the bins become sums of those up to and with each.  Ends with a barrier.
+// Sums of weights and counts up to and with each bin, of given weights and the counts that stand there.  Ends with a barrier.
 template <int BINS>
-__device__ __forceinline__ void running_sums(u64 (&weights)[BINS], uint32_t (&counts)[BINS], Shared &s) {
+__device__ __forceinline__ void running_sums(const u64 (&given)[BINS / kThreads], u64 (&weights)[BINS], uint32_t (&counts)[BINS], Shared &s) {
   constexpr int kOwn = BINS / kThreads;
   const int tid = threadIdx.x, wave = tid >> 6;
   u64 w[kOwn], w_sum = 0;
   uint32_t c[kOwn], c_sum = 0;
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) {
-    w[i] = w_sum += weights[tid * kOwn + i];
+    w[i] = w_sum += given[i];
     c[i] = c_sum += counts[tid * kOwn + i];
   }
   u64 w_before = wave_inclusive_sum(w_sum);
@@ -241,6 +243,16 @@ __device__ __forceinline__ void running_sums(u64 (&weights)[BINS], uint32_t (&co
   }
   __syncthreads();
 }
+// Of a row's bins.
+__device__ __forceinline__ void sum_bins(const Weights &weights, Shared &s) {
+  u64 whole[kBins / kThreads];
+#pragma unroll
+  for (int i = 0; i < kBins / kThreads; ++i) {
+    const int b = threadIdx.x * (kBins / kThreads) + i;
+    whole[i] = weights.whole(b, s.bins.inside[b]);
+  }
+  running_sums(whole, s.bins.weights, s.bins.counts, s);
+}
 
 // The first bin up to whose end there are `amount` tokens, or as much weight: into s.at, with what lies before it and in it.  Ends with a barrier.
 template <int BINS>
@@ -259,32 +271,46 @@ __device__ __forceinline__ void find(const u64 (&weights)[BINS], const uint32_t 
   __syncthreads();
 }
 
-// A place in the order: the logit, what lies before its first token, its tokens and the weight of each.
+// A place in the order: the logit, its bin, what lies before its first token (tokens; units before the bin, and units of the bin), its tokens, and units of the bin of each.
 struct Place {
   uint32_t key, before_count, tokens;
-  u64 before_weight, weight;
+  int bin;
+  u64 before_bin, before_inside, weight;
 };
+// A place after so many of its tokens: weight of all up to there, and units of its bin.
+struct End {
+  int bin;
+  u64 total, inside;
+};
+__device__ __forceinline__ End end_at(const Weights &weights, const Place &place, u64 tokens) {
+  const u64 inside = place.before_inside + tokens * place.weight;
+  return {place.bin, place.before_bin + weights.whole(place.bin, inside), inside};
+}
 
-// The logit at which the running count, or the running sum of the weights, reaches `amount` (at least one, and no more than there is).
+// The logit at which the running count, or the running sum of the weights, reaches `amount` (at least one, and no more than there is), and how much that is in units of its bin, which
+// are at least one, and no more than there are: in the bin, or in what is kept of it.
 template <typename Reader>
-__device__ __forceinline__ Place locate(const Reader &reader, const Weights &weights, bool by_count, u64 amount, Shared &s) {
+__device__ __forceinline__ Place locate(const Reader &reader, const Weights &weights, bool by_count, u64 amount, const End &kept, u64 &inside, Shared &s) {
   __syncthreads();
   if (threadIdx.x == 0) {
     s.low = 0xffffffffu;
     s.high = 0;
   }
   find(s.bins.weights, s.bins.counts, by_count, amount, s);
-  const int bin = s.at;
   Place place;
+  place.bin = s.at;
   place.before_count = s.before_count;
-  place.before_weight = s.before_weight;
-  u64 inside = s.at_weight;
+  place.before_bin = s.before_weight;
+  place.before_inside = 0;
+  u64 in_all = s.bins.inside[place.bin];
+  inside = by_count ? 0
+                    : min(max((u64)ceil((double)(amount - place.before_bin) / weights.share(place.bin)), (u64)1), place.bin == kept.bin ? min(kept.inside, in_all) : in_all);
   uint32_t low = 0xffffffffu, high = 0, count = 0;
-  const float from = weights.lowest(bin), to = weights.highest(bin);
+  const float from = weights.lowest(place.bin), to = weights.highest(place.bin);
   reader.template each<2>([&](float x, int, int) {
     if (x >= from && x <= to) {
-      double y;
-      if (weights.of(x, y) && weights.bin(y) == bin) {
+      u64 w;
+      if (weights.of(x, w) == place.bin) {
         low = min(low, key_of(x));
         high = max(high, key_of(x));
         ++count;
@@ -308,28 +334,30 @@ __device__ __forceinline__ Place locate(const Reader &reader, const Weights &wei
     reader.each([&](float x, int, int) {
       const uint32_t key = key_of(x);
       if (key >= low && key <= high) {
-        double y;
-        const u64 w = weights.of(x, y);
-        if (w) {
+        u64 w;
+        if (weights.of(x, w) == place.bin) {
           atomicAdd(&s.bins.fine_counts[(high - key) >> shift], 1u);
           atomicAdd(&s.bins.fine_weights[(high - key) >> shift], w);
         }
       }
     });
     __syncthreads();
-    running_sums(s.bins.fine_weights, s.bins.fine_counts, s);
-    find(s.bins.fine_weights, s.bins.fine_counts, by_count, by_count ? amount - place.before_count : amount - place.before_weight, s);
+    u64 fine[kFine / kThreads];
+#pragma unroll
+    for (int i = 0; i < kFine / kThreads; ++i) fine[i] = s.bins.fine_weights[threadIdx.x * (kFine / kThreads) + i];
+    running_sums(fine, s.bins.fine_weights, s.bins.fine_counts, s);
+    find(s.bins.fine_weights, s.bins.fine_counts, by_count, by_count ? amount - place.before_count : inside - place.before_inside, s);
     place.before_count += s.before_count;
-    place.before_weight += s.before_weight;
+    place.before_inside += s.before_weight;
     place.tokens = s.at_count;
-    inside = s.at_weight;
-    const uint32_t from = high - ((uint32_t)s.at << shift), rest = (1u << shift) - 1u;
-    high = from;
-    low = max(low, from - min(from, rest));
+    in_all = s.at_weight;
+    const uint32_t first = high - ((uint32_t)s.at << shift), rest = (1u << shift) - 1u;
+    high = first;
+    low = max(low, first - min(first, rest));
     __syncthreads();
   }
   place.key = low;
-  place.weight = inside / place.tokens;  // (tokens of one logit weigh the same)
+  place.weight = in_all / place.tokens;  // (tokens of one logit weigh the same)
   return place;
 }
 
@@ -361,29 +389,28 @@ __device__ __forceinline__ int index_of(const Reader &reader, uint32_t key, uint
   return (int)low;
 }
 
-// The reader's logits into the bins, whose sums are what s.bins then holds.  counted: tokens, too.
+// The reader's logits into the bins.  counted: tokens, too.  Ends with a barrier.
 template <typename Reader>
 __device__ __forceinline__ void fill_bins(const Reader &reader, const Weights &weights, bool counted, Shared &s) {
   for (int b = threadIdx.x; b < kBins; b += kThreads) {
-    s.bins.weights[b] = 0;
+    s.bins.inside[b] = 0;
     s.bins.counts[b] = 0;
   }
   __syncthreads();
-  if (counted)
+  if (counted || weights.infinite)
     reader.each([&](float x, int, int) {
-      double y;
-      const u64 w = weights.of(x, y);
-      if (w) {
-        const int b = weights.bin(y);
+      u64 w;
+      const int b = weights.of(x, w);
+      if (b < kBins - 1) {
         atomicAdd(&s.bins.counts[b], 1u);
-        atomicAdd(&s.bins.weights[b], w);
+        atomicAdd(&s.bins.inside[b], w);
       }
     });
   else
     reader.each([&](float x, int, int) {
-      double y;
-      const u64 w = weights.of(x, y);
-      if (w) atomicAdd(&s.bins.weights[weights.bin(y)], w);
+      u64 w;
+      const int b = weights.units(weights.distance(x), w);
+      if (b < kBins - 1) atomicAdd(&s.bins.inside[b], w);
     });
   __syncthreads();
 }
@@ -394,21 +421,20 @@ __device__ __forceinline__ u64 drawn_amount(float u, u64 total) { return min((u6
 // The draw, with the row's sums in s.bins; of the bins in which the sums that it asks for end, the reader has the logits.
 template <typename Reader>
 __device__ __forceinline__ void draw(const Reader &reader, const Setting &setting, const Weights &weights, float u, int vocab, Shared &s, int &token, float &probability) {
-  u64 total = s.bins.weights[kBins - 1];
+  End kept = {-1, s.bins.weights[kBins - 1], 0};
+  u64 inside;
   if (setting.top_k > 0 && (uint32_t)setting.top_k < s.bins.counts[kBins - 1]) {
-    const Place place = locate(reader, weights, true, (u64)setting.top_k, s);
-    total = place.before_weight + (u64)((uint32_t)setting.top_k - place.before_count) * place.weight;
+    const Place place = locate(reader, weights, true, (u64)setting.top_k, kept, inside, s);
+    kept = end_at(weights, place, (u64)((uint32_t)setting.top_k - place.before_count));
   }
   if (setting.top_p < 1.f) {
-    const u64 amount = top_p_amount(setting.top_p, total);
-    const Place place = locate(reader, weights, false, amount, s);
+    const Place place = locate(reader, weights, false, top_p_amount(setting.top_p, kept.total), kept, inside, s);
     // (the first of its tokens that reaches the amount is the last one kept)
-    total = place.before_weight + (amount - place.before_weight + place.weight - 1) / place.weight * place.weight;
+    kept = end_at(weights, place, (inside - place.before_inside + place.weight - 1) / place.weight);
   }
-  const u64 amount = drawn_amount(u, total);
-  const Place place = locate(reader, weights, false, amount, s);
-  token = index_of(reader, place.key, (uint32_t)((amount - place.before_weight - 1) / place.weight), vocab, s);
-  probability = (float)((double)place.weight / (double)total);
+  const Place place = locate(reader, weights, false, drawn_amount(u, kept.total), kept, inside, s);
+  token = index_of(reader, place.key, (uint32_t)((inside - place.before_inside - 1) / place.weight), vocab, s);
+  probability = (float)((double)place.weight * weights.share(place.bin) / (double)kept.total);
 }
 
 // A logit onto the list, as far as it has room; s.listed counts all.
@@ -432,7 +458,7 @@ __device__ __forceinline__ Ranges ends_of(const Setting &setting, const Weights 
   const auto ends = [&](float &from, float &to, bool by_count, u64 first, u64 last) {  // bins in which sums of first .. last end
     find(s.bins.weights, s.bins.counts, by_count, first, s);
     const int low = s.at;
-    least = s.before_weight + 1;
+    least = max(s.before_weight, (u64)1);
     __syncthreads();
     find(s.bins.weights, s.bins.counts, by_count, last, s);
     const int high = s.at;
@@ -568,7 +594,7 @@ __device__ __forceinline__ void finish(const SampleArgs &p, const Setting &setti
     if (!binned) {
       if (fits) fill_bins(listed, weights, true, s);
       else fill_bins(reader, weights, true, s);
-      running_sums(s.bins.weights, s.bins.counts, s);
+      sum_bins(weights, s);
     }
     if (fits) draw(listed, setting, weights, uniform_of(p, r), p.vocab, s, token, probability);
     else draw(reader, setting, weights, uniform_of(p, r), p.vocab, s, token, probability);
@@ -594,7 +620,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_tokens_kernel(const Sample
   if (!setting.few()) {
     const Weights weights(setting, most);
     fill_bins(reader, weights, setting.top_k > 0, s);
-    running_sums(s.bins.weights, s.bins.counts, s);
+    sum_bins(weights, s);
     list_ranges(reader, ends_of(setting, weights, uniform_of(p, r), s), s);
   }
   finish(p, setting, r, reader, most, !setting.few(), s.listed <= kList, s);
@@ -678,7 +704,7 @@ __device__ __forceinline__ bool take_lists(const SampleArgs &p, const Between &b
 }
 
 // The row's sums from its parts' bins.  Ends with a barrier.
-__device__ __forceinline__ void take_bins(const SampleArgs &p, const Between &b, int r, bool counted, Shared &s) {
+__device__ __forceinline__ void take_bins(const SampleArgs &p, const Between &b, int r, const Weights &weights, bool counted, Shared &s) {
   const long long first = (long long)r * p.parts * kBins;
   for (int i = threadIdx.x; i < kBins; i += kThreads) {
     u64 weight = 0;
@@ -690,11 +716,11 @@ __device__ __forceinline__ void take_bins(const SampleArgs &p, const Between &b,
       weight += j < p.parts ? w : 0;
       if (counted) count += j < p.parts ? b.counts[at] : 0;
     }
-    s.bins.weights[i] = weight;
+    s.bins.inside[i] = weight;
     s.bins.counts[i] = count;
   }
   __syncthreads();
-  running_sums(s.bins.weights, s.bins.counts, s);
+  sum_bins(weights, s);
 }
 
 // First: every part's largest, and where top_k is small a list of its first.
@@ -741,7 +767,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_bins_kernel(const SampleAr
   fill_bins(part_of<T>(p, r, part), Weights(setting, most), counted, s);
   const long long own = ((long long)r * p.parts + part) * kBins;
   for (int i = threadIdx.x; i < kBins; i += kThreads) {
-    b.weights[own + i] = s.bins.weights[i];
+    b.weights[own + i] = s.bins.inside[i];
     if (counted) b.counts[own + i] = s.bins.counts[i];
   }
 }
@@ -756,8 +782,9 @@ __global__ __launch_bounds__(kThreads, 4) void sample_ends_kernel(const SampleAr
   const long long at = (long long)r * p.parts + part;
   const float most = largest_of_parts(p, b.parts + (long long)r * p.parts);
   if (setting.few() || most == -INFINITY) return;
-  take_bins(p, b, r, setting.top_k > 0, s);
-  list_ranges(part_of<T>(p, r, part), ends_of(setting, Weights(setting, most), uniform_of(p, r), s), s);
+  const Weights weights(setting, most);
+  take_bins(p, b, r, weights, setting.top_k > 0, s);
+  list_ranges(part_of<T>(p, r, part), ends_of(setting, weights, uniform_of(p, r), s), s);
   leave_list(b, at, s);
   if (threadIdx.x == 0) b.parts[at].count = s.listed;
 }
@@ -771,13 +798,16 @@ __global__ __launch_bounds__(kThreads, 4) void sample_draw_kernel(const SampleAr
   const Setting setting(p, r);
   const float most = largest_of_parts(p, b.parts + (long long)r * p.parts);
   if (setting.few() || most == -INFINITY) return;
-  take_bins(p, b, r, setting.top_k > 0, s);
+  take_bins(p, b, r, Weights(setting, most), setting.top_k > 0, s);
   const bool fits = take_lists(p, b, r, 0, s);
   finish(p, setting, r, all_of<T>(p, r), most, true, fits, s);
 }
 
-// Rows that are too few for the chip's 512 places for workgroups are taken in parts of 8192 logits or more.
-int parts_of(int rows, int vocab) { return max(1, min(min(kMostParts, 512 / rows), vocab / 8192)); }
+// Rows that are too few for the chip's 512 places for workgroups are taken in three parts or more, of 16384 logits or more.
+int parts_of(int rows, int vocab) {
+  const int parts = min(min(kMostParts, 512 / rows), vocab / 16384);
+  return parts < 3 ? 1 : parts;
+}
 
 template <typename T>
 hipError_t launch(const SampleArgs &a, hipStream_t stream) {
