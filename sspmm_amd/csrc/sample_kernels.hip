@@ -10,6 +10,11 @@
 // in LDS, and the draw is the list's.  Else the row is put into bins by z, which is to say by weight; where a sum ends is then known up to a bin, and the logits of the few
 // bins that matter become the list.  A bin is split by its logits until one logit is left, and equal logits by their indices.  Where the list has no room, the row
 // in memory stands in its place.
+//
+// What bounds it: a row is read three times (its largest logit, its bins, its list), the second and third time from the caches; 256 rows of 2^17 bf16 logits, a row a CU: 27 us
+// for the largest alone (2.5 TB/s; greedy rows end there), 79 us with no limit, of which the weights in 64 bits and their atomics are some 26 (22 and 9 cycles a CU for 64 logits);
+// 92 us with top_p, whose second sum reads its list again, 52 with a top_k of 50, which needs no bins of the row.  Few rows are bound by the chain of steps: a row of 2000
+// takes 5 us greedy, 10 with no limit, 13 with top_p and top_k.
 #include "sample_kernels.h"
 
 #include "lane_ops.h"
@@ -21,9 +26,10 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kThreads = 512, kWaves = kThreads / 64;
-constexpr int kBins = 1024, kFine = 512;  // of a row or its list (the last one for what weighs nothing), and of a range of logits
-constexpr int kList = 6144;               // logits of a list
+// Threads of a workgroup (N, below).
+constexpr int kThreads = 512, kManyThreads = 1024;
+constexpr int kBins = 1024;                // of a row or its list, the last one for what weighs nothing
+constexpr int kList = 6144;                // logits of a list
 constexpr int kMostTopK = 1200;            // that the threads' four large ones each give a bound for
 
 struct F32 {};
@@ -130,19 +136,25 @@ struct Bins {
   u64 inside[kBins];   // units of the bin
   u64 weights[kBins];  // units of the largest, of this bin and those before
   uint32_t counts[kBins];
-  u64 fine_weights[kFine];
-  uint32_t fine_counts[kFine];
 };
+template <int N>
 struct Shared {
   Bins bins;
+  u64 fine_weights[N];  // of a range of logits, or of indices
+  uint32_t fine_counts[N];
   uint32_t keys[kList], indices[kList];
-  u64 wave_weights[kWaves];
-  uint32_t wave_counts[kWaves];
+  u64 wave_weights[N / 64];
+  uint32_t wave_counts[N / 64];
   uint32_t low, high, listed;
-  int at, token;
+  int at;
   u64 before_weight, at_weight;
   uint32_t before_count, at_count;
 };
+// How far a range that ends `span` further is shifted to leave numbers below N.
+template <int N>
+__device__ __forceinline__ int shift_of(uint32_t span) {
+  return max(0, 32 - __builtin_ctz(N) - (int)__builtin_clz(span));
+}
 
 // A row in memory, or a part of it.
 template <typename T>
@@ -169,7 +181,7 @@ struct RowReader {
   __device__ __forceinline__ void each(const F &f) const {
     const unsigned char *const blocks = row - lead * E::kBytes;
 #pragma unroll UNROLL
-    for (int b = first + (int)threadIdx.x; b < end; b += kThreads) {
+    for (int b = first + (int)threadIdx.x; b < end; b += (int)blockDim.x) {
       float x[E::kCount];
       E::take(*reinterpret_cast<const uintx4 *>(blocks + (long long)b * 16), x);
 #pragma unroll
@@ -187,13 +199,13 @@ struct ListReader {
   int count;
   template <int UNROLL = 1, typename F>
   __device__ __forceinline__ void each(const F &f) const {
-    for (int i = threadIdx.x; i < count; i += kThreads) f(logit_of(keys[i]), (int)indices[i], 0);
+    for (int i = threadIdx.x; i < count; i += (int)blockDim.x) f(logit_of(keys[i]), (int)indices[i], 0);
   }
 };
 
 // Sum of v over the threads in front of the own one; and, in `all`, over all.  Two barriers.
-template <typename V>
-__device__ __forceinline__ V sum_before(V v, V (&waves)[kWaves], V &all) {
+template <typename V, int W>
+__device__ __forceinline__ V sum_before(V v, V (&waves)[W], V &all) {
   const int wave = threadIdx.x >> 6;
   const V upto = wave_inclusive_sum(v);
   if ((threadIdx.x & 63) == 63) waves[wave] = upto;
@@ -201,7 +213,7 @@ __device__ __forceinline__ V sum_before(V v, V (&waves)[kWaves], V &all) {
   V before = upto - v;
   all = 0;
 #pragma unroll
-  for (int i = 0; i < kWaves; ++i) {
+  for (int i = 0; i < W; ++i) {
     const V w = waves[i];
     before += i < wave ? w : 0;
     all += w;
@@ -211,9 +223,9 @@ __device__ __forceinline__ V sum_before(V v, V (&waves)[kWaves], V &all) {
 }
 
 // Sums of weights and counts up to and with each bin, of given weights and the counts that stand there.  Ends with a barrier.
-template <int BINS>
-__device__ __forceinline__ void running_sums(const u64 (&given)[BINS / kThreads], u64 (&weights)[BINS], uint32_t (&counts)[BINS], Shared &s) {
-  constexpr int kOwn = BINS / kThreads;
+template <int BINS, int N>
+__device__ __forceinline__ void running_sums(const u64 (&given)[BINS / N], u64 (&weights)[BINS], uint32_t (&counts)[BINS], Shared<N> &s) {
+  constexpr int kOwn = BINS / N;
   const int tid = threadIdx.x, wave = tid >> 6;
   u64 w[kOwn], w_sum = 0;
   uint32_t c[kOwn], c_sum = 0;
@@ -232,7 +244,7 @@ __device__ __forceinline__ void running_sums(const u64 (&given)[BINS / kThreads]
   c_before -= c_sum;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kWaves; ++i) {
+  for (int i = 0; i < N / 64; ++i) {
     w_before += i < wave ? s.wave_weights[i] : 0;
     c_before += i < wave ? s.wave_counts[i] : 0;
   }
@@ -244,20 +256,21 @@ __device__ __forceinline__ void running_sums(const u64 (&given)[BINS / kThreads]
   __syncthreads();
 }
 // Of a row's bins.
-__device__ __forceinline__ void sum_bins(const Weights &weights, Shared &s) {
-  u64 whole[kBins / kThreads];
+template <int N>
+__device__ __forceinline__ void sum_bins(const Weights &weights, Shared<N> &s) {
+  u64 whole[kBins / N];
 #pragma unroll
-  for (int i = 0; i < kBins / kThreads; ++i) {
-    const int b = threadIdx.x * (kBins / kThreads) + i;
+  for (int i = 0; i < kBins / N; ++i) {
+    const int b = threadIdx.x * (kBins / N) + i;
     whole[i] = weights.whole(b, s.bins.inside[b]);
   }
-  running_sums(whole, s.bins.weights, s.bins.counts, s);
+  running_sums<kBins>(whole, s.bins.weights, s.bins.counts, s);
 }
 
 // The first bin up to whose end there are `amount` tokens, or as much weight: into s.at, with what lies before it and in it.  Ends with a barrier.
-template <int BINS>
-__device__ __forceinline__ void find(const u64 (&weights)[BINS], const uint32_t (&counts)[BINS], bool by_count, u64 amount, Shared &s) {
-  for (int b = threadIdx.x; b < BINS; b += kThreads) {
+template <int BINS, int N>
+__device__ __forceinline__ void find(const u64 (&weights)[BINS], const uint32_t (&counts)[BINS], bool by_count, u64 amount, Shared<N> &s) {
+  for (int b = threadIdx.x; b < BINS; b += N) {
     const u64 w0 = b ? weights[b - 1] : 0, w1 = weights[b];
     const uint32_t c0 = b ? counts[b - 1] : 0, c1 = counts[b];
     if (by_count ? c0 < amount && amount <= c1 : w0 < amount && amount <= w1) {
@@ -289,8 +302,8 @@ __device__ __forceinline__ End end_at(const Weights &weights, const Place &place
 
 // The logit at which the running count, or the running sum of the weights, reaches `amount` (at least one, and no more than there is), and how much that is in units of its bin, which
 // are at least one, and no more than there are: in the bin, or in what is kept of it.
-template <typename Reader>
-__device__ __forceinline__ Place locate(const Reader &reader, const Weights &weights, bool by_count, u64 amount, const End &kept, u64 &inside, Shared &s) {
+template <typename Reader, int N>
+__device__ __forceinline__ Place locate(const Reader &reader, const Weights &weights, bool by_count, u64 amount, const End &kept, u64 &inside, Shared<N> &s) {
   __syncthreads();
   if (threadIdx.x == 0) {
     s.low = 0xffffffffu;
@@ -325,28 +338,24 @@ __device__ __forceinline__ Place locate(const Reader &reader, const Weights &wei
   low = s.low;
   high = s.high;
   while (low < high) {
-    const int shift = max(0, 23 - (int)__builtin_clz(high - low));  // (high - low) >> shift is below kFine
-    for (int b = threadIdx.x; b < kFine; b += kThreads) {
-      s.bins.fine_weights[b] = 0;
-      s.bins.fine_counts[b] = 0;
-    }
+    const int shift = shift_of<N>(high - low);
+    s.fine_weights[threadIdx.x] = 0;
+    s.fine_counts[threadIdx.x] = 0;
     __syncthreads();
     reader.each([&](float x, int, int) {
       const uint32_t key = key_of(x);
       if (key >= low && key <= high) {
         u64 w;
         if (weights.of(x, w) == place.bin) {
-          atomicAdd(&s.bins.fine_counts[(high - key) >> shift], 1u);
-          atomicAdd(&s.bins.fine_weights[(high - key) >> shift], w);
+          atomicAdd(&s.fine_counts[(high - key) >> shift], 1u);
+          atomicAdd(&s.fine_weights[(high - key) >> shift], w);
         }
       }
     });
     __syncthreads();
-    u64 fine[kFine / kThreads];
-#pragma unroll
-    for (int i = 0; i < kFine / kThreads; ++i) fine[i] = s.bins.fine_weights[threadIdx.x * (kFine / kThreads) + i];
-    running_sums(fine, s.bins.fine_weights, s.bins.fine_counts, s);
-    find(s.bins.fine_weights, s.bins.fine_counts, by_count, by_count ? amount - place.before_count : inside - place.before_inside, s);
+    const u64 fine[1] = {s.fine_weights[threadIdx.x]};
+    running_sums<N>(fine, s.fine_weights, s.fine_counts, s);
+    find(s.fine_weights, s.fine_counts, by_count, by_count ? amount - place.before_count : inside - place.before_inside, s);
     place.before_count += s.before_count;
     place.before_inside += s.before_weight;
     place.tokens = s.at_count;
@@ -362,19 +371,19 @@ __device__ __forceinline__ Place locate(const Reader &reader, const Weights &wei
 }
 
 // The index of the token number `which` among those of one logit: the range of indices is split as ranges of logits are.
-template <typename Reader>
-__device__ __forceinline__ int index_of(const Reader &reader, uint32_t key, uint32_t which, int vocab, Shared &s) {
+template <typename Reader, int N>
+__device__ __forceinline__ int index_of(const Reader &reader, uint32_t key, uint32_t which, int vocab, Shared<N> &s) {
   uint32_t low = 0, high = (uint32_t)vocab - 1;
   while (low < high) {
-    const int shift = max(0, 23 - (int)__builtin_clz(high - low));
-    s.bins.fine_counts[threadIdx.x] = 0;
+    const int shift = shift_of<N>(high - low);
+    s.fine_counts[threadIdx.x] = 0;
     __syncthreads();
     reader.each([&](float x, int i, int) {
-      if (key_of(x) == key && (uint32_t)i >= low && (uint32_t)i <= high) atomicAdd(&s.bins.fine_counts[((uint32_t)i - low) >> shift], 1u);
+      if (key_of(x) == key && (uint32_t)i >= low && (uint32_t)i <= high) atomicAdd(&s.fine_counts[((uint32_t)i - low) >> shift], 1u);
     });
     __syncthreads();
     uint32_t all;
-    const uint32_t own = s.bins.fine_counts[threadIdx.x], before = sum_before(own, s.wave_counts, all);
+    const uint32_t own = s.fine_counts[threadIdx.x], before = sum_before(own, s.wave_counts, all);
     if (which >= before && which < before + own) {
       s.at = threadIdx.x;
       s.before_count = before;
@@ -390,9 +399,9 @@ __device__ __forceinline__ int index_of(const Reader &reader, uint32_t key, uint
 }
 
 // The reader's logits into the bins.  counted: tokens, too.  Ends with a barrier.
-template <typename Reader>
-__device__ __forceinline__ void fill_bins(const Reader &reader, const Weights &weights, bool counted, Shared &s) {
-  for (int b = threadIdx.x; b < kBins; b += kThreads) {
+template <typename Reader, int N>
+__device__ __forceinline__ void fill_bins(const Reader &reader, const Weights &weights, bool counted, Shared<N> &s) {
+  for (int b = threadIdx.x; b < kBins; b += N) {
     s.bins.inside[b] = 0;
     s.bins.counts[b] = 0;
   }
@@ -419,8 +428,8 @@ __device__ __forceinline__ u64 top_p_amount(float top_p, u64 total) { return min
 __device__ __forceinline__ u64 drawn_amount(float u, u64 total) { return min((u64)((double)u * (double)total) + 1, total); }
 
 // The draw, with the row's sums in s.bins; of the bins in which the sums that it asks for end, the reader has the logits.
-template <typename Reader>
-__device__ __forceinline__ void draw(const Reader &reader, const Setting &setting, const Weights &weights, float u, int vocab, Shared &s, int &token, float &probability) {
+template <typename Reader, int N>
+__device__ __forceinline__ void draw(const Reader &reader, const Setting &setting, const Weights &weights, float u, int vocab, Shared<N> &s, int &token, float &probability) {
   End kept = {-1, s.bins.weights[kBins - 1], 0};
   u64 inside;
   if (setting.top_k > 0 && (uint32_t)setting.top_k < s.bins.counts[kBins - 1]) {
@@ -438,7 +447,8 @@ __device__ __forceinline__ void draw(const Reader &reader, const Setting &settin
 }
 
 // A logit onto the list, as far as it has room; s.listed counts all.
-__device__ __forceinline__ void list(float x, int i, Shared &s) {
+template <int N>
+__device__ __forceinline__ void list(float x, int i, Shared<N> &s) {
   const uint32_t at = atomicAdd(&s.listed, 1u);
   if (at < kList) {
     s.keys[at] = key_of(x);
@@ -452,7 +462,8 @@ struct Ranges {
 };
 
 // Those of the bins in which what draw() asks for may end, as far as the sums in s.bins say.  Ends with a barrier.
-__device__ __forceinline__ Ranges ends_of(const Setting &setting, const Weights &weights, float u, Shared &s) {
+template <int N>
+__device__ __forceinline__ Ranges ends_of(const Setting &setting, const Weights &weights, float u, Shared<N> &s) {
   Ranges r = {{INFINITY, INFINITY, INFINITY}, {-INFINITY, -INFINITY, -INFINITY}};
   u64 least = s.bins.weights[kBins - 1], most = least;  // that the kept tokens weigh
   const auto ends = [&](float &from, float &to, bool by_count, u64 first, u64 last) {  // bins in which sums of first .. last end
@@ -474,8 +485,8 @@ __device__ __forceinline__ Ranges ends_of(const Setting &setting, const Weights 
 }
 
 // The reader's logits in these ranges become the list.  Ends with a barrier.
-template <typename Reader>
-__device__ __forceinline__ void list_ranges(const Reader &reader, const Ranges &r, Shared &s) {
+template <typename Reader, int N>
+__device__ __forceinline__ void list_ranges(const Reader &reader, const Ranges &r, Shared<N> &s) {
   if (threadIdx.x == 0) s.listed = 0;
   __syncthreads();
   reader.template each<4>([&](float x, int i, int) {
@@ -486,26 +497,26 @@ __device__ __forceinline__ void list_ranges(const Reader &reader, const Ranges &
 }
 
 // The largest of the reader's logits, -infinity if there is none.
-template <typename Reader>
-__device__ __forceinline__ float largest_of(const Reader &reader, Shared &s) {
+template <typename Reader, int N>
+__device__ __forceinline__ float largest_of(const Reader &reader, Shared<N> &s) {
   float most = -INFINITY;
   reader.template each<4>([&](float x, int, int) { most = fmaxf(most, x); });
   most = wave_max_all(most);
   if ((threadIdx.x & 63) == 0) s.wave_counts[threadIdx.x >> 6] = __float_as_uint(most);
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kWaves; ++i) most = fmaxf(most, __uint_as_float(s.wave_counts[i]));
+  for (int i = 0; i < N / 64; ++i) most = fmaxf(most, __uint_as_float(s.wave_counts[i]));
   __syncthreads();
   return most;
 }
 
 // The first `wanted` of the reader's logits, and others, onto the list: those that reach a logit which so many of the threads' largest reach.  Its number, or
 // 0 where the list has all.  Ends with a barrier.
-template <typename T>
-__device__ __forceinline__ uint32_t list_first(const RowReader<T> &reader, uint32_t wanted, float &largest, Shared &s) {
+template <typename T, int N>
+__device__ __forceinline__ uint32_t list_first(const RowReader<T> &reader, uint32_t wanted, float &largest, Shared<N> &s) {
   const int tid = threadIdx.x;
   constexpr int kPairs = 2;  // (the largest and the one behind it, of the even and of the odd places of all blocks)
-  const bool one = wanted <= kThreads / 4;
+  const bool one = wanted <= N / 4;
   float large[2 * kPairs];
 #pragma unroll
   for (float &x : large) x = -INFINITY;
@@ -521,10 +532,10 @@ __device__ __forceinline__ uint32_t list_first(const RowReader<T> &reader, uint3
   // ---- bins of equal width from the smallest of these to the largest
   if (tid == 0) {
     s.low = s.high = 0;
-    s.at = kFine;
+    s.at = N;
     s.listed = 0;
   }
-  s.bins.fine_counts[tid] = 0;
+  s.fine_counts[tid] = 0;
   __syncthreads();
   float most = -INFINITY, least = INFINITY;  // of the finite ones
 #pragma unroll
@@ -540,26 +551,26 @@ __device__ __forceinline__ uint32_t list_first(const RowReader<T> &reader, uint3
   }
   __syncthreads();
   const float top = logit_of(s.high), bottom = logit_of(~s.low);
-  const float scale = (float)(kFine - 1) / fmaxf(top - bottom, 1e-30f);
-  const auto bin = [&](float x) { return (int)fminf(fmaxf((top - x) * scale, 0.f), (float)(kFine - 1)); };
+  const float scale = (float)(N - 1) / fmaxf(top - bottom, 1e-30f);
+  const auto bin = [&](float x) { return (int)fminf(fmaxf((top - x) * scale, 0.f), (float)(N - 1)); };
 #pragma unroll
   for (float x : large)
-    if (x > -INFINITY) atomicAdd(&s.bins.fine_counts[bin(x)], 1u);
+    if (x > -INFINITY) atomicAdd(&s.fine_counts[bin(x)], 1u);
   __syncthreads();
   uint32_t all;
-  const uint32_t own = s.bins.fine_counts[tid], before = sum_before(own, s.wave_counts, all);
+  const uint32_t own = s.fine_counts[tid], before = sum_before(own, s.wave_counts, all);
   if (before < wanted && wanted <= before + own) s.at = tid;
   if (tid == 0) s.low = 0xffffffffu;
   __syncthreads();
   const int last = s.at;
-  if (last < kFine) {
+  if (last < N) {
 #pragma unroll
     for (float x : large)
       if (x > -INFINITY && bin(x) <= last) atomicMin(&s.low, key_of(x));
   }
   __syncthreads();
-  const uint32_t from = last < kFine ? s.low : 0;
-  const float reaches = last < kFine ? logit_of(from) : -INFINITY;
+  const uint32_t from = last < N ? s.low : 0;
+  const float reaches = last < N ? logit_of(from) : -INFINITY;
   reader.template each<2>([&](float x, int i, int) {
     if (x >= reaches && x > -INFINITY) list(x, i, s);
   });
@@ -582,8 +593,8 @@ __device__ __forceinline__ void result(const SampleArgs &p, int r, int token, fl
 __device__ __forceinline__ float uniform_of(const SampleArgs &p, int r) { return fminf(fmaxf(p.uniform[r], 0.f), 0x1.fffffep-1f); }  // (NaN: 0)
 
 // The row's token, and it is written: from the list in s, of some bins of those in s.bins (binned) or of the row's first logits; or where there were too many for it, from the row itself.
-template <typename T>
-__device__ __forceinline__ void finish(const SampleArgs &p, const Setting &setting, int r, const RowReader<T> &reader, float most, bool binned, bool fits, Shared &s) {
+template <typename T, int N>
+__device__ __forceinline__ void finish(const SampleArgs &p, const Setting &setting, int r, const RowReader<T> &reader, float most, bool binned, bool fits, Shared<N> &s) {
   const Weights weights(setting, most);
   const ListReader listed = {s.keys, s.indices, (int)s.listed};
   int token;
@@ -603,9 +614,9 @@ __device__ __forceinline__ void finish(const SampleArgs &p, const Setting &setti
 }
 
 // A workgroup a row.
-template <typename T>
-__global__ __launch_bounds__(kThreads, 4) void sample_tokens_kernel(const SampleArgs p) {
-  __shared__ Shared s;
+template <typename T, int N>
+__global__ __launch_bounds__(N, 4) void sample_tokens_kernel(const SampleArgs p) {
+  __shared__ Shared<N> s;
   const int r = blockIdx.x;
   const unsigned char *const row = row_at<T>(p, r);
   const RowReader<T> reader(row, p.vocab, 0, RowReader<T>::blocks(row, p.vocab));
@@ -669,15 +680,17 @@ __device__ __forceinline__ Part part_here(const SampleArgs &p, const Part *parts
 __device__ __forceinline__ float largest_of_parts(const SampleArgs &p, const Part *parts) { return wave_max_all(part_here(p, parts).most); }
 
 // The list in s to memory.
-__device__ __forceinline__ void leave_list(const Between &b, long long at, const Shared &s) {
+template <int N>
+__device__ __forceinline__ void leave_list(const Between &b, long long at, const Shared<N> &s) {
   const int count = min((int)s.listed, kList);
-  for (int i = threadIdx.x; i < count; i += kThreads) {
+  for (int i = threadIdx.x; i < count; i += N) {
     b.keys[at * kList + i] = s.keys[i];
     b.indices[at * kList + i] = s.indices[i];
   }
 }
 // The parts' lists as one in s, but for logits that some part's list does not hold; false if some part's, or all together, are too many, or fewer than `wanted`.  Ends with a barrier.
-__device__ __forceinline__ bool take_lists(const SampleArgs &p, const Between &b, int r, uint32_t wanted, Shared &s) {
+template <int N>
+__device__ __forceinline__ bool take_lists(const SampleArgs &p, const Between &b, int r, uint32_t wanted, Shared<N> &s) {
   if (threadIdx.x == 0) s.listed = 0;
   __syncthreads();
   const Part mine = part_here(p, b.parts + (long long)r * p.parts);
@@ -686,7 +699,7 @@ __device__ __forceinline__ bool take_lists(const SampleArgs &p, const Between &b
   const uint32_t behind = wave_inclusive_sum(min(mine.count, (uint32_t)kList)), all = from_last_lane(behind);
   const long long first = (long long)r * p.parts * kList;
 #pragma unroll 2
-  for (uint32_t i = threadIdx.x; i < all; i += kThreads) {
+  for (uint32_t i = threadIdx.x; i < all; i += N) {
     int part = 0;
     uint32_t before = 0;
 #pragma unroll
@@ -704,9 +717,10 @@ __device__ __forceinline__ bool take_lists(const SampleArgs &p, const Between &b
 }
 
 // The row's sums from its parts' bins.  Ends with a barrier.
-__device__ __forceinline__ void take_bins(const SampleArgs &p, const Between &b, int r, const Weights &weights, bool counted, Shared &s) {
+template <int N>
+__device__ __forceinline__ void take_bins(const SampleArgs &p, const Between &b, int r, const Weights &weights, bool counted, Shared<N> &s) {
   const long long first = (long long)r * p.parts * kBins;
-  for (int i = threadIdx.x; i < kBins; i += kThreads) {
+  for (int i = threadIdx.x; i < kBins; i += N) {
     u64 weight = 0;
     uint32_t count = 0;
 #pragma unroll
@@ -726,7 +740,7 @@ __device__ __forceinline__ void take_bins(const SampleArgs &p, const Between &b,
 // First: every part's largest, and where top_k is small a list of its first.
 template <typename T>
 __global__ __launch_bounds__(kThreads, 4) void sample_first_kernel(const SampleArgs p) {
-  __shared__ Shared s;
+  __shared__ Shared<kThreads> s;
   const int part = blockIdx.x, r = blockIdx.y;
   const Between b(p.workspace, p.rows, p.parts);
   const RowReader<T> reader = part_of<T>(p, r, part);
@@ -734,8 +748,8 @@ __global__ __launch_bounds__(kThreads, 4) void sample_first_kernel(const SampleA
   const long long at = (long long)r * p.parts + part;
   Part mine = {-INFINITY, 0, 0};
   if (setting.few()) {
-    // (twice a part's share and some, of logits in any order)
-    mine.from = list_first(reader, (uint32_t)min(setting.top_k, 2 * setting.top_k / p.parts + 64), mine.most, s);
+    // (half as many again as a part's share, and some, of logits in any order)
+    mine.from = list_first(reader, (uint32_t)min(setting.top_k, 3 * setting.top_k / (2 * p.parts) + 48), mine.most, s);
     mine.count = s.listed;
     leave_list(b, at, s);
   } else {
@@ -744,25 +758,15 @@ __global__ __launch_bounds__(kThreads, 4) void sample_first_kernel(const SampleA
   if (threadIdx.x == 0) b.parts[at] = mine;
 }
 
-// Second: the draw from these lists, and else every part's bins.
+// Second: every part's bins, where it has no such list.
 template <typename T>
 __global__ __launch_bounds__(kThreads, 4) void sample_bins_kernel(const SampleArgs p) {
-  __shared__ Shared s;
+  __shared__ Shared<kThreads> s;
   const int part = blockIdx.x, r = blockIdx.y;
   const Between b(p.workspace, p.rows, p.parts);
   const Setting setting(p, r);
-  if (setting.few() && part > 0) return;
-  const Part *const parts = b.parts + (long long)r * p.parts;
-  const float most = largest_of_parts(p, parts);
-  if (most == -INFINITY) {
-    if (part == 0) result(p, r, -1, 0.f);
-    return;
-  }
-  if (setting.few()) {
-    const bool fits = take_lists(p, b, r, (uint32_t)setting.top_k, s);
-    finish(p, setting, r, all_of<T>(p, r), most, false, fits, s);
-    return;
-  }
+  const float most = largest_of_parts(p, b.parts + (long long)r * p.parts);
+  if (setting.few() || most == -INFINITY) return;
   const bool counted = setting.top_k > 0;
   fill_bins(part_of<T>(p, r, part), Weights(setting, most), counted, s);
   const long long own = ((long long)r * p.parts + part) * kBins;
@@ -775,7 +779,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_bins_kernel(const SampleAr
 // Third: from all parts' bins the ranges of logits that matter, and every part's list of its own in these.
 template <typename T>
 __global__ __launch_bounds__(kThreads, 4) void sample_ends_kernel(const SampleArgs p) {
-  __shared__ Shared s;
+  __shared__ Shared<kThreads> s;
   const int part = blockIdx.x, r = blockIdx.y;
   const Between b(p.workspace, p.rows, p.parts);
   const Setting setting(p, r);
@@ -789,30 +793,38 @@ __global__ __launch_bounds__(kThreads, 4) void sample_ends_kernel(const SampleAr
   if (threadIdx.x == 0) b.parts[at].count = s.listed;
 }
 
-// Fourth: the draw from those.
+// Fourth: the draw from the lists.
 template <typename T>
-__global__ __launch_bounds__(kThreads, 4) void sample_draw_kernel(const SampleArgs p) {
-  __shared__ Shared s;
+__global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs p) {
+  __shared__ Shared<kThreads> s;
   const int r = blockIdx.x;
   const Between b(p.workspace, p.rows, p.parts);
   const Setting setting(p, r);
   const float most = largest_of_parts(p, b.parts + (long long)r * p.parts);
-  if (setting.few() || most == -INFINITY) return;
-  take_bins(p, b, r, Weights(setting, most), setting.top_k > 0, s);
-  const bool fits = take_lists(p, b, r, 0, s);
-  finish(p, setting, r, all_of<T>(p, r), most, true, fits, s);
+  if (most == -INFINITY) {
+    result(p, r, -1, 0.f);
+    return;
+  }
+  if (!setting.few()) take_bins(p, b, r, Weights(setting, most), setting.top_k > 0, s);
+  const bool fits = take_lists(p, b, r, (uint32_t)setting.top_k, s);
+  finish(p, setting, r, all_of<T>(p, r), most, !setting.few(), fits, s);
 }
 
-// Rows that are too few for the chip's 512 places for workgroups are taken in three parts or more, of 16384 logits or more.
+// Rows that are too few for the chip's 512 places for workgroups are taken in five parts or more, of 16384 logits or more: four launches, which cost some 9 us.  (bf16, us in
+// parts and as a row each: one row of 131072 logits with no limit 31 and 51, top_k 28 and 35; 64 rows in eight parts 52 and 64, 39 and 46, top_p 67 and 78; 128 rows in four 65
+// and 65, 46 and 46, all settings mixed 77 and 73; one row of 50000 in three 30 and 29, 23 and 20.)
 int parts_of(int rows, int vocab) {
   const int parts = min(min(kMostParts, 512 / rows), vocab / 16384);
-  return parts < 3 ? 1 : parts;
+  return parts < 5 ? 1 : parts;
 }
 
 template <typename T>
 hipError_t launch(const SampleArgs &a, hipStream_t stream) {
   if (a.parts == 1) {
-    hipLaunchKernelGGL((sample_tokens_kernel<T>), dim3(a.rows), dim3(kThreads), 0, stream, a);
+    // Where a row has a CU of its own, 1024 threads, unless it is short, when their barriers cost more (us with 1024 and with 512 threads, no limit: 1 row of 2000 11.7 and 9.8, of
+    // 20000 17.9 and 17.5, of 32000 20.7 and 21.8; 200 rows of 50000 36 and 39; 256 rows of 131072 79 and 93).  More rows have two workgroups a CU.
+    if (a.rows <= 256 && a.vocab > 24576) hipLaunchKernelGGL((sample_tokens_kernel<T, kManyThreads>), dim3(a.rows), dim3(kManyThreads), 0, stream, a);
+    else hipLaunchKernelGGL((sample_tokens_kernel<T, kThreads>), dim3(a.rows), dim3(kThreads), 0, stream, a);
   } else {
     const dim3 grid(a.parts, a.rows);
     hipLaunchKernelGGL((sample_first_kernel<T>), grid, dim3(kThreads), 0, stream, a);
