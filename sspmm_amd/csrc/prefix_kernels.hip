@@ -21,7 +21,8 @@ constexpr int kWaves = 4;   // of a workgroup, which share a job's units
 constexpr int kPlaces = 512;     // for workgroups, two a CU
 constexpr int kJobKeys = 1280;   // that a workgroup goes over in the time that it takes to begin and to end
 constexpr int kLeastKeys = 256;  // of a job, as far as there are
-constexpr int kMostStates = 2 * (kPlaces + 1);  // of a query
+constexpr int kMostRounds = 4;   // jobs for each place, and one a tile more, are the most that a plan makes
+constexpr int kMostStates = kMostRounds * kPlaces + 2;  // of a query: jobs of two tiles
 
 // ---- the plan: 32-bit words, in this order
 //   header  jobs, 0, 0, 0
@@ -184,7 +185,8 @@ __global__ __launch_bounds__(kMostPlanRows) void plan_prefixes_kernel(PrefixPlan
   // Units of a job, at most: as few as leave no more jobs than there are places, so that all run at once, found by halving; or, with too many tiles for that, so many that
   // the last jobs' time and what beginning and ending take of all together are least.
   const int least = kLeastKeys / unit;
-  int size = max(least, (int)sqrtf((float)units * (float)(kJobKeys / unit) / (float)shape.target));
+  const u64 most_jobs = (u64)kMostRounds * shape.target;  // (and one a tile more; the buffers have room for so many)
+  int size = max(max(least, (int)sqrtf((float)units * (float)(kJobKeys / unit) / (float)shape.target)), (int)min((units + most_jobs - 1) / most_jobs, (u64)1 << 27));
   if (4 * all_tiles <= 3 * (u64)shape.target) {
     // (jobs of n units in all tiles are fewer than n / size + tiles)
     u64 low = max((u64)least, (units + shape.target - 1) / shape.target), high = max(low, (units + shape.target - all_tiles - 1) / (shape.target - all_tiles));
@@ -556,7 +558,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefix_attention_kernel(const 
 template <typename T, int D>
 __global__ __launch_bounds__(256) void prefix_attention_join_kernel(const PrefixAttentionArgs p) {
   constexpr int kSets = 1024 / D;
-  __shared__ float weights[kMostStates];  // (jobs of two tiles)
+  __shared__ float weights[kMostStates];
   __shared__ __align__(16) float part[kSets][D];
   __shared__ float largest[4], totals[4];
   const PrefixPlan plan(const_cast<int32_t *>(p.plan), p.shape, p.rows);
@@ -622,9 +624,9 @@ PrefixShape prefix_shape(int rows, int queries, int heads, int kv_heads) {
   // own tiles; shared ones, full but for one in a group of two rows or more
   s.tiles = (long long)rows * ((s.row_queries + kRows - 1) / kRows) + (long long)rows * s.row_queries / kRows + rows / 2;
   s.target = max(1, kPlaces / kv_heads);
-  s.jobs = s.tiles + s.target;  // (a tile of n units has fewer than n / size + 1)
+  s.jobs = s.tiles + kMostRounds * s.target;  // (a tile of n units has fewer than n / size + 1, and all tiles' n / size are that many rounds of places at most)
   // a job's queries, 32 at most, are a tile's, and all tiles' no more than twice the rows'
-  s.state_rows = 2ll * rows * s.row_queries + (long long)s.target * kRows;
+  s.state_rows = 2ll * rows * s.row_queries + (long long)kMostRounds * s.target * kRows;
   return s;
 }
 size_t prefix_plan_ints(const PrefixShape &shape, int rows) { return (size_t)PrefixPlan(nullptr, shape, rows).words(rows); }

@@ -424,7 +424,7 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     top_k below 0, and NaN: temperature as 0, the others as what keeps everything).  Logits of -infinity, and NaN, are never drawn; of +infinity they share the draw; a row without any other gives -1.
     probabilities: (tokens, float32 [rows] of the probabilities with which they were drawn).
 
-    Weights are whole multiples of 2^-b of the largest, vocab * 2^b <= 2^62 (at most 52), so that no order of sums changes a token.  Rows may lie apart, at any element;
+    Weights are whole multiples of 2^-b (vocab * 2^b <= 2^62, b at most 50) of the power of 2^(1/16) nearest to them, so that no order of sums changes a token.  Rows may lie apart, at any element;
     other strides are copied first.  At most 2^24 tokens in a vocabulary."""
     kind, device = LOGIT_TYPES.get(logits.dtype), logits.get_device()
     if kind is None or device < 0:

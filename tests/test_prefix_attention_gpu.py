@@ -114,6 +114,23 @@ def test_as_many_rows_as_a_plan_takes(built_library):
     assert (got.float() - want.float()).abs().max() < 0.02
 
 
+@pytest.mark.parametrize("groups,heads,kv,page", [([(0, [4096 + 120 * i]) for i in range(32)], 16, 16, 32), ([(0, [22000 + 900 * i]) for i in range(8)], 64, 64, 64),
+                                                  ([(3200, [3000 + 5 * i, 3500]) for i in range(200)], 2, 1, 64), ([(30000, [500, 9000, 20000]), (25000, [4000] * 5)], 32, 32, 64)])
+def test_more_tiles_than_places_and_long_rows(built_library, groups, heads, kv, page):
+    """Jobs are no more than the plan has room for, where their number grows with the root of the rows' lengths, and where it is bounded."""
+    table, lengths, pages = _tables(groups, page)
+    rows, d = lengths.numel(), 32
+    pool = _pool(pages, kv, page, d, torch.int8, 1)
+    q = _randn((rows, 1, heads, d), 2).half()
+    plan = sspmm_amd.plan_prefixes(table, lengths, 1, heads, kv, page)
+    assert rows < int(plan.data[0]) <= (plan.data.numel() - 4 - 12 * rows) // 12
+    got = sspmm_amd.prefix_attention(q, table, plan, *pool)
+    at = list(range(0, rows, 1 + rows // 9)) + [rows - 1]
+    check_step(got[at], q[at], table[at], lengths[at], *pool, d ** -0.5)
+    want = sspmm_amd.cache_attention(q, table, lengths, *pool)
+    assert (got.float() - want.float()).abs().max() < 0.02
+
+
 def test_what_a_plan_shares(built_library):
     page, rows = 32, 6
     table = _ints([[1, 2, 3, 4, 5], [1, 2, 3, 9, 8], [1, 2, 3, 4, 7], [1, 10, 11, 12, 13], [20, 21, -1, -1, -1], [-1, 2, 3, 4, 5]])

@@ -1,6 +1,7 @@
-"""Drawn tokens against the rule in 64 bits.  Weights there are doubles, here whole multiples of 2^-45 of the largest or finer: a running sum of n of them is off by
-n / 2 of these steps at most, and a token differs where a uniform number's place lies that near to a border, which is to say (borders up to 2^17, sums of
-one or more) in one draw of 2^45 / 2^17 / 2^17, some 2^11, at the very worst, in one of millions with the errors' signs mixed.  Logits and numbers here are fixed."""
+"""Drawn tokens against the rule in 64 bits.  Weights there are doubles, here whole multiples of 2^-45 or finer of the
+power of 2^(1/16) that is nearest to them, and so within 2^-45 of themselves; the sum of those of one power is brought to multiples of 2^-45 of the largest.  A running sum
+is off by 2^-45 of itself and 2^10 halves of such a step at most, and a token differs where a uniform number's place lies that near to a border, which is to say (borders up to
+2^17, sums of one or more) in one draw of 2^45 / (1 + 2^9) / 2^17, some 2^18, at the worst.  Logits and numbers here are fixed."""
 import math
 
 import numpy as np
