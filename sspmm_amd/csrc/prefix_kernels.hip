@@ -194,7 +194,8 @@ __global__ __launch_bounds__(kMostPlanRows) void plan_prefixes_kernel(PrefixPlan
       const u64 step = (high - low + 3) / 4;
       u64 mine = 0, counts;
       for (int i = 0; i < 3; ++i) {  // three sizes at a time; a thread's jobs matter up to the places
-        const u64 at = low + i * step, jobs = (u64)group_tiles * ((group_units + at - 1) / at) + (u64)own_tiles * ((own_units + at - 1) / at);
+        const uint32_t at = (uint32_t)(low + i * step);  // (below 2^29; 32 bits divide much faster than 64)
+        const u64 jobs = (u64)group_tiles * (((uint32_t)group_units + at - 1) / at) + (u64)own_tiles * (((uint32_t)own_units + at - 1) / at);
         mine |= min(jobs, (u64)2 * kPlaces) << 21 * i;
       }
       sum_before(mine, waves, counts);
@@ -240,8 +241,9 @@ __global__ __launch_bounds__(kMostPlanRows) void plan_prefixes_kernel(PrefixPlan
     const int tiles = ((of_group ? group_queries[row] : shape.row_queries) + kRows - 1) / kRows;
     const int tile = which % tiles, cut = which / tiles, first = tile * kRows;
     const int count = min(kRows, (of_group ? group_queries[row] : shape.row_queries) - first);
-    const int unit0 = of_group ? 0 : start / unit;
-    plan.jobs[j] = {row, unit0 + (int)((long long)row_units * cut / cuts), unit0 + (int)((long long)row_units * (cut + 1) / cuts), of_group ? start : stop,
+    const int each = row_units / cuts, more = row_units % cuts;  // units of a job, and the first jobs that have one more
+    const int unit0 = (of_group ? 0 : start / unit) + cut * each + min(cut, more);
+    plan.jobs[j] = {row, unit0, unit0 + each + (cut < more), of_group ? start : stop,
                     of_group ? INT_MAX : lengths_of[row] - queries + 1, in_orders[row], first, count,
                     (of_group ? shared_states[row] : own_states[row]) + first * cuts + cut * count, {0, 0, 0}};
   }
