@@ -624,6 +624,7 @@ int sspmm_compact_pages(int32_t *page_refs, int pages, int32_t *page_table, int 
  * Attention of packed queries over packed states of other lengths, as a decoder's over its encoder's: query i of sequence b (rows offsets[b] ..
  * offsets[b + 1] - 1 of q and out) sees rows source_offsets[b] .. source_offsets[b + 1] - 1 of k and v, all of them.  Both lists as offsets in
  * sspmm_prompt_attention, the second within 0 .. source_tokens; a sequence without states, or whose scores are all -infinity, is zeros.  Strides, limits and out as there.
+ * tokens * heads / kv_heads is below 2^31.
  * workspace: sspmm_cross_attention_workspace_bytes of the same sizes, 16-byte aligned (may be 0 bytes).
  */
 size_t sspmm_cross_attention_workspace_bytes(int sequences, int tokens, int source_tokens, int heads, int kv_heads, int head_dim);

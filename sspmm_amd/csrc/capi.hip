@@ -847,7 +847,7 @@ int sspmm_cross_attention(int type, int sequences, int tokens, int source_tokens
   if (sequences == 0 || tokens == 0) return 0;
   if (!offsets || !source_offsets || !operand_fits(q, q_row, q_head, head_dim) || !operand_fits(out, out_row, out_head, head_dim)) return kInvalid;
   if (source_tokens > 0 && (!operand_fits(k, k_row, k_head, head_dim) || !operand_fits(v, v_row, v_head, head_dim))) return kInvalid;
-  if (tokens > (1 << 30) || source_tokens > (1 << 30)) return kInvalid;
+  if (tokens > (1 << 30) || source_tokens > (1 << 30) || (int64_t)tokens * (heads / kv_heads) >= 1ll << 31) return kInvalid;
   sspmm::PromptArgs a{};
   a.q = q;
   a.k = k;

@@ -34,6 +34,8 @@ def test_cross_attention(L):
                  (18, float("nan")), (18, float("inf")), (18, 3.0e38), (19, None), (19, A + 2), (20, 60), (21, 3), (22, None), (22, A + 8), (23, need - 1)):
         assert run((i, v)) == 1, (i, v)
     assert run((1, 0), (7, None), (8, None)) == 0 and run((2, 0), (9, None)) == 0
+    # queries times heads of a group are counted in 31 bits
+    assert run((2, 1 << 30)) == 1
 
 
 def test_plan_and_prefix_attention(L):
