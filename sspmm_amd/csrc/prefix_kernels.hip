@@ -82,42 +82,58 @@ __device__ __forceinline__ int full_pages(int length, int queries, int page_size
   return (int)min((long long)slots, max(0ll, (long long)length - queries + 1) / page_size);
 }
 
-// A wave a row: the lowest row that begins with the same page, and the pages that the two share.
-__global__ __launch_bounds__(64) void plan_prefixes_compare_kernel(PrefixPlan plan, const int32_t *table, int rows, int slots, const int32_t *lengths, int page_size, int queries) {
-  const int row = blockIdx.x, lane = threadIdx.x;
+// A workgroup a row: the lowest row that begins with the same page, and the pages that the two share.
+constexpr int kCompareWaves = 4;
+__global__ __launch_bounds__(64 * kCompareWaves) void plan_prefixes_compare_kernel(PrefixPlan plan, const int32_t *table, int rows, int slots, const int32_t *lengths, int page_size,
+                                                                                   int queries) {
+  __shared__ int ends[kCompareWaves];
+  const int row = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int32_t *const own = table + (long long)row * slots;
   const int first = own[0], full = full_pages(lengths[row], queries, page_size, slots);
   int leader = -1, shared = 0;
   if (first >= 0 && full > 0) {
+    int most = 0;
     for (int at = 0; at < rows && leader < 0; at += 64) {
       const int r = at + lane;
-      const bool same = r < rows && table[(long long)r * slots] == first && full_pages(lengths[r], queries, page_size, slots) > 0;
-      const u64 those = __ballot(same);
-      if (those) leader = at + __builtin_ctzll(those);
+      const int begins = r < rows ? table[(long long)r * slots] : -1, pages = r < rows ? full_pages(lengths[r], queries, page_size, slots) : 0;
+      const u64 those = __ballot(begins == first && pages > 0);
+      if (those) {
+        const int lowest = __builtin_ctzll(those);
+        leader = at + lowest;
+        most = min(full, __builtin_amdgcn_readlane(pages, lowest));
+      }
     }
     const int32_t *const other = table + (long long)leader * slots;
-    const int most = min(full, full_pages(lengths[leader], queries, page_size, slots));
+    // (a wave looks at 512 slots at a time)
     constexpr int kAtOnce = 8;
-    bool more = true;
-    for (shared = 0; more && shared < most;) {
+    for (shared = 0; shared < most;) {
+      const int from = shared + 64 * kAtOnce * wave;
       bool same[kAtOnce];
-      const int from = shared;
 #pragma unroll
       for (int i = 0; i < kAtOnce; ++i) {
         const int s = from + 64 * i + lane, at = min(s, most - 1);
         const int mine = own[at];
         same[i] = s < most && mine >= 0 && mine == other[at];
       }
+      int end = INT_MAX;  // the first that differs
 #pragma unroll
-      for (int i = 0; i < kAtOnce; ++i) {
+      for (int i = kAtOnce - 1; i >= 0; --i) {
         const u64 differ = __ballot(!same[i]);
-        if (more) shared += differ ? __builtin_ctzll(differ) : 64;
-        more = more && differ == 0;
+        end = differ ? from + 64 * i + __builtin_ctzll(differ) : end;
+      }
+      __syncthreads();
+      if (lane == 0) ends[wave] = end;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kCompareWaves; ++i) end = min(end, ends[i]);
+      shared += 64 * kAtOnce * kCompareWaves;
+      if (end != INT_MAX) {
+        shared = min(end, most);
+        break;
       }
     }
-    shared = min(shared, most);
   }
-  if (lane == 0) {
+  if (threadIdx.x == 0) {
     plan.leaders[row] = leader;
     plan.shared[row] = shared;
   }
@@ -645,7 +661,7 @@ size_t prefix_attention_floats(const PrefixShape &shape, int kv_heads, int d) {
 hipError_t launch_plan_prefixes(const PrefixShape &shape, const int32_t *table, int rows, int slots, const int32_t *lengths, int page_size, int queries, int32_t *plan,
                                 hipStream_t stream) {
   const PrefixPlan at(plan, shape, rows);
-  hipLaunchKernelGGL(plan_prefixes_compare_kernel, dim3(rows), dim3(64), 0, stream, at, table, rows, slots, lengths, page_size, queries);
+  hipLaunchKernelGGL(plan_prefixes_compare_kernel, dim3(rows), dim3(64 * kCompareWaves), 0, stream, at, table, rows, slots, lengths, page_size, queries);
   hipLaunchKernelGGL(plan_prefixes_kernel, dim3(1), dim3(max(256, (rows + 63) / 64 * 64)), 0, stream, at, rows, slots, lengths, page_size, queries, shape);
   return hipGetLastError();
 }

@@ -151,6 +151,19 @@ def test_what_a_plan_shares(built_library):
     assert _units(empty) == 0
 
 
+def test_where_long_rows_part(built_library):
+    """Rows of thousands of pages, as far as they are the same."""
+    slots = 5000
+    base = torch.arange(slots, dtype=torch.int32, device="cuda")
+    for shared in (1, 63, 64, 511, 512, 513, 1536, 2047, 2048, 2049, 4095, 4096, 4097, 4999, 5000):
+        table = torch.stack([base, base])
+        table[1, shared:] += slots
+        if shared + 1 < slots:
+            table[1, shared + 1] -= slots  # (the same again behind it)
+        plan = sspmm_amd.plan_prefixes(table, _ints([32 * slots + 1, 32 * slots]), 1, 1, 1, 32)
+        assert _units(plan) == shared + 2 * (slots - shared), shared
+
+
 @pytest.mark.parametrize("form", FORMATS)
 def test_short_empty_and_overlong_rows(built_library, form):
     """Rows without a token, with fewer tokens than queries, and with more than their table has room for; queries that see nothing are zeros."""
