@@ -11,9 +11,9 @@
 // bins that matter become the list.  A bin is split by its logits until one logit is left, and equal logits by their indices.  Where the list has no room, the row
 // in memory stands in its place.
 //
-// What bounds it: a row is read three times (its largest logit, its bins, its list), the second and third time from the caches; 256 rows of 2^17 bf16 logits, a row a CU: 27 us
-// for the largest alone (2.5 TB/s; greedy rows end there), 79 us with no limit, of which the weights in 64 bits and their atomics are some 26 (22 and 9 cycles a CU for 64 logits);
-// 92 us with top_p, whose second sum reads its list again, 52 with a top_k of 50, which needs no bins of the row.  Few rows are bound by the chain of steps: a row of 2000
+// What bounds it: a row is read three times (its largest logit, its bins, its list), the second and third time from the caches; 256 rows of 2^17 bf16 logits, a row a CU: 18 us
+// greedy (3.7 TB/s), 79 us with no limit, of which the weights in 64 bits and their atomics are some 26 (22 and 9 cycles a CU for 64 logits); 92 us with top_p, whose second
+// sum reads its list again; 29 with a top_k of 50, which needs no bins of the row and reads it once, 53 with one of 1000, which reads it twice.  Few rows are bound by the chain of steps: a row of 2000
 // takes 5 us greedy, 10 with no limit, 13 with top_p and top_k.
 #include "sample_kernels.h"
 
@@ -176,21 +176,27 @@ struct RowReader {
     return ((int)(reinterpret_cast<uintptr_t>(row) & 15) / E::kBytes + vocab + E::kCount - 1) / E::kCount;
   }
   __device__ __forceinline__ float one(int i) const { return E::one(row + (long long)i * E::kBytes); }
-  // f(logit, index, place in its block) of every element, in any order
-  template <int UNROLL = 1, typename F>
-  __device__ __forceinline__ void each(const F &f) const {
-    const unsigned char *const blocks = row - lead * E::kBytes;
-#pragma unroll UNROLL
-    for (int b = first + (int)threadIdx.x; b < end; b += (int)blockDim.x) {
-      float x[E::kCount];
-      E::take(*reinterpret_cast<const uintx4 *>(blocks + (long long)b * 16), x);
+  // f(logit, index, place in its block) of a block's elements
+  template <typename F>
+  __device__ __forceinline__ void block(int b, const F &f) const {
+    float x[E::kCount];
+    E::take(*reinterpret_cast<const uintx4 *>(row - lead * E::kBytes + (long long)b * 16), x);
 #pragma unroll
-      for (int i = 0; i < E::kCount; ++i) f(x[i], b * E::kCount - lead + i, i);
-    }
-    // (what lies in front of the whole blocks and behind them, an element a thread)
+    for (int i = 0; i < E::kCount; ++i) f(x[i], b * E::kCount - lead + i, i);
+  }
+  // of what lies in front of the whole blocks and behind them, an element a thread
+  template <typename F>
+  __device__ __forceinline__ void edge(const F &f) const {
     const int tid = threadIdx.x, head_end = min(to, first * E::kCount - lead), tail = max(head_end, end * E::kCount - lead);
     const int i = from + tid < head_end ? from + tid : tail + tid - (head_end - from);
     if (i < head_end || (i >= tail && i < to)) f(one(i), i, 0);
+  }
+  // and of every element, in any order
+  template <int UNROLL = 1, typename F>
+  __device__ __forceinline__ void each(const F &f) const {
+#pragma unroll UNROLL
+    for (int b = first + (int)threadIdx.x; b < end; b += (int)blockDim.x) block(b, f);
+    edge(f);
   }
 };
 
@@ -560,7 +566,10 @@ __device__ __forceinline__ uint32_t list_first(const RowReader<T> &reader, uint3
   uint32_t all;
   const uint32_t own = s.fine_counts[tid], before = sum_before(own, s.wave_counts, all);
   if (before < wanted && wanted <= before + own) s.at = tid;
-  if (tid == 0) s.low = 0xffffffffu;
+  if (tid == 0) {
+    s.low = 0xffffffffu;
+    s.high = 0;
+  }
   __syncthreads();
   const int last = s.at;
   if (last < N) {
@@ -571,9 +580,27 @@ __device__ __forceinline__ uint32_t list_first(const RowReader<T> &reader, uint3
   __syncthreads();
   const uint32_t from = last < N ? s.low : 0;
   const float reaches = last < N ? logit_of(from) : -INFINITY;
-  reader.template each<2>([&](float x, int i, int) {
+  const auto take = [&](float x, int i, int) {
     if (x >= reaches && x > -INFINITY) list(x, i, s);
-  });
+  };
+  // Where few threads' largest reach it, those threads' blocks are all that has to be read again, by all threads (256 rows of
+  // 131072 in bf16, greedy 18 us instead of 27, top_k of 50 29 instead of 38, of 128 34 instead of 38).
+  bool few = one && last < N;
+  if (few) {
+    if (large[0] >= reaches) s.fine_counts[atomicAdd(&s.high, 1u)] = (uint32_t)tid;
+    __syncthreads();
+    few = s.high <= N / 4;
+  }
+  if (few) {
+    const int threads = (int)s.high, blocks = (reader.end - reader.first + N - 1) / N * threads;
+    for (int j = tid; j < blocks; j += N) {
+      const int b = reader.first + (int)s.fine_counts[j % threads] + N * (j / threads);
+      if (b < reader.end) reader.block(b, take);
+    }
+    reader.edge(take);
+  } else {
+    reader.template each<2>(take);
+  }
   __syncthreads();
   largest = top;
   return from;
