@@ -82,12 +82,10 @@ __device__ __forceinline__ int full_pages(int length, int queries, int page_size
   return (int)min((long long)slots, max(0ll, (long long)length - queries + 1) / page_size);
 }
 
-// A workgroup a row: the lowest row that begins with the same page, and the pages that the two share.
-constexpr int kCompareWaves = 4;
-__global__ __launch_bounds__(64 * kCompareWaves) void plan_prefixes_compare_kernel(PrefixPlan plan, const int32_t *table, int rows, int slots, const int32_t *lengths, int page_size,
-                                                                                   int queries) {
-  __shared__ int ends[kCompareWaves];
-  const int row = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+// The lowest row that begins with the same page as `row`, and the pages that the two share: by WAVES waves, of which this is number `wave`; with more than one, a workgroup.
+template <int WAVES>
+__device__ __forceinline__ int2 compare(int row, int wave, const int32_t *table, int rows, int slots, const int32_t *lengths, int page_size, int queries, int (&ends)[WAVES]) {
+  const int lane = threadIdx.x & 63;
   const int32_t *const own = table + (long long)row * slots;
   const int first = own[0], full = full_pages(lengths[row], queries, page_size, slots);
   int leader = -1, shared = 0;
@@ -121,21 +119,33 @@ __global__ __launch_bounds__(64 * kCompareWaves) void plan_prefixes_compare_kern
         const u64 differ = __ballot(!same[i]);
         end = differ ? from + 64 * i + __builtin_ctzll(differ) : end;
       }
-      __syncthreads();
-      if (lane == 0) ends[wave] = end;
-      __syncthreads();
+      if constexpr (WAVES > 1) {
+        __syncthreads();
+        if (lane == 0) ends[wave] = end;
+        __syncthreads();
 #pragma unroll
-      for (int i = 0; i < kCompareWaves; ++i) end = min(end, ends[i]);
-      shared += 64 * kAtOnce * kCompareWaves;
+        for (int i = 0; i < WAVES; ++i) end = min(end, ends[i]);
+      }
+      shared += 64 * kAtOnce * WAVES;
       if (end != INT_MAX) {
         shared = min(end, most);
         break;
       }
     }
   }
+  return {leader, shared};
+}
+
+// A workgroup a row.
+constexpr int kCompareWaves = 4;
+__global__ __launch_bounds__(64 * kCompareWaves) void plan_prefixes_compare_kernel(PrefixPlan plan, const int32_t *table, int rows, int slots, const int32_t *lengths, int page_size,
+                                                                                   int queries) {
+  __shared__ int ends[kCompareWaves];
+  const int row = blockIdx.x;
+  const int2 found = compare<kCompareWaves>(row, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), table, rows, slots, lengths, page_size, queries, ends);
   if (threadIdx.x == 0) {
-    plan.leaders[row] = leader;
-    plan.shared[row] = shared;
+    plan.leaders[row] = found.x;
+    plan.shared[row] = found.y;
   }
 }
 
@@ -152,8 +162,11 @@ __device__ __forceinline__ u64 sum_before(u64 v, u64 (&waves)[kMostPlanRows / 64
   return upto - v + (wave ? of(wave - 1) : 0);
 }
 
-// One workgroup, a thread a row (and more threads than that).
-__global__ __launch_bounds__(kMostPlanRows) void plan_prefixes_kernel(PrefixPlan plan, int rows, int slots, const int32_t *lengths, int page_size, int queries, PrefixShape shape) {
+// One workgroup, a thread a row (and more threads than that).  table: no launch has compared the rows, but here a wave does it for each
+// (up to 8: 3 rows 7.6 us and, with the launch, 9.2, 8 rows 8.7 and 9.5, 16 rows 15.3 and 11.8).
+constexpr int kFewRows = 8;
+__global__ __launch_bounds__(kMostPlanRows) void plan_prefixes_kernel(PrefixPlan plan, const int32_t *table, int rows, int slots, const int32_t *lengths, int page_size, int queries,
+                                                                      PrefixShape shape) {
   __shared__ int2 found[kMostPlanRows];  // leader, shared pages
   __shared__ int base[kMostPlanRows];
   __shared__ int in_orders[kMostPlanRows], lengths_of[kMostPlanRows], group_queries[kMostPlanRows];
@@ -161,10 +174,21 @@ __global__ __launch_bounds__(kMostPlanRows) void plan_prefixes_kernel(PrefixPlan
   __shared__ u64 best[kMostPlanRows], waves[kMostPlanRows / 64];
   const int r = threadIdx.x;
   const bool there = r < rows;
-  const int leader = there ? plan.leaders[r] : -1, mine = there ? plan.shared[r] : 0;
-  found[r] = {leader, mine};
+  found[r] = {-1, 0};
   best[r] = 0;
+  if (table) {
+    const int wave = __builtin_amdgcn_readfirstlane(r >> 6);
+    int none[1];
+    __syncthreads();
+    if (wave < rows) {
+      const int2 of_row = compare<1>(wave, 0, table, rows, slots, lengths, page_size, queries, none);
+      if ((r & 63) == 0) found[wave] = of_row;
+    }
+  } else if (there) {
+    found[r] = {plan.leaders[r], plan.shared[r]};
+  }
   __syncthreads();
+  const int leader = found[r].x, mine = found[r].y;
   // ---- the pages that a group shares: of its rows' numbers the one that saves most
   if (leader >= 0) {
     int as_many = 0;
@@ -661,8 +685,10 @@ size_t prefix_attention_floats(const PrefixShape &shape, int kv_heads, int d) {
 hipError_t launch_plan_prefixes(const PrefixShape &shape, const int32_t *table, int rows, int slots, const int32_t *lengths, int page_size, int queries, int32_t *plan,
                                 hipStream_t stream) {
   const PrefixPlan at(plan, shape, rows);
-  hipLaunchKernelGGL(plan_prefixes_compare_kernel, dim3(rows), dim3(64 * kCompareWaves), 0, stream, at, table, rows, slots, lengths, page_size, queries);
-  hipLaunchKernelGGL(plan_prefixes_kernel, dim3(1), dim3(max(256, (rows + 63) / 64 * 64)), 0, stream, at, rows, slots, lengths, page_size, queries, shape);
+  const bool few = rows <= kFewRows;
+  if (!few) hipLaunchKernelGGL(plan_prefixes_compare_kernel, dim3(rows), dim3(64 * kCompareWaves), 0, stream, at, table, rows, slots, lengths, page_size, queries);
+  hipLaunchKernelGGL(plan_prefixes_kernel, dim3(1), dim3(few ? max(256, 64 * rows) : max(256, (rows + 63) / 64 * 64)), 0, stream, at, few ? table : nullptr, rows, slots, lengths,
+                     page_size, queries, shape);
   return hipGetLastError();
 }
 

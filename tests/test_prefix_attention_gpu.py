@@ -151,8 +151,9 @@ def test_what_a_plan_shares(built_library):
     assert _units(empty) == 0
 
 
-def test_where_long_rows_part(built_library):
-    """Rows of thousands of pages, as far as they are the same."""
+@pytest.mark.parametrize("others", [0, 9])
+def test_where_long_rows_part(built_library, others):
+    """Rows of thousands of pages, as far as they are the same; alone, and among others without a token."""
     slots = 5000
     base = torch.arange(slots, dtype=torch.int32, device="cuda")
     for shared in (1, 63, 64, 511, 512, 513, 1536, 2047, 2048, 2049, 4095, 4096, 4097, 4999, 5000):
@@ -160,7 +161,8 @@ def test_where_long_rows_part(built_library):
         table[1, shared:] += slots
         if shared + 1 < slots:
             table[1, shared + 1] -= slots  # (the same again behind it)
-        plan = sspmm_amd.plan_prefixes(table, _ints([32 * slots + 1, 32 * slots]), 1, 1, 1, 32)
+        table = torch.cat([table, table[:1].expand(others, slots)])
+        plan = sspmm_amd.plan_prefixes(table, _ints([32 * slots + 1, 32 * slots] + [0] * others), 1, 1, 1, 32)
         assert _units(plan) == shared + 2 * (slots - shared), shared
 
 
