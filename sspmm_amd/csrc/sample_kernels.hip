@@ -37,6 +37,7 @@ struct F32 {};
 template <typename T>
 struct Elements {  // of 16 bytes
   static constexpr int kCount = 8, kBytes = 2;
+  static constexpr int kGrain = __is_same(T, Bf16) ? 16 : 13;  // bits at the end that are the same in all logits of one sign, taken as 32 bits
   static __device__ __forceinline__ void take(uintx4 w, float (&x)[8]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -48,7 +49,7 @@ struct Elements {  // of 16 bytes
 };
 template <>
 struct Elements<F32> {
-  static constexpr int kCount = 4, kBytes = 4;
+  static constexpr int kCount = 4, kBytes = 4, kGrain = 0;
   static __device__ __forceinline__ void take(uintx4 w, float (&x)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
@@ -141,11 +142,11 @@ template <int N>
 struct Shared {
   Bins bins;
   u64 fine_weights[N];  // of a range of logits, or of indices
-  uint32_t fine_counts[N];
+  __align__(16) uint32_t fine_counts[N];
   uint32_t keys[kList], indices[kList];
   u64 wave_weights[N / 64];
   uint32_t wave_counts[N / 64];
-  uint32_t low, high, listed;
+  uint32_t low, high, listed, alike;
   int at;
   u64 before_weight, at_weight;
   uint32_t before_count, at_count;
@@ -160,6 +161,7 @@ __device__ __forceinline__ int shift_of(uint32_t span) {
 template <typename T>
 struct RowReader {
   typedef Elements<T> E;
+  static constexpr int kGrain = E::kGrain;
   const unsigned char *row;  // aligned to an element
   int first, end;            // whole blocks of 16 aligned bytes in it, counted from the one that holds its first element
   int lead, from, to;        // elements in front of the row in that block; the part's elements
@@ -200,7 +202,9 @@ struct RowReader {
   }
 };
 
+template <typename T>
 struct ListReader {
+  static constexpr int kGrain = Elements<T>::kGrain;
   const uint32_t *keys, *indices;
   int count;
   template <int UNROLL = 1, typename F>
@@ -344,7 +348,8 @@ __device__ __forceinline__ Place locate(const Reader &reader, const Weights &wei
   low = s.low;
   high = s.high;
   while (low < high) {
-    const int shift = shift_of<N>(high - low);
+    // (no finer than the type: with 16 bits a bin has few logits, and one round finds the right one)
+    const int shift = max(shift_of<N>(high - low), Reader::kGrain);
     s.fine_weights[threadIdx.x] = 0;
     s.fine_counts[threadIdx.x] = 0;
     __syncthreads();
@@ -367,8 +372,12 @@ __device__ __forceinline__ Place locate(const Reader &reader, const Weights &wei
     place.tokens = s.at_count;
     in_all = s.at_weight;
     const uint32_t first = high - ((uint32_t)s.at << shift), rest = (1u << shift) - 1u;
-    high = first;
-    low = max(low, first - min(first, rest));
+    if (shift == Reader::kGrain) {  // one logit (a negative one ends in ones, the others in zeros)
+      low = high = Reader::kGrain > 0 && first < 0x80000000u && (first & rest) == 0 ? first - 1 : first;
+    } else {
+      high = first;
+      low = max(low, first - min(first, rest));
+    }
     __syncthreads();
   }
   place.key = low;
@@ -376,9 +385,35 @@ __device__ __forceinline__ Place locate(const Reader &reader, const Weights &wei
   return place;
 }
 
-// The index of the token number `which` among those of one logit: the range of indices is split as ranges of logits are.
+constexpr uint32_t kFewAlike = 256;  // (ranked by the first four waves at a time; 512 by eight cost 256 rows of 131072 83 us instead of 78)
+// The index of the token number `which` among those of one logit: of few, by counting the smaller ones; else the range of indices is split as ranges of logits are.
 template <typename Reader, int N>
 __device__ __forceinline__ int index_of(const Reader &reader, uint32_t key, uint32_t which, int vocab, Shared<N> &s) {
+  s.fine_counts[threadIdx.x] = 0xffffffffu;
+  if (threadIdx.x == 0) s.alike = 0;
+  __syncthreads();
+  reader.each([&](float x, int i, int) {
+    if (key_of(x) == key) {
+      const uint32_t at = atomicAdd(&s.alike, 1u);
+      if (at < N) s.fine_counts[at] = (uint32_t)i;
+    }
+  });
+  __syncthreads();
+  const uint32_t those = s.alike;
+  if (those <= kFewAlike) {
+    if (threadIdx.x < those) {
+      const uint32_t own = s.fine_counts[threadIdx.x];
+      uint32_t smaller = 0;
+      for (uint32_t i = 0; i < those; i += 4) {
+        const uintx4 four = *reinterpret_cast<const uintx4 *>(&s.fine_counts[i]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) smaller += four[j] < own;
+      }
+      if (smaller == which) s.at = (int)own;
+    }
+    __syncthreads();
+    return s.at;
+  }
   uint32_t low = 0, high = (uint32_t)vocab - 1;
   while (low < high) {
     const int shift = shift_of<N>(high - low);
@@ -623,7 +658,7 @@ __device__ __forceinline__ float uniform_of(const SampleArgs &p, int r) { return
 template <typename T, int N>
 __device__ __forceinline__ void finish(const SampleArgs &p, const Setting &setting, int r, const RowReader<T> &reader, float most, bool binned, bool fits, Shared<N> &s) {
   const Weights weights(setting, most);
-  const ListReader listed = {s.keys, s.indices, (int)s.listed};
+  const ListReader<T> listed = {s.keys, s.indices, (int)s.listed};
   int token;
   float probability = 1.f;
   if (setting.greedy) {

@@ -207,6 +207,39 @@ def test_captured_streams_and_twice_the_same(built_library):
     assert torch.equal(beside, want)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_first_ones_at_any_place(built_library, dtype):
+    """Settings that list few logits of a row: rows that begin and end at any element, their first ones at the edges and in the middle, values of both signs."""
+    for vocab in (1025, 5003, 33001):
+        base = _logits(1, vocab + 40, dtype, seed=vocab)[0][0]
+        for start in range(9):
+            x = base.clone()
+            row = x[16 + start:16 + start + vocab]
+            x[:16 + start] = INF
+            x[16 + start + vocab:] = INF
+            row -= 14  # (all below zero)
+            row[0], row[vocab - 1], row[vocab // 2] = 3.0, 2.5, 2.75
+            for top_k in (1, 3, 20, 128):
+                _check(row[None], torch.tensor([0.93], device="cuda"), 4.0, top_k, 0.99)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("alike", [1, 2, 255, 256, 257, 511, 513, 1500])
+def test_equal_logits_among_others(built_library, dtype, alike):
+    """So many equal ones, far apart in the row, at the place that is drawn; and logits about zero, whose order the signs decide."""
+    vocab = 20000
+    logits = _logits(3, vocab, dtype, seed=alike, spread=0.01)[0].float()
+    at = torch.randperm(vocab, device="cuda", generator=torch.Generator(device="cuda").manual_seed(alike))[:alike]
+    logits[0, at] = 1.5
+    logits[1, at] = -0.0
+    logits[2, at] = 0.0
+    logits = logits.to(dtype)
+    for u in (0.0, 0.3, 0.999):
+        _check(logits, torch.full((3,), u, device="cuda"), 1.0)
+        _check(logits, torch.full((3,), u, device="cuda"), 0.05, 0, 0.9)
+        _check(logits, torch.full((3,), u, device="cuda"), 1.0, max(1, alike // 2))
+
+
 def test_frequencies_are_the_probabilities(built_library):
     """A number for each of n equal parts of [0, 1): a token of probability p is drawn n p times, give or take one (its run has two ends)."""
     n, vocab = 4096, 37
