@@ -889,9 +889,13 @@ hipError_t launch(const SampleArgs &a, hipStream_t stream) {
     else hipLaunchKernelGGL((sample_tokens_kernel<T, kThreads>), dim3(a.rows), dim3(kThreads), 0, stream, a);
   } else {
     const dim3 grid(a.parts, a.rows);
+    // (settings that the host knows may say that no row has bins: 64 rows of 131072, top_k of 50 23.5 -> 20.3 us)
+    const bool no_bins = (!a.top_k && a.top_k_all > 0 && a.top_k_all <= kMostTopK) || (!a.temperature && !(a.temperature_all > 0.f));
     hipLaunchKernelGGL((sample_first_kernel<T>), grid, dim3(kThreads), 0, stream, a);
-    hipLaunchKernelGGL((sample_bins_kernel<T>), grid, dim3(kThreads), 0, stream, a);
-    hipLaunchKernelGGL((sample_ends_kernel<T>), grid, dim3(kThreads), 0, stream, a);
+    if (!no_bins) {
+      hipLaunchKernelGGL((sample_bins_kernel<T>), grid, dim3(kThreads), 0, stream, a);
+      hipLaunchKernelGGL((sample_ends_kernel<T>), grid, dim3(kThreads), 0, stream, a);
+    }
     hipLaunchKernelGGL((sample_draw_kernel<T>), dim3(a.rows), dim3(kThreads), 0, stream, a);
   }
   return hipGetLastError();
