@@ -131,6 +131,21 @@ def test_more_tiles_than_places_and_long_rows(built_library, groups, heads, kv, 
     assert (got.float() - want.float()).abs().max() < 0.02
 
 
+@pytest.mark.parametrize("rows,n,heads,kv", [(1024, 128, 32, 1), (1024, 1, 4096, 512), (3, 32768, 32, 4)])
+def test_the_largest_sizes(built_library, rows, n, heads, kv):
+    """As many queries and heads as a plan is for, of many rows and of few."""
+    page, d = 32, 32
+    groups = [(130, [n + 1 + (7 * i) % 50 for i in range(rows // 2)]), (64, [n + 3 + (5 * i) % 70 for i in range(rows - rows // 2)])]
+    table, lengths, pages = _tables(groups, page)
+    pool = _pool(pages, kv, page, d, torch.int8, 1)
+    q = _randn((rows, n, heads, d), 2).half()
+    plan = sspmm_amd.plan_prefixes(table, lengths, n, heads, kv, page)
+    assert rows <= int(plan.data[0]) <= (plan.data.numel() - 4 - 12 * rows) // 12
+    got = sspmm_amd.prefix_attention(q, table, plan, *pool)
+    want = sspmm_amd.cache_attention(q, table, lengths, *pool)
+    assert (got.float() - want.float()).abs().max() < 0.02
+
+
 def test_what_a_plan_shares(built_library):
     page, rows = 32, 6
     table = _ints([[1, 2, 3, 4, 5], [1, 2, 3, 9, 8], [1, 2, 3, 4, 7], [1, 10, 11, 12, 13], [20, 21, -1, -1, -1], [-1, 2, 3, 4, 5]])
