@@ -336,7 +336,9 @@ Shape shape_of(int sequences, int tokens, int key_tokens, int heads, int kv_head
   const double theirs = (double)keys * (d == 128 ? 18e-3 : d == 64 ? 11e-3 : 8e-3) *
                         max(1.0, (double)live * ((tokens + live * 128 - 1) / (live * 128)) * heads / 256);
   const double ours = (double)wide * keys * d * 4 / 4.8e6 + (s.splits > 1 ? 4 : 0);
-  if (theirs < ours || s.tiles * kv_heads * max(s.splits, 32) >= 1 << 23) s.row_tiles = 0;  // (a launch has less than 2^32 threads)
+  // (32768 tokens on 20 states each, 16 heads on 8 of 64: 1237 us, by the prompts' kernel 3166)
+  const long long blocks = s.tiles * kv_heads * (s.splits > 8 ? max(s.splits, 16 * s.row_tiles) : s.splits);  // of the larger launch
+  if (theirs < ours || blocks >= 1 << 23) s.row_tiles = 0;  // (a launch has less than 2^32 threads)
   return s;
 }
 

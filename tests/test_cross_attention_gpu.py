@@ -76,6 +76,23 @@ def test_thousands_of_single_tokens(built_library):
             check(got[row:row + 1, h], want, off, "sequence %d" % i)
 
 
+@pytest.mark.parametrize("n", [33000, 300000])
+def test_more_sequences_than_a_batch(built_library, n):
+    """One token each, of tens and hundreds of thousands of sequences with up to four states."""
+    heads, kv, d = 16, 8, 32
+    sources = torch.arange(n, device="cuda") % 5
+    offsets, source_offsets = torch.arange(n + 1, dtype=torch.int32, device="cuda"), torch.cat([sources.new_zeros(1), sources.cumsum(0)]).int()
+    q = _randn((n, heads, d), 1, torch.float16)
+    kvs = _randn((int(source_offsets[-1]), 2, kv, d), 2, torch.float16)
+    got = sspmm_amd.cross_attention(q, kvs[:, 0], kvs[:, 1], offsets, source_offsets)
+    assert not got[sources == 0].any()
+    for i in list(range(0, n, n // 40)) + list(range(n - 6, n)):
+        at, m = int(source_offsets[i]), int(sources[i])
+        for h in range(heads) if m else ():
+            want, off = attention(q[i:i + 1, h], kvs[at:at + m, 0, h // 2], kvs[at:at + m, 1, h // 2], torch.tensor([m], device="cuda"), d ** -0.5, q.dtype, q.dtype)
+            check(got[i:i + 1, h], want, off, "sequence %d" % i)
+
+
 @pytest.mark.parametrize("scaling", [1e-3, 0.125, 3.0, 100.0])
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("lengths,sources", [([1, 3], [300, 77]), ([150, 20], [300, 77])])
