@@ -326,8 +326,14 @@ __device__ __forceinline__ Place locate(const Reader &reader, const Weights &wei
   place.before_bin = s.before_weight;
   place.before_inside = 0;
   u64 in_all = s.bins.inside[place.bin];
-  inside = by_count ? 0
-                    : min(max((u64)ceil((double)(amount - place.before_bin) / weights.share(place.bin)), (u64)1), place.bin == kept.bin ? min(kept.inside, in_all) : in_all);
+  if (by_count) {
+    inside = 0;
+  } else {
+    // (units of the largest's weight are the first bin's own: as they are, since 53 bits lose the one that u times equal weights is to be exceeded by)
+    const u64 rest = amount - place.before_bin;
+    inside = place.bin == 0 ? rest : max((u64)ceil((double)rest / weights.share(place.bin)), (u64)1);
+    inside = min(inside, place.bin == kept.bin ? min(kept.inside, in_all) : in_all);
+  }
   uint32_t low = 0xffffffffu, high = 0, count = 0;
   const float from = weights.lowest(place.bin), to = weights.highest(place.bin);
   reader.template each<2>([&](float x, int, int) {
