@@ -157,47 +157,54 @@ __device__ __forceinline__ int shift_of(uint32_t span) {
   return max(0, 32 - __builtin_ctz(N) - (int)__builtin_clz(span));
 }
 
-// A row in memory, or a part of it.
+// A row in memory, or one of the parts that its lines of 128 bytes are dealt to in turn: tokens that are likely often stand side by side, a vocabulary's first ones for
+// instance, and a part that had them all would list too few of them (64 rows of 131072 whose first tokens are likely, top_k of 100: 20.7 us, by parts of one stretch each 114).
 template <typename T>
 struct RowReader {
   typedef Elements<T> E;
   static constexpr int kGrain = E::kGrain;
+  static constexpr int kLine = 8;  // blocks of 16 bytes of a line
+  static constexpr int kLineLogits = kLine * E::kCount;
   const unsigned char *row;  // aligned to an element
-  int first, end;            // whole blocks of 16 aligned bytes in it, counted from the one that holds its first element
-  int lead, from, to;        // elements in front of the row in that block; the part's elements
-  // the part of a row in the blocks first_block .. end_block - 1 as they are counted here
-  __device__ __forceinline__ RowReader(const void *row_, int vocab, int first_block, int end_block) {
+  int vocab, lead;           // elements; those in front of the row in the line that holds its first one, from where on blocks are counted
+  int first, end;            // of the part's blocks, counted as if they lay side by side, those that lie whole in the row
+  int part, parts;
+  __device__ __forceinline__ RowReader(const void *row_, int vocab_, int part_, int parts_) {
     row = static_cast<const unsigned char *>(row_);
-    lead = (int)(reinterpret_cast<uintptr_t>(row_) & 15) / E::kBytes;
-    from = max(0, first_block * E::kCount - lead);
-    to = min((long long)vocab, (long long)end_block * E::kCount - lead);
-    first = (from + lead + E::kCount - 1) / E::kCount;
-    end = max(first, (to + lead) / E::kCount);
+    vocab = vocab_;
+    part = part_;
+    parts = parts_;
+    lead = (int)(reinterpret_cast<uintptr_t>(row_) & (16 * kLine - 1)) / E::kBytes;
+    const int whole = (int)(((long long)vocab + lead) / E::kCount), lines = whole / kLine;
+    first = part == 0 ? (lead + E::kCount - 1) / E::kCount : 0;  // (a line's at most)
+    end = max(first, (lines - part + parts - 1) / parts * kLine + (lines % parts == part ? whole % kLine : 0));
   }
-  static __device__ __forceinline__ int blocks(const void *row, int vocab) {
-    return ((int)(reinterpret_cast<uintptr_t>(row) & 15) / E::kBytes + vocab + E::kCount - 1) / E::kCount;
-  }
+  // Where the part's block number i lies.
+  __device__ __forceinline__ int place(int i) const { return parts == 1 ? i : (i / kLine * parts + part) * kLine + i % kLine; }
   __device__ __forceinline__ float one(int i) const { return E::one(row + (long long)i * E::kBytes); }
-  // f(logit, index, place in its block) of a block's elements
+  // f(logit, index, place in its block) of the elements of the part's block number i
   template <typename F>
-  __device__ __forceinline__ void block(int b, const F &f) const {
+  __device__ __forceinline__ void block(int i, const F &f) const {
+    const int b = place(i);
     float x[E::kCount];
     E::take(*reinterpret_cast<const uintx4 *>(row - lead * E::kBytes + (long long)b * 16), x);
 #pragma unroll
-    for (int i = 0; i < E::kCount; ++i) f(x[i], b * E::kCount - lead + i, i);
+    for (int j = 0; j < E::kCount; ++j) f(x[j], b * E::kCount - lead + j, j);
   }
-  // of what lies in front of the whole blocks and behind them, an element a thread
+  // of what lies in front of the row's whole blocks and behind them, an element a thread: the first part's
   template <typename F>
   __device__ __forceinline__ void edge(const F &f) const {
-    const int tid = threadIdx.x, head_end = min(to, first * E::kCount - lead), tail = max(head_end, end * E::kCount - lead);
-    const int i = from + tid < head_end ? from + tid : tail + tid - (head_end - from);
-    if (i < head_end || (i >= tail && i < to)) f(one(i), i, 0);
+    if (part != 0) return;
+    const int blocks = (lead + E::kCount - 1) / E::kCount, whole = (int)(((long long)vocab + lead) / E::kCount);
+    const int tid = threadIdx.x, head_end = min(vocab, blocks * E::kCount - lead), tail = max(head_end, whole * E::kCount - lead);
+    const int i = tid < head_end ? tid : tail + tid - head_end;
+    if (i < vocab) f(one(i), i, 0);
   }
   // and of every element, in any order
   template <int UNROLL = 1, typename F>
   __device__ __forceinline__ void each(const F &f) const {
 #pragma unroll UNROLL
-    for (int b = first + (int)threadIdx.x; b < end; b += (int)blockDim.x) block(b, f);
+    for (int i = first + (int)threadIdx.x; i < end; i += (int)blockDim.x) block(i, f);
     edge(f);
   }
 };
@@ -563,7 +570,9 @@ template <typename T, int N>
 __device__ __forceinline__ uint32_t list_first(const RowReader<T> &reader, uint32_t wanted, float &largest, Shared<N> &s) {
   const int tid = threadIdx.x;
   constexpr int kPairs = 2;  // (the largest and the one behind it, of the even and of the odd places of all blocks)
-  const bool one = wanted <= N / 4;
+  // (where first ones stand side by side, a list has all logits of as many blocks, and the parts' lists have to fit one: 8 parts of a sorted row, 16 bits, top_k of 200 34 us, more than fit 288;
+  // in any order, top_k of 300, 22.6 and, with four a thread, 26.1)
+  const bool one = wanted <= min(N / 4, (kList - kFewAlike) / (RowReader<T>::E::kCount * reader.parts));
   float large[2 * kPairs];
 #pragma unroll
   for (float &x : large) x = -INFINITY;
@@ -635,8 +644,8 @@ __device__ __forceinline__ uint32_t list_first(const RowReader<T> &reader, uint3
   if (few) {
     const int threads = (int)s.high, blocks = (reader.end - reader.first + N - 1) / N * threads;
     for (int j = tid; j < blocks; j += N) {
-      const int b = reader.first + (int)s.fine_counts[j % threads] + N * (j / threads);
-      if (b < reader.end) reader.block(b, take);
+      const int i = reader.first + (int)s.fine_counts[j % threads] + N * (j / threads);
+      if (i < reader.end) reader.block(i, take);
     }
     reader.edge(take);
   } else {
@@ -687,7 +696,7 @@ __global__ __launch_bounds__(N, 4) void sample_tokens_kernel(const SampleArgs p)
   __shared__ Shared<N> s;
   const int r = blockIdx.x;
   const unsigned char *const row = row_at<T>(p, r);
-  const RowReader<T> reader(row, p.vocab, 0, RowReader<T>::blocks(row, p.vocab));
+  const RowReader<T> reader(row, p.vocab, 0, 1);
   const Setting setting(p, r);
   float most;
   if (setting.few()) list_first(reader, (uint32_t)setting.top_k, most, s);
@@ -731,14 +740,11 @@ struct Between {
 
 template <typename T>
 __device__ __forceinline__ RowReader<T> part_of(const SampleArgs &p, int r, int part) {
-  const unsigned char *const row = row_at<T>(p, r);
-  const long long blocks = RowReader<T>::blocks(row, p.vocab);
-  return RowReader<T>(row, p.vocab, (int)(blocks * part / p.parts), (int)(blocks * (part + 1) / p.parts));
+  return RowReader<T>(row_at<T>(p, r), p.vocab, part, p.parts);
 }
 template <typename T>
 __device__ __forceinline__ RowReader<T> all_of(const SampleArgs &p, int r) {
-  const unsigned char *const row = row_at<T>(p, r);
-  return RowReader<T>(row, p.vocab, 0, RowReader<T>::blocks(row, p.vocab));
+  return RowReader<T>(row_at<T>(p, r), p.vocab, 0, 1);
 }
 // (a lane a part)
 __device__ __forceinline__ Part part_here(const SampleArgs &p, const Part *parts) {
@@ -816,8 +822,9 @@ __global__ __launch_bounds__(kThreads, 4) void sample_first_kernel(const SampleA
   const long long at = (long long)r * p.parts + part;
   Part mine = {-INFINITY, 0, 0};
   if (setting.few()) {
-    // (half as many again as a part's share, and some, of logits in any order)
-    mine.from = list_first(reader, (uint32_t)min(setting.top_k, 3 * setting.top_k / (2 * p.parts) + 48), mine.most, s);
+    // (its share and a line, which no part exceeds of first ones that stand side by side; half as many again, and some, of logits in any order)
+    const int share = max((setting.top_k + p.parts - 1) / p.parts + RowReader<T>::kLineLogits, 3 * setting.top_k / (2 * p.parts) + 48);
+    mine.from = list_first(reader, (uint32_t)min(setting.top_k, share), mine.most, s);
     mine.count = s.listed;
     leave_list(b, at, s);
   } else {

@@ -181,3 +181,34 @@ def test_captured_streams_and_twice_the_same(built_library):
     torch.cuda.synchronize()
     for i, out in enumerate(got):
         assert torch.equal(out[0], want[i % 2][0]) and torch.equal(out[1], want[i % 2][1])
+
+
+@pytest.mark.parametrize("order", ["likely ones first", "sorted"])
+@pytest.mark.parametrize("top_k", [100, 200, 1000])
+def test_likely_tokens_side_by_side_take_no_longer(built_library, top_k, order):
+    """The parts' lists suffice, wherever a row's first tokens lie: in less than twice the time of the same logits in any order (the whole row by one workgroup takes five
+    times as long and more)."""
+    rows, vocab, calls = 64, 131072, 20
+    x, uniform = _logits(rows, vocab, torch.float32, seed=top_k, spread=2.0)
+    x = x.sort(1, descending=True).values if order == "sorted" else x - 0.8 * torch.log(1.0 + torch.arange(vocab, device="cuda"))
+    anywhere = x[:, torch.randperm(vocab, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")]
+    graphs, times = [], ([], [])
+    for logits in (x.bfloat16(), anywhere.bfloat16()):
+        _check(logits[:2], uniform[:2], 0.8, top_k)
+        logits = logits.contiguous()
+        sspmm_amd.sample_tokens(logits, uniform, 0.8, top_k)
+        torch.cuda.synchronize()
+        graphs.append((torch.cuda.CUDAGraph(), logits))
+        with torch.cuda.graph(graphs[-1][0]):
+            for _ in range(calls):
+                sspmm_amd.sample_tokens(logits, uniform, 0.8, top_k)
+    for turn in range(9):
+        for (graph, _), took in zip(graphs, times):
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            begin.record()
+            graph.replay()
+            end.record()
+            end.synchronize()
+            took.append(begin.elapsed_time(end) * 1e3 / calls)
+    first, other = (sorted(took)[len(took) // 2] for took in times)
+    assert first < 2 * other, "%.1f us, in any order %.1f" % (first, other)
