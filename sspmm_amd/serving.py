@@ -350,11 +350,11 @@ def plan_prefixes(page_table, lengths, queries, heads, kv_heads, page_size, plan
     if plan is None:
         plan = PrefixPlan(rows, slots, queries, heads, kv_heads, page_size, page_table.new_empty(size >> 2))
     elif ((plan.rows, plan.slots, plan.queries, plan.heads, plan.kv_heads, plan.page_size) != (rows, slots, queries, heads, kv_heads, page_size) or
-          plan.data.get_device() != device):
+          not _listed(plan.data, 1, device) or 4 * plan.data.numel() < size):
         raise ValueError("plan is of other sizes, or on another GPU")
     if rows and queries:
         rc = _lib.call(_lib.lib().sspmm_plan_prefixes, page_table.device, page_table.data_ptr(), rows, slots, lengths.data_ptr(), page_size, queries, heads, kv_heads,
-                       plan.data.data_ptr(), size)
+                       plan.data.data_ptr(), 4 * plan.data.numel())
         if rc:
             _lib.check(rc, "sspmm_plan_prefixes")
     return plan
@@ -375,8 +375,8 @@ def prefix_attention(q, page_table, plan, keys, values, scales, scaling=None, ou
     _heads(heads, kv, d)
     if not _listed(page_table, 2, device):
         _ints("page_table", page_table, 2, device)
-    if plan.data.get_device() != device:
-        raise TypeError("plan must be on the other arguments' GPU")
+    if not _listed(plan.data, 1, device):
+        _ints("plan's data", plan.data, 1, device)
     slots = page_table.size(1)
     if (plan.rows, plan.slots, plan.queries, plan.heads, plan.kv_heads, plan.page_size) != (rows, slots, n, heads, kv, page_size) or page_table.size(0) != rows:
         raise ValueError("plan is for %d rows of %d slots, %d queries, %d heads on %d, pages of %d" %
