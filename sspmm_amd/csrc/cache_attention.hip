@@ -99,7 +99,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_attention_kernel(const C
   float run_max[TILES], run_sum[TILES];
 #pragma unroll
   for (int t = 0; t < TILES; ++t) {
-    run_max[t] = -3.0e38f;
+    run_max[t] = kLowest;
     run_sum[t] = 0.f;
 #pragma unroll
     for (int part = 0; part < kParts; ++part) o[t][part] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -317,7 +317,7 @@ __global__ __launch_bounds__(256) void cache_attention_join_kernel(const CacheAt
   const float *const own = base + (long long)kRows * D + r;
   // (a split a thread: there are no more than 256)
   const bool mine = tid < p.splits;
-  const float max_here = mine ? own[tid * pitch] : -3.0e38f, sum_here = mine ? own[tid * pitch + kRows] : 0.f;
+  const float max_here = mine ? own[tid * pitch] : kLowest, sum_here = mine ? own[tid * pitch + kRows] : 0.f;
   float most = wave_max_all(max_here);
   if ((tid & 63) == 0) largest[tid >> 6] = most;
   __syncthreads();

@@ -99,7 +99,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cross_step_kernel(const Prompt
     constexpr bool again = decltype(again_)::value;
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
-      run_max[t] = -3.0e38f;
+      run_max[t] = kLowest;
       run_sum[t] = 0.f;
 #pragma unroll
       for (int part = 0; part < kParts; ++part) o[t][part] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -259,7 +259,7 @@ __global__ __launch_bounds__(256) void cross_join_kernel(const PromptArgs p, int
   for (int at = threadIdx.x; at < kRows * D / 4; at += 256) {
     const int r = at / (D / 4), d = (at % (D / 4)) * 4, row = tile.row0 + r;
     if (row >= tile.rows) return;
-    float most = -3.0e38f, total = 0.f;
+    float most = kLowest, total = 0.f;
     floatx4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int s = 0; s < splits; ++s) {
@@ -291,7 +291,7 @@ __global__ __launch_bounds__(256) void cross_join_many_kernel(const PromptArgs p
   const float *const from = partial + ((long long)number * p.kv_heads + head) * splits * state_floats(kRows, D);
   const int tid = threadIdx.x, lane = tid & 63, set = tid / (D / 4), d = (tid % (D / 4)) * 4;
   const float *const own = from + (long long)lane * state_floats(kRows, D) + (long long)kRows * D + r;
-  const float max_here = lane < splits ? own[0] : -3.0e38f, sum_here = lane < splits ? own[kRows] : 0.f;
+  const float max_here = lane < splits ? own[0] : kLowest, sum_here = lane < splits ? own[kRows] : 0.f;
   const float down = half_way_down((wave_max_all(max_here) - max_here) * p.scale_log2e);
   const float total = wave_sum_all(sum_here * down * down);
   if (tid < splits) weights[tid] = down;

@@ -139,6 +139,9 @@ __device__ __forceinline__ float sum_over_rows(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// Where a running maximum of scores begins: no finite score is below it, and -infinity stays apart.
+constexpr float kLowest = -0x1.fffffep127f;
+
 // The factor that, taken twice, brings a sum of exponentials or of what they weigh to a reference point x >= 0 powers of two above its own.  (One factor
 // ends at 2^-126, and 2^-126 of a value near the end of the range is a number like any other.  At 2^-252 nothing is left of it, and what is infinite stays so.)
 __device__ __forceinline__ float half_way_down(float x) { return __builtin_amdgcn_exp2f(-0.5f * fminf(x, 252.0f)); }

@@ -350,7 +350,7 @@ struct CacheRows {
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
-      run_max[t] = -3.0e38f;
+      run_max[t] = kLowest;
       run_sum[t] = 0.f;
 #pragma unroll
       for (int part = 0; part < kParts; ++part) o[t][part] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -622,7 +622,7 @@ __global__ __launch_bounds__(256) void prefix_attention_join_kernel(const Prefix
   const long long own_at = (long long)row.own_states + own_first * row.own_jobs + r % kRows;
   const int states = row.shared_jobs + row.own_jobs;
   const auto place = [&](int s) { return s < row.shared_jobs ? shared_at + (long long)s * shared_step : own_at + (long long)(s - row.shared_jobs) * own_step; };
-  float most = -3.0e38f;
+  float most = kLowest;
   for (int s = tid; s < states; s += 256) most = fmaxf(most, sums[2 * place(s)]);
   most = wave_max_all(most);
   if ((tid & 63) == 0) largest[tid >> 6] = most;

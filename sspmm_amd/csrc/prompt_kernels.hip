@@ -199,7 +199,7 @@ __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void prompt_attention_kern
     for (int part = 0; part < kParts; ++part)
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[part][i] = 0.f;
-    run_max = -3.0e38f;
+    run_max = kLowest;
     run_sum = 0.f;
   };
   const auto move_by = [&](float grown) __attribute__((always_inline)) {  // the reference point, by so many powers of two

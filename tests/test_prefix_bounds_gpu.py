@@ -101,3 +101,19 @@ def test_every_page_once_at_the_largest_sizes(built_library, rows, n, heads, kv)
         for h in range(0, heads, max(1, heads // 5)):
             want, off = attention(q[b, at, h], k[:, h // (heads // kv)], v[:, h // (heads // kv)], length - n + 1 + at, d ** -0.5, torch.float16, q.dtype)
             check(got[b, at, h], want, off, "row %d of %d, head %d" % (b, length, h))
+
+
+@pytest.mark.parametrize("form", FORMATS)
+def test_equal_scores_near_the_lowest(built_library, form):
+    """-104 * 2^121 * 0.8 log2(e), about -3.19e38, for every position: finite and equal, each has the same share."""
+    page, d, heads, kv = 32, 32, 2, 1
+    table, lengths = _ints([[1, 2, 3, 4], [1, 2, 5, -1], [6, 7, 8, 0]]), _ints([100, 70, 128])
+    keys, values, scales = sspmm_amd.new_cache(9, kv, page, d, form)
+    keys[..., 0] = -104
+    values.fill_(52)
+    scales[:, 0], scales[:, 1] = 2.0 ** 121, 0.25
+    q = torch.zeros(3, 1, heads, d, dtype=torch.float16, device="cuda")
+    q[..., 0] = 1.0
+    plan = sspmm_amd.plan_prefixes(table, lengths, 1, heads, kv, page)
+    for got in (sspmm_amd.prefix_attention(q, table, plan, keys, values, scales, scaling=0.8), sspmm_amd.cache_attention(q, table, lengths, keys, values, scales, scaling=0.8)):
+        assert (got == 13).all()
