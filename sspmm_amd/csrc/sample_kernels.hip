@@ -133,6 +133,12 @@ struct Weights {
   }
 };
 
+// A logit that none which weighs something beside the largest is below: z of the last bin but one ends at (kBins - 3/2) / (16 log2(e)), 44.3.
+__device__ __forceinline__ float least_of(const Setting &s, float largest) {
+  const float x = fmaf(-44.4f, s.temperature, largest);
+  return s.greedy ? largest : largest == INFINITY ? -INFINITY : x - fmaf(fabsf(x), 0x1p-20f, 1e-44f);
+}
+
 struct Bins {
   u64 inside[kBins];   // units of the bin
   u64 weights[kBins];  // units of the largest, of this bin and those before
@@ -564,10 +570,11 @@ __device__ __forceinline__ float largest_of(const Reader &reader, Shared<N> &s) 
   return most;
 }
 
-// The first `wanted` of the reader's logits, and others, onto the list: those that reach a logit which so many of the threads' largest reach.  Its number, or
-// 0 where the list has all.  Ends with a barrier.
+// The first `wanted` of the reader's logits, and others, onto the list: those that reach a logit which so many of the threads' largest reach, but for what weighs nothing beside
+// the largest (tokens ruled out by a low number instead of -infinity would fill it: 64 rows of 131072 with some 20 others, top_k of 50 23 us instead of 146; with -infinity 17).  Its number, or
+// 0 where the list has all that weighs something.  Ends with a barrier.
 template <typename T, int N>
-__device__ __forceinline__ uint32_t list_first(const RowReader<T> &reader, uint32_t wanted, float &largest, Shared<N> &s) {
+__device__ __forceinline__ uint32_t list_first(const RowReader<T> &reader, const Setting &setting, uint32_t wanted, float &largest, Shared<N> &s) {
   const int tid = threadIdx.x;
   constexpr int kPairs = 2;  // (the largest and the one behind it, of the even and of the odd places of all blocks)
   // (where first ones stand side by side, a list has all logits of as many blocks, and the parts' lists have to fit one: 8 parts of a sorted row, 16 bits, top_k of 200 34 us, more than fit 288;
@@ -628,8 +635,9 @@ __device__ __forceinline__ uint32_t list_first(const RowReader<T> &reader, uint3
       if (x > -INFINITY && bin(x) <= last) atomicMin(&s.low, key_of(x));
   }
   __syncthreads();
-  const uint32_t from = last < N ? s.low : 0;
-  const float reaches = last < N ? logit_of(from) : -INFINITY;
+  const float reached = last < N ? logit_of(s.low) : -INFINITY, weighs = least_of(setting, top);
+  const uint32_t from = last < N && reached >= weighs ? s.low : 0;
+  const float reaches = fmaxf(reached, weighs);
   const auto take = [&](float x, int i, int) {
     if (x >= reaches && x > -INFINITY) list(x, i, s);
   };
@@ -699,7 +707,7 @@ __global__ __launch_bounds__(N, 4) void sample_tokens_kernel(const SampleArgs p)
   const RowReader<T> reader(row, p.vocab, 0, 1);
   const Setting setting(p, r);
   float most;
-  if (setting.few()) list_first(reader, (uint32_t)setting.top_k, most, s);
+  if (setting.few()) list_first(reader, setting, (uint32_t)setting.top_k, most, s);
   else most = largest_of(reader, s);
   if (most == -INFINITY) {  // (nothing may be drawn)
     result(p, r, -1, 0.f);
@@ -762,12 +770,14 @@ __device__ __forceinline__ void leave_list(const Between &b, long long at, const
     b.indices[at * kList + i] = s.indices[i];
   }
 }
-// The parts' lists as one in s, but for logits that some part's list does not hold; false if some part's, or all together, are too many, or fewer than `wanted`.  Ends with a barrier.
+// The parts' lists as one in s, but for logits that some part's list does not hold, and parts whose largest is below `least`; false if some part's, or all together, are too many, or
+// fewer than `wanted`.  Ends with a barrier.
 template <int N>
-__device__ __forceinline__ bool take_lists(const SampleArgs &p, const Between &b, int r, uint32_t wanted, Shared<N> &s) {
+__device__ __forceinline__ bool take_lists(const SampleArgs &p, const Between &b, int r, uint32_t wanted, float least, Shared<N> &s) {
   if (threadIdx.x == 0) s.listed = 0;
   __syncthreads();
-  const Part mine = part_here(p, b.parts + (long long)r * p.parts);
+  Part mine = part_here(p, b.parts + (long long)r * p.parts);
+  if (mine.most < least) mine = {mine.most, 0, 0};
   const uint32_t from = from_last_lane(wave_inclusive_max(mine.from));
   bool fits = from_last_lane(wave_inclusive_max(mine.count)) <= (uint32_t)kList;
   const uint32_t behind = wave_inclusive_sum(min(mine.count, (uint32_t)kList)), all = from_last_lane(behind);
@@ -824,7 +834,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_first_kernel(const SampleA
   if (setting.few()) {
     // (its share and a line, which no part exceeds of first ones that stand side by side; half as many again, and some, of logits in any order)
     const int share = max((setting.top_k + p.parts - 1) / p.parts + RowReader<T>::kLineLogits, 3 * setting.top_k / (2 * p.parts) + 48);
-    mine.from = list_first(reader, (uint32_t)min(setting.top_k, share), mine.most, s);
+    mine.from = list_first(reader, setting, (uint32_t)min(setting.top_k, share), mine.most, s);
     mine.count = s.listed;
     leave_list(b, at, s);
   } else {
@@ -881,7 +891,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
     return;
   }
   if (!setting.few()) take_bins(p, b, r, Weights(setting, most), setting.top_k > 0, s);
-  const bool fits = take_lists(p, b, r, (uint32_t)setting.top_k, s);
+  const bool fits = take_lists(p, b, r, (uint32_t)setting.top_k, setting.few() ? least_of(setting, most) : -INFINITY, s);
   finish(p, setting, r, all_of<T>(p, r), most, !setting.few(), fits, s);
 }
 

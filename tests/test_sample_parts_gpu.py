@@ -183,32 +183,59 @@ def test_captured_streams_and_twice_the_same(built_library):
         assert torch.equal(out[0], want[i % 2][0]) and torch.equal(out[1], want[i % 2][1])
 
 
-@pytest.mark.parametrize("order", ["likely ones first", "sorted"])
-@pytest.mark.parametrize("top_k", [100, 200, 1000])
-def test_likely_tokens_side_by_side_take_no_longer(built_library, top_k, order):
-    """The parts' lists suffice, wherever a row's first tokens lie: in less than twice the time of the same logits in any order (the whole row by one workgroup takes five
-    times as long and more)."""
-    rows, vocab, calls = 64, 131072, 20
-    x, uniform = _logits(rows, vocab, torch.float32, seed=top_k, spread=2.0)
-    x = x.sort(1, descending=True).values if order == "sorted" else x - 0.8 * torch.log(1.0 + torch.arange(vocab, device="cuda"))
-    anywhere = x[:, torch.randperm(vocab, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")]
-    graphs, times = [], ([], [])
-    for logits in (x.bfloat16(), anywhere.bfloat16()):
-        _check(logits[:2], uniform[:2], 0.8, top_k)
-        logits = logits.contiguous()
-        sspmm_amd.sample_tokens(logits, uniform, 0.8, top_k)
+def _in_turn(*calls):
+    """us of each call: medians of captured runs of 20, timed in turn."""
+    graphs, times = [], [[] for _ in calls]
+    for call in calls:
+        call()
         torch.cuda.synchronize()
-        graphs.append((torch.cuda.CUDAGraph(), logits))
-        with torch.cuda.graph(graphs[-1][0]):
-            for _ in range(calls):
-                sspmm_amd.sample_tokens(logits, uniform, 0.8, top_k)
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            for _ in range(20):
+                call()
     for turn in range(9):
-        for (graph, _), took in zip(graphs, times):
+        for graph, took in zip(graphs, times):
             begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
             begin.record()
             graph.replay()
             end.record()
             end.synchronize()
-            took.append(begin.elapsed_time(end) * 1e3 / calls)
-    first, other = (sorted(took)[len(took) // 2] for took in times)
+            took.append(begin.elapsed_time(end) * 1e3 / 20)
+    return [sorted(took)[len(took) // 2] for took in times]
+
+
+@pytest.mark.parametrize("order", ["likely ones first", "sorted"])
+@pytest.mark.parametrize("top_k", [100, 200, 1000])
+def test_likely_tokens_side_by_side_take_no_longer(built_library, top_k, order):
+    """The parts' lists suffice, wherever a row's first tokens lie: in less than twice the time of the same logits in any order (the whole row by one workgroup takes five
+    times as long and more)."""
+    rows, vocab = 64, 131072
+    x, uniform = _logits(rows, vocab, torch.float32, seed=top_k, spread=2.0)
+    x = x.sort(1, descending=True).values if order == "sorted" else x - 0.8 * torch.log(1.0 + torch.arange(vocab, device="cuda"))
+    anywhere = x[:, torch.randperm(vocab, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")]
+    x, anywhere = x.bfloat16(), anywhere.bfloat16().contiguous()
+    for logits in (x, anywhere):
+        _check(logits[:2], uniform[:2], 0.8, top_k)
+    first, other = _in_turn(lambda: sspmm_amd.sample_tokens(x, uniform, 0.8, top_k), lambda: sspmm_amd.sample_tokens(anywhere, uniform, 0.8, top_k))
     assert first < 2 * other, "%.1f us, in any order %.1f" % (first, other)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab", [(40, 20000), (12, 131072)])
+def test_tokens_ruled_out_by_a_low_number(built_library, rows, vocab, dtype):
+    """Few tokens are left, fewer than top_k, and the others have the type's lowest value, or one that is far enough below: as if it were -infinity, also in its time (with lists that overflow eight
+    times as long)."""
+    logits, uniform = _logits(rows, vocab, dtype, seed=vocab)
+    out = torch.rand(rows, vocab, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda") >= 20 / vocab
+    out[:, 7] = False
+    never = logits.masked_fill(out, -INF)
+    for low in (torch.finfo(dtype).min, -1e4):
+        lowest = logits.masked_fill(out, low)
+        for settings in ((0.8, 10, 1.0, 0.0), (0.8, 50, 0.9, 0.0), (0.8, 1000, 1.0, 0.01), (0.0, 0, 1.0, 0.0), (0.8, 0, 1.0, 0.0)):
+            _check(lowest, uniform, *settings)
+            assert torch.equal(sspmm_amd.sample_tokens(lowest, uniform, *settings), sspmm_amd.sample_tokens(never, uniform, *settings))
+        for temperature in (1e4, 1e38):  # (where they count again)
+            _check(lowest, uniform, temperature, 50)
+        for top_k in (10, 50, 1000) if _in_parts(lowest) else ():
+            took, other = _in_turn(lambda: sspmm_amd.sample_tokens(lowest, uniform, 0.8, top_k), lambda: sspmm_amd.sample_tokens(never, uniform, 0.8, top_k))
+            assert took < 4 * other, "top_k %d: %.1f us, with -infinity %.1f" % (top_k, took, other)
