@@ -655,10 +655,10 @@ int sspmm_prefix_attention(int type, int format, int rows, int queries, int head
  * uniform[i] in [0, 1).  With the weights w = exp((l - max l) / temperature): kept are those with w >= min_p; of these the top_k first in the order of falling
  * logits, equal ones by rising index; of these the shortest run, at least one, whose weights reach top_p of the sum of all of these.  The token is the first in that order
  * at which the running sum of the weights exceeds uniform * their sum.  temperature <= 0 (or NaN): the largest logit's first index; top_k <= 0, top_p >= 1 (or NaN), min_p <= 0
- * (or NaN): everything is kept.  NaN logits are taken as -infinity, which is never drawn; infinite ones share the draw.  A row that is all -infinity gives -1.
+ * (or NaN): everything is kept.  top_p below 0 is taken as 0 and min_p above 1 as 1, which keeps the largest logits; uniform below 0 (or NaN) as 0, of 1 and above as the last number below.  NaN logits are taken as -infinity, which is never drawn; infinite ones share the draw.  A row that is all -infinity gives -1.
  * Weights are whole multiples of 2^-b of the power of 2^(1/16) nearest to them, vocab * 2^b <= 2^62, b <= 50: the result does not depend on the order of the sums.
  * temperature, top_k, top_p, min_p: one value a row, or NULL and the value beside it for all.  probabilities (may be NULL): weight over sum, of the token (0 with -1).
- * vocab 1 .. 2^24.  workspace: sspmm_sample_tokens_workspace_bytes of the same sizes (0 where a workgroup takes a row), 16-byte aligned.
+ * rows below 2^22, vocab 1 .. 2^24.  workspace: sspmm_sample_tokens_workspace_bytes of the same sizes (0 where a workgroup takes a row), 16-byte aligned.
  */
 size_t sspmm_sample_tokens_workspace_bytes(int rows, int vocab);
 int sspmm_sample_tokens(int type, int rows, int vocab, const void *logits, int64_t row_stride, const float *uniform, const float *temperature, float temperature_all,

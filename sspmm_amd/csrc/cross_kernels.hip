@@ -1,7 +1,7 @@
 // Attention of a sequence's few queries, a token's as a rule, over its packed states in 16 bits:
 //   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^((q . k_j - m) scale log2(e)).
-// Bound by the bytes of k and v, each read once for all queries and heads of a group: a token of each of 64 sequences on 50 to 2000 states, 32 heads on 8 of 128, bf16 (276 MB), 58 us, 4.8 TB/s, which is
-// what a large copy reaches.  Four tokens on 40 states or fewer, 4 heads of 64, 4.6 us: the launch and its chain of look-ups.
+// Bound by the bytes of k and v, each read once for all queries and heads of a group: a token of each of 64 sequences on 50 to 2000 states, 32 heads on 8 of 128, bf16 (276 MB), 57 us, 4.8 TB/s, again and
+// again (the last-level cache has a part of it), 70 us, 4.0 TB/s, where nothing is cached.  Four tokens on 40 states or fewer, 4 heads of 64, 4.6 us: the launch and its chain of look-ups.
 #include "prompt_kernels.h"
 
 #include "lane_ops.h"
@@ -50,7 +50,8 @@ template <typename T, int D, int TILES>
 __global__ __launch_bounds__(64 * kWaves, 2) void cross_step_kernel(const PromptArgs p, int splits, float *partial) {
   constexpr int kRows = 16 * TILES, kSteps = D / 32, kParts = D / 16, kPieces = D / 8, kLoads = kUnit * kPieces / 64;
   // fp16 loses what is below 2^-25, and many keys of small probabilities are not nothing: their largest is 2^7 or more there.  bf16 does not, but its v may be as large as
-  // 32 bits hold: probabilities are 2^-16 at most, and 2^16 keys' sum does not overflow (v below 2^-102 loses what is then below 2^-149).
+  // 32 bits hold: probabilities are 2^-16 at most, and 2^16 keys' sum does not overflow (v below 2^-102 loses what is then below 2^-149).  In 16 bits the second product is a matrix
+  // instruction's, as in the package's other attentions; root mean square errors are 1.0 to 1.3 (fp16) and 1.2 to 1.41 (bf16) times those of probabilities in 32 bits.
   constexpr float kHeadroom = __is_same(T, Fp16) ? 7.f : -24.f;
   constexpr int kTileBytes = kUnit * D * 2;
   typedef float Sums[kWaves][kRows][D];
@@ -316,6 +317,7 @@ __global__ __launch_bounds__(256) void cross_join_many_kernel(const PromptArgs p
 // of the mean lengths, which are what the host knows.  us, this kernel and that: 64 sequences of a token on 1500 keys, 32 heads on 8 of 128 features, 78 and 235; 16 of
 // 16 tokens 40 and 64, 8 of 32 33 and 31, 8 of 64 40 and 32; one of 64 on 16000 keys, 16 heads on 2, 36 and 207; two of 100 on 4000, 8 heads of 64, 17 and 40; 8 of 32
 // on 512, 12 heads of 64, 14 and 10; 32 of one 16 and 14.
+// A sequence that is many times longer than the mean has as few shares as the others: a token of each of 64 sequences, one on 65536 states and the others on 100, 798 us (alone 51); on 16000 145 (22).
 // Shares are of 256 keys or more (of 128: four of one token on 8000 keys 46 us instead of 42), as many as fill the 512 places for workgroups, or a few times as many where the last round
 // of them would leave more than a tenth of the places empty.
 struct Shape {

@@ -7,9 +7,9 @@
 //
 // What bounds it: the bytes of the pages, and two launches with a chain of look-ups in each (job, queries, page, keys), some 12 us for a call that reads next to nothing of 128
 // features.  64 rows of 64 to 4000 tokens that share nothing, 32 heads on 8 of 128, int8: 59 us, 4.0 TB/s (cache_attention 52).  64 rows behind 7936 shared tokens, 16 heads on 4, e4m3:
-// 37 (cache_attention 73); 16 rows behind 99968, int8: 45 (182).  In these the first-level caches hand on 127 and 210 MB, every tile its own, at 4 to 5.5 TB/s; loads alone, as many
-// in flight, in these sizes reach that and no more.  Tiles of 32 rows, as two share the codes' way to fp16: more would leave one wave a SIMD; fewer instructions do not help (codes
-// of int8 as subnormal numbers with the offset of 128 taken off by the products, 600 -> 480 vector instructions for 64 keys and 32 rows: 1 to 3 % of the time).
+// 37 (cache_attention 73); 16 rows behind 99968, int8: 43 (182).  In these the first-level caches hand on 127 and 210 MB, every tile its own, at 4 to 5.5 TB/s; loads alone, as many
+// in flight and nothing cached, take 23 us for 100 MB and 39 for 200.  Tiles of 32 rows, as two share the codes' way to fp16: a wave with more would leave one wave a SIMD, while four waves on the
+// same keys, 32 rows each, were not tried; fewer instructions do not help (codes of int8 as subnormal numbers with the offset of 128 taken off by the products, 600 -> 480 vector instructions for 64 keys and 32 rows: 1 to 3 % of the time).
 #include "prefix_kernels.h"
 
 #include "cache_codes.h"
@@ -452,7 +452,8 @@ struct CacheRows {
           for (int i = 0; i < 4; ++i) most = fmaxf(most, s[t][kt][i]);
         most = max_over_rows(most);
         // The reference point moves only when a row's maximum has grown by more than 2^8, and lies 2^7 below it then: fp16 holds 2^15, but loses what is
-        // below 2^-25, and many keys of small probabilities are not nothing.
+        // below 2^-25, and many keys of small probabilities are not nothing.  (fp16 for the matrix instructions, as the codes; root mean square errors are 1.0 to 1.3 times those of
+        // probabilities in 32 bits.)
         const float new_max = fmaxf(run_max[t], most - 7.0f);
         if (__ballot(new_max - run_max[t] > 8.0f) != 0) {
           const float down = half_way_down(new_max - run_max[t]);

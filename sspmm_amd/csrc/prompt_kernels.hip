@@ -88,7 +88,8 @@ __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void prompt_attention_kern
   // Numbers offsets[b] / 128 + b .. are sequence b's, enough for its tiles however it lies; a workgroup with one too many ends at once.  (Summing up
   // the tiles of the sequences before: 4096 sequences of 64 tokens, 8 heads 947 us instead of 360.)  Of 64 sequences at a time those with the most
   // keys go first: level x (a causal tile has about as many keys as places before it in its sequence, another as many as its sequence) is
-  // the largest at which more tiles than those before this one are of x or more.
+  // the largest at which more tiles than those before this one are of x or more.  CROSS: those with the most queries, whatever keys they see, and of as many queries the first (64 sequences
+  // of 128 queries on 50 to 3893 states, 32 heads on 8 of 128, the longest in front 301 us, behind 333).
   int first = 0, length = -1, q0 = 0;  // the sequence's first row and rows, the workgroup's first query in it
   int key_first = 0, keys = 0;  // its first key's row, and keys
   const auto base = [&](int chunk) { return max(0, min(p.offsets[64 * chunk], p.tokens)) / kTileQueries + 64 * chunk; };

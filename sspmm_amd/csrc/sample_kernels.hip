@@ -30,7 +30,9 @@ typedef unsigned long long u64;
 constexpr int kThreads = 512, kManyThreads = 1024;
 constexpr int kBins = 1024;                // of a row or its list, the last one for what weighs nothing
 constexpr int kList = 6144;                // logits of a list
-constexpr int kMostTopK = 1200;            // that the threads' four large ones each give a bound for
+// The largest top_k that the threads' four large ones give a bound for; above it rows have bins.  By a list and by bins, us: 30 rows of 5000 logits, top_k of 1200 28 and 25, 30 of 20000
+// 32 and 31, 200 of 50000 37 and 43, 64 of 131072 37 and 61, 384 of 100003 (fp32) 91 and 126; top_k of 2000 34 and 25, 42 and 33, 44 and 45, 41 and 62, 115 and 127.
+constexpr int kMostTopK = 1200;
 
 struct F32 {};
 
@@ -164,7 +166,7 @@ __device__ __forceinline__ int shift_of(uint32_t span) {
 }
 
 // A row in memory, or one of the parts that its lines of 128 bytes are dealt to in turn: tokens that are likely often stand side by side, a vocabulary's first ones for
-// instance, and a part that had them all would list too few of them (64 rows of 131072 whose first tokens are likely, top_k of 100: 20.7 us, by parts of one stretch each 114).
+// instance, and a part that had them all would list too few of them (64 rows of 131072 whose first tokens are likely, top_k of 100: 22 us, by parts of one stretch each 114).
 template <typename T>
 struct RowReader {
   typedef Elements<T> E;
@@ -577,8 +579,8 @@ template <typename T, int N>
 __device__ __forceinline__ uint32_t list_first(const RowReader<T> &reader, const Setting &setting, uint32_t wanted, float &largest, Shared<N> &s) {
   const int tid = threadIdx.x;
   constexpr int kPairs = 2;  // (the largest and the one behind it, of the even and of the odd places of all blocks)
-  // (where first ones stand side by side, a list has all logits of as many blocks, and the parts' lists have to fit one: 8 parts of a sorted row, 16 bits, top_k of 200 34 us, more than fit 288;
-  // in any order, top_k of 300, 22.6 and, with four a thread, 26.1)
+  // (Where first ones stand side by side, a list has all logits of as many blocks, and the parts' lists have to fit one: 64 sorted rows of 131072 in bf16, top_k of 200, 38 us, and
+  // 288 with lists that do not.  In any order one a thread takes 21.7 us there and four 25.1.)
   const bool one = wanted <= min(N / 4, (kList - kFewAlike) / (RowReader<T>::E::kCount * reader.parts));
   float large[2 * kPairs];
 #pragma unroll
@@ -722,7 +724,7 @@ __global__ __launch_bounds__(N, 4) void sample_tokens_kernel(const SampleArgs p)
   finish(p, setting, r, reader, most, !setting.few(), s.listed <= kList, s);
 }
 
-// ---- The same where rows are few: p.parts workgroups a row, four launches.  What they leave for each other:
+// ---- The same where rows are few: p.parts workgroups a row, four launches, or the first and the last where no row has bins.  What they leave for each other:
 constexpr int kMostParts = 8;  // (the third launch's workgroups go over all parts' bins)
 struct Part {
   float most;

@@ -212,7 +212,8 @@ def cross_attention(q, k, v, offsets, source_offsets, scaling=None, out=None):
     """softmax(q k^T * scaling) v of packed queries over packed states of other lengths, a decoder's over its encoder's: q [tokens, heads, d], k and v
     [source_tokens, kv_heads, d]; the queries of sequence b, offsets[b] .. offsets[b + 1] - 1, see all of source_offsets[b] .. source_offsets[b + 1] - 1 and
     nothing else.  Types, head widths, strides, scaling and out as in prompt_attention; single tokens are sequences of one.  A sequence without states is
-    zeros; tokens of no sequence are not written."""
+    zeros; tokens of no sequence are not written.  Work is shared out by the mean length of the sources, which the host knows: one that is many times longer than the mean is faster in a call of its
+    own (single tokens, 32 heads on 8 of 128: 65536 states 51 us alone, 798 beside 63 sequences of 100)."""
     dtype, device = q.dtype, q.get_device()
     kind = TYPES.get(dtype)
     if (kind is None or device < 0 or k.dtype is not dtype or v.dtype is not dtype or k.get_device() != device or v.get_device() != device or
@@ -420,12 +421,13 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     With the weights w = exp((l - max l) / temperature), kept are those with w >= min_p; of these the top_k first in the order of falling logits, equal ones by
     rising index; of these the shortest run, at least one, whose weights reach top_p of the sum of all of these.  The token is the first in that order at which
     the running sum of the weights exceeds uniform times their sum.  Each setting is a number or a tensor with one for every row (float32, top_k int32).
-    temperature 0: the largest logit, its first index; top_k 0, top_p 1, min_p 0: everything is kept (of tensors, which the host does not look at, also temperature and
-    top_k below 0, and NaN: temperature as 0, the others as what keeps everything).  Logits of -infinity, and NaN, are never drawn; of +infinity they share the draw; a row without any other gives -1.
+    temperature 0: the largest logit, its first index; top_k 0, top_p 1, min_p 0: everything is kept.  What tensors hold, which the host does not look at, is taken to the nearer end:
+    temperature, top_k, top_p and min_p below 0 as 0, top_p and min_p above 1 as 1 (a min_p of 1 keeps the largest logits), uniform below 0 as 0, of 1 and above as the last number below; and NaN as
+    temperature 0, as what keeps everything, and as uniform 0.  Logits of -infinity, and NaN, are never drawn; of +infinity they share the draw; a row without any other gives -1.
     probabilities: (tokens, float32 [rows] of the probabilities with which they were drawn).
 
     Weights are whole multiples of 2^-b (vocab * 2^b <= 2^62, b at most 50) of the power of 2^(1/16) nearest to them, so that no order of sums changes a token.  Rows may lie apart, at any element;
-    other strides are copied first.  At most 2^24 tokens in a vocabulary."""
+    other strides are copied first.  At most 2^24 tokens in a vocabulary, and fewer than 2^22 rows."""
     kind, device = LOGIT_TYPES.get(logits.dtype), logits.get_device()
     if kind is None or device < 0:
         raise TypeError("logits must be a float16, bfloat16 or float32 tensor on a GPU")
