@@ -207,8 +207,8 @@ def _in_turn(*calls):
 @pytest.mark.parametrize("order", ["likely ones first", "sorted"])
 @pytest.mark.parametrize("top_k", [100, 200, 1000])
 def test_likely_tokens_side_by_side_take_no_longer(built_library, top_k, order):
-    """The parts' lists suffice, wherever a row's first tokens lie: in less than twice the time of the same logits in any order (the whole row by one workgroup takes five
-    times as long and more)."""
+    """The parts' lists suffice, wherever a row's first tokens lie: in less than three times the time of the same logits in any order (the lists are up to eight times as long
+    where they are sorted, 1.05 to 1.75 times the time; the whole row by one workgroup takes 3.9 to 13 times)."""
     rows, vocab = 64, 131072
     x, uniform = _logits(rows, vocab, torch.float32, seed=top_k, spread=2.0)
     x = x.sort(1, descending=True).values if order == "sorted" else x - 0.8 * torch.log(1.0 + torch.arange(vocab, device="cuda"))
@@ -217,7 +217,7 @@ def test_likely_tokens_side_by_side_take_no_longer(built_library, top_k, order):
     for logits in (x, anywhere):
         _check(logits[:2], uniform[:2], 0.8, top_k)
     first, other = _in_turn(lambda: sspmm_amd.sample_tokens(x, uniform, 0.8, top_k), lambda: sspmm_amd.sample_tokens(anywhere, uniform, 0.8, top_k))
-    assert first < 2 * other, "%.1f us, in any order %.1f" % (first, other)
+    assert first < 3 * other, "%.1f us, in any order %.1f" % (first, other)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
